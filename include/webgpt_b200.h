@@ -306,6 +306,88 @@ int32_t wgpt_session_generate_sample(wgpt_session *session, int32_t n_new, int32
 int32_t wgpt_sample_topk(wgpt_device *dev, const float *logits, int32_t n_rows, int32_t V, int32_t top_k,
                          double temperature, const double *uniforms, uint32_t *ids_out);
 
+/* ---- serving sequences of different lengths: a paged key-value cache, attention over it, its eviction, and the
+ *      verification of drafted tokens. No counterpart in the reference, which recomputes one window per token
+ *      (model.js:69,104-268); the attention is that of instructions.js:1101-1214 and the softmax and pick are those of
+ *      globals.js:47-74. All of these calls only enqueue; what a kernel finds wrong in device memory (a page id, a length,
+ *      row offsets, a token id out of range, a row of logits without a distribution) is skipped as said below and reported
+ *      by the next wgpt_device_check as WGPT_ERR_ARG. Nothing of a captured call depends on host memory. */
+
+enum { WGPT_TYPE_F32 = 0, WGPT_TYPE_F16 = 1, WGPT_TYPE_BF16 = 2 };
+
+/* One layer's cache: position j of sequence s lies in page table[s * table_stride + j / page_size], slot j % page_size, and
+ * its key row of head h begins at k[page * page_stride + slot * position_stride + h * head_stride] (v likewise; strides in
+ * elements, so that pools [page][position][head][head_size] and [page][head][position][head_size] both fit). Several layers
+ * may share table and lengths; sequences may share pages that are only read. The descriptor is read during the call; the
+ * arrays it names are read when the kernels run. Requirements, otherwise WGPT_ERR_SHAPE / WGPT_ERR_ALIGN: head_size a
+ * multiple of 8 up to 256, table_stride * page_size >= max_length, k and v 16-byte aligned, strides that are not negative and multiples of
+ * 16 bytes. Of what lies in the pages, only positions below a sequence's length are read. */
+typedef struct wgpt_paged_cache {
+  void *k, *v;              /* pools of n_pages pages, elements of `type` */
+  const uint32_t *table;    /* [n_seq, table_stride] page ids; entries behind a sequence's last page are not read */
+  int32_t *lengths;         /* [n_seq] positions held, the new tokens of the step at hand among them */
+  int64_t page_stride, position_stride, head_stride;
+  int32_t type;             /* WGPT_TYPE_* */
+  int32_t n_pages, page_size, n_kv_head, head_size, n_seq, table_stride;
+  int32_t max_length;       /* no sequence is longer; a longer one is read and written up to here and reported */
+} wgpt_paged_cache;
+
+/* The rows of the new tokens of a step lie behind one another, sequence by sequence: sequence s has the rows
+ * starts[s] .. starts[s+1] - 1 (starts: n_seq + 1 numbers in device memory, not decreasing, the last at most n_rows), or
+ * n_rows / n_seq rows each where starts is NULL. Row i of a sequence's n new rows is its position lengths[s] - n + i.
+ * Rows from starts[n_seq] on, and rows whose position would be negative, belong to no token.
+ *
+ * Writes the new tokens' key and value rows (n_kv_head * head_size f32 values each, rows ld apart) into the cache, rounded
+ * once to its type. Two sequences must not write to the same slot. ld a multiple of 4. */
+int32_t wgpt_paged_append(wgpt_device *dev, const wgpt_paged_cache *cache, int32_t n_rows, const int32_t *starts,
+                          const float *k, const float *v, int64_t ld);
+
+/* Attention of the new tokens over the cache, their own rows included (append first). Row r of q has n_head heads of
+ * head_size f32 values, rows ld_q apart; head h reads the cache's head h / (n_head / n_kv_head). The row of position t sees
+ * the positions j <= t, and of these j > t - window where window > 0:
+ *   out = sum_j softmax_j(scale * q . k_j) v_j,
+ * f32 throughout (half-precision caches go through the tensor cores as they are, q and the probabilities as sums of half-precision values). A row
+ * that belongs to a token but sees nothing (it has no position, or a page id of its is out of range throughout) is set to zeros; positions in a page whose id is out of range are not seen. Rows that belong to no sequence are left as they were.
+ * weights, or NULL: [n_seq, ld_weights] f32, ld_weights >= max_length; the attention weight that each position got, summed
+ * over the heads and new tokens of its sequence, is added to weights[s * ld_weights + j]. The order of all sums is fixed:
+ * the same call gives the same bits. */
+int32_t wgpt_paged_attention(wgpt_device *dev, const wgpt_paged_cache *cache, int32_t n_rows, const int32_t *starts,
+                             int32_t n_head, float scale, int32_t window, const float *q, int64_t ld_q, float *out,
+                             int64_t ld_out, float *weights, int64_t ld_weights);
+
+/* Thins out every sequence that holds more than `keep` positions: the `recent` newest stay and, of the older ones, the
+ * keep - recent with the largest accumulated weight (the lowest position among equals; NaN counts as the largest). What
+ * stays keeps its order and goes to the positions 0, 1, ... of the cache `to`, which has the shape and type of `from` and
+ * pages, a table and lengths of its own; its lengths are set to min(length, keep). Sequences of up to `keep` positions are copied
+ * whole. The pages of `to` must not overlap the pages of `from` (slots that are read may be shared by sequences, so
+ * nothing is moved in place): hand over free pages and take back the old ones. Key and value rows are copied as they are.
+ * weights [n_seq, ld_weights] as above; weights_to [n_seq, ld_weights_to >= keep], or NULL: the weights of what stays, zeros
+ * behind it; kept [n_seq, keep]: the positions in `from` that stayed, -1 behind them. 0 <= recent <= keep, keep >= 1,
+ * to->max_length >= min(keep, from->max_length). A position whose page id is out of range, on either side, is not copied. */
+int32_t wgpt_paged_evict(wgpt_device *dev, const wgpt_paged_cache *from, const wgpt_paged_cache *to, int32_t keep,
+                         int32_t recent, const float *weights, int64_t ld_weights, float *weights_to,
+                         int64_t ld_weights_to, int32_t *kept);
+
+/* Speculative sampling's accept step. Sequence s has drafted n_drafted[s] tokens (n_draft where n_drafted is NULL), ids
+ * draft_ids[s * n_draft + i]; target holds n_draft + 1 rows of V logits per sequence (rows ld_target apart), row i those
+ * behind the i-th draft (row 0: before any); draft, or NULL, n_draft rows per sequence, the logits that the drafts were drawn
+ * from. With p_i and q_i the softmax of logits / temperature, over the top_k largest where top_k > 0 (NULL draft: q_i is one
+ * at the drafted id), draft i is accepted while uniforms[s * (n_draft + 1) + i] * q_i(x_i) < p_i(x_i). At the first that is not, the
+ * next token is drawn from max(p_i - q_i, 0), or from p_i if that is zero everywhere; behind the last accepted one from
+ * p_i. Drawn: with the number uniforms[s * (n_draft + 1) + n_draft] in [0,1), the first id whose running sum exceeds number * total, in
+ * the order of the ids, or of descending logits where top_k > 0 (so that no drafts and a top_k give wgpt_sample_topk's
+ * pick). Probabilities that decide are in double precision. NaN logits count as -infinity; a row with no finite value or with +infinity has no distribution:
+ * as a target it accepts nothing and draws id 0, as a draft it accepts nothing and counts as q = 0, and both are reported. A drafted id >= V is not
+ * accepted and reported.
+ * ids_out [n_seq, n_draft + 1]: the accepted drafts, the drawn token, WGPT_NO_ID behind it; n_accepted [n_seq].
+ * 0 <= n_draft <= WGPT_MAX_DRAFT, 0 <= top_k <= min(WGPT_MAX_TOP_K, V). */
+#define WGPT_MAX_DRAFT 64
+#define WGPT_NO_ID 0xFFFFFFFFu
+int32_t wgpt_verify_drafts(wgpt_device *dev, int32_t n_seq, int32_t n_draft, int32_t V, const float *target,
+                           int64_t ld_target, const float *draft, int64_t ld_draft, const uint32_t *draft_ids,
+                           const int32_t *n_drafted, int32_t top_k, double temperature, const double *uniforms,
+                           uint32_t *ids_out, int32_t *n_accepted);
+
 /* GPT.externalBuffer tap (model.js:18,211-222): copies the residual stream before ln_f of the most recent
  * forward ([rows, n_embd], rows = n_seq * tokens of that call) into dst (device memory). */
 int32_t wgpt_session_tap(wgpt_session *session, float *dst, uint64_t max_floats, uint64_t *floats_written);

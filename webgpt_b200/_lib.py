@@ -32,8 +32,21 @@ class Params(C.Structure):
     _fields_ = [(k, C.c_int32) for k in ("n_layer", "n_head", "n_embd", "n_ctx", "vocab_size", "bias")]
 
 
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2  # WGPT_TYPE_*
+MAX_DRAFT, NO_ID = 64, 0xFFFFFFFF
+
+
+class PagedCache(C.Structure):
+    """wgpt_paged_cache: one layer's pools, page table and lengths (device addresses) and their shape."""
+    _fields_ = [(k, C.c_void_p) for k in ("k", "v", "table", "lengths")] + \
+               [(k, C.c_int64) for k in ("page_stride", "position_stride", "head_stride")] + \
+               [(k, C.c_int32) for k in ("type", "n_pages", "page_size", "n_kv_head", "head_size", "n_seq", "table_stride",
+                                         "max_length")]
+
+
 vp, vpp = C.c_void_p, C.POINTER(C.c_void_p)
-i32, u64, f32 = C.c_int32, C.c_uint64, C.c_float
+i32, u64, f32, i64 = C.c_int32, C.c_uint64, C.c_float, C.c_int64
+cache = C.POINTER(PagedCache)
 
 # name -> argument types; every function returns int32 status unless listed in _SPECIAL
 SIGNATURES = {
@@ -94,6 +107,10 @@ SIGNATURES = {
     "wgpt_session_generate_sample": [vp, i32, i32, C.c_double, vp],
     "wgpt_sample_topk": [vp, vp, i32, i32, i32, C.c_double, vp, vp],
     "wgpt_visuals_render": [vp, vp, i32, i32, vp],
+    "wgpt_paged_append": [vp, cache, i32, vp, vp, vp, i64],
+    "wgpt_paged_attention": [vp, cache, i32, vp, i32, f32, i32, vp, i64, vp, i64, vp, i64],
+    "wgpt_paged_evict": [vp, cache, cache, i32, i32, vp, i64, vp, i64, vp],
+    "wgpt_verify_drafts": [vp, i32, i32, i32, vp, i64, vp, i64, vp, vp, i32, C.c_double, vp, vp, vp],
     "wgpt_session_tap": [vp, vp, u64, C.POINTER(u64)],
 }
 _SPECIAL = {"wgpt_abi_version": (i32, []), "wgpt_last_error": (C.c_char_p, [])}

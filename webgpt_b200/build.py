@@ -6,11 +6,12 @@ else, so it loads on a machine without a GPU (where every device call then repor
 import os
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libwebgpt_b200.so")
-SOURCES = ["api.cu"]
+SOURCES = ["api.cu", "serving.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--use_fast_math=false",
     "-Xcompiler", "-fPIC,-fvisibility=hidden,-O3", "-shared", "-cudart", "static",
@@ -35,15 +36,24 @@ def needs_build():
 def build(force=False, verbose=False):
     if not force and not needs_build():
         return LIB
-    flags = [f for f in NVCC_FLAGS if f != "--use_fast_math=false"]
-    cmd = [_nvcc()] + flags + (["-Xptxas", "-v"] if verbose else []) + \
-          [os.path.join(CSRC, s) for s in SOURCES] + ["-o", LIB]
-    res = subprocess.run(cmd, capture_output=True, text=True)
+    flags = [f for f in NVCC_FLAGS if f not in ("--use_fast_math=false", "-shared")]
+    with tempfile.TemporaryDirectory() as tmp:
+        objects = [os.path.join(tmp, s + ".o") for s in SOURCES]
+        jobs = [subprocess.Popen([_nvcc()] + flags + (["-Xptxas", "-v"] if verbose else []) +
+                                 ["-c", os.path.join(CSRC, s), "-o", o],
+                                 stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+                for s, o in zip(SOURCES, objects)]
+        said = [j.communicate()[0] for j in jobs]
+        if any(j.returncode for j in jobs):
+            sys.stderr.write("".join(said))
+            raise RuntimeError("nvcc failed")
+        res = subprocess.run([_nvcc()] + NVCC_FLAGS[:2] + ["-shared", "-cudart", "static", "-o", LIB] + objects,
+                             capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
         raise RuntimeError("nvcc failed")
     if verbose:
-        sys.stderr.write(res.stderr)
+        sys.stderr.write("".join(said))
     return LIB
 
 

@@ -1,6 +1,4 @@
-// C ABI of webgpt_b200 (declared in include/webgpt_b200.h): device/buffer management, the per-operator entry
 // points mirroring the reference's instruction classes, and the model/session level that mirrors class GPT.
-#include "../../include/webgpt_b200.h"
 
 #include <cuda_runtime.h>
 
@@ -29,6 +27,7 @@
 #include "gemm_split.cuh"
 #include "gemm_stream.cuh"
 #include "gemv_ring.cuh"
+#include "host.cuh"
 #include "int8.cuh"
 #include "sampling.cuh"
 #include "matmul.cuh"
@@ -36,12 +35,10 @@
 
 using namespace wgpt;
 
-#define WGPT_EXPORT extern "C" __attribute__((visibility("default")))
-
-// ------------------------------------------------------------------------------------------ errors
+// ------------------------------------------------------------------------------------------ errors, device
 static thread_local char g_err[512] = "";
 
-static int32_t fail(int32_t code, const char *fmt, ...) {
+int32_t fail(int32_t code, const char *fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
   vsnprintf(g_err, sizeof g_err, fmt, ap);
@@ -49,185 +46,14 @@ static int32_t fail(int32_t code, const char *fmt, ...) {
   return code;
 }
 
-#define CK(call)                                                                                   \
-  do {                                                                                             \
-    cudaError_t e__ = (call);                                                                      \
-    if (e__ != cudaSuccess)                                                                        \
-      return fail(e__ == cudaErrorMemoryAllocation ? WGPT_ERR_OOM : WGPT_ERR_CUDA, "%s: %s", #call, \
-                  cudaGetErrorString(e__));                                                        \
-  } while (0)
-
-#define TRY(call)                 \
-  do {                            \
-    int32_t rc__ = (call);        \
-    if (rc__ != WGPT_OK) return rc__; \
-  } while (0)
-
-#define REQUIRE(cond, code, ...) \
-  do {                           \
-    if (!(cond)) return fail((code), __VA_ARGS__); \
-  } while (0)
-
-static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-// ------------------------------------------------------------------------------------------ device
-struct wgpt_device {
-  int ordinal;
-  cudaStream_t stream;
-  int precision;
-  uint64_t launches;
-  int sm_count;
-  size_t smem_optin;
-  void *scratch;  // library-owned workspace (split-K partial sums, temporaries of wgpt_attention)
-  size_t scratch_cap;
-  uint64_t scratch_gen;  // bumped whenever the workspace moves: recorded pass lists hold its old address
-  int *d_err;     // device-side error word (out-of-range token id)
-  float *tc_scratch;  // split-K partial tiles of the tensor-core GEMM (fixed size)
-  size_t tc_scratch_bytes;
-  bool pdl;       // launch the decode-chain kernels with programmatic dependent launch (WGPT_PDL=0 turns it off)
-  bool graphs;    // replay decode steps as a CUDA graph (WGPT_GRAPH=0 turns it off)
-  bool capturing;   // between wgpt_graph_begin and wgpt_graph_end
-  uint64_t capture_launch0;
-  bool block_gemv;  // layer GEMVs through gemv_block_kernel (WGPT_BLOCK_GEMV=0: register-streaming kernel)
-  int deembed_tc_min_rows;   // fewest sequences whose de-embedding runs on the tensor-core GEMM (WGPT_DEEMBED_TC_ROWS)
-  int gemv_stream_max_rows;  // most rows the register-streaming GEMV takes for a layer product (WGPT_GEMV_MAX_ROWS)
-  unsigned int *d_work;  // two counters of gemv_loop_kernel (left zero by every launch)
-  bool loop_gemv;     // products against matrices larger than L2 through gemv_loop_kernel (WGPT_LOOP_GEMV=0: off)
-  int max_clusters[9];  // clusters of S CTAs of gemm_split_kernel resident at once with one CTA per SM
-  bool fused_decode;  // single-sequence decode with two kernels per block (WGPT_FUSED_DECODE=0 turns it off)
-};
-
-#define LAUNCH(dev, kernel, grid, block, smem, ...)                       \
-  do {                                                                    \
-    kernel<<<(grid), (block), (smem), (dev)->stream>>>(__VA_ARGS__);      \
-    (dev)->launches++;                                                    \
-    CK(cudaGetLastError());                                               \
-  } while (0)
-
-// Lets a kernel take all the dynamic shared memory that its static part leaves, once per kernel and device. The limit is
-// never lowered again: two threads that drive two devices handles share it, and one setting its own launch's size could
-// undercut the other's between that one's setting and its launch.
-static cudaError_t allow_smem_raw(const wgpt_device *dev, const void *kern, bool whole_carveout) {
-  static std::mutex mu;
-  static std::set<std::pair<const void *, int>> done;
-  std::lock_guard<std::mutex> lock(mu);
-  if (done.count({kern, dev->ordinal})) return cudaSuccess;
-  cudaFuncAttributes at;
-  cudaError_t e = cudaFuncGetAttributes(&at, kern);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(dev->smem_optin - at.sharedSizeBytes));
-  // the whole carveout, so that the next kernel's CTA fits on the SM beside this one's and fetches its weights early
-  if (e == cudaSuccess && whole_carveout)
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, (int)cudaSharedmemCarveoutMaxShared);
-  if (e == cudaSuccess) done.insert({kern, dev->ordinal});
-  return e;
-}
-template <typename K>
-static cudaError_t allow_smem(const wgpt_device *dev, K kern, bool whole_carveout = false) {
-  return allow_smem_raw(dev, reinterpret_cast<const void *>(kern), whole_carveout);
-}
-
-// Launch for kernels that call pdl_wait() before touching anything an earlier kernel wrote: with dev->pdl they
-// carry the programmatic-serialisation attribute and may start while their predecessor is still running.
-template <typename... KArgs, typename... Args>
-static cudaError_t launch_ex(bool pdl, int cluster_z, cudaStream_t stream, void (*kernel)(KArgs...), dim3 grid,
-                             dim3 block, size_t smem, Args... args);
-// The same with clusters of cluster_x CTAs along x.
-template <typename... KArgs, typename... Args>
-static cudaError_t launch_ex_x(bool pdl, int cluster_x, cudaStream_t stream, void (*kernel)(KArgs...), dim3 grid,
-                               dim3 block, size_t smem, const Args &...args) {
-  cudaLaunchConfig_t cfg;
-  memset(&cfg, 0, sizeof cfg);
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  int n = 0;
-  if (pdl) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n].val.programmaticStreamSerializationAllowed = 1;
-    n++;
-  }
-  attr[n].id = cudaLaunchAttributeClusterDimension;
-  attr[n].val.clusterDim.x = (unsigned)cluster_x;
-  attr[n].val.clusterDim.y = 1;
-  attr[n].val.clusterDim.z = 1;
-  n++;
-  cfg.attrs = attr;
-  cfg.numAttrs = n;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
-// Launch with thread-block clusters of cluster_x CTAs along x (and programmatic dependent launch if pdl).
-template <typename P>
-static cudaError_t launch_cluster_x(bool pdl, int cluster_x, cudaStream_t stream, void (*kernel)(P), dim3 grid,
-                                    dim3 block, size_t smem, const P &arg) {
-  cudaLaunchConfig_t cfg;
-  memset(&cfg, 0, sizeof cfg);
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  int n = 0;
-  if (pdl) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n].val.programmaticStreamSerializationAllowed = 1;
-    n++;
-  }
-  attr[n].id = cudaLaunchAttributeClusterDimension;
-  attr[n].val.clusterDim.x = (unsigned)cluster_x;
-  attr[n].val.clusterDim.y = 1;
-  attr[n].val.clusterDim.z = 1;
-  n++;
-  cfg.attrs = attr;
-  cfg.numAttrs = n;
-  return cudaLaunchKernelEx(&cfg, kernel, arg);
-}
-
-template <typename... KArgs, typename... Args>
-static cudaError_t launch_ex(bool pdl, int cluster_z, cudaStream_t stream, void (*kernel)(KArgs...), dim3 grid,
-                             dim3 block, size_t smem, Args... args) {
-  cudaLaunchConfig_t cfg;
-  memset(&cfg, 0, sizeof cfg);
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  int n = 0;
-  if (pdl) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n].val.programmaticStreamSerializationAllowed = 1;
-    n++;
-  }
-  if (cluster_z > 1) {  // thread-block clusters along z
-    attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = 1;
-    attr[n].val.clusterDim.y = 1;
-    attr[n].val.clusterDim.z = (unsigned)cluster_z;
-    n++;
-  }
-  cfg.attrs = attr;
-  cfg.numAttrs = n;
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
-}
-
-#define LAUNCH_PDL(dev, kernel, grid, block, smem, ...)                                          \
-  do {                                                                                           \
-    CK(launch_ex((dev)->pdl, 0, (dev)->stream, kernel, dim3(grid), dim3(block), (smem), __VA_ARGS__)); \
-    (dev)->launches++;                                                                           \
-  } while (0)
-
-static int32_t use(wgpt_device *dev) {
+int32_t use(wgpt_device *dev) {
   REQUIRE(dev != nullptr, WGPT_ERR_ARG, "device handle is null");
   CK(cudaSetDevice(dev->ordinal));
   return WGPT_OK;
 }
 
 // Grows the workspace. Work already enqueued may still be using the old block, so drain first.
-static int32_t scratch_reserve(wgpt_device *dev, size_t bytes) {
+int32_t scratch_reserve(wgpt_device *dev, size_t bytes) {
   if (bytes <= dev->scratch_cap) return WGPT_OK;
   REQUIRE(!dev->capturing, WGPT_ERR_STATE,
           "the workspace would have to grow while a pass list is being recorded: run the pass list once first");
@@ -235,17 +61,18 @@ static int32_t scratch_reserve(wgpt_device *dev, size_t bytes) {
   if (dev->scratch) CK(cudaFree(dev->scratch));
   dev->scratch = nullptr;
   dev->scratch_cap = 0;
+  dev->scratch_gen++;  // with the old block gone, whether or not a new one is found
   size_t cap = (bytes + (size_t(1) << 20) - 1) & ~((size_t(1) << 20) - 1);
-  CK(cudaMalloc(&dev->scratch, cap));
+  cudaError_t e = cudaMalloc(&dev->scratch, cap);
+  if (e != cudaSuccess) {
+    dev->scratch = nullptr;
+    cudaGetLastError();  // the next launch's check is not to find it
+    return fail(e == cudaErrorMemoryAllocation ? WGPT_ERR_OOM : WGPT_ERR_CUDA, "workspace of %zu bytes: %s", cap,
+                cudaGetErrorString(e));
+  }
   dev->scratch_cap = cap;
-  dev->scratch_gen++;
   return WGPT_OK;
 }
-
-// Calls that synchronise the stream (or free memory a recording may name) are not valid while a pass list is
-// being recorded: a synchronise on a capturing stream would invalidate the capture.
-#define NOT_RECORDING(dev, what)                                                                       \
-  REQUIRE(!(dev)->capturing, WGPT_ERR_STATE, "%s is not valid between wgpt_graph_begin and wgpt_graph_end", what)
 
 WGPT_EXPORT int32_t wgpt_abi_version(void) { return WGPT_ABI_VERSION; }
 WGPT_EXPORT const char *wgpt_last_error(void) { return g_err; }
@@ -273,6 +100,7 @@ WGPT_EXPORT int32_t wgpt_device_create(int32_t ordinal, wgpt_device **out) {
   dev->scratch_gen = 0;
   dev->d_err = nullptr;
   dev->d_work = nullptr;
+  dev->d_join = nullptr;
   const char *ev = getenv("WGPT_PDL");
   dev->pdl = !(ev && ev[0] == '0');
   ev = getenv("WGPT_GRAPH");
@@ -295,6 +123,8 @@ WGPT_EXPORT int32_t wgpt_device_create(int32_t ordinal, wgpt_device **out) {
   if (e == cudaSuccess) e = cudaMalloc(&dev->d_err, sizeof(int));
   if (e == cudaSuccess) e = cudaMalloc(&dev->d_work, 2 * sizeof(unsigned int));
   if (e == cudaSuccess) e = cudaMemsetAsync(dev->d_work, 0, 2 * sizeof(unsigned int), dev->stream);
+  if (e == cudaSuccess) e = cudaMalloc(&dev->d_join, kJoinCounters * sizeof(unsigned int));
+  if (e == cudaSuccess) e = cudaMemsetAsync(dev->d_join, 0, kJoinCounters * sizeof(unsigned int), dev->stream);
   if (e == cudaSuccess) e = cudaMalloc(&dev->tc_scratch, dev->tc_scratch_bytes);
   if (e == cudaSuccess) e = cudaMemsetAsync(dev->d_err, 0, sizeof(int), dev->stream);
   if (e != cudaSuccess) {
@@ -328,6 +158,7 @@ WGPT_EXPORT int32_t wgpt_device_destroy(wgpt_device *dev) {
   if (dev->scratch) cudaFree(dev->scratch);
   if (dev->d_err) cudaFree(dev->d_err);
   if (dev->d_work) cudaFree(dev->d_work);
+  if (dev->d_join) cudaFree(dev->d_join);
   if (dev->tc_scratch) cudaFree(dev->tc_scratch);
   cudaStreamDestroy(dev->stream);
   delete dev;
@@ -1490,6 +1321,10 @@ static int32_t check_err_word(wgpt_device *dev, const char *what) {
     if (h == 4) return fail(WGPT_ERR_TIMEOUT, "%s: the whole-token decode kernel gave up at a grid barrier", what);
     if (h == 2) return fail(WGPT_ERR_TIMEOUT, "%s: a bulk copy into shared memory did not complete in time", what);
     if (h == 3) return fail(WGPT_ERR_TIMEOUT, "%s: the tensor-core GEMM pipeline gave up waiting on a barrier", what);
+    if (h == 5)
+      return fail(WGPT_ERR_ARG, "%s: a paged cache's page id, length or row offsets are out of range", what);
+    if (h == 7) return fail(WGPT_ERR_ARG, "%s: a sequence's number of drafts is out of range", what);
+    if (h == 6) return fail(WGPT_ERR_ARG, "%s: a row of logits has no finite value or one of +infinity", what);
     return fail(WGPT_ERR_ARG, "%s: token id out of range", what);
   }
   return WGPT_OK;

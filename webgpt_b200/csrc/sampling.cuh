@@ -16,22 +16,12 @@
 // The kernel then writes the token and advances the session like argmax_kernel.
 #pragma once
 #include "common.cuh"
+#include "sample_key.cuh"
 
 namespace wgpt {
 
 constexpr int kSampleThreads = 1024;
 constexpr int kMaxTopK = 128;
-
-__device__ __forceinline__ unsigned long long sample_key(float v, int idx) {
-  uint32_t u = __float_as_uint(v);
-  if (u == 0x80000000u) u = 0u;  // -0 and +0 compare equal in the reference's sort
-  uint32_t k = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-  return ((unsigned long long)k << 32) | (unsigned long long)(0xFFFFFFFFu - (uint32_t)idx);
-}
-
-__device__ __forceinline__ int sample_key_index(unsigned long long c) {
-  return (int)(0xFFFFFFFFu - (uint32_t)(c & 0xFFFFFFFFull));
-}
 
 // Dynamic shared memory: (1024 + cap) 64-bit keys, cap = top_k * ceil(V / 1024).
 // uniforms: [steps][gridDim.x] doubles in [0,1), indexed by the session's step counter.
@@ -176,10 +166,6 @@ sample_topk_kernel(const float *__restrict__ logits, int V, int top_k, double te
 //      as sample_topk_kernel does from its sorted list, with the logits taken out of the keys.
 constexpr int kPickThreads = 512, kPickVals = 16, kPickCap = 256, kPickTopK = 48, kPickCluster = 8;
 
-__device__ __forceinline__ float sample_key_value(unsigned long long c) {
-  const uint32_t k = (uint32_t)(c >> 32);
-  return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
-}
 __device__ __forceinline__ unsigned long long max64(unsigned long long a, unsigned long long b) { return a > b ? a : b; }
 
 __global__ void __launch_bounds__(kPickThreads)

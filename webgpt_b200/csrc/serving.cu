@@ -1,0 +1,192 @@
+// The operators that serve sequences of different lengths: the paged key-value cache (append, attention, eviction) and the
+// verification of drafted tokens, behind the C ABI of include/webgpt_b200.h.
+#include <algorithm>
+
+#include "host.cuh"
+#include "paged.cuh"
+#include "verify.cuh"
+
+using namespace wgpt;
+
+// ------------------------------------------------------------------------------------------ checks
+static int type_bytes(int type) { return type == WGPT_TYPE_F32 ? 4 : 2; }
+
+static int32_t check_cache(wgpt_device *dev, const wgpt_paged_cache *c, PagedView *out) {
+  REQUIRE(c && c->k && c->v && c->table && c->lengths, WGPT_ERR_ARG, "null pointer in the cache");
+  REQUIRE(c->type >= WGPT_TYPE_F32 && c->type <= WGPT_TYPE_BF16, WGPT_ERR_ARG, "unknown cache type %d", c->type);
+  REQUIRE(c->n_pages >= 1 && c->page_size >= 1 && c->n_kv_head >= 1 && c->n_seq >= 1 && c->table_stride >= 1 &&
+              c->max_length >= 1,
+          WGPT_ERR_SHAPE, "empty cache: %d pages of %d, %d heads, %d sequences of up to %d positions, %d pages a table row",
+          c->n_pages, c->page_size, c->n_kv_head, c->n_seq, c->max_length, c->table_stride);
+  REQUIRE(c->head_size >= 8 && c->head_size <= 256 && c->head_size % 8 == 0, WGPT_ERR_SHAPE,
+          "head_size %d is not a multiple of 8 up to 256", c->head_size);
+  REQUIRE((int64_t)c->table_stride * c->page_size >= c->max_length, WGPT_ERR_SHAPE,
+          "%d pages of %d positions a sequence hold fewer than max_length %d", c->table_stride, c->page_size, c->max_length);
+  const int per16 = 16 / type_bytes(c->type);
+  REQUIRE(c->page_stride >= 0 && c->position_stride >= 0 && c->head_stride >= 0, WGPT_ERR_SHAPE, "a stride is negative");
+  REQUIRE(aligned16(c->k) && aligned16(c->v) && c->page_stride % per16 == 0 && c->position_stride % per16 == 0 &&
+              c->head_stride % per16 == 0,
+          WGPT_ERR_ALIGN, "pools must be 16-byte aligned and their strides multiples of 16 bytes");
+  *out = PagedView{c->k,          c->v,         c->table,     c->lengths, c->page_stride,  c->position_stride,
+                   c->head_stride, (uint32_t)c->n_pages, (uint32_t)c->page_size, c->n_kv_head, c->head_size, c->n_seq,
+                   c->table_stride, c->max_length, dev->d_err};
+  return WGPT_OK;
+}
+
+static int32_t check_rows(const wgpt_paged_cache *c, int32_t n_rows, const int32_t *starts, NewRows *out) {
+  REQUIRE(n_rows >= 1, WGPT_ERR_SHAPE, "no rows");
+  REQUIRE(starts || n_rows % c->n_seq == 0, WGPT_ERR_SHAPE, "%d rows do not divide among %d sequences", n_rows, c->n_seq);
+  *out = NewRows{starts, n_rows, n_rows / c->n_seq};
+  return WGPT_OK;
+}
+
+static int32_t check_matrix(const void *p, int64_t ld, int64_t cols, const char *what) {
+  REQUIRE(p != nullptr, WGPT_ERR_ARG, "%s is null", what);
+  REQUIRE(ld >= cols, WGPT_ERR_SHAPE, "rows of %s are %lld values, fewer than %lld", what, (long long)ld, (long long)cols);
+  REQUIRE(aligned16(p) && ld % 4 == 0, WGPT_ERR_ALIGN, "%s must be 16-byte aligned, its rows a multiple of 4 values", what);
+  return WGPT_OK;
+}
+
+// ------------------------------------------------------------------------------------------ cache
+WGPT_EXPORT int32_t wgpt_paged_append(wgpt_device *dev, const wgpt_paged_cache *cache, int32_t n_rows,
+                                      const int32_t *starts, const float *k, const float *v, int64_t ld) {
+  TRY(use(dev));
+  PagedView c;
+  NewRows r;
+  TRY(check_cache(dev, cache, &c));
+  TRY(check_rows(cache, n_rows, starts, &r));
+  TRY(check_matrix(k, ld, (int64_t)c.n_kv * c.hs, "k"));
+  TRY(check_matrix(v, ld, (int64_t)c.n_kv * c.hs, "v"));
+  const int grid = std::min(n_rows, dev->sm_count * 16);
+  if (cache->type == WGPT_TYPE_F32)
+    LAUNCH_PDL(dev, paged_append_kernel<float>, grid, kAppendThreads, 0, c, r, k, v, (long long)ld);
+  else if (cache->type == WGPT_TYPE_F16)
+    LAUNCH_PDL(dev, paged_append_kernel<__half>, grid, kAppendThreads, 0, c, r, k, v, (long long)ld);
+  else
+    LAUNCH_PDL(dev, paged_append_kernel<__nv_bfloat16>, grid, kAppendThreads, 0, c, r, k, v, (long long)ld);
+  return WGPT_OK;
+}
+
+WGPT_EXPORT int32_t wgpt_paged_attention(wgpt_device *dev, const wgpt_paged_cache *cache, int32_t n_rows,
+                                         const int32_t *starts, int32_t n_head, float scale, int32_t window,
+                                         const float *q, int64_t ld_q, float *out, int64_t ld_out, float *weights,
+                                         int64_t ld_weights) {
+  TRY(use(dev));
+  PagedAttention a;
+  TRY(check_cache(dev, cache, &a.c));
+  TRY(check_rows(cache, n_rows, starts, &a.r));
+  REQUIRE(n_head >= 1 && n_head % cache->n_kv_head == 0, WGPT_ERR_SHAPE, "%d heads do not divide among %d of the cache",
+          n_head, cache->n_kv_head);
+  REQUIRE(window >= 0, WGPT_ERR_SHAPE, "window %d is negative", window);
+  const int64_t E = (int64_t)n_head * cache->head_size;
+  TRY(check_matrix(q, ld_q, E, "q"));
+  TRY(check_matrix(out, ld_out, E, "out"));
+  REQUIRE(!weights || ld_weights >= cache->max_length, WGPT_ERR_SHAPE, "rows of weights are %lld values, fewer than max_length %d",
+          (long long)ld_weights, cache->max_length);
+  a.n_head = n_head;
+  a.group = n_head / cache->n_kv_head;
+  a.window = window;
+  a.scale = scale;
+  a.q = q;
+  a.out = out;
+  a.ld_q = ld_q;
+  a.ld_out = ld_out;
+  a.scores = a.stats = nullptr;
+  if (weights) {
+    const size_t rows = (size_t)n_rows * n_head;
+    TRY(scratch_reserve(dev, rows * ((size_t)cache->max_length + 1) * 4));
+    a.stats = static_cast<float *>(dev->scratch);
+    a.scores = a.stats + rows;
+  }
+  REQUIRE(n_rows <= 65535, WGPT_ERR_SHAPE, "%d rows", n_rows);
+  const dim3 grid(n_head, n_rows), block(kPagedWarps * 32);
+  if (cache->type == WGPT_TYPE_F32)
+    LAUNCH_PDL(dev, paged_attention_kernel<float>, grid, block, 0, a);
+  else if (cache->type == WGPT_TYPE_F16)
+    LAUNCH_PDL(dev, paged_attention_kernel<__half>, grid, block, 0, a);
+  else
+    LAUNCH_PDL(dev, paged_attention_kernel<__nv_bfloat16>, grid, block, 0, a);
+  if (weights) {
+    const int blocks = std::min((cache->max_length + 255) / 256, std::max(1, 8 * dev->sm_count / cache->n_seq));
+    LAUNCH_PDL(dev, paged_weights_kernel, dim3(blocks, cache->n_seq), dim3(256), 0, a, weights, (long long)ld_weights);
+  }
+  return WGPT_OK;
+}
+
+WGPT_EXPORT int32_t wgpt_paged_evict(wgpt_device *dev, const wgpt_paged_cache *from, const wgpt_paged_cache *to,
+                                     int32_t keep, int32_t recent, const float *weights, int64_t ld_weights,
+                                     float *weights_to, int64_t ld_weights_to, int32_t *kept) {
+  TRY(use(dev));
+  PagedEvict e;
+  TRY(check_cache(dev, from, &e.from));
+  TRY(check_cache(dev, to, &e.to));
+  REQUIRE(weights && kept, WGPT_ERR_ARG, "null pointer");
+  REQUIRE(from->type == to->type && from->n_kv_head == to->n_kv_head && from->head_size == to->head_size &&
+              from->n_seq == to->n_seq,
+          WGPT_ERR_SHAPE, "the two caches differ in type, heads or sequences");
+  REQUIRE(keep >= 1 && recent >= 0 && recent <= keep, WGPT_ERR_SHAPE, "keep %d and recent %d: 0 <= recent <= keep, keep >= 1",
+          keep, recent);
+  REQUIRE(to->max_length >= std::min(keep, from->max_length), WGPT_ERR_SHAPE, "%d positions do not hold the %d that stay",
+          to->max_length, std::min(keep, from->max_length));
+  REQUIRE(ld_weights >= from->max_length && (!weights_to || ld_weights_to >= keep), WGPT_ERR_SHAPE,
+          "rows of weights are shorter than their sequences");
+  e.keep = keep;
+  e.recent = recent;
+  e.weights = weights;
+  e.weights_to = weights_to;
+  e.kept = kept;
+  e.ld = ld_weights;
+  e.ld_to = ld_weights_to;
+  LAUNCH_PDL(dev, paged_select_kernel, from->n_seq, kEvictThreads, 0, e);
+  const int most = std::min(keep, from->max_length);
+  const int blocks = std::min((most + 7) / 8, std::max(1, 8 * dev->sm_count / from->n_seq));
+  LAUNCH_PDL(dev, paged_gather_kernel, dim3(blocks, from->n_seq), dim3(256), 0, e, type_bytes(from->type));
+  return WGPT_OK;
+}
+
+// ------------------------------------------------------------------------------------------ drafts
+WGPT_EXPORT int32_t wgpt_verify_drafts(wgpt_device *dev, int32_t n_seq, int32_t n_draft, int32_t V, const float *target,
+                                       int64_t ld_target, const float *draft, int64_t ld_draft, const uint32_t *draft_ids,
+                                       const int32_t *n_drafted, int32_t top_k, double temperature,
+                                       const double *uniforms, uint32_t *ids_out, int32_t *n_accepted) {
+  TRY(use(dev));
+  REQUIRE(target && uniforms && ids_out && n_accepted && (draft_ids || n_draft == 0), WGPT_ERR_ARG, "null pointer");
+  REQUIRE(n_seq >= 1 && n_seq <= 65535 && V >= 1, WGPT_ERR_SHAPE, "empty logits, or %d sequences", n_seq);
+  REQUIRE(n_draft >= 0 && n_draft <= WGPT_MAX_DRAFT, WGPT_ERR_SHAPE, "n_draft %d outside 0..%d", n_draft, WGPT_MAX_DRAFT);
+  REQUIRE(top_k >= 0 && top_k <= WGPT_MAX_TOP_K && top_k <= V, WGPT_ERR_SHAPE, "top_k %d outside 0..%d", top_k,
+          std::min<int>(WGPT_MAX_TOP_K, V));
+  REQUIRE(temperature > 0.0, WGPT_ERR_ARG, "temperature must be positive");
+  REQUIRE(ld_target >= V && (!draft || n_draft == 0 || ld_draft >= V), WGPT_ERR_SHAPE, "rows of logits are shorter than %d", V);
+  Verify a;
+  a.n_seq = n_seq;
+  a.n_draft = n_draft;
+  a.V = V;
+  a.top_k = top_k;
+  a.chunks = (V + kVerifyChunk - 1) / kVerifyChunk;
+  a.target = target;
+  a.draft = n_draft ? draft : nullptr;
+  a.ld_target = ld_target;
+  a.ld_draft = ld_draft;
+  a.draft_ids = draft_ids;
+  a.n_drafted = n_drafted;
+  a.temperature = temperature;
+  a.uniforms = uniforms;
+  a.ids_out = ids_out;
+  a.n_accepted = n_accepted;
+  a.err = dev->d_err;
+  const int rows = a.draft ? 2 * n_draft + 1 : n_draft + 1;
+  const size_t places = (size_t)n_seq * (2 * n_draft + 1);
+  if (top_k > 0) {
+    TRY(scratch_reserve(dev, places * top_k * 8));
+    a.list_value = static_cast<float *>(dev->scratch);
+    a.list_id = reinterpret_cast<int *>(a.list_value + places * top_k);
+    LAUNCH_PDL(dev, verify_list_kernel, dim3(rows, n_seq), dim3(kListThreads), 0, a);
+    LAUNCH_PDL(dev, verify_draw_list_kernel, n_seq, 128, 0, a);
+    return WGPT_OK;
+  }
+  TRY(scratch_reserve(dev, places * a.chunks * sizeof(float2)));
+  a.partial = static_cast<float2 *>(dev->scratch);
+  LAUNCH_PDL(dev, verify_sums_kernel, dim3(a.chunks, rows, n_seq), dim3(kVerifyThreads), 0, a);
+  LAUNCH_PDL(dev, verify_draw_kernel, n_seq, kDrawThreads, 0, a);
+  return WGPT_OK;
+}

@@ -5,7 +5,8 @@ import random
 import numpy as np
 
 from .instructions import (AttentionBlockClass, DeEmbedBlockClass, EmbedBlockClass, FastMatMulBlockClass,
-                           GeluBlockClass, LayerNormBlockClass, ResidualBlockClass, SoftmaxBlockClass)
+                           GeluBlockClass, LayerNormBlockClass, PagedAppendBlockClass, PagedAttentionBlockClass,
+                           PagedEvictBlockClass, ResidualBlockClass, SoftmaxBlockClass, VerifyDraftsBlockClass)
 
 # globals.js:1-8
 FastMatMulBlock = FastMatMulBlockClass()
@@ -16,10 +17,14 @@ DeEmbedBlock = DeEmbedBlockClass()
 GeluBlock = GeluBlockClass()
 LayerNormBlock = LayerNormBlockClass()
 SoftmaxBlock = SoftmaxBlockClass()
+PagedAppendBlock = PagedAppendBlockClass()
+PagedAttentionBlock = PagedAttentionBlockClass()
+PagedEvictBlock = PagedEvictBlockClass()
+VerifyDraftsBlock = VerifyDraftsBlockClass()
 
 # globals.js:11
 operations = [FastMatMulBlock, AttentionBlock, ResidualBlock, EmbedBlock, DeEmbedBlock, GeluBlock, LayerNormBlock,
-              SoftmaxBlock]
+              SoftmaxBlock, PagedAppendBlock, PagedAttentionBlock, PagedEvictBlock, VerifyDraftsBlock]
 
 
 def initializeOperations(device):  # globals.js:13

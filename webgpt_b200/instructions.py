@@ -1,4 +1,5 @@
-"""Operator ("instruction") classes with the surface of the reference's instructions.js.
+"""Operator ("instruction") classes with the surface of the reference's instructions.js, and behind them those of
+serving over a paged key-value cache, which the reference has no counterpart of.
 
 Each class keeps the reference's name, its `newInstance(...)` argument order and its return shape
 `{"resultBuffer", "passes"}`; a pass is either `{"flag": "compute", "run": callable}` (one call into the C
@@ -196,3 +197,65 @@ class AttentionBlockClass(Block):
                                          head_size, inputBuffer, qWeightsBuffer, qBiasBuffer,
                                          kWeightsBuffer, kBiasBuffer, vWeightsBuffer, vBiasBuffer,
                                          linearWeightsBuffer, linearBiasBuffer, resultBuffer)]}
+
+
+class PagedAppendBlockClass(Block):
+    def __init__(self):
+        super().__init__()
+        self.name = "pagedAppend"
+
+    def newInstance(self, cache, n_rows, startsBuffer, kBuffer, vBuffer, ld):
+        """New tokens' key and value rows (n_kv_head * head_size values, ld apart) into a layer's pages. cache is what
+        PagedCache.layer() gives; startsBuffer as in wgpt_paged_append, or None for as many rows for each sequence."""
+        return {"resultBuffer": None,
+                "passes": [self._compute("wgpt_paged_append", cache, n_rows, startsBuffer, kBuffer, vBuffer, ld)]}
+
+
+class PagedAttentionBlockClass(Block):
+    def __init__(self):
+        super().__init__()
+        self.name = "pagedAttention"
+
+    def newInstance(self, cache, n_rows, startsBuffer, n_head, attentionDotProductScale, qBuffer, ld_q, window=0,
+                    weightsBuffer=None):
+        """Attention of the new tokens over a layer's pages, their own rows included: [n_rows, n_head * head_size].
+        weightsBuffer [n_seq, max_length], or None: the weight that each position got is added to it."""
+        E = n_head * cache.head_size
+        resultBuffer = self.initResultBuffer([n_rows, E])
+        return {"resultBuffer": resultBuffer,
+                "passes": [self._compute("wgpt_paged_attention", cache, n_rows, startsBuffer, n_head,
+                                         float(attentionDotProductScale), window, qBuffer, ld_q, resultBuffer, E, weightsBuffer,
+                                         cache.max_length if weightsBuffer is not None else 0)]}
+
+
+class PagedEvictBlockClass(Block):
+    def __init__(self):
+        super().__init__()
+        self.name = "pagedEvict"
+
+    def newInstance(self, cache, toCache, keep, recent, weightsBuffer, weightsToBuffer=None):
+        """What stays of each sequence goes to toCache: the recent newest positions and the heaviest of the others, keep in
+        all. The result is [n_seq, keep], the positions that stayed, -1 behind them. weightsBuffer is
+        [n_seq, max_length], weightsToBuffer [n_seq, keep] or None."""
+        resultBuffer = self.initResultBuffer([cache.n_seq, keep])
+        return {"resultBuffer": resultBuffer,
+                "passes": [self._compute("wgpt_paged_evict", cache, toCache, keep, recent, weightsBuffer, cache.max_length,
+                                         weightsToBuffer, keep, resultBuffer)]}
+
+
+class VerifyDraftsBlockClass(Block):
+    def __init__(self):
+        super().__init__()
+        self.name = "verifyDrafts"
+
+    def newInstance(self, n_seq, n_draft, vocab_size, targetBuffer, draftBuffer, idsBuffer, countsBuffer, top_k,
+                    temperature, uniformsBuffer):
+        """Accepts or replaces drafted tokens: the result holds [n_seq, n_draft + 1] ids (the accepted drafts, the drawn
+        token, 0xFFFFFFFF behind it), acceptedBuffer how many drafts each sequence keeps. targetBuffer
+        [n_seq, n_draft + 1, vocab_size] and draftBuffer [n_seq, n_draft, vocab_size] (or None) are logits."""
+        resultBuffer = self.initResultBuffer([n_seq, n_draft + 1])
+        accepted = self.initResultBuffer([n_seq])
+        return {"resultBuffer": resultBuffer, "acceptedBuffer": accepted,
+                "passes": [self._compute("wgpt_verify_drafts", n_seq, n_draft, vocab_size, targetBuffer, vocab_size, draftBuffer,
+                                         vocab_size, idsBuffer, countsBuffer, top_k, float(temperature), uniformsBuffer,
+                                         resultBuffer, accepted)]}

@@ -1,0 +1,167 @@
+"""Host side of the paged key-value cache: which pages each sequence has, and how long it is.
+
+The pools, the page table and the lengths lie on the device, where wgpt_paged_append / _attention / _evict read them; this
+class keeps the free pages and a mirror of table and lengths, and hands out the descriptors. All layers share one table.
+A step is: advance() by the new tokens, append and attend per layer, retreat() by the drafts that were not accepted.
+"""
+import ctypes as C
+
+import numpy as np
+
+from . import _lib
+
+_TYPES = {"f32": (_lib.TYPE_F32, 4), "f16": (_lib.TYPE_F16, 2), "bf16": (_lib.TYPE_BF16, 2)}
+
+
+class Layer:
+    """One layer's cache as the operator calls take it (`ptr`: the descriptor's address, read during each call)."""
+
+    def __init__(self, owner, descriptor):
+        self._owner = owner  # its buffers have to outlive the descriptor
+        self.descriptor = descriptor
+        self.ptr = C.byref(descriptor)
+        self.head_size, self.n_kv_head = descriptor.head_size, descriptor.n_kv_head
+        self.n_seq, self.max_length = descriptor.n_seq, descriptor.max_length
+
+
+class PagedCache:
+    def __init__(self, device, n_seq, n_kv_head, head_size, n_pages, page_size=16, type="f16", n_layer=1, max_length=None,
+                 weights=False):
+        """n_pages pages of page_size positions for all sequences together, per layer; no sequence longer than max_length
+        (default: what all pages hold). weights: keep each position's accumulated attention weight, which evict() goes by."""
+        if type not in _TYPES:
+            raise ValueError(f"unknown cache type {type!r}: one of {', '.join(_TYPES)}")
+        self.type, elem = _TYPES[type]
+        self.device, self.n_seq, self.n_layer = device, n_seq, n_layer
+        self.n_pages, self.page_size = n_pages, page_size
+        self.max_length = n_pages * page_size if max_length is None else max_length
+        self.width = -(-self.max_length // page_size)
+        self.lengths = np.zeros(n_seq, np.int32)
+        self.pages = [[] for _ in range(n_seq)]
+        self.free = list(range(n_pages - 1, -1, -1))
+        self._shape = (n_kv_head, head_size)
+        nbytes = n_pages * page_size * n_kv_head * head_size * elem
+        # every buffer once more for evict(): a table and lengths to write to beside those that are read
+        self._tables = [device.buffer(n_seq * self.width * 4) for _ in range(2)]
+        self._lengths = [device.buffer(n_seq * 4) for _ in range(2)]
+        self._pools = [(device.buffer(nbytes), device.buffer(nbytes)) for _ in range(n_layer)]
+        self._weights = [device.buffer(n_seq * self.max_length * 4) for _ in range(n_layer)] if weights else None
+        self._kept = None
+        for b in self._weights or []:
+            b.write(np.zeros(n_seq * self.max_length, np.float32))
+        self._upload()
+
+    # ------------------------------------------------------------------ what the calls take
+    def layer(self, i=0, which=0):
+        """The descriptor of layer i's cache (which = 1: the one that evict() writes to)."""
+        k, v = self._pools[i]
+        n_kv, hs = self._shape
+        return Layer(self, _lib.PagedCache(k.ptr, v.ptr, self._tables[which].ptr, self._lengths[which].ptr,
+                                           self.page_size * n_kv * hs, n_kv * hs, hs, self.type, self.n_pages, self.page_size,
+                                           n_kv, hs, self.n_seq, self.width, self.max_length))
+
+    def weights(self, i=0):
+        """Layer i's accumulated weights, [n_seq, max_length]."""
+        return self._weights[i]
+
+    # ------------------------------------------------------------------ lengths
+    def advance(self, new):
+        """Makes room for new[s] more tokens of each sequence (a number: as many for each). Changes nothing if a sequence
+        would grow past max_length or there are too few pages."""
+        new = np.broadcast_to(np.asarray(new, np.int64), (self.n_seq,))
+        if (new < 0).any():
+            raise ValueError("a sequence cannot advance by a negative number of tokens: use retreat()")
+        want = self.lengths + new
+        if (want > self.max_length).any():
+            raise ValueError(f"a sequence would hold {int(want.max())} positions, more than max_length {self.max_length}")
+        need = [-(-int(L) // self.page_size) - len(p) for L, p in zip(want, self.pages)]
+        if sum(need) > len(self.free):
+            raise MemoryError(f"{sum(need)} pages are needed, {len(self.free)} are free")
+        for s, n in enumerate(need):
+            self.pages[s] += [self.free.pop() for _ in range(n)]
+        self.lengths[:] = want
+        self._upload()
+
+    def retreat(self, by):
+        """Drops the by[s] newest positions of each sequence (a number: as many of each)."""
+        by = np.broadcast_to(np.asarray(by, np.int64), (self.n_seq,))
+        if (by < 0).any() or (by > self.lengths).any():
+            raise ValueError("a sequence cannot retreat by a negative number of positions or past its beginning")
+        for s in range(self.n_seq):
+            L = int(self.lengths[s] - by[s])
+            if self._weights and by[s]:
+                for w in self._weights:
+                    w.write(np.zeros(int(by[s]), np.float32), offset=(s * self.max_length + L) * 4)
+            self._cut(s, L)
+        self._upload()
+
+    def release(self, s):
+        """Ends sequence s: its pages are free again."""
+        by = np.zeros(self.n_seq, np.int64)
+        by[s] = self.lengths[s]
+        self.retreat(by)
+
+    def starts(self, new):
+        """The starts array of a step of new[s] tokens per sequence, on the device."""
+        return self.device.tensor(np.concatenate([[0], np.cumsum(new)]).astype(np.int32))
+
+    # ------------------------------------------------------------------ eviction
+    def evict(self, keep, recent):
+        """Thins out the sequences that hold more than keep positions, in every layer by its own weights; returns the
+        positions that stayed, [n_layer, n_seq, keep], -1 behind them. Needs as many free pages as what stays fills in the
+        sequences that are thinned out."""
+        if self._weights is None:
+            raise ValueError("the cache keeps no weights: create it with weights=True")
+        keep = min(int(keep), self.max_length)
+        after = np.minimum(self.lengths, keep)
+        need = [-(-int(L) // self.page_size) for L in after]
+        if sum(need) > len(self.free):
+            raise MemoryError(f"{sum(need)} pages are needed, {len(self.free)} are free")
+        pages = [[self.free.pop() for _ in range(n)] for n in need]
+        self._tables[1].write(self._table_of(pages))
+        kept = self.device.buffer(self.n_seq * keep * 4)
+        moved = self.device.buffer(self.n_seq * keep * 4)
+        out = []
+        try:
+            for i in range(self.n_layer):
+                w = self._weights[i]
+                _lib.call("wgpt_paged_evict", self.device.handle, self.layer(i).ptr, self.layer(i, 1).ptr, keep, int(recent), w.ptr,
+                          self.max_length, moved.ptr, keep, kept.ptr)
+                out.append(kept.read(np.int32, self.n_seq * keep).reshape(self.n_seq, keep))
+                rows = np.zeros((self.n_seq, self.max_length), np.float32)
+                rows[:, :keep] = moved.read(np.float32, self.n_seq * keep).reshape(self.n_seq, keep)
+                w.write(rows)
+        except Exception:
+            for p in pages:
+                self.free += p
+            raise
+        finally:
+            kept.destroy()
+            moved.destroy()
+        for s in range(self.n_seq):
+            self.free += self.pages[s]
+        self.pages = pages
+        self.lengths[:] = after
+        self._upload()
+        return np.stack(out)
+
+    # ------------------------------------------------------------------ inside
+    def _cut(self, s, length):
+        n = -(-length // self.page_size)
+        self.free += self.pages[s][n:]
+        self.pages[s] = self.pages[s][:n]
+        self.lengths[s] = length
+
+    def _table_of(self, pages):
+        table = np.zeros((self.n_seq, self.width), np.uint32)
+        for s, p in enumerate(pages):
+            table[s, :len(p)] = p
+        return table
+
+    def _upload(self):
+        self._tables[0].write(self._table_of(self.pages))
+        self._lengths[0].write(self.lengths)
+
+    def destroy(self):
+        for b in self._tables + self._lengths + [x for p in self._pools for x in p] + (self._weights or []):
+            b.destroy()
