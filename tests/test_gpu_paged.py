@@ -218,19 +218,22 @@ def test_attention_masked_positions_may_hold_anything(dev, type):
     rng = np.random.default_rng(13)
     lengths, new = [40, 70, 33], [4, 3, 1]
     pages = make(rng, lengths, 16, 1, 64, type)
-    clean, _ = check_attention(dev, pages, type, "positions", new, 2, window=20)
+    q = (np.random.default_rng(1).standard_normal((8, 2, 64)) * 1.5).astype(np.float32)
+    want, _, size, top = ref.attend(pages, [0, 4, 7, 8], 2, 0.125, 20, q)
     pages.k[pages.place(0, 39)] = np.nan      # the last draft: its own row alone sees it
     pages.v[pages.place(0, 39)] = np.inf
     pages.k[pages.place(1, 47)] = -np.inf     # in the window of the first row alone
     pages.v[pages.place(1, 48)] = np.nan      # in those of the first two (48 .. 67, 49 .. 68, 50 .. 69: the first alone)
     pages.v[pages.place(2, 3)] = np.nan       # behind every window
     cache = OnDevice(dev, pages, type)
-    q = (np.random.default_rng(1).standard_normal((8, 2, 64)) * 1.5).astype(np.float32)
     got, _ = attend(dev, cache, [0, 4, 7, 8], 8, 2, 0.125, 20, q)
     assert np.isnan(got[3]).all()
     assert np.isnan(got[4]).all()
-    for row in (0, 1, 2, 5, 6, 7):
-        assert np.array_equal(got[row], clean[row])
+    # The other rows are what they are without those positions, each within its own tolerance: two results of f32 arithmetic
+    # in different orders (rows beside one that sees such a value are added up apart) lie that near to the same 64-bit value,
+    # though not at the same bits.
+    rows = [0, 1, 2, 5, 6, 7]
+    assert (np.abs(got[rows] - want[rows]) <= ref.attend_tolerance(pages, size, top)[rows]).all()
 
 
 @pytest.mark.parametrize("type", ["f32", "f16", "bf16"])

@@ -2,6 +2,8 @@
 #pragma once
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "sample_key.cuh"
 
@@ -128,89 +130,818 @@ __device__ __forceinline__ float paged_value(const float *p) { return __ldcg(p);
 __device__ __forceinline__ float paged_value(const __half *p) { return __half2float(__ldcg(p)); }
 __device__ __forceinline__ float paged_value(const __nv_bfloat16 *p) { return __bfloat162float(__ldcg(p)); }
 
+//   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = 2^(c s_ij - m_i),  s_ij = q_i . k_j,  c = scale / ln 2,  m_i = max_j c s_ij
+// in one pass over the keys, with the running maximum and sum in f32 (sums and values are multiplied by 2^(old - new maximum)
+// when it moves).
+//
+// What bounds it is the cache's bytes: a row of K and V is read once for all the query rows that share it (the heads of its
+// group, times the new tokens), at most ROWS of them, a row tile. All (sequence, head of the cache, row tile) groups lie
+// behind one another as units of 64 positions; every CTA takes as many units as any other, whatever the lengths are, so a CTA
+// may hold the end of one group, whole ones, and the beginning of another. A group that is shared is joined by the CTA that
+// finishes last, in the order of the positions.
+//
+// Inside a CTA four warps take 16 positions each of a unit and never meet until the group ends: each has a ring of tiles in
+// shared memory that cp.async fills, K and V tiles in turn, its own running maximum and its own sums.
+constexpr int kPagedWarps = 4, kPagedThreads = 32 * kPagedWarps, kTile = 16, kUnit = kPagedWarps * kTile;
+
 struct PagedAttention {
   PagedView c;
   NewRows r;
   int n_head, group, window;
-  float scale;
+  float scale2;  // scale / ln 2
   const float *q;
   float *out;
   long long ld_q, ld_out;
-  float *scores, *stats;  // [n_rows * n_head][max_length] and [n_rows * n_head] (log-sum), or NULL
+  int least;             // fewest units a CTA takes
+  float *partial;        // [2 * CTAs][paged_slot(ROWS, hs)]
+  unsigned int *join;    // a counter per CTA, zero on entry and left zero
+  float *scores, *stats; // [n_rows * n_head][max_length] and [n_rows * n_head], in units of log 2, or NULL
 };
 
-// One CTA per (row, head); its warps take the positions in turn, a lane holds up to eight dimensions, and the warps' running
-// maxima, sums and values meet in shared memory.
-constexpr int kPagedWarps = 4;
+// A sequence's share of the work.
+struct PagedSeq {
+  int first, n, L, begin;  // rows, length, position of the first unit
+  int tiles, units;        // row tiles, units of each
+};
 
-template <typename T>
-__global__ void __launch_bounds__(kPagedWarps * 32)
-paged_attention_kernel(PagedAttention a) {
-  const PagedView &c = a.c;
-  pdl_launch_dependents();
-  pdl_wait();
-  __shared__ float sm[kPagedWarps], sl[kPagedWarps], so[kPagedWarps][256];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = blockIdx.x, row = blockIdx.y, kvh = h / a.group;
-  const int s = sequence_of(c, a.r, row, lane);
-  if (s < 0) return;
-  int first, n;
-  new_rows(c, a.r, s, first, n);
-  if ((unsigned)(row - first) >= (unsigned)n) return;
-  const int end = paged_length(c, s) - n + (row - first) + 1, begin = a.window > 0 ? max(0, end - a.window) : 0;
-  const float *q = a.q + (long long)row * a.ld_q + h * c.hs;
-  float qv[8], o[8], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    qv[i] = lane + 32 * i < c.hs ? __ldcg(q + lane + 32 * i) : 0.f;
-    o[i] = 0.f;
-  }
-  for (int j = begin + warp; j < end; j += kPagedWarps) {
-    const long long at = paged_offset(c, s, j);
-    float sc = -INFINITY;
-    if (at >= 0) {
-      const T *k = static_cast<const T *>(c.k) + at + kvh * c.head_stride, *v = static_cast<const T *>(c.v) + at + kvh * c.head_stride;
-      float d = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (lane + 32 * i < c.hs) d += qv[i] * paged_value(k + lane + 32 * i);
-      sc = warp_sum(d) * a.scale;
-      if (sc != -INFINITY) {
-        const float nm = fmaxf(m, sc), f = expf(m - nm), p = expf(sc - nm);
-        l = l * f + p;
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-          if (lane + 32 * i < c.hs) o[i] = o[i] * f + p * paged_value(v + lane + 32 * i);
-        m = nm;
-      }
-    }
-    if (a.scores && lane == 0) a.scores[((long long)row * a.n_head + h) * c.max_length + j] = sc;
-  }
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; i++) so[warp][lane + 32 * i] = o[i];
-  __syncthreads();
-  float top = sm[0], sum = 0.f;
-#pragma unroll
-  for (int w = 1; w < kPagedWarps; w++) top = fmaxf(top, sm[w]);
-  float f[kPagedWarps];
-#pragma unroll
-  for (int w = 0; w < kPagedWarps; w++) {
-    f[w] = sl[w] != 0.f ? expf(sm[w] - top) : 0.f;
-    sum += f[w] * sl[w];
-  }
-  for (int d = threadIdx.x; d < c.hs; d += kPagedWarps * 32) {
-    float v = 0.f;
-#pragma unroll
-    for (int w = 0; w < kPagedWarps; w++) v += f[w] != 0.f ? f[w] * so[w][d] : 0.f;
-    a.out[(long long)row * a.ld_out + h * c.hs + d] = sum != 0.f ? v / sum : 0.f;
-  }
-  if (a.stats && threadIdx.x == 0) a.stats[(long long)row * a.n_head + h] = top + logf(sum);
+template <int ROWS>
+__device__ __forceinline__ PagedSeq paged_seq(const PagedAttention &a, int s) {
+  PagedSeq q;
+  new_rows(a.c, a.r, s, q.first, q.n);
+  q.L = paged_length(a.c, s);
+  const int lowest = a.window > 0 ? max(0, q.L - q.n + 1 - a.window) : 0;
+  q.begin = min(lowest, q.L) / kUnit * kUnit;
+  q.tiles = (int)(((long long)q.n * a.group + ROWS - 1) / ROWS);
+  q.units = max(1, (q.L - q.begin + kUnit - 1) / kUnit);  // one even if there is nothing to see: the rows are set to zero
+  return q;
 }
 
-// weights[s][j] += sum over the sequence's rows and heads, in their order, of exp(score - log-sum).
+// What a part of a group leaves for the others: the rows' values, maxima and sums.
+__host__ __device__ constexpr int paged_slot(int rows, int hs) { return rows * hs + (2 * rows + 3) / 4 * 4; }
+
+// The row tile that a CTA works on.
+struct PagedGroup {
+  int s, kvh, r0, rows;    // sequence, head of the cache, first row of the tile (token * group + head in the group), rows
+  int lowest, highest;     // positions that some row sees: [lowest, highest)
+  int inner_low, inner_high;  // positions that every row sees
+};
+
+__device__ __forceinline__ void row_range(const PagedAttention &a, const PagedSeq &q, int token, int &lo, int &hi) {
+  hi = max(0, q.L - q.n + token + 1);
+  lo = a.window > 0 ? max(0, hi - a.window) : 0;
+}
+
+__device__ __forceinline__ long long row_offset(const PagedAttention &a, const PagedSeq &q, const PagedGroup &g, int r, long long ld) {
+  const int token = (g.r0 + r) / a.group, head = g.kvh * a.group + (g.r0 + r) % a.group;
+  return (long long)(q.first + token) * ld + (long long)head * a.c.hs;
+}
+__device__ __forceinline__ long long row_index(const PagedAttention &a, const PagedSeq &q, const PagedGroup &g, int r) {
+  const int token = (g.r0 + r) / a.group, head = g.kvh * a.group + (g.r0 + r) % a.group;
+  return (long long)(q.first + token) * a.n_head + head;
+}
+
+// Copies 16 bytes, or writes zeros where there is nothing to copy.
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t to, const void *from, bool there) {
+  const int bytes = there ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ float exp2_of(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// What the kernel of a type, a (padded) head size and a number of rows takes of shared memory.
+template <typename T, int HSP, int RT>
+struct PagedShape {
+  static constexpr bool kWide = sizeof(T) == 4;  // f32: products on the CUDA cores, RT rows; else on the tensor cores, 8 RT rows
+  static constexpr int kRows = kWide ? RT : 8 * RT;
+  static constexpr int kTerms = kWide ? 1 : std::is_same<T, __half>::value ? 2 : 3;  // values that a query or probability is split into
+  static constexpr int kPitch = HSP * (int)sizeof(T) + 16;  // of a row in shared memory: 16-byte pieces of 8 rows meet all banks
+  static constexpr int kTileBytes = kTile * kPitch;
+  static constexpr int kQPitch = kWide ? HSP * 4 : HSP * 2 + 16;
+  static constexpr int kQBytes = kRows * kTerms * kQPitch;
+  static constexpr int kPBytes = kWide ? kPagedWarps * kRows * kTile * 4 : 0;  // probabilities of a tile
+  // half the ring's tiles are of K and half of V; enough that two CTAs share an SM, where a row is small enough
+  static constexpr int kStages = kTileBytes <= 2304 ? 6 : kTileBytes <= 4352 ? 6 : 3;
+  static constexpr int kRing = kStages * kTileBytes;
+  static constexpr int kSmem = kQBytes + kPBytes + kPagedWarps * kRing;
+  static_assert(kRing >= kRows * HSP * 4 || kWide || HSP * RT <= 512, "");
+};
+
+// Rows of a tile that a warp saw something non-finite in (an infinity or NaN in V, in a key, in q, also where a row's mask
+// leaves it out: zero times infinity): the same again one position at a time, each row from what it sees alone. Leaves the row's
+// maximum, sum and values as the fast path does.
+template <typename T>
+__device__ __noinline__ void paged_rows_apart(const PagedAttention &a, const PagedSeq &q, const PagedGroup &g, int u0, int u1,
+                                              int warp, int lane, float *o_out, float *m_out, float *l_out) {
+  const PagedView &c = a.c;
+  for (int r = 0; r < g.rows; r++) {
+    int lo, hi;
+    row_range(a, q, (g.r0 + r) / a.group, lo, hi);
+    const float *x = a.q + row_offset(a, q, g, r, a.ld_q);
+    float qv[8], o[8], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      qv[i] = lane + 32 * i < c.hs ? __ldcg(x + lane + 32 * i) : 0.f;
+      o[i] = 0.f;
+    }
+    for (int u = u0; u < u1; u++) {
+      const int base = q.begin + u * kUnit + warp * kTile;
+      for (int j = max(base, lo); j < min(base + kTile, hi); j++) {
+        const long long at = paged_offset(c, g.s, j);
+        float sc = -INFINITY;
+        if (at >= 0) {
+          const T *k = static_cast<const T *>(c.k) + at + g.kvh * c.head_stride, *v = static_cast<const T *>(c.v) + at + g.kvh * c.head_stride;
+          float d = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; i++)
+            if (lane + 32 * i < c.hs) d += qv[i] * paged_value(k + lane + 32 * i);
+          sc = warp_sum(d) * a.scale2;
+          if (sc != -INFINITY) {
+            const float nm = fmaxf(m, sc), f = exp2f(m - nm), p = exp2f(sc - nm);
+            l = l * f + p;
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+              if (lane + 32 * i < c.hs) o[i] = o[i] * f + p * paged_value(v + lane + 32 * i);
+            m = nm;
+          }
+        }
+        if (a.scores && lane == 0) a.scores[row_index(a, q, g, r) * c.max_length + j] = sc;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (lane + 32 * i < c.hs) o_out[r * c.hs + lane + 32 * i] = o[i];
+    if (lane == 0) {
+      m_out[r] = m;
+      l_out[r] = l;
+    }
+  }
+}
+
+// A warp's view of its ring: fills K and V tiles in turn, half-stage 2 t for the keys of its t-th tile and 2 t + 1 for its values.
+template <typename T, int HSP, int RT>
+struct PagedRing {
+  using S = PagedShape<T, HSP, RT>;
+  static constexpr int kPerRow = HSP * (int)sizeof(T) / 16;          // 16-byte pieces of a row
+  static constexpr int kLanes = kPerRow < 32 ? kPerRow : 32;         // lanes that share a row
+  static constexpr int kAtOnce = 32 / kLanes, kSteps = kTile / kAtOnce, kWidth = kPerRow / kLanes;
+  const PagedView &c;
+  const T *k, *v;      // this head's rows of page 0
+  const uint32_t *table;
+  uint32_t base;       // shared-memory address of the ring
+  uint32_t *ok;        // [kStages] which of a tile's positions are there
+  int lowest, highest, pos, lane, pieces;
+  uint32_t page, slot; // of this lane's position of the next tile to fill
+  long long at;        // where this lane's position of the tile at hand begins, or -1
+
+  __device__ __forceinline__ PagedRing(const PagedView &c_, int s, int kvh, uint32_t base_, uint32_t *ok_, int lane_)
+      : c(c_), k(static_cast<const T *>(c_.k) + kvh * c_.head_stride), v(static_cast<const T *>(c_.v) + kvh * c_.head_stride),
+        table(c_.table + (size_t)s * c_.table_stride), base(base_), ok(ok_), lane(lane_), pieces(c_.hs * (int)sizeof(T) / 16) {}
+
+  __device__ __forceinline__ void look_up() {  // the page of this lane's position, asked for a tile ahead
+    page = 0xFFFFFFFFu;
+    slot = 0;
+    if (pos >= lowest && pos < highest) {
+      const uint32_t index = (uint32_t)pos / c.page_size;
+      slot = (uint32_t)pos - index * c.page_size;
+      page = __ldcg(table + index);
+    }
+  }
+  __device__ __forceinline__ void begin(int first, int lowest_, int highest_) {
+    lowest = lowest_;
+    highest = highest_;
+    pos = first + (lane & (kTile - 1));
+    look_up();
+  }
+  // Fills half-stage h (in ring order) and commits it.
+  __device__ __forceinline__ void fill(int h, bool any) {
+    const int stage = h % S::kStages;
+    if (any) {
+      if ((h & 1) == 0) {
+        const bool wanted = pos >= lowest && pos < highest;
+        at = -1;
+        if (page < c.n_pages)
+          at = (long long)page * c.page_stride + (long long)slot * c.position_stride;
+        else if (wanted)
+          *c.err = kErrCache;
+        const uint32_t there = __ballot_sync(0xffffffffu, at >= 0) & 0xffffu;
+        if (lane == 0) ok[stage] = there;
+        pos += kUnit;
+        look_up();
+      }
+      const T *from = (h & 1) ? v : k;
+      const uint32_t to = base + stage * S::kTileBytes;
+#pragma unroll
+      for (int i = 0; i < kSteps; i++) {
+        const int row = i * kAtOnce + lane / kLanes;
+        const long long x = __shfl_sync(0xffffffffu, at, row);
+#pragma unroll
+        for (int w = 0; w < kWidth; w++) {
+          const int piece = lane % kLanes + w * 32;
+          if (piece < pieces)
+            cp_async16_or_zero(to + row * S::kPitch + piece * 16, reinterpret_cast<const char *>(from + (x < 0 ? 0 : x)) + piece * 16, x >= 0);
+        }
+      }
+    }
+    cp_async_commit();
+  }
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Two values rounded to the 16-bit type, packed, and what is left of them.
+template <typename T>
+__device__ __forceinline__ uint32_t split2(float &x, float &y) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    x -= f.x;
+    y -= f.y;
+    return *reinterpret_cast<const uint32_t *>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    const float2 f = __bfloat1622float2(h);
+    x -= f.x;
+    y -= f.y;
+    return *reinterpret_cast<const uint32_t *>(&h);
+  }
+}
+
+template <typename T, int HSP, int RT>
+__global__ void __launch_bounds__(kPagedThreads)
+paged_attention_kernel(const __grid_constant__ PagedAttention a) {
+  using S = PagedShape<T, HSP, RT>;
+  constexpr int ROWS = S::kRows, TERMS = S::kTerms, D = S::kStages;
+  // f32: a lane holds four dimensions of kQuads pieces of a row; where 16 lanes hold a row, the halves of the warp take even and odd keys
+  constexpr int kQuads = HSP <= 128 ? 1 : HSP / 128, kHalves = HSP <= 64 ? 2 : 1;
+  constexpr float kLift = std::is_same<T, __half>::value ? 14.f : 0.f;  // probabilities are held times 2^14, in the middle of a half's range
+  extern __shared__ __align__(16) unsigned char paged_smem[];
+  __shared__ float s_m[kPagedWarps][ROWS], s_l[kPagedWarps][ROWS], s_qscale[ROWS];
+  __shared__ int s_lo[ROWS], s_hi[ROWS];
+  __shared__ long long s_row[ROWS];
+  __shared__ uint32_t s_ok[kPagedWarps][D];
+  __shared__ long long s_sum[kPagedWarps], s_excl;
+  __shared__ int s_seq, s_last;
+  const PagedView &c = a.c;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hs = c.hs;
+  unsigned char *q_smem = paged_smem, *ring_smem = paged_smem + S::kQBytes + S::kPBytes + warp * S::kRing;
+  float *p_smem = reinterpret_cast<float *>(paged_smem + S::kQBytes) + warp * ROWS * kTile;
+  pdl_launch_dependents();
+  // where 32 does not divide the head size, what lies behind a row takes part in products: zeros, times zeros of the query's
+  const bool padded = !S::kWide && (hs & 31) != 0;
+  auto clear_ring = [&]() {
+    for (int i = lane; i < S::kRing / 16; i += 32) reinterpret_cast<uint4 *>(ring_smem)[i] = make_uint4(0, 0, 0, 0);
+    __syncwarp();
+  };
+  if (padded) clear_ring();
+  pdl_wait();
+
+  // ---- this CTA's units
+  auto weight_of = [&](int s) -> long long {
+    if (s >= c.n_seq) return 0;
+    const PagedSeq q = paged_seq<ROWS>(a, s);
+    return (long long)q.tiles * q.units * c.n_kv;
+  };
+  auto scan = [&](long long mine, long long &all) {  // sum over the threads before this one, and over all
+    long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    __syncthreads();
+    if (lane == 31) s_sum[warp] = upto;
+    __syncthreads();
+    all = 0;
+    for (int w = 0; w < kPagedWarps; w++) {
+      if (w < warp) upto += s_sum[w];
+      all += s_sum[w];
+    }
+    return upto - mine;
+  };
+  long long total = 0, mine = 0, before = 0;
+  for (int s0 = 0; s0 < c.n_seq; s0 += kPagedThreads) {
+    long long all;
+    mine = weight_of(s0 + tid);
+    before = total + scan(mine, all);
+    total += all;
+  }
+  const long long per = max((long long)a.least, (total + gridDim.x - 1) / gridDim.x);
+  const long long x0 = blockIdx.x * per, x1 = min(total, x0 + per);
+  if (x0 >= x1) return;
+  if (c.n_seq <= kPagedThreads) {
+    if (before <= x0 && x0 < before + mine) {
+      s_seq = tid;
+      s_excl = before;
+    }
+  } else {
+    long long sum = 0;
+    for (int s0 = 0; s0 < c.n_seq && sum <= x0; s0 += kPagedThreads) {
+      long long all;
+      mine = weight_of(s0 + tid);
+      before = sum + scan(mine, all);
+      if (before <= x0 && x0 < before + mine) {
+        s_seq = s0 + tid;
+        s_excl = before;
+      }
+      sum += all;
+    }
+  }
+  __syncthreads();
+  int s = s_seq;
+  long long seq_begin = s_excl, x = x0;
+  PagedSeq q = paged_seq<ROWS>(a, s);
+
+  while (x < x1) {
+    while (x >= seq_begin + (long long)q.tiles * q.units * c.n_kv) {
+      seq_begin += (long long)q.tiles * q.units * c.n_kv;
+      q = paged_seq<ROWS>(a, ++s);
+    }
+    const long long gi = (x - seq_begin) / q.units, g_begin = seq_begin + gi * q.units, g_end = g_begin + q.units;
+    PagedGroup g;
+    g.s = s;
+    g.kvh = (int)(gi / q.tiles);
+    g.r0 = (int)(gi % q.tiles) * ROWS;
+    g.rows = (int)min((long long)ROWS, (long long)q.n * a.group - g.r0);
+    {
+      int lo, hi;
+      row_range(a, q, g.r0 / a.group, lo, hi);
+      g.lowest = lo;
+      g.inner_high = hi;
+      row_range(a, q, (g.r0 + g.rows - 1) / a.group, lo, hi);
+      g.inner_low = lo;
+      g.highest = hi;
+    }
+    // units [u0, u1) of the group are this CTA's; those that no row of the tile sees are left out
+    int u0 = (int)(x - g_begin), u1 = (int)(min(x1, g_end) - g_begin);
+    x = min(x1, g_end);
+    u0 = max(u0, (g.lowest - q.begin) / kUnit);
+    u1 = min(u1, (g.highest - q.begin + kUnit - 1) / kUnit);
+    const int n_tiles = max(0, u1 - u0);
+
+    PagedRing<T, HSP, RT> ring(c, s, g.kvh, smem_addr(ring_smem), s_ok[warp], lane);
+    if (n_tiles > 0) ring.begin(q.begin + u0 * kUnit + warp * kTile, g.lowest, g.highest);
+#pragma unroll
+    for (int h = 0; h < D - 1; h++) ring.fill(h, h < 2 * n_tiles);
+
+    // ---- the queries
+    if constexpr (S::kWide) {
+      float4 *q4 = reinterpret_cast<float4 *>(q_smem);
+      for (int i = tid; i < ROWS * (HSP / 4); i += kPagedThreads) {
+        const int r = i / (HSP / 4), d = i % (HSP / 4);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < g.rows && 4 * d < hs) v = __ldcg(reinterpret_cast<const float4 *>(a.q + row_offset(a, q, g, r, a.ld_q)) + d);
+        q4[i] = v;
+      }
+    } else {
+      for (int r = warp; r < ROWS; r += kPagedWarps) {
+        float v[HSP / 32], top = 0.f;
+        const float *row = r < g.rows ? a.q + row_offset(a, q, g, r, a.ld_q) : nullptr;
+#pragma unroll
+        for (int i = 0; i < HSP / 64; i++) {
+          const int d = 2 * lane + 64 * i;
+          const float2 f = row && d < hs ? __ldcg(reinterpret_cast<const float2 *>(row + d)) : make_float2(0.f, 0.f);
+          v[2 * i] = f.x;
+          v[2 * i + 1] = f.y;
+          top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+        int e = 0;
+        if constexpr (TERMS == 2) {  // a power of two that brings the row's largest value near 2^13
+          top = warp_max(top);
+          e = top > 0.f && top < INFINITY ? ilogbf(top) - 13 : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < HSP / 64; i++) {
+          float f0 = scalbnf(v[2 * i], -e), f1 = scalbnf(v[2 * i + 1], -e);
+#pragma unroll
+          for (int t = 0; t < TERMS; t++)
+            *reinterpret_cast<uint32_t *>(q_smem + (t * ROWS + r) * S::kQPitch + (2 * lane + 64 * i) * 2) = split2<T>(f0, f1);
+        }
+        if (lane == 0) s_qscale[r] = scalbnf(a.scale2, e);
+      }
+    }
+    if (tid < ROWS) {
+      int lo = 0, hi = 0;
+      if (tid < g.rows) row_range(a, q, (g.r0 + tid) / a.group, lo, hi);
+      s_lo[tid] = lo;
+      s_hi[tid] = hi;
+      s_row[tid] = row_index(a, q, g, tid) * c.max_length;
+    }
+    __syncthreads();
+
+    bool finite = true;
+    float *o_smem = reinterpret_cast<float *>(ring_smem);
+    if constexpr (S::kWide) {
+      const int key = lane & 15, half = lane >> 4;
+      float m[ROWS], l[ROWS];
+      float4 o[ROWS][kQuads];
+#pragma unroll
+      for (int r = 0; r < ROWS; r++) {
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+#pragma unroll
+        for (int w = 0; w < kQuads; w++) o[r][w] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      for (int t = 0; t < n_tiles; t++) {
+        const int pos0 = q.begin + (u0 + t) * kUnit + warp * kTile;
+        // ---- scores: a lane takes one key and every other quad of its row
+        cp_async_wait<D - 2>();
+        __syncwarp();
+        ring.fill(2 * t + D - 1, 2 * t + D - 1 < 2 * n_tiles);
+        const uint32_t ok = s_ok[warp][(2 * t) % D];
+        const float4 *kt = reinterpret_cast<const float4 *>(ring_smem + ((2 * t) % D) * S::kTileBytes + key * S::kPitch);
+        float sc[ROWS];
+#pragma unroll
+        for (int r = 0; r < ROWS; r++) sc[r] = 0.f;
+#pragma unroll 4
+        for (int d = half; d < hs / 4; d += 2) {
+          const float4 kv = kt[d];
+#pragma unroll
+          for (int r = 0; r < ROWS; r++) {
+            const float4 qv = reinterpret_cast<const float4 *>(q_smem)[r * (HSP / 4) + d];
+            sc[r] = fmaf(qv.x, kv.x, sc[r]);
+            sc[r] = fmaf(qv.y, kv.y, sc[r]);
+            sc[r] = fmaf(qv.z, kv.z, sc[r]);
+            sc[r] = fmaf(qv.w, kv.w, sc[r]);
+          }
+        }
+        const bool whole = ok == 0xffffu && pos0 >= g.inner_low && pos0 + kTile <= g.inner_high;
+        float f[ROWS];
+        bool moved = false;
+#pragma unroll
+        for (int r = 0; r < ROWS; r++) {
+          sc[r] = (sc[r] + __shfl_xor_sync(0xffffffffu, sc[r], 16)) * a.scale2;
+          if (!whole && !((ok >> key & 1u) && pos0 + key >= s_lo[r] && pos0 + key < s_hi[r])) sc[r] = -INFINITY;
+          if (a.scores && half == 0 && r < g.rows && pos0 + key >= s_lo[r] && pos0 + key < s_hi[r])
+            a.scores[s_row[r] + pos0 + key] = sc[r];
+          float top = sc[r];
+#pragma unroll
+          for (int w = 8; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+          top = fmaxf(top, m[r]);
+          f[r] = m[r] == top ? 1.f : exp2_of(m[r] - top);
+          moved |= m[r] != top;
+          const float p = sc[r] == -INFINITY ? 0.f : exp2_of(sc[r] - top);
+          m[r] = top;
+          l[r] = l[r] * f[r] + p;
+          if (half == 0) p_smem[r * kTile + key] = p;
+        }
+        if (moved) {
+#pragma unroll
+          for (int r = 0; r < ROWS; r++)
+#pragma unroll
+            for (int w = 0; w < kQuads; w++) {
+              o[r][w].x *= f[r];
+              o[r][w].y *= f[r];
+              o[r][w].z *= f[r];
+              o[r][w].w *= f[r];
+            }
+        }
+        // ---- values: a lane takes four dimensions (times kQuads) of each key, or of every other one
+        cp_async_wait<D - 2>();
+        __syncwarp();
+        ring.fill(2 * t + D, 2 * t + D < 2 * n_tiles);
+        const unsigned char *vt = ring_smem + ((2 * t + 1) % D) * S::kTileBytes;
+        const int dim4 = kHalves == 2 ? key : lane;
+#pragma unroll
+        for (int j0 = 0; j0 < kTile; j0 += 4 * kHalves) {
+          float4 vv[4][kQuads];
+#pragma unroll
+          for (int jj = 0; jj < 4; jj++)
+#pragma unroll
+            for (int w = 0; w < kQuads; w++) {
+              const int j = j0 + (kHalves == 2 ? 4 * half : 0) + jj;
+              vv[jj][w] = 4 * (dim4 + 32 * w) < hs ? *reinterpret_cast<const float4 *>(vt + j * S::kPitch + (dim4 + 32 * w) * 16)
+                                                   : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+          for (int r = 0; r < ROWS; r++) {
+            const float4 p = *reinterpret_cast<const float4 *>(p_smem + r * kTile + j0 + (kHalves == 2 ? 4 * half : 0));
+            const float pj[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+            for (int jj = 0; jj < 4; jj++)
+#pragma unroll
+              for (int w = 0; w < kQuads; w++) {
+                o[r][w].x = fmaf(pj[jj], vv[jj][w].x, o[r][w].x);
+                o[r][w].y = fmaf(pj[jj], vv[jj][w].y, o[r][w].y);
+                o[r][w].z = fmaf(pj[jj], vv[jj][w].z, o[r][w].z);
+                o[r][w].w = fmaf(pj[jj], vv[jj][w].w, o[r][w].w);
+              }
+          }
+        }
+      }
+      cp_async_wait<0>();
+      __syncwarp();
+#pragma unroll
+      for (int r = 0; r < ROWS; r++) {
+#pragma unroll
+        for (int w = 8; w > 0; w >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], w);
+#pragma unroll
+        for (int w = 0; w < kQuads; w++) {
+          float4 &v = o[r][w];
+          if (kHalves == 2) {
+            v.x += __shfl_xor_sync(0xffffffffu, v.x, 16);
+            v.y += __shfl_xor_sync(0xffffffffu, v.y, 16);
+            v.z += __shfl_xor_sync(0xffffffffu, v.z, 16);
+            v.w += __shfl_xor_sync(0xffffffffu, v.w, 16);
+          }
+          const int d = (kHalves == 2 ? key : lane) + 32 * w;
+          finite = finite && fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) < INFINITY;
+          if (r < g.rows && 4 * d < hs && (kHalves == 1 || half == 0)) *reinterpret_cast<float4 *>(o_smem + r * hs + 4 * d) = v;
+        }
+        finite = finite && fabsf(l[r]) < INFINITY;
+        if (lane == 0) {
+          s_m[warp][r] = m[r];
+          s_l[warp][r] = l[r];
+        }
+      }
+    } else {
+      // The keys are the matrix instruction's 16 rows and the queries its 8 columns: scores come out with a lane holding two
+      // queries of keys lane / 4 and lane / 4 + 8, and the probabilities, transposed inside the warp, are the second operand
+      // of the values' product, whose rows are dimensions.
+      constexpr int KS = HSP / 16;
+      const int gr = lane >> 2, cc = lane & 3;
+      const uint32_t ring0 = smem_addr(ring_smem), q0 = smem_addr(q_smem);
+      const int k_row = (lane & 7) + (lane & 8), k_col = (lane >> 4) * 8;             // a lane's row and piece of a K tile's fragment
+      const int v_row = (lane & 7) + ((lane >> 4) << 3), v_col = lane & 8;            // of a V tile's
+      const int q_row = lane & 7, q_col = (lane >> 3) * 8;                            // of 32 dimensions of eight queries
+      float m[RT][2], l[RT][2], qs[RT][2];
+      float o[KS][RT][4];
+#pragma unroll
+      for (int n = 0; n < RT; n++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          m[n][e] = -INFINITY;
+          l[n][e] = 0.f;
+          qs[n][e] = s_qscale[8 * n + 2 * cc + e];
+        }
+#pragma unroll
+      for (int i = 0; i < KS; i++)
+#pragma unroll
+        for (int n = 0; n < RT; n++) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
+      for (int t = 0; t < n_tiles; t++) {
+        const int pos0 = q.begin + (u0 + t) * kUnit + warp * kTile;
+        cp_async_wait<D - 2>();
+        __syncwarp();
+        ring.fill(2 * t + D - 1, 2 * t + D - 1 < 2 * n_tiles);
+        const uint32_t ok = s_ok[warp][(2 * t) % D];
+        const uint32_t kt = ring0 + ((2 * t) % D) * S::kTileBytes + k_row * S::kPitch + k_col * 2;
+        float sc[TERMS][RT][4];
+#pragma unroll
+        for (int u = 0; u < TERMS; u++)
+#pragma unroll
+          for (int n = 0; n < RT; n++) sc[u][n][0] = sc[u][n][1] = sc[u][n][2] = sc[u][n][3] = 0.f;
+#pragma unroll
+        for (int i = 0; i < KS; i += 2) {
+          if (16 * i < hs) {
+            uint32_t a0[4], a1[4];
+            ldmatrix4(kt + i * 32, a0);
+            if (HSP >= 32) ldmatrix4(kt + (i + 1) * 32, a1);
+#pragma unroll
+            for (int u = 0; u < TERMS; u++)
+#pragma unroll
+              for (int n = 0; n < RT; n++) {
+                uint32_t b[4];
+                ldmatrix4(q0 + (u * ROWS + 8 * n + q_row) * S::kQPitch + (i * 16 + q_col) * 2, b);
+                mma_16x8x16<T>(sc[u][n], a0, b[0], b[1]);
+                mma_16x8x16<T>(sc[u][n], a1, b[2], b[3]);
+              }
+          }
+        }
+        const bool whole = ok == 0xffffu && pos0 >= g.inner_low && pos0 + kTile <= g.inner_high;
+        uint32_t p[TERMS][RT][2];
+        float f[RT][2];
+        bool moved = false;
+#pragma unroll
+        for (int n = 0; n < RT; n++) {
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            float x0 = sc[TERMS - 1][n][e], x1 = sc[TERMS - 1][n][2 + e];
+#pragma unroll
+            for (int u = TERMS - 2; u >= 0; u--) {
+              x0 += sc[u][n][e];
+              x1 += sc[u][n][2 + e];
+            }
+            x0 *= qs[n][e];
+            x1 *= qs[n][e];
+            const int r = 8 * n + 2 * cc + e;
+            if (!whole) {
+              const int lo = s_lo[r], hi = s_hi[r];
+              if (!((ok >> gr & 1u) && pos0 + gr >= lo && pos0 + gr < hi)) x0 = -INFINITY;
+              if (!((ok >> (gr + 8) & 1u) && pos0 + gr + 8 >= lo && pos0 + gr + 8 < hi)) x1 = -INFINITY;
+            }
+            if (a.scores && r < g.rows) {
+              float *to = a.scores + s_row[r] + pos0 + gr;
+              if (pos0 + gr >= s_lo[r] && pos0 + gr < s_hi[r]) to[0] = x0;
+              if (pos0 + gr + 8 >= s_lo[r] && pos0 + gr + 8 < s_hi[r]) to[8] = x1;
+            }
+            float top = fmaxf(x0, x1);
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+            top = fmaxf(top, m[n][e]);
+            f[n][e] = m[n][e] == top ? 1.f : exp2_of(m[n][e] - top);
+            moved |= m[n][e] != top;
+            m[n][e] = top;
+            sc[0][n][e] = x0 == -INFINITY ? 0.f : exp2_of(x0 - top + kLift);
+            sc[0][n][2 + e] = x1 == -INFINITY ? 0.f : exp2_of(x1 - top + kLift);
+            l[n][e] = l[n][e] * f[n][e] + (sc[0][n][e] + sc[0][n][2 + e]);
+          }
+#pragma unroll
+          for (int u = 0; u < TERMS; u++) {
+            p[u][n][0] = transpose8x8(split2<T>(sc[0][n][0], sc[0][n][1]));
+            p[u][n][1] = transpose8x8(split2<T>(sc[0][n][2], sc[0][n][3]));
+          }
+        }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+          for (int i = 0; i < KS; i++)
+#pragma unroll
+            for (int n = 0; n < RT; n++) {
+              o[i][n][0] *= f[n][0];
+              o[i][n][1] *= f[n][1];
+              o[i][n][2] *= f[n][0];
+              o[i][n][3] *= f[n][1];
+            }
+        }
+        cp_async_wait<D - 2>();
+        __syncwarp();
+        ring.fill(2 * t + D, 2 * t + D < 2 * n_tiles);
+        const uint32_t vt = ring0 + ((2 * t + 1) % D) * S::kTileBytes + v_row * S::kPitch + v_col * 2;
+#pragma unroll
+        for (int i = 0; i < KS; i++)
+          if (16 * i < hs) {
+            uint32_t av[4];
+            ldmatrix4_trans(vt + i * 32, av);
+#pragma unroll
+            for (int u = TERMS - 1; u >= 0; u--)
+#pragma unroll
+              for (int n = 0; n < RT; n++) mma_16x8x16<T>(o[i][n], av, p[u][n][0], p[u][n][1]);
+          }
+      }
+      cp_async_wait<0>();
+      __syncwarp();
+      const float down = kLift != 0.f ? 1.f / 16384.f : 1.f;
+#pragma unroll
+      for (int n = 0; n < RT; n++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const int r = 8 * n + 2 * cc + e;
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], w);
+          finite = finite && fabsf(l[n][e]) < INFINITY;
+          if (gr == 0) {
+            s_m[warp][r] = m[n][e];
+            s_l[warp][r] = l[n][e] * down;
+          }
+#pragma unroll
+          for (int i = 0; i < KS; i++)
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+              const float v = o[i][n][2 * y + e] * down;
+              const int d = 16 * i + gr + 8 * y;
+              finite = finite && fabsf(v) < INFINITY;
+              if (r < g.rows && d < hs) o_smem[r * hs + d] = v;
+            }
+        }
+    }
+    if (!__all_sync(0xffffffffu, finite)) {
+      __syncwarp();
+      paged_rows_apart<T>(a, q, g, u0, u1, warp, lane, o_smem, s_m[warp], s_l[warp]);
+    }
+    __syncthreads();
+
+    // ---- the four warps' results, and the group's if other CTAs have a part of it
+    const int first_cta = (int)(g_begin / per), last_cta = (int)((g_end - 1) / per), parts = last_cta - first_cta + 1;
+    const int quads = hs / 4, items = g.rows * quads;
+    const int slot_floats = paged_slot(ROWS, hs);
+    float *slot = a.partial + (2ll * blockIdx.x + ((int)blockIdx.x == first_cta ? 1 : 0)) * slot_floats;
+    for (int i = tid; i < items; i += kPagedThreads) {
+      const int r = i / quads, d = i % quads;
+      float top = s_m[0][r], sum = 0.f;
+#pragma unroll
+      for (int w = 1; w < kPagedWarps; w++) top = fmaxf(top, s_m[w][r]);
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kPagedWarps; w++) {
+        if (s_m[w][r] == -INFINITY && s_l[w][r] == 0.f) continue;
+        const float f = exp2f(s_m[w][r] - top);
+        const float4 o = reinterpret_cast<const float4 *>(paged_smem + S::kQBytes + S::kPBytes + w * S::kRing)[i];
+        sum += f * s_l[w][r];
+        v.x += f * o.x;
+        v.y += f * o.y;
+        v.z += f * o.z;
+        v.w += f * o.w;
+      }
+      if (parts == 1) {
+        const float inv = sum != 0.f ? 1.f / sum : 0.f;
+        if (sum != 0.f) v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+        reinterpret_cast<float4 *>(a.out + row_offset(a, q, g, r, a.ld_out))[d] = v;
+        if (a.stats && d == 0) a.stats[row_index(a, q, g, r)] = top + log2f(sum);
+      } else {
+        __stcg(reinterpret_cast<float4 *>(slot) + i, v);
+        if (d == 0) {
+          __stcg(slot + ROWS * hs + r, top);
+          __stcg(slot + ROWS * hs + ROWS + r, sum);
+        }
+      }
+    }
+    if (parts > 1) {
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        const unsigned int done = atomicAdd(a.join + first_cta, 1u);
+        s_last = done == (unsigned)parts - 1;
+        if (s_last) a.join[first_cta] = 0;
+      }
+      __syncthreads();
+      if (s_last) {
+        __threadfence();
+        // where a row tile has few values, several threads share a quad and take every so many parts
+        float4 *red = reinterpret_cast<float4 *>(paged_smem);
+        float *red_sum = reinterpret_cast<float *>(red + kPagedThreads);
+        auto part_of = [&](int k) { return a.partial + (2ll * (first_cta + k) + (k == 0 ? 1 : 0)) * slot_floats; };
+        const int share = items >= kPagedThreads ? 1 : kPagedThreads / items;
+        for (int i0 = 0; i0 < items; i0 += kPagedThreads) {
+          const int i = share > 1 ? tid % items : i0 + tid, sh = share > 1 ? tid / items : 0;
+          const bool live = i < items && sh < share;
+          const int r = live ? i / quads : 0;
+          float top = -INFINITY, sum = 0.f;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (live) {
+#pragma unroll 8
+            for (int k = 0; k < parts; k++) top = fmaxf(top, __ldcg(part_of(k) + ROWS * hs + r));
+#pragma unroll 4
+            for (int k = sh; k < parts; k += share) {
+              const float *part = part_of(k);
+              const float m = __ldcg(part + ROWS * hs + r), l = __ldcg(part + ROWS * hs + ROWS + r);
+              const float4 o = __ldcg(reinterpret_cast<const float4 *>(part) + i);
+              const float f = m == -INFINITY && l == 0.f ? 0.f : exp2f(m - top);
+              sum += f * l;
+              v.x += f * o.x;
+              v.y += f * o.y;
+              v.z += f * o.z;
+              v.w += f * o.w;
+            }
+          }
+          if (share > 1) {
+            red[tid] = v;
+            red_sum[tid] = sum;
+            __syncthreads();
+            if (tid < items)
+              for (int w = 1; w < share; w++) {
+                const float4 o = red[w * items + tid];
+                v.x += o.x;
+                v.y += o.y;
+                v.z += o.z;
+                v.w += o.w;
+                sum += red_sum[w * items + tid];
+              }
+          }
+          if (live && sh == 0) {
+            if (sum != 0.f) {
+              const float inv = 1.f / sum;
+              v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+            }
+            reinterpret_cast<float4 *>(a.out + row_offset(a, q, g, r, a.ld_out))[i % quads] = v;
+            if (a.stats && i % quads == 0) a.stats[row_index(a, q, g, r)] = top + log2f(sum);
+          }
+        }
+      }
+    }
+    __syncthreads();
+    if (padded && x < x1) clear_ring();  // the results lay there
+  }
+}
+
+// weights[s][j] += sum over the sequence's rows and heads, in their order, of 2^(score - log2 of the sum).
 __global__ void __launch_bounds__(256)
 paged_weights_kernel(PagedAttention a, float *__restrict__ weights, long long ld) {
   pdl_launch_dependents();
@@ -228,7 +959,7 @@ paged_weights_kernel(PagedAttention a, float *__restrict__ weights, long long ld
       for (int h = 0; h < a.n_head; h++) {
         const long long rh = (long long)(first + t) * a.n_head + h;
         const float sc = __ldcg(a.scores + rh * c.max_length + j);
-        if (sc != -INFINITY) w += expf(sc - __ldcg(a.stats + rh));
+        if (sc != -INFINITY) w += exp2f(sc - __ldcg(a.stats + rh));
       }
     }
     weights[s * ld + j] += w;

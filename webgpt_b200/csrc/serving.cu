@@ -1,6 +1,7 @@
 // The operators that serve sequences of different lengths: the paged key-value cache (append, attention, eviction) and the
 // verification of drafted tokens, behind the C ABI of include/webgpt_b200.h.
 #include <algorithm>
+#include <atomic>
 
 #include "host.cuh"
 #include "paged.cuh"
@@ -67,6 +68,68 @@ WGPT_EXPORT int32_t wgpt_paged_append(wgpt_device *dev, const wgpt_paged_cache *
   return WGPT_OK;
 }
 
+// CTAs of a kernel that an SM holds, asked once per kernel and GPU.
+template <typename T, int HSP, int RT>
+static int32_t paged_ctas(wgpt_device *dev, int *out) {
+  static std::atomic<int> known[64];
+  using S = PagedShape<T, HSP, RT>;
+  REQUIRE(dev->ordinal < 64, WGPT_ERR_UNSUPPORTED, "device ordinal %d not supported", dev->ordinal);
+  int n = known[dev->ordinal].load();
+  if (n == 0) {
+    CK(allow_smem(dev, paged_attention_kernel<T, HSP, RT>, true));
+    CK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, paged_attention_kernel<T, HSP, RT>, kPagedThreads, S::kSmem));
+    REQUIRE(n >= 1, WGPT_ERR_UNSUPPORTED, "the attention kernel does not fit an SM");
+    known[dev->ordinal].store(n);
+  }
+  *out = n;
+  return WGPT_OK;
+}
+
+template <typename T, int HSP, int RT>
+static int32_t launch_paged_attention(wgpt_device *dev, PagedAttention &a) {
+  using S = PagedShape<T, HSP, RT>;
+  int per_sm = 0;
+  TRY((paged_ctas<T, HSP, RT>(dev, &per_sm)));
+  const int grid = std::min(per_sm * dev->sm_count, kJoinCounters);
+  const size_t rows = a.stats ? (size_t)a.r.n_rows * a.n_head : 0, scores = rows * (size_t)a.c.max_length;
+  const size_t partial = (size_t)2 * grid * paged_slot(S::kRows, a.c.hs);
+  TRY(scratch_reserve(dev, (partial + rows + scores) * 4));
+  a.partial = static_cast<float *>(dev->scratch);
+  if (a.stats) {
+    a.stats = a.partial + partial;
+    a.scores = a.stats + rows;
+  }
+  a.join = dev->d_join;
+  a.least = 1;
+  LAUNCH_PDL(dev, (paged_attention_kernel<T, HSP, RT>), grid, kPagedThreads, S::kSmem, a);
+  return WGPT_OK;
+}
+
+// How many of the rows that share a head of the cache a CTA takes at once: what a sequence has of them on average. More row
+// tiles read the cache again, fewer rows leave room for more keys in flight.
+template <typename T, int HSP>
+static int32_t launch_paged_rows(wgpt_device *dev, PagedAttention &a, long long rows) {
+  if constexpr (sizeof(T) == 4) {
+    if (rows <= 1) return launch_paged_attention<T, HSP, 1>(dev, a);
+    if (rows <= 2) return launch_paged_attention<T, HSP, 2>(dev, a);
+    if (rows <= 4) return launch_paged_attention<T, HSP, 4>(dev, a);
+    return launch_paged_attention<T, HSP, 8>(dev, a);
+  } else {
+    if (rows <= 8) return launch_paged_attention<T, HSP, 1>(dev, a);
+    if (rows <= 16 || HSP > 128) return launch_paged_attention<T, HSP, 2>(dev, a);
+    if constexpr (HSP <= 128) return launch_paged_attention<T, HSP, 4>(dev, a);
+  }
+  return WGPT_ERR_UNSUPPORTED;
+}
+
+template <typename T>
+static int32_t launch_paged_type(wgpt_device *dev, PagedAttention &a) {
+  const long long tokens = ((long long)a.r.n_rows + a.c.n_seq - 1) / a.c.n_seq, rows = tokens * a.group;
+  if (a.c.hs <= 64) return launch_paged_rows<T, 64>(dev, a, rows);
+  if (a.c.hs <= 128) return launch_paged_rows<T, 128>(dev, a, rows);
+  return launch_paged_rows<T, 256>(dev, a, rows);
+}
+
 WGPT_EXPORT int32_t wgpt_paged_attention(wgpt_device *dev, const wgpt_paged_cache *cache, int32_t n_rows,
                                          const int32_t *starts, int32_t n_head, float scale, int32_t window,
                                          const float *q, int64_t ld_q, float *out, int64_t ld_out, float *weights,
@@ -86,26 +149,19 @@ WGPT_EXPORT int32_t wgpt_paged_attention(wgpt_device *dev, const wgpt_paged_cach
   a.n_head = n_head;
   a.group = n_head / cache->n_kv_head;
   a.window = window;
-  a.scale = scale;
+  a.scale2 = scale * 1.44269504088896f;
   a.q = q;
   a.out = out;
   a.ld_q = ld_q;
   a.ld_out = ld_out;
-  a.scores = a.stats = nullptr;
-  if (weights) {
-    const size_t rows = (size_t)n_rows * n_head;
-    TRY(scratch_reserve(dev, rows * ((size_t)cache->max_length + 1) * 4));
-    a.stats = static_cast<float *>(dev->scratch);
-    a.scores = a.stats + rows;
-  }
-  REQUIRE(n_rows <= 65535, WGPT_ERR_SHAPE, "%d rows", n_rows);
-  const dim3 grid(n_head, n_rows), block(kPagedWarps * 32);
+  a.scores = nullptr;
+  a.stats = weights;  // that there are any; their place is found with the rest of the workspace
   if (cache->type == WGPT_TYPE_F32)
-    LAUNCH_PDL(dev, paged_attention_kernel<float>, grid, block, 0, a);
+    TRY(launch_paged_type<float>(dev, a));
   else if (cache->type == WGPT_TYPE_F16)
-    LAUNCH_PDL(dev, paged_attention_kernel<__half>, grid, block, 0, a);
+    TRY(launch_paged_type<__half>(dev, a));
   else
-    LAUNCH_PDL(dev, paged_attention_kernel<__nv_bfloat16>, grid, block, 0, a);
+    TRY(launch_paged_type<__nv_bfloat16>(dev, a));
   if (weights) {
     const int blocks = std::min((cache->max_length + 255) / 256, std::max(1, 8 * dev->sm_count / cache->n_seq));
     LAUNCH_PDL(dev, paged_weights_kernel, dim3(blocks, cache->n_seq), dim3(256), 0, a, weights, (long long)ld_weights);
