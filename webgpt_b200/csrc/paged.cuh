@@ -293,7 +293,7 @@ struct PagedRing {
   const uint32_t *table;
   uint32_t base;       // shared-memory address of the ring
   uint32_t *ok;        // [kStages] which of a tile's positions are there
-  int lowest, highest, pos, lane, pieces;
+  int lowest, highest, pos, lane, pieces, next = 0;
   uint32_t page, slot; // of this lane's position of the next tile to fill
   long long at;        // where this lane's position of the tile at hand begins, or -1
 
@@ -316,11 +316,12 @@ struct PagedRing {
     pos = first + (lane & (kTile - 1));
     look_up();
   }
-  // Fills half-stage h (in ring order) and commits it.
-  __device__ __forceinline__ void fill(int h, bool any) {
-    const int stage = h % S::kStages;
+  // Fills the next half-stage in ring order, of keys or of values, and commits it.
+  __device__ __forceinline__ void fill(bool keys, bool any) {
+    const int stage = next;
+    next = next + 1 == S::kStages ? 0 : next + 1;
     if (any) {
-      if ((h & 1) == 0) {
+      if (keys) {
         const bool wanted = pos >= lowest && pos < highest;
         at = -1;
         if (page < c.n_pages)
@@ -332,7 +333,7 @@ struct PagedRing {
         pos += kUnit;
         look_up();
       }
-      const T *from = (h & 1) ? v : k;
+      const T *from = keys ? k : v;
       const uint32_t to = base + stage * S::kTileBytes;
 #pragma unroll
       for (int i = 0; i < kSteps; i++) {
@@ -511,7 +512,8 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
     PagedRing<T, HSP, RT> ring(c, s, g.kvh, smem_addr(ring_smem), s_ok[warp], lane);
     if (n_tiles > 0) ring.begin(q.begin + u0 * kUnit + warp * kTile, g.lowest, g.highest);
 #pragma unroll
-    for (int h = 0; h < D - 1; h++) ring.fill(h, h < 2 * n_tiles);
+    for (int h = 0; h < D - 1; h++) ring.fill((h & 1) == 0, h < 2 * n_tiles);
+    int now = 0;  // the stage that is next to be used up
 
     // ---- the queries
     if constexpr (S::kWide) {
@@ -576,9 +578,10 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
         // ---- scores: a lane takes one key and every other quad of its row
         cp_async_wait<D - 2>();
         __syncwarp();
-        ring.fill(2 * t + D - 1, 2 * t + D - 1 < 2 * n_tiles);
-        const uint32_t ok = s_ok[warp][(2 * t) % D];
-        const float4 *kt = reinterpret_cast<const float4 *>(ring_smem + ((2 * t) % D) * S::kTileBytes + key * S::kPitch);
+        ring.fill((D & 1) != 0, 2 * t + D - 1 < 2 * n_tiles);
+        const uint32_t ok = s_ok[warp][now];
+        const float4 *kt = reinterpret_cast<const float4 *>(ring_smem + now * S::kTileBytes + key * S::kPitch);
+        now = now + 1 == D ? 0 : now + 1;
         float sc[ROWS];
 #pragma unroll
         for (int r = 0; r < ROWS; r++) sc[r] = 0.f;
@@ -628,8 +631,9 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
         // ---- values: a lane takes four dimensions (times kQuads) of each key, or of every other one
         cp_async_wait<D - 2>();
         __syncwarp();
-        ring.fill(2 * t + D, 2 * t + D < 2 * n_tiles);
-        const unsigned char *vt = ring_smem + ((2 * t + 1) % D) * S::kTileBytes;
+        ring.fill((D & 1) == 0, 2 * t + D < 2 * n_tiles);
+        const unsigned char *vt = ring_smem + now * S::kTileBytes;
+        now = now + 1 == D ? 0 : now + 1;
         const int dim4 = kHalves == 2 ? key : lane;
 #pragma unroll
         for (int j0 = 0; j0 < kTile; j0 += 4 * kHalves) {
@@ -711,9 +715,10 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
         const int pos0 = q.begin + (u0 + t) * kUnit + warp * kTile;
         cp_async_wait<D - 2>();
         __syncwarp();
-        ring.fill(2 * t + D - 1, 2 * t + D - 1 < 2 * n_tiles);
-        const uint32_t ok = s_ok[warp][(2 * t) % D];
-        const uint32_t kt = ring0 + ((2 * t) % D) * S::kTileBytes + k_row * S::kPitch + k_col * 2;
+        ring.fill((D & 1) != 0, 2 * t + D - 1 < 2 * n_tiles);
+        const uint32_t ok = s_ok[warp][now];
+        const uint32_t kt = ring0 + now * S::kTileBytes + k_row * S::kPitch + k_col * 2;
+        now = now + 1 == D ? 0 : now + 1;
         float sc[TERMS][RT][4];
 #pragma unroll
         for (int u = 0; u < TERMS; u++)
@@ -739,7 +744,6 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
         const bool whole = ok == 0xffffu && pos0 >= g.inner_low && pos0 + kTile <= g.inner_high;
         uint32_t p[TERMS][RT][2];
         float f[RT][2];
-        bool moved = false;
 #pragma unroll
         for (int n = 0; n < RT; n++) {
 #pragma unroll
@@ -768,7 +772,6 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
             for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
             top = fmaxf(top, m[n][e]);
             f[n][e] = m[n][e] == top ? 1.f : exp2_of(m[n][e] - top);
-            moved |= m[n][e] != top;
             m[n][e] = top;
             sc[0][n][e] = x0 == -INFINITY ? 0.f : exp2_of(x0 - top + kLift);
             sc[0][n][2 + e] = x1 == -INFINITY ? 0.f : exp2_of(x1 - top + kLift);
@@ -780,30 +783,28 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
             p[u][n][1] = transpose8x8(split2<T>(sc[0][n][2], sc[0][n][3]));
           }
         }
-        if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-          for (int i = 0; i < KS; i++)
-#pragma unroll
-            for (int n = 0; n < RT; n++) {
-              o[i][n][0] *= f[n][0];
-              o[i][n][1] *= f[n][1];
-              o[i][n][2] *= f[n][0];
-              o[i][n][3] *= f[n][1];
-            }
-        }
         cp_async_wait<D - 2>();
         __syncwarp();
-        ring.fill(2 * t + D, 2 * t + D < 2 * n_tiles);
-        const uint32_t vt = ring0 + ((2 * t + 1) % D) * S::kTileBytes + v_row * S::kPitch + v_col * 2;
+        ring.fill((D & 1) == 0, 2 * t + D < 2 * n_tiles);
+        const uint32_t vt = ring0 + now * S::kTileBytes + v_row * S::kPitch + v_col * 2;
+        now = now + 1 == D ? 0 : now + 1;
 #pragma unroll
         for (int i = 0; i < KS; i++)
           if (16 * i < hs) {
             uint32_t av[4];
             ldmatrix4_trans(vt + i * 32, av);
 #pragma unroll
-            for (int u = TERMS - 1; u >= 0; u--)
+            for (int n = 0; n < RT; n++) {
+              // a tile's values first, smallest terms ahead, then the running sums: the instruction cuts its sum off, which a
+              // long row of additions to one accumulator would show
+              float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-              for (int n = 0; n < RT; n++) mma_16x8x16<T>(o[i][n], av, p[u][n][0], p[u][n][1]);
+              for (int u = TERMS - 1; u >= 0; u--) mma_16x8x16<T>(d, av, p[u][n][0], p[u][n][1]);
+              o[i][n][0] = fmaf(o[i][n][0], f[n][0], d[0]);
+              o[i][n][1] = fmaf(o[i][n][1], f[n][1], d[1]);
+              o[i][n][2] = fmaf(o[i][n][2], f[n][0], d[2]);
+              o[i][n][3] = fmaf(o[i][n][3], f[n][1], d[3]);
+            }
           }
       }
       cp_async_wait<0>();
