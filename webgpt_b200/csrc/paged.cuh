@@ -18,6 +18,7 @@ struct PagedView {
   int *lengths;
   long long page_stride, position_stride, head_stride;
   uint32_t n_pages, page_size;
+  int page_shift;  // log2 of the page size, or -1 where it is no power of two
   int n_kv, hs, n_seq, table_stride, max_length;
   int *err;
 };
@@ -136,13 +137,13 @@ __device__ __forceinline__ float paged_value(const __nv_bfloat16 *p) { return __
 //
 // What bounds it is the cache's bytes: a row of K and V is read once for all the query rows that share it (the heads of its
 // group, times the new tokens), at most ROWS of them, a row tile. All (sequence, head of the cache, row tile) groups lie
-// behind one another as units of 64 positions; every CTA takes as many units as any other, whatever the lengths are, so a CTA
+// behind one another as units of four tiles of positions; every CTA takes as many units as any other, whatever the lengths are, so a CTA
 // may hold the end of one group, whole ones, and the beginning of another. A group that is shared is joined by the CTA that
 // finishes last, in the order of the positions.
 //
-// Inside a CTA four warps take 16 positions each of a unit and never meet until the group ends: each has a ring of tiles in
+// Inside a CTA four warps take a tile of positions each of a unit and never meet until the group ends: each has a ring of tiles in
 // shared memory that cp.async fills, K and V tiles in turn, its own running maximum and its own sums.
-constexpr int kPagedWarps = 4, kPagedThreads = 32 * kPagedWarps, kTile = 16, kUnit = kPagedWarps * kTile;
+constexpr int kPagedWarps = 4, kPagedThreads = 32 * kPagedWarps;
 
 struct PagedAttention {
   PagedView c;
@@ -164,15 +165,15 @@ struct PagedSeq {
   int tiles, units;        // row tiles, units of each
 };
 
-template <int ROWS>
+template <int ROWS, int UNIT>
 __device__ __forceinline__ PagedSeq paged_seq(const PagedAttention &a, int s) {
   PagedSeq q;
   new_rows(a.c, a.r, s, q.first, q.n);
   q.L = paged_length(a.c, s);
   const int lowest = a.window > 0 ? max(0, q.L - q.n + 1 - a.window) : 0;
-  q.begin = min(lowest, q.L) / kUnit * kUnit;
-  q.tiles = (int)(((long long)q.n * a.group + ROWS - 1) / ROWS);
-  q.units = max(1, (q.L - q.begin + kUnit - 1) / kUnit);  // one even if there is nothing to see: the rows are set to zero
+  q.begin = min(lowest, q.L) / UNIT * UNIT;
+  q.tiles = (q.n * a.group + ROWS - 1) / ROWS;
+  q.units = max(1, (q.L - q.begin + UNIT - 1) / UNIT);  // one even if there is nothing to see: the rows are set to zero
   return q;
 }
 
@@ -219,21 +220,23 @@ struct PagedShape {
   static constexpr int kRows = kWide ? RT : 8 * RT;
   static constexpr int kTerms = kWide ? 1 : std::is_same<T, __half>::value ? 2 : 3;  // values that a query or probability is split into
   static constexpr int kPitch = HSP * (int)sizeof(T) + 16;  // of a row in shared memory: 16-byte pieces of 8 rows meet all banks
+  static constexpr int kTile = HSP * (int)sizeof(T) <= 256 ? 32 : 16;  // positions of a warp's tile
+  static constexpr int kUnit = kPagedWarps * kTile;
   static constexpr int kTileBytes = kTile * kPitch;
   static constexpr int kQPitch = kWide ? HSP * 4 : HSP * 2 + 16;
   static constexpr int kQBytes = kRows * kTerms * kQPitch;
   static constexpr int kPBytes = kWide ? kPagedWarps * kRows * kTile * 4 : 0;  // probabilities of a tile
-  // half the ring's tiles are of K and half of V; enough that two CTAs share an SM, where a row is small enough
-  static constexpr int kStages = kTileBytes <= 2304 ? 6 : kTileBytes <= 4352 ? 6 : 3;
+  // tiles of a ring, of K and V in turn: two CTAs or more share an SM, where a row is small enough
+  static constexpr int kStages = 3;
   static constexpr int kRing = kStages * kTileBytes;
   static constexpr int kSmem = kQBytes + kPBytes + kPagedWarps * kRing;
-  static_assert(kRing >= kRows * HSP * 4 || kWide || HSP * RT <= 512, "");
+  static_assert(kRing >= kRows * HSP * 4, "a warp's values go where its ring was");
 };
 
 // Rows of a tile that a warp saw something non-finite in (an infinity or NaN in V, in a key, in q, also where a row's mask
 // leaves it out: zero times infinity): the same again one position at a time, each row from what it sees alone. Leaves the row's
 // maximum, sum and values as the fast path does.
-template <typename T>
+template <typename T, int TILE>
 __device__ __noinline__ void paged_rows_apart(const PagedAttention &a, const PagedSeq &q, const PagedGroup &g, int u0, int u1,
                                               int warp, int lane, float *o_out, float *m_out, float *l_out) {
   const PagedView &c = a.c;
@@ -248,8 +251,8 @@ __device__ __noinline__ void paged_rows_apart(const PagedAttention &a, const Pag
       o[i] = 0.f;
     }
     for (int u = u0; u < u1; u++) {
-      const int base = q.begin + u * kUnit + warp * kTile;
-      for (int j = max(base, lo); j < min(base + kTile, hi); j++) {
+      const int base = q.begin + (u * kPagedWarps + warp) * TILE;
+      for (int j = max(base, lo); j < min(base + TILE, hi); j++) {
         const long long at = paged_offset(c, g.s, j);
         float sc = -INFINITY;
         if (at >= 0) {
@@ -281,31 +284,36 @@ __device__ __noinline__ void paged_rows_apart(const PagedAttention &a, const Pag
   }
 }
 
-// A warp's view of its ring: fills K and V tiles in turn, half-stage 2 t for the keys of its t-th tile and 2 t + 1 for its values.
+// A warp's view of its ring: fills tiles of K and of V in turn.
 template <typename T, int HSP, int RT>
 struct PagedRing {
   using S = PagedShape<T, HSP, RT>;
+  static constexpr int kTile = S::kTile;
   static constexpr int kPerRow = HSP * (int)sizeof(T) / 16;          // 16-byte pieces of a row
   static constexpr int kLanes = kPerRow < 32 ? kPerRow : 32;         // lanes that share a row
-  static constexpr int kAtOnce = 32 / kLanes, kSteps = kTile / kAtOnce, kWidth = kPerRow / kLanes;
+  static constexpr int kAtOnce = 32 / kLanes, kWidth = kPerRow / kLanes;
   const PagedView &c;
   const T *k, *v;      // this head's rows of page 0
   const uint32_t *table;
   uint32_t base;       // shared-memory address of the ring
   uint32_t *ok;        // [kStages] which of a tile's positions are there
-  int lowest, highest, pos, lane, pieces, next = 0;
+  int lowest, highest, pos, lane, next = 0;
   uint32_t page, slot; // of this lane's position of the next tile to fill
   long long at;        // where this lane's position of the tile at hand begins, or -1
+  bool blocks;         // whether 16 positions from a multiple of 16 on always share a page
+  bool plain;          // the tile at hand: all of its positions are there, and in blocks
 
   __device__ __forceinline__ PagedRing(const PagedView &c_, int s, int kvh, uint32_t base_, uint32_t *ok_, int lane_)
       : c(c_), k(static_cast<const T *>(c_.k) + kvh * c_.head_stride), v(static_cast<const T *>(c_.v) + kvh * c_.head_stride),
-        table(c_.table + (size_t)s * c_.table_stride), base(base_), ok(ok_), lane(lane_), pieces(c_.hs * (int)sizeof(T) / 16) {}
+        table(c_.table + (size_t)s * c_.table_stride), base(base_), ok(ok_), lane(lane_) {
+    blocks = c.page_size % 16 == 0;
+  }
 
   __device__ __forceinline__ void look_up() {  // the page of this lane's position, asked for a tile ahead
     page = 0xFFFFFFFFu;
     slot = 0;
     if (pos >= lowest && pos < highest) {
-      const uint32_t index = (uint32_t)pos / c.page_size;
+      const uint32_t index = c.page_shift >= 0 ? (uint32_t)pos >> c.page_shift : (uint32_t)pos / c.page_size;
       slot = (uint32_t)pos - index * c.page_size;
       page = __ldcg(table + index);
     }
@@ -316,34 +324,49 @@ struct PagedRing {
     pos = first + (lane & (kTile - 1));
     look_up();
   }
-  // Fills the next half-stage in ring order, of keys or of values, and commits it.
+  // Fills the next stage with a tile of keys or of values, and commits it.
   __device__ __forceinline__ void fill(bool keys, bool any) {
     const int stage = next;
     next = next + 1 == S::kStages ? 0 : next + 1;
     if (any) {
       if (keys) {
-        const bool wanted = pos >= lowest && pos < highest;
         at = -1;
         if (page < c.n_pages)
           at = (long long)page * c.page_stride + (long long)slot * c.position_stride;
-        else if (wanted)
+        else if (pos >= lowest && pos < highest)
           *c.err = kErrCache;
-        const uint32_t there = __ballot_sync(0xffffffffu, at >= 0) & 0xffffu;
+        const uint32_t there = __ballot_sync(0xffffffffu, at >= 0);
+        plain = blocks && there == 0xffffffffu;
         if (lane == 0) ok[stage] = there;
-        pos += kUnit;
+        pos += S::kUnit;
         look_up();
       }
       const T *from = keys ? k : v;
-      const uint32_t to = base + stage * S::kTileBytes;
+      const uint32_t to = base + stage * S::kTileBytes + lane / kLanes * S::kPitch + lane % kLanes * 16;
+      if (plain) {  // one address per 16 positions, the others at a fixed distance
+        const long long step = (long long)kAtOnce * c.position_stride * (int)sizeof(T);
 #pragma unroll
-      for (int i = 0; i < kSteps; i++) {
-        const int row = i * kAtOnce + lane / kLanes;
-        const long long x = __shfl_sync(0xffffffffu, at, row);
+        for (int b = 0; b < kTile / 16; b++) {
+          const char *p = reinterpret_cast<const char *>(from + __shfl_sync(0xffffffffu, at, 16 * b) + lane / kLanes * c.position_stride) + lane % kLanes * 16;
 #pragma unroll
-        for (int w = 0; w < kWidth; w++) {
-          const int piece = lane % kLanes + w * 32;
-          if (piece < pieces)
-            cp_async16_or_zero(to + row * S::kPitch + piece * 16, reinterpret_cast<const char *>(from + (x < 0 ? 0 : x)) + piece * 16, x >= 0);
+          for (int i = 0; i < 16 / kAtOnce; i++) {
+#pragma unroll
+            for (int w = 0; w < kWidth; w++)
+              if ((lane % kLanes + w * 32) * 16 < c.hs * (int)sizeof(T))
+                cp_async16(to + (16 * b + i * kAtOnce) * S::kPitch + w * 512, p + w * 512);
+            p += step;
+          }
+        }
+      } else {
+#pragma unroll 4
+        for (int i = 0; i < kTile / kAtOnce; i++) {
+          const long long x = __shfl_sync(0xffffffffu, at, i * kAtOnce + lane / kLanes);
+#pragma unroll
+          for (int w = 0; w < kWidth; w++) {
+            const int piece = (lane % kLanes + w * 32) * 16;
+            if (piece < c.hs * (int)sizeof(T))
+              cp_async16_or_zero(to + i * kAtOnce * S::kPitch + w * 512, reinterpret_cast<const char *>(from + (x < 0 ? 0 : x)) + piece, x >= 0);
+          }
         }
       }
     }
@@ -401,7 +424,7 @@ template <typename T, int HSP, int RT>
 __global__ void __launch_bounds__(kPagedThreads)
 paged_attention_kernel(const __grid_constant__ PagedAttention a) {
   using S = PagedShape<T, HSP, RT>;
-  constexpr int ROWS = S::kRows, TERMS = S::kTerms, D = S::kStages;
+  constexpr int ROWS = S::kRows, TERMS = S::kTerms, D = S::kStages, kTile = S::kTile;
   // f32: a lane holds four dimensions of kQuads pieces of a row; where 16 lanes hold a row, the halves of the warp take even and odd keys
   constexpr int kQuads = HSP <= 128 ? 1 : HSP / 128, kHalves = HSP <= 64 ? 2 : 1;
   constexpr float kLift = std::is_same<T, __half>::value ? 14.f : 0.f;  // probabilities are held times 2^14, in the middle of a half's range
@@ -410,8 +433,9 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
   __shared__ int s_lo[ROWS], s_hi[ROWS];
   __shared__ long long s_row[ROWS];
   __shared__ uint32_t s_ok[kPagedWarps][D];
-  __shared__ long long s_sum[kPagedWarps], s_excl;
+  __shared__ uint32_t s_sum[kPagedWarps], s_excl;
   __shared__ int s_seq, s_last;
+  __shared__ PagedSeq s_q;
   const PagedView &c = a.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hs = c.hs;
   unsigned char *q_smem = paged_smem, *ring_smem = paged_smem + S::kQBytes + S::kPBytes + warp * S::kRing;
@@ -427,16 +451,17 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
   pdl_wait();
 
   // ---- this CTA's units
-  auto weight_of = [&](int s) -> long long {
+  PagedSeq q;
+  auto weight_of = [&](int s) -> uint32_t {
     if (s >= c.n_seq) return 0;
-    const PagedSeq q = paged_seq<ROWS>(a, s);
-    return (long long)q.tiles * q.units * c.n_kv;
+    q = paged_seq<ROWS, S::kUnit>(a, s);
+    return (uint32_t)q.tiles * (uint32_t)q.units * (uint32_t)c.n_kv;
   };
-  auto scan = [&](long long mine, long long &all) {  // sum over the threads before this one, and over all
-    long long upto = mine;
+  auto scan = [&](uint32_t mine, uint32_t &all) {  // sum over the threads before this one, and over all
+    uint32_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+      const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += x;
     }
     __syncthreads();
@@ -449,50 +474,52 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
     }
     return upto - mine;
   };
-  long long total = 0, mine = 0, before = 0;
+  uint32_t total = 0, mine = 0, before = 0;
   for (int s0 = 0; s0 < c.n_seq; s0 += kPagedThreads) {
-    long long all;
+    uint32_t all;
     mine = weight_of(s0 + tid);
     before = total + scan(mine, all);
     total += all;
   }
-  const long long per = max((long long)a.least, (total + gridDim.x - 1) / gridDim.x);
-  const long long x0 = blockIdx.x * per, x1 = min(total, x0 + per);
+  const uint32_t per = max((uint32_t)a.least, (total + gridDim.x - 1) / gridDim.x);
+  const uint32_t x0 = blockIdx.x * per, x1 = min(total, x0 + per);  // the caller sees to it that neither passes 2^31
   if (x0 >= x1) return;
   if (c.n_seq <= kPagedThreads) {
     if (before <= x0 && x0 < before + mine) {
       s_seq = tid;
       s_excl = before;
+      s_q = q;
     }
   } else {
-    long long sum = 0;
+    uint32_t sum = 0;
     for (int s0 = 0; s0 < c.n_seq && sum <= x0; s0 += kPagedThreads) {
-      long long all;
+      uint32_t all;
       mine = weight_of(s0 + tid);
       before = sum + scan(mine, all);
       if (before <= x0 && x0 < before + mine) {
         s_seq = s0 + tid;
         s_excl = before;
+        s_q = q;
       }
       sum += all;
     }
   }
   __syncthreads();
   int s = s_seq;
-  long long seq_begin = s_excl, x = x0;
-  PagedSeq q = paged_seq<ROWS>(a, s);
+  uint32_t seq_begin = s_excl, x = x0;
+  q = s_q;
 
   while (x < x1) {
-    while (x >= seq_begin + (long long)q.tiles * q.units * c.n_kv) {
-      seq_begin += (long long)q.tiles * q.units * c.n_kv;
-      q = paged_seq<ROWS>(a, ++s);
+    while (x >= seq_begin + (uint32_t)q.tiles * (uint32_t)q.units * (uint32_t)c.n_kv) {
+      seq_begin += (uint32_t)q.tiles * (uint32_t)q.units * (uint32_t)c.n_kv;
+      q = paged_seq<ROWS, S::kUnit>(a, ++s);
     }
-    const long long gi = (x - seq_begin) / q.units, g_begin = seq_begin + gi * q.units, g_end = g_begin + q.units;
+    const uint32_t gi = (x - seq_begin) / (uint32_t)q.units, g_begin = seq_begin + gi * q.units, g_end = g_begin + q.units;
     PagedGroup g;
     g.s = s;
-    g.kvh = (int)(gi / q.tiles);
-    g.r0 = (int)(gi % q.tiles) * ROWS;
-    g.rows = (int)min((long long)ROWS, (long long)q.n * a.group - g.r0);
+    g.kvh = (int)(gi / (uint32_t)q.tiles);
+    g.r0 = (int)(gi - (uint32_t)g.kvh * (uint32_t)q.tiles) * ROWS;
+    g.rows = min(ROWS, q.n * a.group - g.r0);
     {
       int lo, hi;
       row_range(a, q, g.r0 / a.group, lo, hi);
@@ -505,12 +532,12 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
     // units [u0, u1) of the group are this CTA's; those that no row of the tile sees are left out
     int u0 = (int)(x - g_begin), u1 = (int)(min(x1, g_end) - g_begin);
     x = min(x1, g_end);
-    u0 = max(u0, (g.lowest - q.begin) / kUnit);
-    u1 = min(u1, (g.highest - q.begin + kUnit - 1) / kUnit);
+    u0 = max(u0, (g.lowest - q.begin) / S::kUnit);
+    u1 = min(u1, (g.highest - q.begin + S::kUnit - 1) / S::kUnit);
     const int n_tiles = max(0, u1 - u0);
 
     PagedRing<T, HSP, RT> ring(c, s, g.kvh, smem_addr(ring_smem), s_ok[warp], lane);
-    if (n_tiles > 0) ring.begin(q.begin + u0 * kUnit + warp * kTile, g.lowest, g.highest);
+    if (n_tiles > 0) ring.begin(q.begin + (u0 * kPagedWarps + warp) * kTile, g.lowest, g.highest);
 #pragma unroll
     for (int h = 0; h < D - 1; h++) ring.fill((h & 1) == 0, h < 2 * n_tiles);
     int now = 0;  // the stage that is next to be used up
@@ -563,7 +590,8 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
     bool finite = true;
     float *o_smem = reinterpret_cast<float *>(ring_smem);
     if constexpr (S::kWide) {
-      const int key = lane & 15, half = lane >> 4;
+      constexpr int kShare = 32 / kTile;  // lanes that share a key
+      const int key = lane % kTile, share = lane / kTile, half = lane >> 4, dim = lane & 15;
       float m[ROWS], l[ROWS];
       float4 o[ROWS][kQuads];
 #pragma unroll
@@ -574,8 +602,8 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
         for (int w = 0; w < kQuads; w++) o[r][w] = make_float4(0.f, 0.f, 0.f, 0.f);
       }
       for (int t = 0; t < n_tiles; t++) {
-        const int pos0 = q.begin + (u0 + t) * kUnit + warp * kTile;
-        // ---- scores: a lane takes one key and every other quad of its row
+        const int pos0 = q.begin + ((u0 + t) * kPagedWarps + warp) * kTile;
+        // ---- scores: a lane takes one key, or every other quad of its row
         cp_async_wait<D - 2>();
         __syncwarp();
         ring.fill((D & 1) != 0, 2 * t + D - 1 < 2 * n_tiles);
@@ -585,8 +613,8 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
         float sc[ROWS];
 #pragma unroll
         for (int r = 0; r < ROWS; r++) sc[r] = 0.f;
-#pragma unroll 4
-        for (int d = half; d < hs / 4; d += 2) {
+#pragma unroll 8
+        for (int d = share; d < hs / 4; d += kShare) {
           const float4 kv = kt[d];
 #pragma unroll
           for (int r = 0; r < ROWS; r++) {
@@ -597,25 +625,26 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
             sc[r] = fmaf(qv.w, kv.w, sc[r]);
           }
         }
-        const bool whole = ok == 0xffffu && pos0 >= g.inner_low && pos0 + kTile <= g.inner_high;
+        const bool whole = ok == 0xffffffffu && pos0 >= g.inner_low && pos0 + kTile <= g.inner_high;
         float f[ROWS];
         bool moved = false;
 #pragma unroll
         for (int r = 0; r < ROWS; r++) {
-          sc[r] = (sc[r] + __shfl_xor_sync(0xffffffffu, sc[r], 16)) * a.scale2;
+          if (kShare == 2) sc[r] += __shfl_xor_sync(0xffffffffu, sc[r], 16);
+          sc[r] *= a.scale2;
           if (!whole && !((ok >> key & 1u) && pos0 + key >= s_lo[r] && pos0 + key < s_hi[r])) sc[r] = -INFINITY;
-          if (a.scores && half == 0 && r < g.rows && pos0 + key >= s_lo[r] && pos0 + key < s_hi[r])
+          if (a.scores && share == 0 && r < g.rows && pos0 + key >= s_lo[r] && pos0 + key < s_hi[r])
             a.scores[s_row[r] + pos0 + key] = sc[r];
           float top = sc[r];
 #pragma unroll
-          for (int w = 8; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+          for (int w = kTile / 2; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
           top = fmaxf(top, m[r]);
           f[r] = m[r] == top ? 1.f : exp2_of(m[r] - top);
           moved |= m[r] != top;
           const float p = sc[r] == -INFINITY ? 0.f : exp2_of(sc[r] - top);
           m[r] = top;
           l[r] = l[r] * f[r] + p;
-          if (half == 0) p_smem[r * kTile + key] = p;
+          if (share == 0) p_smem[r * kTile + key] = p;
         }
         if (moved) {
 #pragma unroll
@@ -634,7 +663,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
         ring.fill((D & 1) == 0, 2 * t + D < 2 * n_tiles);
         const unsigned char *vt = ring_smem + now * S::kTileBytes;
         now = now + 1 == D ? 0 : now + 1;
-        const int dim4 = kHalves == 2 ? key : lane;
+        const int dim4 = kHalves == 2 ? dim : lane;
 #pragma unroll
         for (int j0 = 0; j0 < kTile; j0 += 4 * kHalves) {
           float4 vv[4][kQuads];
@@ -667,7 +696,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
 #pragma unroll
       for (int r = 0; r < ROWS; r++) {
 #pragma unroll
-        for (int w = 8; w > 0; w >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], w);
+        for (int w = kTile / 2; w > 0; w >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], w);
 #pragma unroll
         for (int w = 0; w < kQuads; w++) {
           float4 &v = o[r][w];
@@ -677,7 +706,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
             v.z += __shfl_xor_sync(0xffffffffu, v.z, 16);
             v.w += __shfl_xor_sync(0xffffffffu, v.w, 16);
           }
-          const int d = (kHalves == 2 ? key : lane) + 32 * w;
+          const int d = (kHalves == 2 ? dim : lane) + 32 * w;
           finite = finite && fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) < INFINITY;
           if (r < g.rows && 4 * d < hs && (kHalves == 1 || half == 0)) *reinterpret_cast<float4 *>(o_smem + r * hs + 4 * d) = v;
         }
@@ -691,7 +720,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
       // The keys are the matrix instruction's 16 rows and the queries its 8 columns: scores come out with a lane holding two
       // queries of keys lane / 4 and lane / 4 + 8, and the probabilities, transposed inside the warp, are the second operand
       // of the values' product, whose rows are dimensions.
-      constexpr int KS = HSP / 16;
+      constexpr int KS = HSP / 16, KB = kTile / 16;  // steps of 16 dimensions, blocks of 16 positions
       const int gr = lane >> 2, cc = lane & 3;
       const uint32_t ring0 = smem_addr(ring_smem), q0 = smem_addr(q_smem);
       const int k_row = (lane & 7) + (lane & 8), k_col = (lane >> 4) * 8;             // a lane's row and piece of a K tile's fragment
@@ -712,76 +741,96 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
 #pragma unroll
         for (int n = 0; n < RT; n++) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
       for (int t = 0; t < n_tiles; t++) {
-        const int pos0 = q.begin + (u0 + t) * kUnit + warp * kTile;
+        const int pos0 = q.begin + ((u0 + t) * kPagedWarps + warp) * kTile;
         cp_async_wait<D - 2>();
         __syncwarp();
         ring.fill((D & 1) != 0, 2 * t + D - 1 < 2 * n_tiles);
         const uint32_t ok = s_ok[warp][now];
         const uint32_t kt = ring0 + now * S::kTileBytes + k_row * S::kPitch + k_col * 2;
         now = now + 1 == D ? 0 : now + 1;
-        float sc[TERMS][RT][4];
+        float sc[TERMS][KB][RT][4];
 #pragma unroll
         for (int u = 0; u < TERMS; u++)
 #pragma unroll
-          for (int n = 0; n < RT; n++) sc[u][n][0] = sc[u][n][1] = sc[u][n][2] = sc[u][n][3] = 0.f;
+          for (int b = 0; b < KB; b++)
+#pragma unroll
+            for (int n = 0; n < RT; n++) sc[u][b][n][0] = sc[u][b][n][1] = sc[u][b][n][2] = sc[u][b][n][3] = 0.f;
 #pragma unroll
         for (int i = 0; i < KS; i += 2) {
           if (16 * i < hs) {
-            uint32_t a0[4], a1[4];
-            ldmatrix4(kt + i * 32, a0);
-            if (HSP >= 32) ldmatrix4(kt + (i + 1) * 32, a1);
+            uint32_t ka[KB][2][4];
+#pragma unroll
+            for (int b = 0; b < KB; b++) {
+              ldmatrix4(kt + b * 16 * S::kPitch + i * 32, ka[b][0]);
+              ldmatrix4(kt + b * 16 * S::kPitch + (i + 1) * 32, ka[b][1]);
+            }
 #pragma unroll
             for (int u = 0; u < TERMS; u++)
 #pragma unroll
               for (int n = 0; n < RT; n++) {
-                uint32_t b[4];
-                ldmatrix4(q0 + (u * ROWS + 8 * n + q_row) * S::kQPitch + (i * 16 + q_col) * 2, b);
-                mma_16x8x16<T>(sc[u][n], a0, b[0], b[1]);
-                mma_16x8x16<T>(sc[u][n], a1, b[2], b[3]);
+                uint32_t qb[4];
+                ldmatrix4(q0 + (u * ROWS + 8 * n + q_row) * S::kQPitch + (i * 16 + q_col) * 2, qb);
+#pragma unroll
+                for (int b = 0; b < KB; b++) mma_16x8x16<T>(sc[u][b][n], ka[b][0], qb[0], qb[1]);
+#pragma unroll
+                for (int b = 0; b < KB; b++) mma_16x8x16<T>(sc[u][b][n], ka[b][1], qb[2], qb[3]);
               }
           }
         }
-        const bool whole = ok == 0xffffu && pos0 >= g.inner_low && pos0 + kTile <= g.inner_high;
-        uint32_t p[TERMS][RT][2];
+        const bool whole = ok == 0xffffffffu && pos0 >= g.inner_low && pos0 + kTile <= g.inner_high;
+        uint32_t p[TERMS][KB][RT][2];
         float f[RT][2];
 #pragma unroll
         for (int n = 0; n < RT; n++) {
 #pragma unroll
           for (int e = 0; e < 2; e++) {
-            float x0 = sc[TERMS - 1][n][e], x1 = sc[TERMS - 1][n][2 + e];
-#pragma unroll
-            for (int u = TERMS - 2; u >= 0; u--) {
-              x0 += sc[u][n][e];
-              x1 += sc[u][n][2 + e];
-            }
-            x0 *= qs[n][e];
-            x1 *= qs[n][e];
             const int r = 8 * n + 2 * cc + e;
+            float x[2 * KB], top = m[n][e];  // of this lane's positions gr + 8 y
+#pragma unroll
+            for (int y = 0; y < 2 * KB; y++) {
+              x[y] = sc[TERMS - 1][y / 2][n][2 * (y & 1) + e];
+#pragma unroll
+              for (int u = TERMS - 2; u >= 0; u--) x[y] += sc[u][y / 2][n][2 * (y & 1) + e];
+              x[y] *= qs[n][e];
+            }
             if (!whole) {
-              const int lo = s_lo[r], hi = s_hi[r];
-              if (!((ok >> gr & 1u) && pos0 + gr >= lo && pos0 + gr < hi)) x0 = -INFINITY;
-              if (!((ok >> (gr + 8) & 1u) && pos0 + gr + 8 >= lo && pos0 + gr + 8 < hi)) x1 = -INFINITY;
+              const int lo = s_lo[r] - pos0, hi = s_hi[r] - pos0;
+#pragma unroll
+              for (int y = 0; y < 2 * KB; y++) {
+                const int j = gr + 8 * y;
+                if (!((ok >> j & 1u) && j >= lo && j < hi)) x[y] = -INFINITY;
+              }
             }
             if (a.scores && r < g.rows) {
               float *to = a.scores + s_row[r] + pos0 + gr;
-              if (pos0 + gr >= s_lo[r] && pos0 + gr < s_hi[r]) to[0] = x0;
-              if (pos0 + gr + 8 >= s_lo[r] && pos0 + gr + 8 < s_hi[r]) to[8] = x1;
+              const int lo = s_lo[r] - pos0, hi = s_hi[r] - pos0;
+#pragma unroll
+              for (int y = 0; y < 2 * KB; y++)
+                if (gr + 8 * y >= lo && gr + 8 * y < hi) to[8 * y] = x[y];
             }
-            float top = fmaxf(x0, x1);
+#pragma unroll
+            for (int y = 0; y < 2 * KB; y++) top = fmaxf(top, x[y]);
 #pragma unroll
             for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-            top = fmaxf(top, m[n][e]);
             f[n][e] = m[n][e] == top ? 1.f : exp2_of(m[n][e] - top);
             m[n][e] = top;
-            sc[0][n][e] = x0 == -INFINITY ? 0.f : exp2_of(x0 - top + kLift);
-            sc[0][n][2 + e] = x1 == -INFINITY ? 0.f : exp2_of(x1 - top + kLift);
-            l[n][e] = l[n][e] * f[n][e] + (sc[0][n][e] + sc[0][n][2 + e]);
+            const float less = top - kLift;
+            float sum = 0.f;
+#pragma unroll
+            for (int y = 0; y < 2 * KB; y++) {
+              x[y] = x[y] == -INFINITY ? 0.f : exp2_of(x[y] - less);
+              sum += x[y];
+              sc[0][y / 2][n][2 * (y & 1) + e] = x[y];
+            }
+            l[n][e] = fmaf(l[n][e], f[n][e], sum);
           }
 #pragma unroll
-          for (int u = 0; u < TERMS; u++) {
-            p[u][n][0] = transpose8x8(split2<T>(sc[0][n][0], sc[0][n][1]));
-            p[u][n][1] = transpose8x8(split2<T>(sc[0][n][2], sc[0][n][3]));
-          }
+          for (int b = 0; b < KB; b++)
+#pragma unroll
+            for (int u = 0; u < TERMS; u++) {
+              p[u][b][n][0] = transpose8x8(split2<T>(sc[0][b][n][0], sc[0][b][n][1]));
+              p[u][b][n][1] = transpose8x8(split2<T>(sc[0][b][n][2], sc[0][b][n][3]));
+            }
         }
         cp_async_wait<D - 2>();
         __syncwarp();
@@ -791,15 +840,18 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
 #pragma unroll
         for (int i = 0; i < KS; i++)
           if (16 * i < hs) {
-            uint32_t av[4];
-            ldmatrix4_trans(vt + i * 32, av);
+            uint32_t va[KB][4];
+#pragma unroll
+            for (int b = 0; b < KB; b++) ldmatrix4_trans(vt + b * 16 * S::kPitch + i * 32, va[b]);
 #pragma unroll
             for (int n = 0; n < RT; n++) {
               // a tile's values first, smallest terms ahead, then the running sums: the instruction cuts its sum off, which a
               // long row of additions to one accumulator would show
               float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-              for (int u = TERMS - 1; u >= 0; u--) mma_16x8x16<T>(d, av, p[u][n][0], p[u][n][1]);
+              for (int u = TERMS - 1; u >= 0; u--)
+#pragma unroll
+                for (int b = 0; b < KB; b++) mma_16x8x16<T>(d, va[b], p[u][b][n][0], p[u][b][n][1]);
               o[i][n][0] = fmaf(o[i][n][0], f[n][0], d[0]);
               o[i][n][1] = fmaf(o[i][n][1], f[n][1], d[1]);
               o[i][n][2] = fmaf(o[i][n][2], f[n][0], d[2]);
@@ -835,7 +887,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
     }
     if (!__all_sync(0xffffffffu, finite)) {
       __syncwarp();
-      paged_rows_apart<T>(a, q, g, u0, u1, warp, lane, o_smem, s_m[warp], s_l[warp]);
+      paged_rows_apart<T, S::kTile>(a, q, g, u0, u1, warp, lane, o_smem, s_m[warp], s_l[warp]);
     }
     __syncthreads();
 
@@ -899,7 +951,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
           if (live) {
 #pragma unroll 8
             for (int k = 0; k < parts; k++) top = fmaxf(top, __ldcg(part_of(k) + ROWS * hs + r));
-#pragma unroll 4
+#pragma unroll 8
             for (int k = sh; k < parts; k += share) {
               const float *part = part_of(k);
               const float m = __ldcg(part + ROWS * hs + r), l = __ldcg(part + ROWS * hs + ROWS + r);

@@ -28,8 +28,11 @@ static int32_t check_cache(wgpt_device *dev, const wgpt_paged_cache *c, PagedVie
   REQUIRE(aligned16(c->k) && aligned16(c->v) && c->page_stride % per16 == 0 && c->position_stride % per16 == 0 &&
               c->head_stride % per16 == 0,
           WGPT_ERR_ALIGN, "pools must be 16-byte aligned and their strides multiples of 16 bytes");
+  int shift = 0;
+  while (shift < 31 && (1 << shift) < c->page_size) shift++;
+  if ((1u << shift) != (uint32_t)c->page_size) shift = -1;
   *out = PagedView{c->k,          c->v,         c->table,     c->lengths, c->page_stride,  c->position_stride,
-                   c->head_stride, (uint32_t)c->n_pages, (uint32_t)c->page_size, c->n_kv_head, c->head_size, c->n_seq,
+                   c->head_stride, (uint32_t)c->n_pages, (uint32_t)c->page_size, shift, c->n_kv_head, c->head_size, c->n_seq,
                    c->table_stride, c->max_length, dev->d_err};
   return WGPT_OK;
 }
@@ -92,6 +95,10 @@ static int32_t launch_paged_attention(wgpt_device *dev, PagedAttention &a) {
   TRY((paged_ctas<T, HSP, RT>(dev, &per_sm)));
   const int grid = std::min(per_sm * dev->sm_count, kJoinCounters);
   const size_t rows = a.stats ? (size_t)a.r.n_rows * a.n_head : 0, scores = rows * (size_t)a.c.max_length;
+  // units and rows are counted in 32 bits
+  REQUIRE((int64_t)a.r.n_rows * a.group < (int64_t)1 << 30 &&
+              ((int64_t)a.r.n_rows * a.group / S::kRows + a.c.n_seq) * (a.c.max_length / S::kUnit + 2) < ((int64_t)1 << 31) / a.c.n_kv,
+          WGPT_ERR_SHAPE, "%d rows over up to %d positions of %d heads: split the call", a.r.n_rows, a.c.max_length, a.c.n_kv);
   const size_t partial = (size_t)2 * grid * paged_slot(S::kRows, a.c.hs);
   TRY(scratch_reserve(dev, (partial + rows + scores) * 4));
   a.partial = static_cast<float *>(dev->scratch);
@@ -100,7 +107,8 @@ static int32_t launch_paged_attention(wgpt_device *dev, PagedAttention &a) {
     a.scores = a.stats + rows;
   }
   a.join = dev->d_join;
-  a.least = 1;
+  static const int least = getenv("LEAST") ? atoi(getenv("LEAST")) : 1;
+  a.least = least;
   LAUNCH_PDL(dev, (paged_attention_kernel<T, HSP, RT>), grid, kPagedThreads, S::kSmem, a);
   return WGPT_OK;
 }
@@ -117,14 +125,16 @@ static int32_t launch_paged_rows(wgpt_device *dev, PagedAttention &a, long long 
   } else {
     if (rows <= 8) return launch_paged_attention<T, HSP, 1>(dev, a);
     if (rows <= 16 || HSP > 128) return launch_paged_attention<T, HSP, 2>(dev, a);
-    if constexpr (HSP <= 128) return launch_paged_attention<T, HSP, 4>(dev, a);
+    if constexpr (HSP <= 128) return launch_paged_attention<T, HSP, 3>(dev, a);
   }
   return WGPT_ERR_UNSUPPORTED;
 }
 
 template <typename T>
 static int32_t launch_paged_type(wgpt_device *dev, PagedAttention &a) {
-  const long long tokens = ((long long)a.r.n_rows + a.c.n_seq - 1) / a.c.n_seq, rows = tokens * a.group;
+  long long tokens = ((long long)a.r.n_rows + a.c.n_seq - 1) / a.c.n_seq;
+  if (a.r.starts && tokens > 1) tokens += (tokens + 1) / 2;  // some have more than the average
+  const long long rows = tokens * a.group;
   if (a.c.hs <= 64) return launch_paged_rows<T, 64>(dev, a, rows);
   if (a.c.hs <= 128) return launch_paged_rows<T, 128>(dev, a, rows);
   return launch_paged_rows<T, 256>(dev, a, rows);
