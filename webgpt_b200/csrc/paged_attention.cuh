@@ -1,0 +1,922 @@
+// Attention of new tokens over a paged cache.
+//   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = 2^(c s_ij - m_i),  s_ij = q_i . k_j,  c = scale / ln 2,  m_i = max_j c s_ij
+// in one pass over the keys, with the running maximum and sum in f32 (sums and values are multiplied by 2^(old - new maximum)
+// when it moves).
+//
+// What bounds it is the cache's bytes: a row of K and V is read once for all the query rows that share it (the heads of its
+// group, times the new tokens), at most a row tile of them. All (sequence, head of the cache, row tile) groups lie behind one
+// another as units of a few tiles of positions; every CTA takes as many units as any other, whatever the lengths are, so a CTA
+// may hold the end of one group, whole ones, and the beginning of another. A group that is shared is joined by the CTA that
+// finishes last, in the order of the positions.
+//
+// Inside a CTA the key groups (of one warp, or of several with eight rows each) take a tile of each unit and do not meet until
+// the group ends: each has a ring of tiles in shared memory that cp.async fills, K and V tiles in turn. While a group's results
+// are put together the first tiles of the next one are on their way.
+#pragma once
+#include <type_traits>
+
+#include "paged.cuh"
+
+namespace wgpt {
+
+__device__ __forceinline__ float paged_value(const float *p) { return __ldcg(p); }
+__device__ __forceinline__ float paged_value(const __half *p) { return __half2float(__ldcg(p)); }
+__device__ __forceinline__ float paged_value(const __nv_bfloat16 *p) { return __bfloat162float(__ldcg(p)); }
+
+constexpr int kPagedKeyGroups = 4, kPagedWarps = 8, kPagedRows = 32;  // at most, in a CTA
+
+struct PagedAttention {
+  PagedView c;
+  NewRows r;
+  int n_head, group, window;
+  float scale2;  // scale / ln 2
+  const float *q;
+  float *out;
+  long long ld_q, ld_out;
+  int key_groups, row_warps, rows;  // of a CTA: key groups of row_warps warps; rows of a row tile
+  int least;             // fewest units a CTA takes
+  int ahead;             // whether the results of a group leave room for the next one's first tiles
+  float *partial;        // [2 * CTAs][paged_slot(rows, hs)]
+  unsigned int *join;    // a counter per CTA, zero on entry and left zero
+  float *scores, *stats; // [n_rows * n_head][max_length] and [n_rows * n_head], in units of log 2, or NULL
+};
+
+// A sequence's share of the work.
+struct PagedSeq {
+  int first, n, L, begin;  // rows, length, position of the first unit
+  int tiles, units;        // row tiles, units of each
+};
+
+__device__ __forceinline__ PagedSeq paged_seq(const PagedAttention &a, int s, int unit) {
+  PagedSeq q;
+  new_rows(a.c, a.r, s, q.first, q.n);
+  q.L = paged_length(a.c, s);
+  const int lowest = a.window > 0 ? max(0, q.L - q.n + 1 - a.window) : 0;
+  q.begin = min(lowest, q.L) & ~(unit - 1);
+  q.tiles = (q.n * a.group + a.rows - 1) / a.rows;
+  q.units = max(1, (q.L - q.begin + unit - 1) / unit);  // one even if there is nothing to see: the rows are set to zero
+  return q;
+}
+__device__ __forceinline__ uint32_t paged_work(const PagedAttention &a, const PagedSeq &q) {
+  return (uint32_t)q.tiles * (uint32_t)q.units * (uint32_t)a.c.n_kv;
+}
+
+// What a part of a group leaves for the others: the rows' values, maxima and sums.
+__host__ __device__ constexpr int paged_slot(int rows, int hs) { return rows * hs + (2 * rows + 3) / 4 * 4; }
+
+// The row tile that a CTA works on.
+struct PagedGroup {
+  int s, kvh, r0, rows;    // sequence, head of the cache, first row of the tile (token * group + head in the group), rows
+  int lowest, highest;     // positions that some row sees: [lowest, highest)
+  int inner_low, inner_high;  // positions that every row sees
+};
+
+// A CTA's part of it, and where the sequence's work begins.
+struct PagedPart {
+  PagedSeq q;
+  PagedGroup g;
+  uint32_t seq_begin, begin, end, next;  // of the sequence, of the group; the unit behind this part
+  int u0, n_tiles;                       // units of the group
+};
+
+__device__ __forceinline__ void row_range(const PagedAttention &a, const PagedSeq &q, int token, int &lo, int &hi) {
+  hi = max(0, q.L - q.n + token + 1);
+  lo = a.window > 0 ? max(0, hi - a.window) : 0;
+}
+__device__ __forceinline__ long long row_offset(const PagedAttention &a, const PagedPart &w, int r, long long ld) {
+  const int token = (w.g.r0 + r) / a.group, head = w.g.kvh * a.group + (w.g.r0 + r) - token * a.group;
+  return (long long)(w.q.first + token) * ld + (long long)head * a.c.hs;
+}
+__device__ __forceinline__ long long row_index(const PagedAttention &a, const PagedPart &w, int r) {
+  const int token = (w.g.r0 + r) / a.group, head = w.g.kvh * a.group + (w.g.r0 + r) - token * a.group;
+  return (long long)(w.q.first + token) * a.n_head + head;
+}
+
+// The part that begins at unit x of sequence s, up to unit end at most; q and seq_begin are the sequence's.
+__device__ __forceinline__ void paged_part(const PagedAttention &a, PagedPart &w, const PagedSeq &q, int s, uint32_t seq_begin, uint32_t x,
+                                           uint32_t end, int unit) {
+  const uint32_t gi = (x - seq_begin) / (uint32_t)q.units;
+  w.q = q;
+  w.seq_begin = seq_begin;
+  w.begin = seq_begin + gi * (uint32_t)q.units;
+  w.end = w.begin + (uint32_t)q.units;
+  w.next = min(end, w.end);
+  w.g.s = s;
+  w.g.kvh = (int)(gi / (uint32_t)q.tiles);
+  w.g.r0 = (int)(gi - (uint32_t)w.g.kvh * (uint32_t)q.tiles) * a.rows;
+  w.g.rows = min(a.rows, q.n * a.group - w.g.r0);
+  row_range(a, q, w.g.r0 / a.group, w.g.lowest, w.g.inner_high);
+  row_range(a, q, (w.g.r0 + w.g.rows - 1) / a.group, w.g.inner_low, w.g.highest);
+  // units that no row of the tile sees are left out
+  w.u0 = max((int)(x - w.begin), (w.g.lowest - q.begin) / unit);
+  w.n_tiles = max(0, min((int)(w.next - w.begin), (w.g.highest - q.begin + unit - 1) / unit) - w.u0);
+}
+
+// Copies 16 bytes, or writes zeros where there is nothing to copy.
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t to, const void *from, bool there) {
+  const int bytes = there ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ float exp2_of(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// What the kernel of a type, a (padded) head size and a number of rows takes of shared memory. f32: products on the CUDA cores, RT
+// rows a warp; else on the tensor cores, eight rows a warp.
+template <typename T, int HSP, int RT, int STAGES>
+struct PagedShape {
+  static constexpr bool kWide = sizeof(T) == 4;
+  static constexpr int kTerms = kWide ? 1 : std::is_same<T, __half>::value ? 2 : 3;  // values that a query or probability is split into
+  static constexpr int kPitch = HSP * (int)sizeof(T) + 16;  // of a row in shared memory: 16-byte pieces of 8 rows meet all banks
+  static constexpr int kTile = HSP * (int)sizeof(T) <= 256 ? 32 : 16;  // positions of a tile
+  static constexpr int kTileBytes = kTile * kPitch;
+  static constexpr int kQPitch = kWide ? HSP * 4 : HSP * 2 + 16;
+  static constexpr int kStages = STAGES;  // tiles of a ring
+  static constexpr int kRing = kStages * kTileBytes;
+  static constexpr int kPBytes = kWide ? RT * kTile * 4 : 0;  // a warp's probabilities of a tile
+  __host__ __device__ static constexpr int q_bytes(int rows) { return rows * kTerms * kQPitch; }
+  __host__ __device__ static constexpr int smem(int key_groups, int rows) { return q_bytes(rows) + key_groups * (kPBytes + kRing); }
+  __host__ __device__ static constexpr bool ahead(int rows, int hs) { return rows * hs * 4 <= kTileBytes; }
+  __host__ __device__ static constexpr bool fits(int rows, int hs) { return rows * hs * 4 <= kRing; }
+};
+
+// Rows of a tile that a warp saw something non-finite in (an infinity or NaN in V, in a key, in q, also where a row's mask
+// leaves it out: zero times infinity): the same again one position at a time, each row from what it sees alone. Leaves the row's
+// maximum, sum and values as the fast path does.
+template <typename T, int TILE>
+__device__ __noinline__ void paged_rows_apart(const PagedAttention &a, const PagedPart &w, int key_group, int key_groups,
+                                              int row0, int row1, int lane, float *o_out, float *m_out, float *l_out) {
+  const PagedView &c = a.c;
+  const PagedSeq &q = w.q;
+  const PagedGroup &g = w.g;
+  for (int r = row0; r < row1; r++) {
+    int lo, hi;
+    row_range(a, q, (g.r0 + r) / a.group, lo, hi);
+    const float *x = a.q + row_offset(a, w, r, a.ld_q);
+    float qv[8], o[8], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      qv[i] = lane + 32 * i < c.hs ? __ldcg(x + lane + 32 * i) : 0.f;
+      o[i] = 0.f;
+    }
+    for (int u = w.u0; u < w.u0 + w.n_tiles; u++) {
+      const int base = q.begin + (u * key_groups + key_group) * TILE;
+      for (int j = max(base, lo); j < min(base + TILE, hi); j++) {
+        const long long at = paged_offset(c, g.s, j);
+        float sc = -INFINITY;
+        if (at >= 0) {
+          const T *k = static_cast<const T *>(c.k) + at + g.kvh * c.head_stride, *v = static_cast<const T *>(c.v) + at + g.kvh * c.head_stride;
+          float d = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; i++)
+            if (lane + 32 * i < c.hs) d += qv[i] * paged_value(k + lane + 32 * i);
+          sc = warp_sum(d) * a.scale2;
+          if (sc != -INFINITY) {
+            const float nm = fmaxf(m, sc), f = exp2f(m - nm), p = exp2f(sc - nm);
+            l = l * f + p;
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+              if (lane + 32 * i < c.hs) o[i] = o[i] * f + p * paged_value(v + lane + 32 * i);
+            m = nm;
+          }
+        }
+        if (a.scores && lane == 0) a.scores[row_index(a, w, r) * c.max_length + j] = sc;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (lane + 32 * i < c.hs) o_out[r * c.hs + lane + 32 * i] = o[i];
+    if (lane == 0) {
+      m_out[r] = m;
+      l_out[r] = l;
+    }
+  }
+}
+
+// A key group's ring: fills tiles of K and of V in turn. Every warp of the group holds a copy and brings its share of the rows.
+template <typename T, int HSP, int RT, int STAGES>
+struct PagedRing {
+  using S = PagedShape<T, HSP, RT, STAGES>;
+  static constexpr int kTile = S::kTile;
+  static constexpr int kPerRow = HSP * (int)sizeof(T) / 16;          // 16-byte pieces of a row
+  static constexpr int kLanes = kPerRow < 32 ? kPerRow : 32;         // lanes that share a row
+  static constexpr int kAtOnce = 32 / kLanes, kWidth = kPerRow / kLanes;
+  const PagedView &c;
+  const T *k, *v;      // this head's rows of page 0
+  const uint32_t *table;
+  uint32_t base;       // shared-memory address of the ring
+  uint32_t *ok;        // [kStages] which of a tile's positions are there
+  int lowest, highest, pos, unit, lane, share, of, next;
+  uint32_t page, slot; // of this lane's position of the next tile to fill
+  long long at;        // where this lane's position of the tile at hand begins, or -1
+  bool plain;          // the tile at hand: all of its positions are there, and 16 from a multiple of 16 on share a page
+
+  __device__ __forceinline__ PagedRing(const PagedView &c_, uint32_t base_, uint32_t *ok_, int lane_, int unit_, int share_, int of_)
+      : c(c_), base(base_), ok(ok_), unit(unit_), lane(lane_), share(share_), of(of_) {}
+
+  __device__ __forceinline__ void look_up() {  // the page of this lane's position, asked for a tile ahead
+    page = 0xFFFFFFFFu;
+    slot = 0;
+    if (pos >= lowest && pos < highest) {
+      const uint32_t index = c.page_shift >= 0 ? (uint32_t)pos >> c.page_shift : (uint32_t)pos / c.page_size;
+      slot = (uint32_t)pos - index * c.page_size;
+      page = __ldcg(table + index);
+    }
+  }
+  // Begins at position `first` (a multiple of 16) of a part, with the first tiles on their way. The ring is empty.
+  __device__ __forceinline__ void begin(const PagedPart &w, int first) {
+    k = static_cast<const T *>(c.k) + w.g.kvh * c.head_stride;
+    v = static_cast<const T *>(c.v) + w.g.kvh * c.head_stride;
+    table = c.table + (size_t)w.g.s * c.table_stride;
+    lowest = w.g.lowest;
+    highest = w.g.highest;
+    pos = first + (lane & (kTile - 1));
+    next = 0;
+    if (w.n_tiles > 0) look_up();
+#pragma unroll
+    for (int h = 0; h < STAGES - 1; h++) fill((h & 1) == 0, h < 2 * w.n_tiles);
+  }
+  // Fills the next stage with a tile of keys or of values, and commits it.
+  __device__ __forceinline__ void fill(bool keys, bool any) {
+    const int stage = next;
+    next = next + 1 == S::kStages ? 0 : next + 1;
+    if (any) {
+      if (keys) {
+        at = -1;
+        if (page < c.n_pages)
+          at = (long long)page * c.page_stride + (long long)slot * c.position_stride;
+        else if (pos >= lowest && pos < highest)
+          *c.err = kErrCache;
+        const uint32_t there = __ballot_sync(0xffffffffu, at >= 0);
+        plain = c.page_size % 16 == 0 && there == 0xffffffffu;
+        if (lane == 0 && share == 0) ok[stage] = there;
+        pos += unit;
+        look_up();
+      }
+      const T *from = keys ? k : v;
+      const uint32_t to = base + stage * S::kTileBytes + lane / kLanes * S::kPitch + lane % kLanes * 16;
+      if (plain && of == 1) {  // one address per 16 positions, the others at a fixed distance
+        const long long step = (long long)kAtOnce * c.position_stride * (int)sizeof(T);
+#pragma unroll
+        for (int b = 0; b < kTile / 16; b++) {
+          const char *p = reinterpret_cast<const char *>(from + __shfl_sync(0xffffffffu, at, 16 * b) + lane / kLanes * c.position_stride) + lane % kLanes * 16;
+#pragma unroll
+          for (int i = 0; i < 16 / kAtOnce; i++) {
+#pragma unroll
+            for (int w = 0; w < kWidth; w++)
+              if ((lane % kLanes + w * 32) * 16 < c.hs * (int)sizeof(T))
+                cp_async16(to + (16 * b + i * kAtOnce) * S::kPitch + w * 512, p + w * 512);
+            p += step;
+          }
+        }
+      } else {
+#pragma unroll 2
+        for (int i = share; i < kTile / kAtOnce; i += of) {
+          const long long x = __shfl_sync(0xffffffffu, at, i * kAtOnce + lane / kLanes);
+#pragma unroll
+          for (int w = 0; w < kWidth; w++) {
+            const int piece = (lane % kLanes + w * 32) * 16;
+            if (piece < c.hs * (int)sizeof(T))
+              cp_async16_or_zero(to + i * kAtOnce * S::kPitch + w * 512, reinterpret_cast<const char *>(from + (x < 0 ? 0 : x)) + piece, x >= 0);
+          }
+        }
+      }
+    }
+    cp_async_commit();
+  }
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Two values rounded to the 16-bit type, packed, and what is left of them.
+template <typename T>
+__device__ __forceinline__ uint32_t split2(float &x, float &y) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    x -= f.x;
+    y -= f.y;
+    return *reinterpret_cast<const uint32_t *>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    const float2 f = __bfloat1622float2(h);
+    x -= f.x;
+    y -= f.y;
+    return *reinterpret_cast<const uint32_t *>(&h);
+  }
+}
+
+
+template <typename T, int HSP, int RT, int STAGES>
+__global__ void __launch_bounds__(sizeof(T) == 4 ? 128 : 32 * kPagedWarps, sizeof(T) == 4 ? (HSP <= 64 ? 3 : HSP <= 128 ? 2 : 1) : HSP <= 128 ? 2 : 1)
+paged_attention_kernel(const __grid_constant__ PagedAttention a) {
+  using S = PagedShape<T, HSP, RT, STAGES>;
+  constexpr int TERMS = S::kTerms, D = S::kStages, kTile = S::kTile;
+  constexpr int MAXROWS = S::kWide ? RT : kPagedRows;
+  // f32: a lane holds four dimensions of kQuads pieces of a row; where 16 lanes hold a row, the halves of the warp take even and odd keys
+  constexpr int kQuads = HSP <= 128 ? 1 : HSP / 128, kHalves = HSP <= 64 ? 2 : 1;
+  constexpr float kLift = std::is_same<T, __half>::value ? 14.f : 0.f;  // probabilities are held times 2^14, in the middle of a half's range
+  extern __shared__ __align__(16) unsigned char paged_smem[];
+  __shared__ float s_m[kPagedKeyGroups][MAXROWS], s_l[kPagedKeyGroups][MAXROWS], s_qscale[MAXROWS];
+  __shared__ int s_lo[MAXROWS], s_hi[MAXROWS];
+  __shared__ long long s_row[MAXROWS];
+  __shared__ uint32_t s_ok[kPagedKeyGroups][D];
+  __shared__ uint32_t s_sum[kPagedWarps];
+  __shared__ PagedPart s_part[2];
+  __shared__ int s_last, s_more;
+  __shared__ float4 s_red[32 * kPagedWarps];
+  __shared__ float s_red_sum[32 * kPagedWarps];
+  const PagedView &c = a.c;
+  const int KG = a.key_groups, RW = S::kWide ? 1 : a.row_warps, ROWS = S::kWide ? RT : a.rows, threads = blockDim.x;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hs = c.hs, unit = KG * kTile;
+  const int kg = S::kWide ? warp : warp / RW, rw = S::kWide ? 0 : warp - kg * RW;
+  unsigned char *q_smem = paged_smem, *rings = paged_smem + S::q_bytes(ROWS) + KG * S::kPBytes, *ring_smem = rings + kg * S::kRing;
+  float *p_smem = reinterpret_cast<float *>(paged_smem + S::q_bytes(ROWS)) + warp * RT * kTile;
+  const int o_at = a.ahead ? (D - 1) * S::kTileBytes : 0;  // a key group's results, in its ring
+  float *o_smem = reinterpret_cast<float *>(ring_smem + o_at);
+  auto meet = [&]() {  // the warps of a key group
+    __syncwarp();
+    if (RW > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + kg), "r"(32 * RW) : "memory");
+  };
+  pdl_launch_dependents();
+  // where 32 does not divide the head size, what lies behind a row takes part in products: zeros, times zeros of the query's
+  const bool padded = !S::kWide && (hs & 31) != 0;
+  auto clear = [&](unsigned char *from, int bytes) {
+    for (int i = rw * 32 + lane; i < bytes / 16; i += 32 * RW) reinterpret_cast<uint4 *>(from)[i] = make_uint4(0, 0, 0, 0);
+    meet();
+  };
+  if (padded) clear(ring_smem, S::kRing);
+  pdl_wait();
+
+  // ---- this CTA's units: [x0, x1)
+  PagedSeq q;
+  auto weight_of = [&](int s) -> uint32_t {
+    if (s >= c.n_seq) return 0;
+    q = paged_seq(a, s, unit);
+    return paged_work(a, q);
+  };
+  auto scan = [&](uint32_t mine, uint32_t &all) {  // sum over the threads before this one, and over all
+    uint32_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    __syncthreads();
+    if (lane == 31) s_sum[warp] = upto;
+    __syncthreads();
+    all = 0;
+    for (int w = 0; w < threads / 32; w++) {
+      if (w < warp) upto += s_sum[w];
+      all += s_sum[w];
+    }
+    return upto - mine;
+  };
+  uint32_t total = 0, mine = 0, before = 0;
+  for (int s0 = 0; s0 < c.n_seq; s0 += threads) {
+    uint32_t all;
+    mine = weight_of(s0 + tid);
+    before = total + scan(mine, all);
+    total += all;
+  }
+  const uint32_t per = max((uint32_t)a.least, (total + gridDim.x - 1) / gridDim.x);
+  const uint32_t x0 = blockIdx.x * per, x1 = min(total, x0 + per);  // the caller sees to it that neither passes 2^32
+  if (x0 >= x1) return;
+  if (c.n_seq <= threads) {
+    if (before <= x0 && x0 < before + mine) paged_part(a, s_part[0], q, tid, before, x0, x1, unit);
+  } else {
+    uint32_t sum = 0;
+    for (int s0 = 0; s0 < c.n_seq && sum <= x0; s0 += threads) {
+      uint32_t all;
+      mine = weight_of(s0 + tid);
+      before = sum + scan(mine, all);
+      if (before <= x0 && x0 < before + mine) paged_part(a, s_part[0], q, s0 + tid, before, x0, x1, unit);
+      sum += all;
+    }
+  }
+  __syncthreads();
+
+  PagedRing<T, HSP, RT, STAGES> ring(c, smem_addr(ring_smem), s_ok[kg], lane, unit, rw, RW);
+  auto start = [&](const PagedPart &w) { ring.begin(w, w.q.begin + (w.u0 * KG + kg) * kTile); };
+  start(s_part[0]);
+  for (int turn = 0;; turn ^= 1) {
+    const PagedPart &w = s_part[turn];
+    const PagedGroup &g = w.g;
+    // ---- the next part, by a thread that has no query to load first
+    if (tid == threads - 1) {
+      uint32_t x = w.next, seq_begin = w.seq_begin;
+      s_more = x < x1;
+      if (x < x1) {
+        PagedSeq nq = w.q;
+        int s = g.s;
+        while (x >= seq_begin + paged_work(a, nq)) {
+          seq_begin += paged_work(a, nq);
+          nq = paged_seq(a, ++s, unit);
+        }
+        paged_part(a, s_part[turn ^ 1], nq, s, seq_begin, x, x1, unit);
+      }
+    }
+    // ---- the queries
+    if constexpr (S::kWide) {
+      float4 *q4 = reinterpret_cast<float4 *>(q_smem);
+      for (int i = tid; i < ROWS * (HSP / 4); i += threads) {
+        const int r = i / (HSP / 4), d = i % (HSP / 4);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < g.rows && 4 * d < hs) v = __ldcg(reinterpret_cast<const float4 *>(a.q + row_offset(a, w, r, a.ld_q)) + d);
+        q4[i] = v;
+      }
+    } else {
+      for (int r = warp; r < ROWS; r += threads / 32) {
+        float v[HSP / 32], top = 0.f;
+        const float *row = r < g.rows ? a.q + row_offset(a, w, r, a.ld_q) : nullptr;
+#pragma unroll
+        for (int i = 0; i < HSP / 64; i++) {
+          const int d = 2 * lane + 64 * i;
+          const float2 f = row && d < hs ? __ldcg(reinterpret_cast<const float2 *>(row + d)) : make_float2(0.f, 0.f);
+          v[2 * i] = f.x;
+          v[2 * i + 1] = f.y;
+          top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+        int e = 0;
+        if constexpr (TERMS == 2) {  // a power of two that brings the row's largest value near 2^13
+          top = warp_max(top);
+          e = top > 0.f && top < INFINITY ? ilogbf(top) - 13 : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < HSP / 64; i++) {
+          float f0 = scalbnf(v[2 * i], -e), f1 = scalbnf(v[2 * i + 1], -e);
+#pragma unroll
+          for (int t = 0; t < TERMS; t++)
+            *reinterpret_cast<uint32_t *>(q_smem + (t * ROWS + r) * S::kQPitch + (2 * lane + 64 * i) * 2) = split2<T>(f0, f1);
+        }
+        if (lane == 0) s_qscale[r] = scalbnf(a.scale2, e);
+      }
+    }
+    if (tid < ROWS) {
+      int lo = 0, hi = 0;
+      if (tid < g.rows) row_range(a, w.q, (g.r0 + tid) / a.group, lo, hi);
+      s_lo[tid] = lo;
+      s_hi[tid] = hi;
+      if (a.scores) s_row[tid] = row_index(a, w, tid) * c.max_length;
+    }
+    __syncthreads();
+
+    const int n_tiles = w.n_tiles, inner_low = g.inner_low, inner_high = g.inner_high, g_rows = g.rows;
+    const bool more = s_more != 0;
+    int pos0 = w.q.begin + (w.u0 * KG + kg) * kTile, now = 0;  // of the tile at hand; the stage that is next to be used up
+    bool finite = true;
+    if constexpr (S::kWide) {
+      constexpr int kShare = 32 / kTile;  // lanes that share a key
+      const int key = lane % kTile, share = lane / kTile, half = lane >> 4, dim = lane & 15;
+      float m[RT], l[RT];
+      float4 o[RT][kQuads];
+#pragma unroll
+      for (int r = 0; r < RT; r++) {
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+#pragma unroll
+        for (int i = 0; i < kQuads; i++) o[r][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      for (int t = 0; t < n_tiles; t++, pos0 += unit) {
+        // ---- scores: a lane takes one key, or every other quad of its row
+        cp_async_wait<D - 2>();
+        __syncwarp();
+        ring.fill((D & 1) != 0, 2 * t + D - 1 < 2 * n_tiles);
+        const uint32_t ok = s_ok[kg][now];
+        const float4 *kt = reinterpret_cast<const float4 *>(ring_smem + now * S::kTileBytes + key * S::kPitch);
+        now = now + 1 == D ? 0 : now + 1;
+        float sc[RT];
+#pragma unroll
+        for (int r = 0; r < RT; r++) sc[r] = 0.f;
+#pragma unroll 8
+        for (int d = share; d < hs / 4; d += kShare) {
+          const float4 kv = kt[d];
+#pragma unroll
+          for (int r = 0; r < RT; r++) {
+            const float4 qv = reinterpret_cast<const float4 *>(q_smem)[r * (HSP / 4) + d];
+            sc[r] = fmaf(qv.x, kv.x, sc[r]);
+            sc[r] = fmaf(qv.y, kv.y, sc[r]);
+            sc[r] = fmaf(qv.z, kv.z, sc[r]);
+            sc[r] = fmaf(qv.w, kv.w, sc[r]);
+          }
+        }
+        const bool whole = ok == 0xffffffffu && pos0 >= inner_low && pos0 + kTile <= inner_high;
+        float f[RT];
+        bool moved = false;
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+          if (kShare == 2) sc[r] += __shfl_xor_sync(0xffffffffu, sc[r], 16);
+          sc[r] *= a.scale2;
+          if (!whole && !((ok >> key & 1u) && pos0 + key >= s_lo[r] && pos0 + key < s_hi[r])) sc[r] = -INFINITY;
+          if (a.scores && share == 0 && r < g_rows && pos0 + key >= s_lo[r] && pos0 + key < s_hi[r])
+            a.scores[s_row[r] + pos0 + key] = sc[r];
+          float top = sc[r];
+#pragma unroll
+          for (int o2 = kTile / 2; o2 > 0; o2 >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o2));
+          top = fmaxf(top, m[r]);
+          f[r] = m[r] == top ? 1.f : exp2_of(m[r] - top);
+          moved |= m[r] != top;
+          const float p = sc[r] == -INFINITY ? 0.f : exp2_of(sc[r] - top);
+          m[r] = top;
+          l[r] = l[r] * f[r] + p;
+          if (share == 0) p_smem[r * kTile + key] = p;
+        }
+        if (moved) {
+#pragma unroll
+          for (int r = 0; r < RT; r++)
+#pragma unroll
+            for (int i = 0; i < kQuads; i++) {
+              o[r][i].x *= f[r];
+              o[r][i].y *= f[r];
+              o[r][i].z *= f[r];
+              o[r][i].w *= f[r];
+            }
+        }
+        // ---- values: a lane takes four dimensions (times kQuads) of each key, or of every other one
+        cp_async_wait<D - 2>();
+        __syncwarp();
+        ring.fill((D & 1) == 0, 2 * t + D < 2 * n_tiles);
+        const unsigned char *vt = ring_smem + now * S::kTileBytes;
+        now = now + 1 == D ? 0 : now + 1;
+        const int dim4 = kHalves == 2 ? dim : lane;
+#pragma unroll
+        for (int j0 = 0; j0 < kTile; j0 += 4 * kHalves) {
+          float4 vv[4][kQuads];  // what lies behind a row's end is not read back
+#pragma unroll
+          for (int jj = 0; jj < 4; jj++)
+#pragma unroll
+            for (int i = 0; i < kQuads; i++)
+              vv[jj][i] = *reinterpret_cast<const float4 *>(vt + (j0 + (kHalves == 2 ? 4 * half : 0) + jj) * S::kPitch + (dim4 + 32 * i) * 16);
+#pragma unroll
+          for (int r = 0; r < RT; r++) {
+            const float4 p = *reinterpret_cast<const float4 *>(p_smem + r * kTile + j0 + (kHalves == 2 ? 4 * half : 0));
+            const float pj[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+            for (int jj = 0; jj < 4; jj++)
+#pragma unroll
+              for (int i = 0; i < kQuads; i++) {
+                o[r][i].x = fmaf(pj[jj], vv[jj][i].x, o[r][i].x);
+                o[r][i].y = fmaf(pj[jj], vv[jj][i].y, o[r][i].y);
+                o[r][i].z = fmaf(pj[jj], vv[jj][i].z, o[r][i].z);
+                o[r][i].w = fmaf(pj[jj], vv[jj][i].w, o[r][i].w);
+              }
+          }
+        }
+      }
+      cp_async_wait<0>();
+      __syncwarp();
+      if (more && a.ahead) start(s_part[turn ^ 1]);
+#pragma unroll
+      for (int r = 0; r < RT; r++) {
+#pragma unroll
+        for (int o2 = kTile / 2; o2 > 0; o2 >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o2);
+#pragma unroll
+        for (int i = 0; i < kQuads; i++) {
+          float4 &v = o[r][i];
+          if (kHalves == 2) {
+            v.x += __shfl_xor_sync(0xffffffffu, v.x, 16);
+            v.y += __shfl_xor_sync(0xffffffffu, v.y, 16);
+            v.z += __shfl_xor_sync(0xffffffffu, v.z, 16);
+            v.w += __shfl_xor_sync(0xffffffffu, v.w, 16);
+          }
+          const int d = (kHalves == 2 ? dim : lane) + 32 * i;
+          if (r < g_rows && 4 * d < hs) {
+            finite = finite && fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) < INFINITY;
+            if (kHalves == 1 || half == 0) *reinterpret_cast<float4 *>(o_smem + r * hs + 4 * d) = v;
+          }
+        }
+        finite = finite && (r >= g_rows || fabsf(l[r]) < INFINITY);
+        if (lane == 0) {
+          s_m[kg][r] = m[r];
+          s_l[kg][r] = l[r];
+        }
+      }
+    } else {
+      // The keys are the matrix instruction's 16 rows and the queries its 8 columns: scores come out with a lane holding two
+      // queries of keys lane / 4 and lane / 4 + 8, and the probabilities, transposed inside the warp, are the second operand
+      // of the values' product, whose rows are dimensions.
+      constexpr int KS = HSP / 16, KB = kTile / 16;  // steps of 16 dimensions, blocks of 16 positions
+      const int gr = lane >> 2, cc = lane & 3;
+      const uint32_t ring0 = smem_addr(ring_smem);
+      const uint32_t q0 = smem_addr(q_smem) + (8 * rw + (lane & 7)) * S::kQPitch + (lane >> 3) * 16;  // 32 dimensions of eight queries
+      const uint32_t k0 = ((lane & 7) + (lane & 8)) * S::kPitch + (lane >> 4) * 16;                  // a K tile's fragment
+      const uint32_t v0 = ((lane & 7) + ((lane >> 4) << 3)) * S::kPitch + (lane & 8) * 2;            // a V tile's
+      const bool active = 8 * rw < g_rows;
+      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+      const float qs[2] = {s_qscale[8 * rw + 2 * cc], s_qscale[8 * rw + 2 * cc + 1]};
+      float o[KS][4];
+#pragma unroll
+      for (int i = 0; i < KS; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+      for (int t = 0; t < n_tiles; t++, pos0 += unit) {
+        cp_async_wait<D - 2>();
+        meet();
+        ring.fill((D & 1) != 0, 2 * t + D - 1 < 2 * n_tiles);
+        uint32_t p[TERMS][KB][2];
+        float f[2];
+        if (active) {
+          const uint32_t ok = s_ok[kg][now];
+          const uint32_t kt = ring0 + now * S::kTileBytes + k0;
+          float sc[TERMS][KB][4];
+#pragma unroll
+          for (int u = 0; u < TERMS; u++)
+#pragma unroll
+            for (int b = 0; b < KB; b++) sc[u][b][0] = sc[u][b][1] = sc[u][b][2] = sc[u][b][3] = 0.f;
+#pragma unroll
+          for (int i = 0; i < KS; i += 2) {
+            if (16 * i < hs) {
+              uint32_t ka[KB][2][4];
+#pragma unroll
+              for (int b = 0; b < KB; b++) {
+                ldmatrix4(kt + b * 16 * S::kPitch + i * 32, ka[b][0]);
+                ldmatrix4(kt + b * 16 * S::kPitch + (i + 1) * 32, ka[b][1]);
+              }
+#pragma unroll
+              for (int u = 0; u < TERMS; u++) {
+                uint32_t qb[4];
+                ldmatrix4(q0 + u * ROWS * S::kQPitch + i * 32, qb);
+#pragma unroll
+                for (int b = 0; b < KB; b++) mma_16x8x16<T>(sc[u][b], ka[b][0], qb[0], qb[1]);
+#pragma unroll
+                for (int b = 0; b < KB; b++) mma_16x8x16<T>(sc[u][b], ka[b][1], qb[2], qb[3]);
+              }
+            }
+          }
+          const bool whole = ok == 0xffffffffu && pos0 >= inner_low && pos0 + kTile <= inner_high;
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const int r = 8 * rw + 2 * cc + e;
+            float x[2 * KB], top = m[e];  // of this lane's positions gr + 8 y
+#pragma unroll
+            for (int y = 0; y < 2 * KB; y++) {
+              x[y] = sc[TERMS - 1][y / 2][2 * (y & 1) + e];
+#pragma unroll
+              for (int u = TERMS - 2; u >= 0; u--) x[y] += sc[u][y / 2][2 * (y & 1) + e];
+              x[y] *= qs[e];
+            }
+            if (!whole) {
+              const int lo = s_lo[r] - pos0, hi = s_hi[r] - pos0;
+#pragma unroll
+              for (int y = 0; y < 2 * KB; y++) {
+                const int j = gr + 8 * y;
+                if (!((ok >> j & 1u) && j >= lo && j < hi)) x[y] = -INFINITY;
+              }
+            }
+            if (a.scores && r < g_rows) {
+              float *to = a.scores + s_row[r] + pos0 + gr;
+              const int lo = s_lo[r] - pos0, hi = s_hi[r] - pos0;
+#pragma unroll
+              for (int y = 0; y < 2 * KB; y++)
+                if (gr + 8 * y >= lo && gr + 8 * y < hi) to[8 * y] = x[y];
+            }
+#pragma unroll
+            for (int y = 0; y < 2 * KB; y++) top = fmaxf(top, x[y]);
+#pragma unroll
+            for (int o2 = 4; o2 < 32; o2 <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o2));
+            f[e] = m[e] == top ? 1.f : exp2_of(m[e] - top);
+            m[e] = top;
+            const float less = top - kLift;
+            float sum = 0.f;
+#pragma unroll
+            for (int y = 0; y < 2 * KB; y++) {
+              x[y] = x[y] == -INFINITY ? 0.f : exp2_of(x[y] - less);
+              sum += x[y];
+              sc[0][y / 2][2 * (y & 1) + e] = x[y];
+            }
+            l[e] = fmaf(l[e], f[e], sum);
+          }
+#pragma unroll
+          for (int b = 0; b < KB; b++)
+#pragma unroll
+            for (int u = 0; u < TERMS; u++) {
+              p[u][b][0] = transpose8x8(split2<T>(sc[0][b][0], sc[0][b][1]));
+              p[u][b][1] = transpose8x8(split2<T>(sc[0][b][2], sc[0][b][3]));
+            }
+        }
+        now = now + 1 == D ? 0 : now + 1;
+        cp_async_wait<D - 2>();
+        meet();
+        ring.fill((D & 1) == 0, 2 * t + D < 2 * n_tiles);
+        if (active) {
+          const uint32_t vt = ring0 + now * S::kTileBytes + v0;
+#pragma unroll
+          for (int i = 0; i < KS; i += 2)
+            if (16 * i < hs) {
+              uint32_t va[2][KB][4];
+#pragma unroll
+              for (int b = 0; b < KB; b++) {
+                ldmatrix4_trans(vt + b * 16 * S::kPitch + i * 32, va[0][b]);
+                ldmatrix4_trans(vt + b * 16 * S::kPitch + (i + 1) * 32, va[1][b]);
+              }
+              // a tile's values first, smallest terms ahead, then the running sums: the instruction cuts its sum off, which a
+              // long row of additions to one accumulator would show
+              float d[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+              for (int u = TERMS - 1; u >= 0; u--)
+#pragma unroll
+                for (int b = 0; b < KB; b++)
+#pragma unroll
+                  for (int y = 0; y < 2; y++) mma_16x8x16<T>(d[y], va[y][b], p[u][b][0], p[u][b][1]);
+#pragma unroll
+              for (int y = 0; y < 2; y++) {
+                o[i + y][0] = fmaf(o[i + y][0], f[0], d[y][0]);
+                o[i + y][1] = fmaf(o[i + y][1], f[1], d[y][1]);
+                o[i + y][2] = fmaf(o[i + y][2], f[0], d[y][2]);
+                o[i + y][3] = fmaf(o[i + y][3], f[1], d[y][3]);
+              }
+            }
+        }
+        now = now + 1 == D ? 0 : now + 1;
+      }
+      cp_async_wait<0>();
+      meet();
+      if (more && a.ahead) start(s_part[turn ^ 1]);
+      const float down = kLift != 0.f ? 1.f / 16384.f : 1.f;
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const int r = 8 * rw + 2 * cc + e;
+#pragma unroll
+        for (int o2 = 4; o2 < 32; o2 <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], o2);
+        if (gr == 0) {
+          s_m[kg][r] = m[e];
+          s_l[kg][r] = l[e] * down;
+        }
+        if (r < g_rows) {
+          finite = finite && fabsf(l[e]) < INFINITY;
+#pragma unroll
+          for (int i = 0; i < KS; i++)
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+              const float v = o[i][2 * y + e] * down;
+              const int d = 16 * i + gr + 8 * y;
+              if (d < hs) {
+                finite = finite && fabsf(v) < INFINITY;
+                o_smem[r * hs + d] = v;
+              }
+            }
+        }
+      }
+    }
+    if (!__all_sync(0xffffffffu, finite)) {
+      __syncwarp();
+      paged_rows_apart<T, kTile>(a, w, kg, KG, S::kWide ? 0 : 8 * rw, S::kWide ? g_rows : min(g_rows, 8 * rw + 8), lane, o_smem, s_m[kg], s_l[kg]);
+    }
+    __syncthreads();
+
+    // ---- the key groups' results, and the group's if other CTAs have a part of it
+    const int first_cta = (int)(w.begin / per), last_cta = (int)((w.end - 1) / per), parts = last_cta - first_cta + 1;
+    const int quads = hs / 4, items = g_rows * quads;
+    const int slot_floats = paged_slot(ROWS, hs);
+    float *slot = a.partial + (2ll * blockIdx.x + ((int)blockIdx.x == first_cta ? 1 : 0)) * slot_floats;
+    for (int i = tid; i < items; i += threads) {
+      const int r = i / quads, d = i - r * quads;
+      float top = s_m[0][r], sum = 0.f;
+      for (int y = 1; y < KG; y++) top = fmaxf(top, s_m[y][r]);
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int y = 0; y < KG; y++) {
+        if (s_m[y][r] == -INFINITY && s_l[y][r] == 0.f) continue;
+        const float f = exp2f(s_m[y][r] - top);
+        const float4 o = reinterpret_cast<const float4 *>(rings + y * S::kRing + o_at)[i];
+        sum += f * s_l[y][r];
+        v.x += f * o.x;
+        v.y += f * o.y;
+        v.z += f * o.z;
+        v.w += f * o.w;
+      }
+      if (parts == 1) {
+        if (sum != 0.f) {
+          const float inv = 1.f / sum;
+          v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+        }
+        reinterpret_cast<float4 *>(a.out + row_offset(a, w, r, a.ld_out))[d] = v;
+        if (a.stats && d == 0) a.stats[row_index(a, w, r)] = top + log2f(sum);
+      } else {
+        __stcg(reinterpret_cast<float4 *>(slot) + i, v);
+        if (d == 0) {
+          __stcg(slot + ROWS * hs + r, top);
+          __stcg(slot + ROWS * hs + ROWS + r, sum);
+        }
+      }
+    }
+    if (parts > 1) {
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        const unsigned int done = atomicAdd(a.join + first_cta, 1u);
+        s_last = done == (unsigned)parts - 1;
+        if (s_last) a.join[first_cta] = 0;
+      }
+      __syncthreads();
+      if (s_last) {
+        __threadfence();
+        // where a row tile has few values, several threads share a quad and take every so many parts
+        auto part_of = [&](int k) { return a.partial + (2ll * (first_cta + k) + (k == 0 ? 1 : 0)) * slot_floats; };
+        const int share = items >= threads ? 1 : threads / items;
+        for (int i0 = 0; i0 < items; i0 += threads) {
+          const int i = share > 1 ? tid % items : i0 + tid, sh = share > 1 ? tid / items : 0;
+          const bool live = i < items && sh < share;
+          const int r = live ? i / quads : 0;
+          float top = -INFINITY, sum = 0.f;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (live) {
+#pragma unroll 8
+            for (int k = 0; k < parts; k++) top = fmaxf(top, __ldcg(part_of(k) + ROWS * hs + r));
+#pragma unroll 8
+            for (int k = sh; k < parts; k += share) {
+              const float *part = part_of(k);
+              const float m = __ldcg(part + ROWS * hs + r), l = __ldcg(part + ROWS * hs + ROWS + r);
+              const float4 o = __ldcg(reinterpret_cast<const float4 *>(part) + i);
+              const float f = m == -INFINITY && l == 0.f ? 0.f : exp2f(m - top);
+              sum += f * l;
+              v.x += f * o.x;
+              v.y += f * o.y;
+              v.z += f * o.z;
+              v.w += f * o.w;
+            }
+          }
+          if (share > 1) {
+            s_red[tid] = v;
+            s_red_sum[tid] = sum;
+            __syncthreads();
+            if (tid < items)
+              for (int y = 1; y < share; y++) {
+                const float4 o = s_red[y * items + tid];
+                v.x += o.x;
+                v.y += o.y;
+                v.z += o.z;
+                v.w += o.w;
+                sum += s_red_sum[y * items + tid];
+              }
+          }
+          if (live && sh == 0) {
+            if (sum != 0.f) {
+              const float inv = 1.f / sum;
+              v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+            }
+            reinterpret_cast<float4 *>(a.out + row_offset(a, w, r, a.ld_out))[i - r * quads] = v;
+            if (a.stats && i == r * quads) a.stats[row_index(a, w, r)] = top + log2f(sum);
+          }
+        }
+      }
+    }
+    __syncthreads();
+    if (!more) break;
+    if (padded) clear(reinterpret_cast<unsigned char *>(o_smem), a.ahead ? S::kTileBytes : S::kRing);
+    if (!a.ahead) start(s_part[turn ^ 1]);
+  }
+}
+
+// weights[s][j] += sum over the sequence's rows and heads, in their order, of 2^(score - log2 of the sum).
+__global__ void __launch_bounds__(256)
+paged_weights_kernel(PagedAttention a, float *__restrict__ weights, long long ld) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const PagedView &c = a.c;
+  const int s = blockIdx.y;
+  int first, n;
+  new_rows(c, a.r, s, first, n);
+  const int L = paged_length(c, s);
+  for (int j = blockIdx.x * 256 + threadIdx.x; j < L; j += gridDim.x * 256) {
+    float w = 0.f;
+    for (int t = 0; t < n; t++) {
+      const int end = L - n + t + 1, begin = a.window > 0 ? max(0, end - a.window) : 0;
+      if (j < begin || j >= end) continue;
+      for (int h = 0; h < a.n_head; h++) {
+        const long long rh = (long long)(first + t) * a.n_head + h;
+        const float sc = __ldcg(a.scores + rh * c.max_length + j);
+        if (sc != -INFINITY) w += exp2f(sc - __ldcg(a.stats + rh));
+      }
+    }
+    weights[s * ld + j] += w;
+  }
+}
+
+}  // namespace wgpt

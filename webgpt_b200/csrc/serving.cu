@@ -2,9 +2,11 @@
 // verification of drafted tokens, behind the C ABI of include/webgpt_b200.h.
 #include <algorithm>
 #include <atomic>
+#include <cstdlib>
 
 #include "host.cuh"
 #include "paged.cuh"
+#include "paged_attention.cuh"
 #include "verify.cuh"
 
 using namespace wgpt;
@@ -71,35 +73,29 @@ WGPT_EXPORT int32_t wgpt_paged_append(wgpt_device *dev, const wgpt_paged_cache *
   return WGPT_OK;
 }
 
-// CTAs of a kernel that an SM holds, asked once per kernel and GPU.
-template <typename T, int HSP, int RT>
-static int32_t paged_ctas(wgpt_device *dev, int *out) {
-  static std::atomic<int> known[64];
-  using S = PagedShape<T, HSP, RT>;
-  REQUIRE(dev->ordinal < 64, WGPT_ERR_UNSUPPORTED, "device ordinal %d not supported", dev->ordinal);
-  int n = known[dev->ordinal].load();
-  if (n == 0) {
-    CK(allow_smem(dev, paged_attention_kernel<T, HSP, RT>, true));
-    CK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, paged_attention_kernel<T, HSP, RT>, kPagedThreads, S::kSmem));
-    REQUIRE(n >= 1, WGPT_ERR_UNSUPPORTED, "the attention kernel does not fit an SM");
-    known[dev->ordinal].store(n);
-  }
-  *out = n;
-  return WGPT_OK;
-}
-
-template <typename T, int HSP, int RT>
+template <typename T, int HSP, int RT, int STAGES>
 static int32_t launch_paged_attention(wgpt_device *dev, PagedAttention &a) {
-  using S = PagedShape<T, HSP, RT>;
-  int per_sm = 0;
-  TRY((paged_ctas<T, HSP, RT>(dev, &per_sm)));
+  using S = PagedShape<T, HSP, RT, STAGES>;
+  const auto kernel = paged_attention_kernel<T, HSP, RT, STAGES>;
+  const int threads = 32 * a.key_groups * a.row_warps, smem = S::smem(a.key_groups, a.rows), unit = a.key_groups * S::kTile;
+  // CTAs that an SM holds, asked once per shape and GPU
+  static std::atomic<int> known[64][5];
+  REQUIRE(dev->ordinal < 64, WGPT_ERR_UNSUPPORTED, "device ordinal %d not supported", dev->ordinal);
+  int per_sm = known[dev->ordinal][a.row_warps].load();
+  if (per_sm == 0) {
+    CK(allow_smem(dev, kernel, true));
+    CK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem));
+    REQUIRE(per_sm >= 1, WGPT_ERR_UNSUPPORTED, "the attention kernel does not fit an SM");
+    known[dev->ordinal][a.row_warps].store(per_sm);
+  }
   const int grid = std::min(per_sm * dev->sm_count, kJoinCounters);
-  const size_t rows = a.stats ? (size_t)a.r.n_rows * a.n_head : 0, scores = rows * (size_t)a.c.max_length;
+  REQUIRE(S::fits(a.rows, a.c.hs), WGPT_ERR_UNSUPPORTED, "%d rows of %d do not fit the ring", a.rows, a.c.hs);
   // units and rows are counted in 32 bits
   REQUIRE((int64_t)a.r.n_rows * a.group < (int64_t)1 << 30 &&
-              ((int64_t)a.r.n_rows * a.group / S::kRows + a.c.n_seq) * (a.c.max_length / S::kUnit + 2) < ((int64_t)1 << 31) / a.c.n_kv,
+              ((int64_t)a.r.n_rows * a.group / a.rows + a.c.n_seq) * (a.c.max_length / unit + 2) < (((int64_t)1 << 32) - ((int64_t)1 << 20)) / a.c.n_kv,
           WGPT_ERR_SHAPE, "%d rows over up to %d positions of %d heads: split the call", a.r.n_rows, a.c.max_length, a.c.n_kv);
-  const size_t partial = (size_t)2 * grid * paged_slot(S::kRows, a.c.hs);
+  const size_t rows = a.stats ? (size_t)a.r.n_rows * a.n_head : 0, scores = rows * (size_t)a.c.max_length;
+  const size_t partial = (size_t)2 * grid * paged_slot(a.rows, a.c.hs);
   TRY(scratch_reserve(dev, (partial + rows + scores) * 4));
   a.partial = static_cast<float *>(dev->scratch);
   if (a.stats) {
@@ -107,9 +103,10 @@ static int32_t launch_paged_attention(wgpt_device *dev, PagedAttention &a) {
     a.scores = a.stats + rows;
   }
   a.join = dev->d_join;
+  a.ahead = S::ahead(a.rows, a.c.hs);
   static const int least = getenv("LEAST") ? atoi(getenv("LEAST")) : 1;
   a.least = least;
-  LAUNCH_PDL(dev, (paged_attention_kernel<T, HSP, RT>), grid, kPagedThreads, S::kSmem, a);
+  LAUNCH_PDL(dev, kernel, grid, threads, smem, a);
   return WGPT_OK;
 }
 
@@ -117,17 +114,28 @@ static int32_t launch_paged_attention(wgpt_device *dev, PagedAttention &a) {
 // tiles read the cache again, fewer rows leave room for more keys in flight.
 template <typename T, int HSP>
 static int32_t launch_paged_rows(wgpt_device *dev, PagedAttention &a, long long rows) {
+  static const int st = getenv("STAGES") ? atoi(getenv("STAGES")) : 0;
   if constexpr (sizeof(T) == 4) {
-    if (rows <= 1) return launch_paged_attention<T, HSP, 1>(dev, a);
-    if (rows <= 2) return launch_paged_attention<T, HSP, 2>(dev, a);
-    if (rows <= 4) return launch_paged_attention<T, HSP, 4>(dev, a);
-    return launch_paged_attention<T, HSP, 8>(dev, a);
+    a.key_groups = 4;
+    a.row_warps = 1;
+    a.rows = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;
+    if (rows <= 1) {
+      if (st == 2) return launch_paged_attention<T, HSP, 1, 2>(dev, a);
+      return launch_paged_attention<T, HSP, 1, 3>(dev, a);
+    }
+    if (rows <= 2) return launch_paged_attention<T, HSP, 2, 3>(dev, a);
+    if (rows <= 4) return launch_paged_attention<T, HSP, 4, 3>(dev, a);
+    return launch_paged_attention<T, HSP, 8, 3>(dev, a);
   } else {
-    if (rows <= 8) return launch_paged_attention<T, HSP, 1>(dev, a);
-    if (rows <= 16 || HSP > 128) return launch_paged_attention<T, HSP, 2>(dev, a);
-    if constexpr (HSP <= 128) return launch_paged_attention<T, HSP, 3>(dev, a);
+    const int most = HSP <= 128 ? 4 : 3;
+    const long long eights = (rows + 7) / 8, tiles = (eights + most - 1) / most;
+    a.row_warps = (int)((eights + tiles - 1) / tiles);
+    a.key_groups = a.row_warps == 1 ? 4 : 2;
+    a.rows = 8 * a.row_warps;
+    if (st == 2) return launch_paged_attention<T, HSP, 1, 2>(dev, a);
+    if (st == 4) return launch_paged_attention<T, HSP, 1, 4>(dev, a);
+    return launch_paged_attention<T, HSP, 1, 3>(dev, a);
   }
-  return WGPT_ERR_UNSUPPORTED;
 }
 
 template <typename T>
