@@ -93,61 +93,96 @@ struct Pack4<__nv_bfloat16> {
 };
 
 // ------------------------------------------------------------------------------------------ new rows into the pages
-// A CTA takes whole rows; four values a thread and step, k and v side by side.
-constexpr int kAppendThreads = 128;
+// A warp takes a row. Three round trips to memory find its place (its sequence, that one's length, the page), so the first values
+// of k and v are asked for ahead of them.
+constexpr int kAppendThreads = 256, kAppendAhead = 6;
 
 template <typename T>
 __global__ void __launch_bounds__(kAppendThreads)
-paged_append_kernel(PagedView c, NewRows r, const float *__restrict__ k, const float *__restrict__ v, long long ld) {
+paged_append_kernel(const __grid_constant__ PagedView c, NewRows r, const float *__restrict__ k, const float *__restrict__ v, long long ld) {
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, row = blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
+  if (row >= r.n_rows) return;
   const int per_head = c.hs / 4, n4 = c.n_kv * per_head;
-  for (int row = blockIdx.x; row < r.n_rows; row += gridDim.x) {
-    const int s = sequence_of(c, r, row, lane);
-    if (s < 0) continue;
-    int first, n;
-    new_rows(c, r, s, first, n);
-    const int pos = paged_length(c, s) - n + (row - first);
-    if ((unsigned)(row - first) >= (unsigned)n || pos < 0) continue;
-    const long long at = paged_offset(c, s, pos);
-    if (at < 0) continue;
-    const float4 *k4 = reinterpret_cast<const float4 *>(k + (long long)row * ld);
-    const float4 *v4 = reinterpret_cast<const float4 *>(v + (long long)row * ld);
-    for (int i = threadIdx.x; i < n4; i += kAppendThreads) {
+  const float4 *k4 = reinterpret_cast<const float4 *>(k + (long long)row * ld);
+  const float4 *v4 = reinterpret_cast<const float4 *>(v + (long long)row * ld);
+  float4 a[kAppendAhead], b[kAppendAhead];
+  auto ask = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < kAppendAhead; u++) {
+      const int i = i0 + lane + 32 * u;
+      if (i < n4) {
+        a[u] = __ldcg(k4 + i);
+        b[u] = __ldcg(v4 + i);
+      }
+    }
+  };
+  ask(0);
+  const int s = sequence_of(c, r, row, lane);
+  if (s < 0) return;
+  int first, n;
+  new_rows(c, r, s, first, n);
+  const int pos = paged_length(c, s) - n + (row - first);
+  if ((unsigned)(row - first) >= (unsigned)n || pos < 0) return;
+  const long long at = paged_offset(c, s, pos);
+  if (at < 0) return;
+  for (int i0 = 0; i0 < n4; i0 += 32 * kAppendAhead) {
+    if (i0 > 0) ask(i0);
+#pragma unroll
+    for (int u = 0; u < kAppendAhead; u++) {
+      const int i = i0 + lane + 32 * u;
+      if (i >= n4) continue;
       const int h = i / per_head;
       const long long to = at + (long long)h * c.head_stride + (i - h * per_head) * 4;
-      const float4 a = __ldcg(k4 + i), b = __ldcg(v4 + i);
-      *reinterpret_cast<Pack4<T> *>(static_cast<T *>(c.k) + to) = Pack4<T>::of(a);
-      *reinterpret_cast<Pack4<T> *>(static_cast<T *>(c.v) + to) = Pack4<T>::of(b);
+      *reinterpret_cast<Pack4<T> *>(static_cast<T *>(c.k) + to) = Pack4<T>::of(a[u]);
+      *reinterpret_cast<Pack4<T> *>(static_cast<T *>(c.v) + to) = Pack4<T>::of(b[u]);
     }
   }
 }
 
 // ------------------------------------------------------------------------------------------ selection
-// The need-th largest of n 32-bit keys by a CTA of NT threads: digits of 11, 11 and 10 bits from the top, a histogram of each
-// digit among the keys that share the digits found so far. Returns the key, and in `ties` how many keys equal to it belong
-// to the need largest. hist: 2048 counters in shared memory, warp_sums: NT / 32, found: 3.
-template <int NT, typename Key>
-__device__ uint32_t radix_threshold(Key key, int n, int need, uint32_t *hist, uint32_t *warp_sums, uint32_t *found,
-                                    int &ties) {
+// The need-th largest of all 32-bit keys of a cluster of C CTAs (or of one) of NT threads: digits of 11, 11 and 10 bits from the
+// top, a histogram of each digit among the keys that share the digits found so far, added up over the cluster. key(u) is a
+// thread's u-th key of n, there(u) whether it has one. Returns the key, and in `ties` how many keys equal to it belong to the
+// need largest. hist: 2 * 2048 counters in shared memory at the same place in every CTA, warp_sums: NT / 32, found: 2.
+template <int NT, typename Key, typename There>
+__device__ uint32_t radix_threshold(Key key, There there, int n, int need, int C, uint32_t *hist2, uint32_t *warp_sums,
+                                    uint32_t *found, int &ties) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t prefix = 0, mask = 0, left = (uint32_t)need;
 #pragma unroll 1
   for (int pass = 0; pass < 3; pass++) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass < 2 ? 2048 : 1024;
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const uint32_t bins = pass < 2 ? 2048 : 1024;
+    uint32_t *hist = hist2 + (pass & 1) * 2048;  // a neighbour may still read the other
     for (int i = tid; i < 2048; i += NT) hist[i] = 0;
     __syncthreads();
-    for (int i = tid; i < n; i += NT) {
-      const uint32_t k = key(i);
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1u);
+#pragma unroll 4
+    for (int u = 0; u < n; u++) {
+      const uint32_t k = there(u) ? key(u) : 0u;
+      if (there(u) && (k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1u);
     }
-    __syncthreads();
-    // from the largest digit down: thread t holds 2048 / NT digits next to one another
+    if (C > 1) {
+      cluster_arrive();
+      cluster_wait();
+    } else {
+      __syncthreads();
+    }
+    // from the largest digit down: a thread holds 2048 / NT digits next to one another
     constexpr int PT = 2048 / NT;
-    uint32_t mine = 0;
+    uint32_t count[PT], mine = 0;
 #pragma unroll
-    for (int u = 0; u < PT; u++) mine += hist[2047 - (tid * PT + u)];
+    for (int u = 0; u < PT; u++) {
+      const uint32_t d = 2047 - (tid * PT + u);
+      count[u] = 0;
+      if (C == 1) {
+        count[u] = hist[d];
+      } else {
+        for (int q = 0; q < C; q++) count[u] += __float_as_uint(dsmem_ld(dsmem_addr(hist + d, q)));
+      }
+      mine += count[u];
+    }
     uint32_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -161,19 +196,17 @@ __device__ uint32_t radix_threshold(Key key, int n, int need, uint32_t *hist, ui
     if (before < left && left <= upto) {
 #pragma unroll
       for (int u = 0; u < PT; u++) {
-        const uint32_t d = 2047 - (tid * PT + u), cnt = hist[d];
-        if (before < left && left <= before + cnt) {
-          found[0] = d;
+        if (before < left && left <= before + count[u]) {
+          found[0] = 2047 - (tid * PT + u);
           found[1] = left - before;
         }
-        before += cnt;
+        before += count[u];
       }
     }
     __syncthreads();
     prefix |= found[0] << shift;
-    mask |= (uint32_t)(bins - 1) << shift;
+    mask |= (bins - 1) << shift;
     left = found[1];
-    __syncthreads();
   }
   ties = (int)left;
   return prefix;
@@ -192,65 +225,132 @@ struct PagedEvict {
 // Order-preserving bits of a weight; NaN is the largest.
 __device__ __forceinline__ uint32_t weight_key(float w) { return isnan(w) ? 0xFFFFFFFFu : value_key(w); }
 
-// One CTA per sequence: the weight that the last position to stay has, then the positions that stay, in order.
-constexpr int kEvictThreads = 1024;
+// A cluster per sequence, each CTA with a stretch of its positions: the weight that the last position to stay has, then the
+// positions that stay, in order. A thread of a stretch takes groups of four positions, 1024 groups from one of its to the next.
+constexpr int kEvictThreads = 1024, kEvictCluster = 8;
 
-__global__ void __launch_bounds__(kEvictThreads) paged_select_kernel(PagedEvict e) {
-  __shared__ uint32_t hist[2048], warp_sums[32], found[2];
+__global__ void __launch_bounds__(kEvictThreads) paged_select_kernel(const __grid_constant__ PagedEvict e) {
+  __shared__ uint32_t hist[2 * 2048], warp_sums[32], found[2];
+  __shared__ float above[kEvictCluster], equal[kEvictCluster];  // of the CTAs' stretches, as bits
+  uint32_t C;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(C));
+  const int rank = (int)cluster_ctarank(), s = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_launch_dependents();
   pdl_wait();
-  const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int L = paged_length(e.from, s), n = min(L, e.keep);
   const float *w = e.weights + (long long)s * e.ld;
   int *kept = e.kept + (long long)s * e.keep;
   float *wt = e.weights_to ? e.weights_to + (long long)s * e.ld_to : nullptr;
   const int old = L > e.keep ? L - e.recent : 0, need = e.keep - e.recent;
+  const int all = (int)C * kEvictThreads, me = rank * kEvictThreads + tid;
   int out = 0;
-  if (old > 0 && need > 0) {
+  if (old > 0 && need > 0) {  // the same for the whole cluster
+    const int share = ((old + (int)C - 1) / (int)C + 3) / 4 * 4, beg = min(old, rank * share), end = min(old, beg + share);
+    const int rounds = (end - beg + 4 * kEvictThreads - 1) / (4 * kEvictThreads);
+    auto at = [&](int u) { return beg + (u >> 2) * 4 * kEvictThreads + 4 * tid + (u & 3); };
+    auto there = [&](int u) { return at(u) < end; };
+    auto next_to = [&](int u) { return beg + u * kEvictThreads + tid; };  // where the order does not matter
     int ties;
-    const uint32_t t = radix_threshold<kEvictThreads>([&](int i) { return weight_key(__ldcg(w + i)); }, old, need, hist,
+    const uint32_t t = radix_threshold<kEvictThreads>([&](int u) { return weight_key(__ldcg(w + next_to(u))); },
+                                                      [&](int u) { return next_to(u) < end; }, 4 * rounds, need, (int)C, hist,
                                                       warp_sums, found, ties);
-    int eq0 = 0, gt0 = 0;  // equal to and above the threshold so far
-    for (int base = 0; base < old; base += kEvictThreads) {
-      const int i = base + tid;
-      const float x = i < old ? __ldcg(w + i) : 0.f;
-      const uint32_t k = i < old ? weight_key(x) : 0u;
-      const bool gt = i < old && k > t, eq = i < old && k == t;
-      const unsigned below = (1u << lane) - 1u, mg = __ballot_sync(0xffffffffu, gt), me = __ballot_sync(0xffffffffu, eq);
-      if (lane == 0) warp_sums[warp] = (uint32_t)__popc(me) << 16 | (uint32_t)__popc(mg);
-      __syncthreads();
-      uint32_t before = 0, all = 0;
-      for (int q = 0; q < 32; q++) {
-        const uint32_t x2 = warp_sums[q];
-        before += q < warp ? x2 : 0u;
-        all += x2;
+    // how many lie above the threshold and on it, in the stretches before this one
+    int gt = 0, eq = 0;
+#pragma unroll 4
+    for (int u = 0; u < 4 * rounds; u++)
+      if (next_to(u) < end) {
+        const uint32_t k = weight_key(__ldcg(w + next_to(u)));
+        gt += k > t ? 1 : 0;
+        eq += k == t ? 1 : 0;
       }
-      const int g = gt0 + (int)(before & 0xffffu) + __popc(mg & below), q = eq0 + (int)(before >> 16) + __popc(me & below);
-      if (gt || (eq && q < ties)) {
-        const int at = g + min(q, ties);
-        kept[at] = i;
-        if (wt) wt[at] = x;
-      }
-      gt0 += (int)(all & 0xffffu);
-      eq0 += (int)(all >> 16);
+    int gt0 = 0, eq0 = 0;
+    if (C > 1) {
+      gt = __reduce_add_sync(0xffffffffu, gt);
+      eq = __reduce_add_sync(0xffffffffu, eq);
       __syncthreads();
+      if (lane == 0) {
+        hist[2048 + warp] = gt;  // a neighbour may still read the first half
+        hist[2080 + warp] = eq;
+      }
+      __syncthreads();
+      if (tid < (int)C) {  // to every CTA
+        uint32_t g = 0, q = 0;
+        for (int i = 0; i < kEvictThreads / 32; i++) {
+          g += hist[2048 + i];
+          q += hist[2080 + i];
+        }
+        dsmem_st(dsmem_addr(&above[rank], tid), __uint_as_float(g));
+        dsmem_st(dsmem_addr(&equal[rank], tid), __uint_as_float(q));
+      }
+      cluster_arrive();
+      cluster_wait();
+      for (int i = 0; i < rank; i++) {
+        gt0 += (int)__float_as_uint(above[i]);
+        eq0 += (int)__float_as_uint(equal[i]);
+      }
+    }
+    for (int u0 = 0; u0 < 4 * rounds; u0 += 4) {
+      float x[4];
+      uint32_t k[4];
+      int g = 0, q = 0;
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        x[u] = there(u0 + u) ? __ldcg(w + at(u0 + u)) : 0.f;
+        k[u] = weight_key(x[u]);
+        g += there(u0 + u) && k[u] > t ? 1 : 0;
+        q += there(u0 + u) && k[u] == t ? 1 : 0;
+      }
+      uint32_t mine = (uint32_t)q << 16 | (uint32_t)g, upto = mine, sum = 0;  // 4096 positions: both fit 16 bits
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+      }
+      __syncthreads();
+      if (lane == 31) warp_sums[warp] = upto;
+      __syncthreads();
+      upto -= mine;
+      const uint32_t ws = warp_sums[lane];
+      upto += __reduce_add_sync(0xffffffffu, lane < warp ? ws : 0u);
+      sum = __reduce_add_sync(0xffffffffu, ws);
+      int gi = gt0 + (int)(upto & 0xffffu), qi = eq0 + (int)(upto >> 16);
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        if (!there(u0 + u)) continue;
+        const bool is_gt = k[u] > t, is_eq = k[u] == t;
+        if (is_gt || (is_eq && qi < ties)) {
+          const int to = gi + min(qi, ties);
+          kept[to] = at(u0 + u);
+          if (wt) wt[to] = x[u];
+        }
+        gi += is_gt ? 1 : 0;
+        qi += is_eq ? 1 : 0;
+      }
+      gt0 += (int)(sum & 0xffffu);
+      eq0 += (int)(sum >> 16);
     }
     out = need;
   }
-  for (int i = out + tid; i < n; i += kEvictThreads) {
+  for (int i = out + me; i < n; i += all) {
     const int from = L - n + i;  // the newest, or all of a sequence that stays whole
     kept[i] = from;
     if (wt) wt[i] = __ldcg(w + from);
   }
-  for (int i = n + tid; i < e.keep; i += kEvictThreads) {
+  for (int i = n + me; i < e.keep; i += all) {
     kept[i] = -1;
     if (wt) wt[i] = 0.f;
   }
-  if (tid == 0) e.to.lengths[s] = n;
+  if (C > 1) {  // shared memory stays until the others have read it; lengths may be one array
+    cluster_arrive();
+    cluster_wait();
+  } else {
+    __syncthreads();
+  }
+  if (me == 0) e.to.lengths[s] = n;
 }
 
 // Copies what stays. A warp takes a position: its rows of all heads in both pools, 16 bytes a lane.
-__global__ void __launch_bounds__(256) paged_gather_kernel(PagedEvict e, int elem) {
+__global__ void __launch_bounds__(256) paged_gather_kernel(const __grid_constant__ PagedEvict e, int elem) {
   pdl_launch_dependents();
   pdl_wait();
   const int s = blockIdx.y, lane = threadIdx.x & 31, n = min(paged_length(e.from, s), e.keep);

@@ -63,7 +63,7 @@ WGPT_EXPORT int32_t wgpt_paged_append(wgpt_device *dev, const wgpt_paged_cache *
   TRY(check_rows(cache, n_rows, starts, &r));
   TRY(check_matrix(k, ld, (int64_t)c.n_kv * c.hs, "k"));
   TRY(check_matrix(v, ld, (int64_t)c.n_kv * c.hs, "v"));
-  const int grid = std::min(n_rows, dev->sm_count * 16);
+  const int grid = (n_rows + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
   if (cache->type == WGPT_TYPE_F32)
     LAUNCH_PDL(dev, paged_append_kernel<float>, grid, kAppendThreads, 0, c, r, k, v, (long long)ld);
   else if (cache->type == WGPT_TYPE_F16)
@@ -104,8 +104,7 @@ static int32_t launch_paged_attention(wgpt_device *dev, PagedAttention &a) {
   }
   a.join = dev->d_join;
   a.ahead = S::ahead(a.rows, a.c.hs);
-  static const int least = getenv("LEAST") ? atoi(getenv("LEAST")) : 1;
-  a.least = least;
+  a.least = 2;
   LAUNCH_PDL(dev, kernel, grid, threads, smem, a);
   return WGPT_OK;
 }
@@ -114,15 +113,11 @@ static int32_t launch_paged_attention(wgpt_device *dev, PagedAttention &a) {
 // tiles read the cache again, fewer rows leave room for more keys in flight.
 template <typename T, int HSP>
 static int32_t launch_paged_rows(wgpt_device *dev, PagedAttention &a, long long rows) {
-  static const int st = getenv("STAGES") ? atoi(getenv("STAGES")) : 0;
   if constexpr (sizeof(T) == 4) {
     a.key_groups = 4;
     a.row_warps = 1;
     a.rows = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;
-    if (rows <= 1) {
-      if (st == 2) return launch_paged_attention<T, HSP, 1, 2>(dev, a);
-      return launch_paged_attention<T, HSP, 1, 3>(dev, a);
-    }
+    if (rows <= 1) return launch_paged_attention<T, HSP, 1, HSP <= 64 ? 2 : 3>(dev, a);
     if (rows <= 2) return launch_paged_attention<T, HSP, 2, 3>(dev, a);
     if (rows <= 4) return launch_paged_attention<T, HSP, 4, 3>(dev, a);
     return launch_paged_attention<T, HSP, 8, 3>(dev, a);
@@ -132,8 +127,7 @@ static int32_t launch_paged_rows(wgpt_device *dev, PagedAttention &a, long long 
     a.row_warps = (int)((eights + tiles - 1) / tiles);
     a.key_groups = a.row_warps == 1 ? 4 : 2;
     a.rows = 8 * a.row_warps;
-    if (st == 2) return launch_paged_attention<T, HSP, 1, 2>(dev, a);
-    if (st == 4) return launch_paged_attention<T, HSP, 1, 4>(dev, a);
+    if (HSP == 128 && a.row_warps == 1) return launch_paged_attention<T, HSP, 1, 2>(dev, a);
     return launch_paged_attention<T, HSP, 1, 3>(dev, a);
   }
 }
@@ -211,7 +205,10 @@ WGPT_EXPORT int32_t wgpt_paged_evict(wgpt_device *dev, const wgpt_paged_cache *f
   e.kept = kept;
   e.ld = ld_weights;
   e.ld_to = ld_weights_to;
-  LAUNCH_PDL(dev, paged_select_kernel, from->n_seq, kEvictThreads, 0, e);
+  // a stretch of up to 4096 positions is one round of a CTA: below that a cluster has nothing to share
+  const int cluster = from->max_length > 4 * kEvictThreads ? kEvictCluster : 1;
+  CK(launch_ex_x(dev->pdl, cluster, dev->stream, paged_select_kernel, dim3(cluster * from->n_seq), dim3(kEvictThreads), 0, e));
+  dev->launches++;
   const int most = std::min(keep, from->max_length);
   const int blocks = std::min((most + 7) / 8, std::max(1, 8 * dev->sm_count / from->n_seq));
   LAUNCH_PDL(dev, paged_gather_kernel, dim3(blocks, from->n_seq), dim3(256), 0, e, type_bytes(from->type));
@@ -254,13 +251,23 @@ WGPT_EXPORT int32_t wgpt_verify_drafts(wgpt_device *dev, int32_t n_seq, int32_t 
     TRY(scratch_reserve(dev, places * top_k * 8));
     a.list_value = static_cast<float *>(dev->scratch);
     a.list_id = reinterpret_cast<int *>(a.list_value + places * top_k);
-    LAUNCH_PDL(dev, verify_list_kernel, dim3(rows, n_seq), dim3(kListThreads), 0, a);
+    const int cap = top_k * ((V + kListThreads - 1) / kListThreads);
+    REQUIRE(cap * sizeof(unsigned long long) <= size_t(200) << 10, WGPT_ERR_SHAPE,
+            "top_k %d with a vocabulary of %d needs %zu bytes of shared memory for the candidate list", top_k, V,
+            cap * sizeof(unsigned long long));
+    CK(allow_smem(dev, verify_list_kernel));
+    LAUNCH_PDL(dev, verify_list_kernel, dim3(rows, n_seq), dim3(kListThreads), cap * sizeof(unsigned long long), a, cap);
     LAUNCH_PDL(dev, verify_draw_list_kernel, n_seq, 128, 0, a);
     return WGPT_OK;
   }
   TRY(scratch_reserve(dev, places * a.chunks * sizeof(float2)));
   a.partial = static_cast<float2 *>(dev->scratch);
   LAUNCH_PDL(dev, verify_sums_kernel, dim3(a.chunks, rows, n_seq), dim3(kVerifyThreads), 0, a);
-  LAUNCH_PDL(dev, verify_draw_kernel, n_seq, kDrawThreads, 0, a);
+  const dim3 grid(kDrawCluster * n_seq), block(kDrawThreads);
+  if (V <= 16 * 32 * kDrawWarps * kDrawCluster)
+    CK(launch_ex_x(dev->pdl, kDrawCluster, dev->stream, verify_draw_kernel<16>, grid, block, 0, a));
+  else
+    CK(launch_ex_x(dev->pdl, kDrawCluster, dev->stream, verify_draw_kernel<0>, grid, block, 0, a));
+  dev->launches++;
   return WGPT_OK;
 }

@@ -9,6 +9,7 @@ namespace wgpt {
 constexpr int kErrRow = 6;     // the error word's value for a row of logits without a distribution
 constexpr int kErrDrafts = 7;  // for a number of drafts out of range
 constexpr uint32_t kNoId = 0xFFFFFFFFu;
+constexpr int kMaxDraft = 64;
 
 struct Verify {
   int n_seq, n_draft, V, top_k, chunks;
@@ -53,86 +54,137 @@ __device__ __forceinline__ double warp_sum64(double v) {
   return v;
 }
 
-// The largest value of each chunk of a row and the sum of exp((x - largest) / temperature) over it.
-constexpr int kVerifyChunk = 8192, kVerifyThreads = 256;
+// The largest value of each chunk of a row and the sum of exp((x - largest) / temperature) over it; a chunk is in registers
+// between the two. Decides whether drafts are accepted: each exponential is good to 2^-22, their sum to a few 1e-8.
+constexpr int kVerifyThreads = 256, kVerifyVals = 16, kVerifyChunk = kVerifyThreads * kVerifyVals;
 
-__global__ void __launch_bounds__(kVerifyThreads) verify_sums_kernel(Verify a) {
-  __shared__ float red[2][kVerifyThreads / 32];
+__global__ void __launch_bounds__(kVerifyThreads) verify_sums_kernel(const __grid_constant__ Verify a) {
+  __shared__ float red[kVerifyThreads / 32];
+  __shared__ double red64[kVerifyThreads / 32];
   pdl_launch_dependents();
   pdl_wait();
-  const int s = blockIdx.z, r = blockIdx.y, tid = threadIdx.x;
+  const int s = blockIdx.z, r = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int beg = blockIdx.x * kVerifyChunk;
   if (!row_wanted(a, r, drafted(a, s))) return;
-  const float *x = logits_row(a, s, r);
-  const int beg = blockIdx.x * kVerifyChunk, end = min(a.V, beg + kVerifyChunk);
-  float m = -INFINITY;
-  for (int i = beg + tid; i < end; i += kVerifyThreads) m = fmaxf(m, logit(x + i));
+  const float *x = logits_row(a, s, r) + beg;
+  const int n = min(a.V - beg, kVerifyChunk);
+  float v[kVerifyVals], m = -INFINITY;
+#pragma unroll
+  for (int u = 0; u < kVerifyVals; u++) v[u] = tid + u * kVerifyThreads < n ? __ldcg(x + tid + u * kVerifyThreads) : -INFINITY;
+#pragma unroll
+  for (int u = 0; u < kVerifyVals; u++) m = fmaxf(m, v[u]);  // NaN is passed over
   m = warp_max(m);
-  if ((tid & 31) == 0) red[0][tid >> 5] = m;
+  if (lane == 0) red[warp] = m;
   __syncthreads();
-  for (int w = 0; w < kVerifyThreads / 32; w++) m = fmaxf(m, red[0][w]);
-  const float inv = (float)(1.0 / a.temperature);
+#pragma unroll
+  for (int w = 0; w < kVerifyThreads / 32; w++) m = fmaxf(m, red[w]);
+  const float c = (float)(1.4426950408889634 / a.temperature);
   float sum = 0.f;
-  if (m > -INFINITY)
-    for (int i = beg + tid; i < end; i += kVerifyThreads) sum += expf((logit(x + i) - m) * inv);
-  sum = warp_sum(sum);
-  if ((tid & 31) == 0) red[1][tid >> 5] = sum;
+#pragma unroll
+  for (int u = 0; u < kVerifyVals; u++) {
+    const float e = exp2f((v[u] - m) * c);
+    sum += v[u] > -INFINITY ? e : 0.f;
+  }
+  double sum64 = warp_sum64((double)sum);
+  if (lane == 0) red64[warp] = sum64;
   __syncthreads();
   if (tid == 0) {
-    sum = 0.f;
-    for (int w = 0; w < kVerifyThreads / 32; w++) sum += red[1][w];
-    a.partial[((long long)s * (2 * a.n_draft + 1) + r) * a.chunks + blockIdx.x] = make_float2(m, sum);
+    sum64 = 0.0;
+    for (int w = 0; w < kVerifyThreads / 32; w++) sum64 += red64[w];
+    a.partial[((long long)s * (2 * a.n_draft + 1) + r) * a.chunks + blockIdx.x] = make_float2(m, (float)sum64);
   }
 }
 
-// top_k > 0: the kept logits of a row in descending order, by one CTA.
+// e^(x / temperature) of x <= 0 in double precision, to about 1e-15: x / temperature = (64 n + j + f) ln 2 / 64 with |f| <= 1/2, so
+// that it is 2^n 2^(j/64) e^(f ln 2 / 64), the second from a table and the third by its series (table-driven exponentials, Tang 1989).
+// scale: 64 / (ln 2 temperature).
+__device__ __forceinline__ double exp_of(double x, double scale, const double *table) {
+  const double t = x * scale;
+  const double shifted = t + 6755399441055744.0;  // 1.5 * 2^52: the integer nearest to t in the low word
+  const int n = __double2loint(shifted);
+  const double f = t - (shifted - 6755399441055744.0);
+  constexpr double z = 0.010830424696249145;  // ln 2 / 64
+  double p = fma(f, z * z * z * z * z / 120.0, z * z * z * z / 24.0);
+  p = fma(p, f, z * z * z / 6.0);
+  p = fma(p, f, z * z / 2.0);
+  p = fma(p, f, z);
+  p = fma(p, f, 1.0);
+  const double y = table[n & 63] * p;
+  return t < -65000.0 ? 0.0 : __hiloint2double(__double2hiint(y) + ((n >> 6) << 20), __double2loint(y));  // 2^-1015 and below: 0
+}
+
+// top_k > 0: the kept logits of a row in descending order, by one CTA. Each thread's largest key (of the value, among equals of the
+// lowest index) is a candidate for the bound: the top_k-th largest of them is a key that at least top_k keys reach, all of them in
+// the top_k threads that hold one. Those read their share again; what reaches the bound is ranked by counting.
 constexpr int kListThreads = 1024;
 
-__global__ void __launch_bounds__(kListThreads) verify_list_kernel(Verify a) {
-  __shared__ uint32_t hist[2048], warp_sums[32], found[2], count[2];
-  __shared__ unsigned long long kept[128];
+__global__ void __launch_bounds__(kListThreads) verify_list_kernel(const __grid_constant__ Verify a, int cap) {
+  extern __shared__ __align__(16) unsigned long long cand[];  // [cap], cap = top_k * ceil(V / kListThreads)
+  __shared__ int count;
   pdl_launch_dependents();
   pdl_wait();
   const int s = blockIdx.y, r = blockIdx.x, tid = threadIdx.x;
   if (!row_wanted(a, r, drafted(a, s))) return;
   const float *x = logits_row(a, s, r);
-  int ties;
-  const uint32_t t = radix_threshold<kListThreads>([&](int i) { return value_key(logit(x + i)); }, a.V, a.top_k, hist,
-                                                   warp_sums, found, ties);
-  if (tid < 2) count[tid] = 0;
-  __syncthreads();
-  for (int i = tid; i < a.V; i += kListThreads) {
-    const float v = logit(x + i);
-    if (value_key(v) > t) kept[atomicAdd(&count[0], 1u)] = sample_key(v, i);
-  }
-  __syncthreads();
-  // of the values at the threshold, the lowest indices
-  const int above = a.top_k - ties, lane = tid & 31, warp = tid >> 5;
-  int eq0 = 0;
-  for (int base = 0; base < a.V && eq0 < ties; base += kListThreads) {
-    const int i = base + tid;
-    const float v = i < a.V ? logit(x + i) : 0.f;
-    const bool eq = i < a.V && value_key(v) == t;
-    const unsigned me = __ballot_sync(0xffffffffu, eq);
-    if (lane == 0) warp_sums[warp] = __popc(me);
-    __syncthreads();
-    int before = eq0, all = 0;
-    for (int q = 0; q < 32; q++) {
-      before += q < warp ? (int)warp_sums[q] : 0;
-      all += (int)warp_sums[q];
+  unsigned long long best = 0ull;
+  for (int i0 = 0; i0 < a.V; i0 += 16 * kListThreads) {
+    float v[16];
+#pragma unroll
+    for (int u = 0; u < 16; u++) {
+      const int i = i0 + tid + u * kListThreads;
+      v[u] = i < a.V ? logit(x + i) : 0.f;
     }
-    before += __popc(me & ((1u << lane) - 1u));
-    if (eq && before < ties) kept[above + before] = sample_key(v, i);
-    eq0 += all;
-    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 16; u++) {
+      const int i = i0 + tid + u * kListThreads;
+      const unsigned long long k = i < a.V ? sample_key(v[u], i) : 0ull;
+      best = k > best ? k : best;
+    }
+  }
+  if (tid == 0) count = 0;
+  // the bound, bit by bit: the value's, and where several threads have that value, the index's
+  const int holders = min(a.V, kListThreads);
+  unsigned long long bound = 1ull;
+  if (holders > a.top_k) {
+    bound = 0ull;
+    for (int bit = 63; bit >= 32; bit--) {
+      const unsigned long long trial = bound | 1ull << bit;
+      if (__syncthreads_count(best >= trial) >= a.top_k) bound = trial;
+    }
+    if (__syncthreads_count(best >= bound) > a.top_k)
+      for (int bit = 31; bit >= 0; bit--) {
+        const unsigned long long trial = bound | 1ull << bit;
+        if (__syncthreads_count(best >= trial) >= a.top_k) bound = trial;
+      }
   }
   __syncthreads();
-  if (tid < a.top_k) {
-    const unsigned long long mine = kept[tid];
+  if (best >= bound)
+    for (int i0 = tid; i0 < a.V; i0 += 16 * kListThreads) {
+      float v[16];
+#pragma unroll
+      for (int u = 0; u < 16; u++) v[u] = i0 + u * kListThreads < a.V ? logit(x + i0 + u * kListThreads) : 0.f;
+#pragma unroll
+      for (int u = 0; u < 16; u++) {
+        const int i = i0 + u * kListThreads;
+        if (i >= a.V) continue;
+        const unsigned long long k = sample_key(v[u], i);
+        if (k >= bound) {
+          const int at = atomicAdd(&count, 1);
+          if (at < cap) cand[at] = k;
+        }
+      }
+    }
+  __syncthreads();
+  const int n = min(count, cap);
+  const long long to = ((long long)s * (2 * a.n_draft + 1) + r) * a.top_k;
+  for (int i = tid; i < n; i += kListThreads) {
+    const unsigned long long mine = cand[i];
     int rank = 0;
-    for (int j = 0; j < a.top_k; j++) rank += kept[j] > mine ? 1 : 0;
-    const long long at = ((long long)s * (2 * a.n_draft + 1) + r) * a.top_k + rank;
-    a.list_value[at] = sample_key_value(mine);
-    a.list_id[at] = sample_key_index(mine);
+    for (int j = 0; j < n; j++) rank += cand[j] > mine ? 1 : 0;
+    if (rank < a.top_k) {
+      a.list_value[to + rank] = sample_key_value(mine);
+      a.list_id[to + rank] = sample_key_index(mine);
+    }
   }
 }
 
@@ -144,146 +196,196 @@ __device__ __forceinline__ void write_ids(const Verify &a, int s, int accepted, 
   if (threadIdx.x == 0) a.n_accepted[s] = accepted;
 }
 
-// The accept step and the draw over the whole vocabulary, one CTA per sequence.
-constexpr int kDrawThreads = 1024;
+// The accept step and the draw over the whole vocabulary, a cluster of CTAs per sequence. The draw needs running sums good to
+// far below the smallest probability, so its exponentials are in double precision: those of the target's row, and of the draft's if a
+// draft was not accepted. Every warp takes a stretch of ids; the sums of the stretches say in which one the running sum passes the
+// number, and that warp adds its stretch up id by id. A lane keeps its exponentials where they fit kVals registers.
+constexpr int kDrawThreads = 512, kDrawWarps = kDrawThreads / 32, kDrawCluster = 8;
 
-__global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(Verify a) {
+template <int kVals>
+__global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const __grid_constant__ Verify a) {
   __shared__ int first_rejected, hit;
-  __shared__ double red[32], red2[32];
+  __shared__ float s_max[2 * kMaxDraft + 1];
+  __shared__ double s_sum[2 * kMaxDraft + 1];
+  __shared__ double table[64];
+  __shared__ double sums[3][kDrawCluster][kDrawWarps];  // of every warp of the cluster: the target's, the draft's, what is drawn from
+  uint32_t C;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(C));
+  const int rank = (int)cluster_ctarank(), s = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  cluster_arrive_relaxed();
+  if (tid < 64) table[tid] = exp2(tid / 64.0);
   pdl_launch_dependents();
   pdl_wait();
-  const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int n = drafted(a, s);
+  const int n = drafted(a, s), rows = 2 * a.n_draft + 1;
   if (tid == 0) {
     first_rejected = n;
     hit = a.V;
   }
-  __syncthreads();
-  const float2 *part = a.partial + (long long)s * (2 * a.n_draft + 1) * a.chunks;
-  // (largest, sum) of a row, by a warp
-  auto row_stats = [&](int r, float &m, double &z) {
-    m = -INFINITY;
+  // every CTA finds the first draft that is not accepted: (largest, sum) of the rows, a warp each
+  const float2 *part = a.partial + (long long)s * rows * a.chunks;
+  for (int r = warp; r < rows; r += kDrawWarps) {
+    if (!row_wanted(a, r, n) || (r > a.n_draft && !a.draft)) continue;
+    float m = -INFINITY;
     for (int c = lane; c < a.chunks; c += 32) m = fmaxf(m, __ldcg(part + r * a.chunks + c).x);
     m = warp_max(m);
-    z = 0.0;
+    double z = 0.0;
     for (int c = lane; c < a.chunks; c += 32) {
       const float2 p = __ldcg(part + r * a.chunks + c);
       if (p.x > -INFINITY) z += (double)p.y * exp(((double)p.x - (double)m) / a.temperature);
     }
     z = warp_sum64(z);
-  };
-  for (int i = warp; i < n; i += kDrawThreads / 32) {
-    float m, mq = 0.f;
-    double z, zq = 1.0;
-    row_stats(i, m, z);
-    if (a.draft) row_stats(a.n_draft + 1 + i, mq, zq);
     if (lane == 0) {
-      const uint32_t x = __ldcg(a.draft_ids + (long long)s * a.n_draft + i);
-      bool ok = false;
-      if (x >= (uint32_t)a.V) {
-        *a.err = 1;
-      } else if (!isinf(m) && !isinf(mq)) {
-        const double p = exp(((double)logit(logits_row(a, s, i) + x) - (double)m) / a.temperature) / z;
-        const double q = a.draft ? exp(((double)logit(logits_row(a, s, a.n_draft + 1 + i) + x) - (double)mq) / a.temperature) / zq : 1.0;
-        ok = __ldcg(a.uniforms + (long long)s * (a.n_draft + 1) + i) * q < p;
-      }
-      if (!ok) atomicMin(&first_rejected, i);
+      s_max[r] = m;
+      s_sum[r] = z;
     }
+  }
+  __syncthreads();
+  if (tid < n) {
+    const int i = tid, rq = a.n_draft + 1 + i;
+    const uint32_t x = __ldcg(a.draft_ids + (long long)s * a.n_draft + i);
+    bool ok = false;
+    if (x >= (uint32_t)a.V) {
+      *a.err = 1;
+    } else if (!isinf(s_max[i]) && !(a.draft && isinf(s_max[rq]))) {
+      const double p = exp(((double)logit(logits_row(a, s, i) + x) - (double)s_max[i]) / a.temperature) / s_sum[i];
+      const double q = a.draft ? exp(((double)logit(logits_row(a, s, rq) + x) - (double)s_max[rq]) / a.temperature) / s_sum[rq] : 1.0;
+      ok = __ldcg(a.uniforms + (long long)s * (a.n_draft + 1) + i) * q < p;
+    }
+    if (!ok) atomicMin(&first_rejected, i);
   }
   __syncthreads();
   const int at = first_rejected;
   const float *x = logits_row(a, s, at), *y = nullptr;
-  float m, mq = 0.f;
-  double z, zq;
-  row_stats(at, m, z);
+  const double m = s_max[at], scale = 64.0 / (0.6931471805599453 * a.temperature);
+  double mq = 0.0;
   uint32_t only = kNoId;
   bool rest = at < n;
-  if (rest) {
-    if (a.draft) {
-      y = logits_row(a, s, a.n_draft + 1 + at);
-      row_stats(a.n_draft + 1 + at, mq, zq);
-      if (isinf(mq)) {
-        if (tid == 0) *a.err = kErrRow;
-        rest = false;
-      }
-    } else {
-      only = __ldcg(a.draft_ids + (long long)s * a.n_draft + at);
+  if (rest && a.draft) {
+    y = logits_row(a, s, a.n_draft + 1 + at);
+    mq = s_max[a.n_draft + 1 + at];
+    if (isinf(mq)) {
+      if (tid == 0) *a.err = kErrRow;
+      rest = false;
     }
+  } else if (rest) {
+    only = __ldcg(a.draft_ids + (long long)s * a.n_draft + at);
   }
-  if (isinf(m)) {
-    if (tid == 0) *a.err = kErrRow;
-    write_ids(a, s, at, 0u);
-    return;
-  }
-  auto block_sum = [&](double v, double *buf) {
+  const bool none = isinf(m);
+  const int stretch = (a.V + (int)C * kDrawWarps - 1) / ((int)C * kDrawWarps);
+  const int beg = min(a.V, (rank * kDrawWarps + warp) * stretch), end = min(a.V, beg + stretch);
+  auto ex = [&](int i) { return exp_of((double)logit(x + i) - m, scale, table); };
+  auto ey = [&](int i) { return exp_of((double)logit(y + i) - mq, scale, table); };
+  const bool two = rest && y != nullptr;
+  double vx[kVals > 0 ? kVals : 1], vy[kVals > 0 ? kVals : 1];
+  // a sum of every warp to every CTA, behind one barrier of the cluster
+  auto tell = [&](int which, double v) {
     v = warp_sum64(v);
-    if (lane == 0) buf[warp] = v;
-    __syncthreads();
-    v = 0.0;
-    for (int w = 0; w < 32; w++) v += buf[w];
+    if (lane < (int)C) dsmem_st64(dsmem_addr(&sums[which][rank][warp], lane), (unsigned long long)__double_as_longlong(v));
+  };
+  auto total_of = [&](int which) {
+    double v = 0.0;
+    for (int q = 0; q < (int)C; q++)
+      for (int w = 0; w < kDrawWarps; w++) v += sums[which][q][w];
     return v;
   };
-  auto e = [&](const float *row, float top, int i) { return exp(((double)logit(row + i) - (double)top) / a.temperature); };
-  // a warp takes V / 32 ids next to one another
-  const int share = (a.V + 31) / 32, beg = min(a.V, warp * share), end = min(a.V, beg + share);
-  double sx = 0.0, sy = 0.0;
-  for (int i = beg + lane; i < end; i += 32) {
-    sx += e(x, m, i);
-    if (rest && y) sy += e(y, mq, i);
-  }
-  z = block_sum(sx, red);
-  zq = block_sum(sy, red2);
-  __syncthreads();
-  const double u = __ldcg(a.uniforms + (long long)s * (a.n_draft + 1) + a.n_draft);
-  for (int attempt = 0; attempt < 2; attempt++) {
-    auto weight = [&](int i) {
-      const double p = e(x, m, i) / z;
-      if (!rest) return p;
-      const double q = y ? e(y, mq, i) / zq : (uint32_t)i == only ? 1.0 : 0.0;
-      return p > q ? p - q : 0.0;
-    };
-    double mine = 0.0;
-    for (int i = beg + lane; i < end; i += 32) mine += weight(i);
-    const double total = block_sum(mine, red);
-    if (total > 0.0) {
-      double before = 0.0;
-      for (int w = 0; w < warp; w++) before += red[w];
-      const double goal = u * total;
-      // only the warp in whose share the running sum passes the goal, and the last one with anything in it
-      if (before + red[warp] > goal && before <= goal) {
-        int last = -1;  // the share's sum was rounded in another order: it may pass the goal where the running sum does not
-        bool found = false;
-        for (int i0 = beg; i0 < end; i0 += 32) {
-          const int i = i0 + lane;
-          double w = i < end ? weight(i) : 0.0, run = w;
+  cluster_wait();  // the others run
+  double zx = 1.0, zq = 1.0;
+  if (!none) {
+    double sx = 0.0, sy = 0.0;
+    if constexpr (kVals > 0) {
 #pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const double up = __shfl_up_sync(0xffffffffu, run, o);
-            if (lane >= o) run += up;
-          }
-          const unsigned past = __ballot_sync(0xffffffffu, i < end && before + run > goal);
-          if (past) {
-            if (lane == 0) atomicMin(&hit, i0 + __ffs(past) - 1);
-            found = true;
-            break;
-          }
-          const unsigned some = __ballot_sync(0xffffffffu, w > 0.0);
-          if (some) last = i0 + 31 - __clz(some);
-          before += __shfl_sync(0xffffffffu, run, 31);
-        }
-        if (!found && last >= 0 && lane == 0) atomicMin(&hit, last);
+      for (int u = 0; u < kVals; u++) {
+        const int i = beg + lane + 32 * u;
+        vx[u] = i < end ? ex(i) : 0.0;
+        vy[u] = two && i < end ? ey(i) : 0.0;
+        sx += vx[u];
+        sy += vy[u];
       }
-      break;
+    } else {
+      for (int i = beg + lane; i < end; i += 32) {
+        sx += ex(i);
+        if (two) sy += ey(i);
+      }
     }
-    rest = false;
-    __syncthreads();
+    tell(0, sx);
+    if (two) tell(1, sy);
   }
-  __syncthreads();
-  write_ids(a, s, at, (uint32_t)min(hit, a.V - 1));
+  cluster_arrive();
+  cluster_wait();
+  const double u01 = __ldcg(a.uniforms + (long long)s * (a.n_draft + 1) + a.n_draft);
+  int which = 0;
+  if (!none) {
+    zx = total_of(0);
+    if (two) zq = total_of(1);
+  }
+  const double ix = 1.0 / zx, iq = 1.0 / zq;
+  // what an id counts: e / sum, less the draft's (or less all of it at the drafted id), none below zero
+  auto weight = [&](double e, double f, int i) {
+    const double p = e * ix, q = two ? f * iq : (uint32_t)i == only ? 1.0 : 0.0;
+    return rest ? fmax(p - q, 0.0) : e;
+  };
+  if (rest && !none) {
+    double sr = 0.0;
+    if constexpr (kVals > 0) {
+#pragma unroll
+      for (int u = 0; u < kVals; u++) {
+        const int i = beg + lane + 32 * u;
+        if (i < end) sr += weight(vx[u], vy[u], i);
+      }
+    } else {
+      for (int i = beg + lane; i < end; i += 32) sr += weight(ex(i), two ? ey(i) : 0.0, i);
+    }
+    tell(2, sr);
+  }
+  cluster_arrive();
+  cluster_wait();
+  double total = zx;
+  if (rest && !none) {
+    total = total_of(2);
+    which = 2;
+    if (!(total > 0.0)) {  // nothing is left: drawn from the target's row itself
+      rest = false;
+      total = zx;
+      which = 0;
+    }
+  }
+  if (!none) {
+    const double goal = u01 * total;
+    double before = 0.0;
+    for (int q = 0; q < rank; q++)
+      for (int w = 0; w < kDrawWarps; w++) before += sums[which][q][w];
+    for (int w = 0; w < warp; w++) before += sums[which][rank][w];
+    // the warp in whose stretch the running sum passes the goal; its id goes to the first CTA
+    if (before + sums[which][rank][warp] > goal && before <= goal) {
+      int last = -1, found = -1;  // the stretch's sum was rounded in another order: it may pass the goal where the running sum does not
+      for (int i0 = beg; i0 < end && found < 0; i0 += 32) {
+        const int i = i0 + lane;
+        const double w = i < end ? weight(ex(i), two ? ey(i) : 0.0, i) : 0.0;
+        double run = w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double up = __shfl_up_sync(0xffffffffu, run, o);
+          if (lane >= o) run += up;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, i < end && before + run > goal);
+        if (past) found = i0 + __ffs(past) - 1;
+        const unsigned some = __ballot_sync(0xffffffffu, w > 0.0);
+        if (some) last = i0 + 31 - __clz(some);
+        before += __shfl_sync(0xffffffffu, run, 31);
+      }
+      if (found < 0) found = last;
+      if (lane == 0 && found >= 0) dsmem_st(dsmem_addr(&hit, 0), __int_as_float(found));
+    }
+  }
+  cluster_arrive();
+  cluster_wait();
+  if (rank != 0) return;
+  if (none && tid == 0) *a.err = kErrRow;
+  write_ids(a, s, at, none ? 0u : (uint32_t)min(hit, a.V - 1));
 }
 
 // The same over the kept lists, one CTA per sequence.
-__global__ void __launch_bounds__(128) verify_draw_list_kernel(Verify a) {
+__global__ void __launch_bounds__(128) verify_draw_list_kernel(const __grid_constant__ Verify a) {
   __shared__ int first_rejected;
   __shared__ double w_list[128];
   pdl_launch_dependents();
