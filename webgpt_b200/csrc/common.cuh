@@ -267,7 +267,7 @@ __device__ __forceinline__ void dsmem_st4(uint32_t addr, float4 v) {
 }
 __device__ __forceinline__ float dsmem_ld(uint32_t addr) {
   float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
   return v;
 }
 __device__ __forceinline__ float4 dsmem_ld4(uint32_t addr) {

@@ -143,12 +143,11 @@ paged_append_kernel(const __grid_constant__ PagedView c, NewRows r, const float 
 
 // ------------------------------------------------------------------------------------------ selection
 // The need-th largest of all 32-bit keys of a cluster of C CTAs (or of one) of NT threads: digits of 11, 11 and 10 bits from the
-// top, a histogram of each digit among the keys that share the digits found so far, added up over the cluster. key(u) is a
-// thread's u-th key of n, there(u) whether it has one. Returns the key, and in `ties` how many keys equal to it belong to the
-// need largest. hist: 2 * 2048 counters in shared memory at the same place in every CTA, warp_sums: NT / 32, found: 2.
-template <int NT, typename Key, typename There>
-__device__ uint32_t radix_threshold(Key key, There there, int n, int need, int C, uint32_t *hist2, uint32_t *warp_sums,
-                                    uint32_t *found, int &ties) {
+// top, a histogram of each digit among the keys that share the digits found so far, added up over the cluster. each(f) calls f
+// with every key of this thread. Returns the key, and in `ties` how many keys equal to it belong to the need largest.
+// hist2: 2 * 2048 counters in shared memory at the same place in every CTA, warp_sums: NT / 32, found: 2.
+template <int NT, typename Each>
+__device__ uint32_t radix_threshold(Each each, int need, int C, uint32_t *hist2, uint32_t *warp_sums, uint32_t *found, int &ties) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t prefix = 0, mask = 0, left = (uint32_t)need;
 #pragma unroll 1
@@ -158,11 +157,9 @@ __device__ uint32_t radix_threshold(Key key, There there, int n, int need, int C
     uint32_t *hist = hist2 + (pass & 1) * 2048;  // a neighbour may still read the other
     for (int i = tid; i < 2048; i += NT) hist[i] = 0;
     __syncthreads();
-#pragma unroll 4
-    for (int u = 0; u < n; u++) {
-      const uint32_t k = there(u) ? key(u) : 0u;
-      if (there(u) && (k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1u);
-    }
+    each([&](uint32_t k) {
+      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1u);
+    });
     if (C > 1) {
       cluster_arrive();
       cluster_wait();
@@ -178,8 +175,12 @@ __device__ uint32_t radix_threshold(Key key, There there, int n, int need, int C
       count[u] = 0;
       if (C == 1) {
         count[u] = hist[d];
-      } else {
-        for (int q = 0; q < C; q++) count[u] += __float_as_uint(dsmem_ld(dsmem_addr(hist + d, q)));
+      } else {  // 8 CTAs at most; the first one's again in the place of those that are not there
+        float part[8];
+#pragma unroll
+        for (int q = 0; q < 8; q++) part[q] = dsmem_ld(dsmem_addr(hist + d, q < C ? q : 0));
+#pragma unroll
+        for (int q = 0; q < 8; q++) count[u] += q < C ? __float_as_uint(part[q]) : 0u;
       }
       mine += count[u];
     }
@@ -191,7 +192,7 @@ __device__ uint32_t radix_threshold(Key key, There there, int n, int need, int C
     }
     if (lane == 31) warp_sums[warp] = upto;
     __syncthreads();
-    for (int w = 0; w < warp; w++) upto += warp_sums[w];
+    upto += __reduce_add_sync(0xffffffffu, lane < warp && lane < NT / 32 ? warp_sums[lane] : 0u);
     uint32_t before = upto - mine;
     if (before < left && left <= upto) {
 #pragma unroll
@@ -226,11 +227,13 @@ struct PagedEvict {
 __device__ __forceinline__ uint32_t weight_key(float w) { return isnan(w) ? 0xFFFFFFFFu : value_key(w); }
 
 // A cluster per sequence, each CTA with a stretch of its positions: the weight that the last position to stay has, then the
-// positions that stay, in order. A thread of a stretch takes groups of four positions, 1024 groups from one of its to the next.
-constexpr int kEvictThreads = 1024, kEvictCluster = 8;
+// positions that stay, in order. A thread's u-th position of a round is u * 1024 + its number, so that a round's flags lie in order
+// as [u][warp][lane]; a stretch of one round (131072 positions a sequence) stays in registers.
+constexpr int kEvictThreads = 1024, kEvictCluster = 8, kEvictVals = 16, kEvictRound = kEvictThreads * kEvictVals;
 
 __global__ void __launch_bounds__(kEvictThreads) paged_select_kernel(const __grid_constant__ PagedEvict e) {
   __shared__ uint32_t hist[2 * 2048], warp_sums[32], found[2];
+  __shared__ uint32_t flags[2][kEvictVals * 32];                // above the threshold and on it, of every 32 positions of a round
   __shared__ float above[kEvictCluster], equal[kEvictCluster];  // of the CTAs' stretches, as bits
   uint32_t C;
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(C));
@@ -245,42 +248,51 @@ __global__ void __launch_bounds__(kEvictThreads) paged_select_kernel(const __gri
   const int all = (int)C * kEvictThreads, me = rank * kEvictThreads + tid;
   int out = 0;
   if (old > 0 && need > 0) {  // the same for the whole cluster
-    const int share = ((old + (int)C - 1) / (int)C + 3) / 4 * 4, beg = min(old, rank * share), end = min(old, beg + share);
-    const int rounds = (end - beg + 4 * kEvictThreads - 1) / (4 * kEvictThreads);
-    auto at = [&](int u) { return beg + (u >> 2) * 4 * kEvictThreads + 4 * tid + (u & 3); };
-    auto there = [&](int u) { return at(u) < end; };
-    auto next_to = [&](int u) { return beg + u * kEvictThreads + tid; };  // where the order does not matter
+    const int share = (old + (int)C - 1) / (int)C, beg = min(old, rank * share), end = min(old, beg + share);
+    const int rounds = (end - beg + kEvictRound - 1) / kEvictRound;
+    float x[kEvictVals];
+    auto fetch = [&](int round) {
+#pragma unroll
+      for (int u = 0; u < kEvictVals; u++) {
+        const int i = beg + round * kEvictRound + u * kEvictThreads + tid;
+        x[u] = i < end ? __ldcg(w + i) : 0.f;
+      }
+    };
+    auto there = [&](int round, int u) { return beg + round * kEvictRound + u * kEvictThreads + tid < end; };
+    auto past = [&](int round, int u) { return beg + round * kEvictRound + u * kEvictThreads >= end; };  // the same for all threads
+    if (rounds == 1) fetch(0);
+    auto each = [&](auto f) {
+      for (int round = 0; round < rounds; round++) {
+        if (rounds > 1) fetch(round);
+#pragma unroll
+        for (int u = 0; u < kEvictVals; u++) {
+          if (past(round, u)) break;
+          if (there(round, u)) f(weight_key(x[u]));
+        }
+      }
+    };
     int ties;
-    const uint32_t t = radix_threshold<kEvictThreads>([&](int u) { return weight_key(__ldcg(w + next_to(u))); },
-                                                      [&](int u) { return next_to(u) < end; }, 4 * rounds, need, (int)C, hist,
-                                                      warp_sums, found, ties);
-    // how many lie above the threshold and on it, in the stretches before this one
-    int gt = 0, eq = 0;
-#pragma unroll 4
-    for (int u = 0; u < 4 * rounds; u++)
-      if (next_to(u) < end) {
-        const uint32_t k = weight_key(__ldcg(w + next_to(u)));
+    const uint32_t t = radix_threshold<kEvictThreads>(each, need, (int)C, hist, warp_sums, found, ties);
+    int gt0 = 0, eq0 = 0;  // above the threshold and on it, before the round at hand
+    if (C > 1) {           // in the stretches before this one
+      int gt = 0, eq = 0;
+      each([&](uint32_t k) {
         gt += k > t ? 1 : 0;
         eq += k == t ? 1 : 0;
-      }
-    int gt0 = 0, eq0 = 0;
-    if (C > 1) {
+      });
       gt = __reduce_add_sync(0xffffffffu, gt);
       eq = __reduce_add_sync(0xffffffffu, eq);
-      __syncthreads();
       if (lane == 0) {
-        hist[2048 + warp] = gt;  // a neighbour may still read the first half
-        hist[2080 + warp] = eq;
+        flags[0][warp] = gt;
+        flags[1][warp] = eq;
       }
       __syncthreads();
-      if (tid < (int)C) {  // to every CTA
-        uint32_t g = 0, q = 0;
-        for (int i = 0; i < kEvictThreads / 32; i++) {
-          g += hist[2048 + i];
-          q += hist[2080 + i];
+      if (warp == 0) {
+        const uint32_t g = __reduce_add_sync(0xffffffffu, flags[0][lane]), q = __reduce_add_sync(0xffffffffu, flags[1][lane]);
+        if (lane < (int)C) {  // to every CTA
+          dsmem_st(dsmem_addr(&above[rank], lane), __uint_as_float(g));
+          dsmem_st(dsmem_addr(&equal[rank], lane), __uint_as_float(q));
         }
-        dsmem_st(dsmem_addr(&above[rank], tid), __uint_as_float(g));
-        dsmem_st(dsmem_addr(&equal[rank], tid), __uint_as_float(q));
       }
       cluster_arrive();
       cluster_wait();
@@ -289,42 +301,55 @@ __global__ void __launch_bounds__(kEvictThreads) paged_select_kernel(const __gri
         eq0 += (int)__float_as_uint(equal[i]);
       }
     }
-    for (int u0 = 0; u0 < 4 * rounds; u0 += 4) {
-      float x[4];
-      uint32_t k[4];
-      int g = 0, q = 0;
+    for (int round = 0; round < rounds; round++) {
+      if (rounds > 1) fetch(round);
+      __syncthreads();
 #pragma unroll
-      for (int u = 0; u < 4; u++) {
-        x[u] = there(u0 + u) ? __ldcg(w + at(u0 + u)) : 0.f;
-        k[u] = weight_key(x[u]);
-        g += there(u0 + u) && k[u] > t ? 1 : 0;
-        q += there(u0 + u) && k[u] == t ? 1 : 0;
+      for (int u = 0; u < kEvictVals; u++) {
+        if (past(round, u)) {
+          if (lane < 2) flags[lane][u * 32 + warp] = 0;
+          continue;
+        }
+        const uint32_t k = weight_key(x[u]);
+        const uint32_t g = __ballot_sync(0xffffffffu, there(round, u) && k > t), q = __ballot_sync(0xffffffffu, there(round, u) && k == t);
+        if (lane == 0) {
+          flags[0][u * 32 + warp] = g;
+          flags[1][u * 32 + warp] = q;
+        }
       }
-      uint32_t mine = (uint32_t)q << 16 | (uint32_t)g, upto = mine, sum = 0;  // 4096 positions: both fit 16 bits
+      __syncthreads();
+      // every warp adds up the counts before its own flags: lane l those of the l-th sixteen
+      uint32_t mine = 0;  // both counts: up to 16384 each
+      const int first = lane * kEvictVals;
+#pragma unroll
+      for (int i0 = 0; i0 < kEvictVals; i0++) {
+        const int i = first + ((i0 + lane) & (kEvictVals - 1));  // in an order that spreads over the banks
+        mine += (uint32_t)__popc(flags[1][i]) << 16 | (uint32_t)__popc(flags[0][i]);
+      }
+      uint32_t upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += y;
       }
-      __syncthreads();
-      if (lane == 31) warp_sums[warp] = upto;
-      __syncthreads();
+      const uint32_t sum = __shfl_sync(0xffffffffu, upto, 31);
       upto -= mine;
-      const uint32_t ws = warp_sums[lane];
-      upto += __reduce_add_sync(0xffffffffu, lane < warp ? ws : 0u);
-      sum = __reduce_add_sync(0xffffffffu, ws);
-      int gi = gt0 + (int)(upto & 0xffffu), qi = eq0 + (int)(upto >> 16);
 #pragma unroll
-      for (int u = 0; u < 4; u++) {
-        if (!there(u0 + u)) continue;
-        const bool is_gt = k[u] > t, is_eq = k[u] == t;
-        if (is_gt || (is_eq && qi < ties)) {
+      for (int u = 0; u < kEvictVals; u++) {
+        if (past(round, u)) break;
+        const int at = u * 32 + warp, of = at / kEvictVals;
+        // what lies before the lane's sixteen that `at` belongs to, and inside them before it
+        const uint32_t base = __shfl_sync(0xffffffffu, upto, of);
+        const int j = of * kEvictVals + (lane & (kEvictVals - 1));
+        const uint32_t in = j < at && lane < kEvictVals ? (uint32_t)__popc(flags[1][j]) << 16 | (uint32_t)__popc(flags[0][j]) : 0u;
+        const uint32_t before = base + __reduce_add_sync(0xffffffffu, in);
+        const uint32_t g = flags[0][at], q = flags[1][at], below = (1u << lane) - 1u;
+        const int gi = gt0 + (int)(before & 0xffffu) + __popc(g & below), qi = eq0 + (int)(before >> 16) + __popc(q & below);
+        if ((g >> lane & 1u) || ((q >> lane & 1u) && qi < ties)) {
           const int to = gi + min(qi, ties);
-          kept[to] = at(u0 + u);
+          kept[to] = beg + round * kEvictRound + u * kEvictThreads + tid;
           if (wt) wt[to] = x[u];
         }
-        gi += is_gt ? 1 : 0;
-        qi += is_eq ? 1 : 0;
       }
       gt0 += (int)(sum & 0xffffu);
       eq0 += (int)(sum >> 16);
@@ -349,6 +374,8 @@ __global__ void __launch_bounds__(kEvictThreads) paged_select_kernel(const __gri
   if (me == 0) e.to.lengths[s] = n;
 }
 
+constexpr int kGatherAhead = 4;
+
 // Copies what stays. A warp takes a position: its rows of all heads in both pools, 16 bytes a lane.
 __global__ void __launch_bounds__(256) paged_gather_kernel(const __grid_constant__ PagedEvict e, int elem) {
   pdl_launch_dependents();
@@ -358,13 +385,26 @@ __global__ void __launch_bounds__(256) paged_gather_kernel(const __grid_constant
   for (int i = blockIdx.x * 8 + (threadIdx.x >> 5); i < n; i += gridDim.x * 8) {
     const long long a = paged_offset(e.from, s, __ldcg(e.kept + (long long)s * e.keep + i)), b = paged_offset(e.to, s, i);
     if (a < 0 || b < 0) continue;
-    for (int j = lane; j < all; j += 32) {
-      const int h = j / chunks, x = (j - h * chunks) * 16;
-      const long long at = (a + h * e.from.head_stride) * elem + x, to = (b + h * e.to.head_stride) * elem + x;
-      const uint4 kk = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const char *>(e.from.k) + at));
-      const uint4 vv = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const char *>(e.from.v) + at));
-      *reinterpret_cast<uint4 *>(static_cast<char *>(e.to.k) + to) = kk;
-      *reinterpret_cast<uint4 *>(static_cast<char *>(e.to.v) + to) = vv;
+    for (int j0 = lane; j0 < all; j0 += 32 * kGatherAhead) {
+      uint4 kk[kGatherAhead], vv[kGatherAhead];
+#pragma unroll
+      for (int u = 0; u < kGatherAhead; u++) {
+        const int j = j0 + 32 * u, h = j / chunks;
+        const long long at = (a + h * e.from.head_stride) * elem + (j - h * chunks) * 16;
+        if (j < all) {
+          kk[u] = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const char *>(e.from.k) + at));
+          vv[u] = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const char *>(e.from.v) + at));
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kGatherAhead; u++) {
+        const int j = j0 + 32 * u, h = j / chunks;
+        const long long to = (b + h * e.to.head_stride) * elem + (j - h * chunks) * 16;
+        if (j < all) {
+          *reinterpret_cast<uint4 *>(static_cast<char *>(e.to.k) + to) = kk[u];
+          *reinterpret_cast<uint4 *>(static_cast<char *>(e.to.v) + to) = vv[u];
+        }
+      }
     }
   }
 }

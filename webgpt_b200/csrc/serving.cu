@@ -205,7 +205,7 @@ WGPT_EXPORT int32_t wgpt_paged_evict(wgpt_device *dev, const wgpt_paged_cache *f
   e.kept = kept;
   e.ld = ld_weights;
   e.ld_to = ld_weights_to;
-  // a stretch of up to 4096 positions is one round of a CTA: below that a cluster has nothing to share
+  // up to a few positions a thread one CTA is done before a cluster has met
   const int cluster = from->max_length > 4 * kEvictThreads ? kEvictCluster : 1;
   CK(launch_ex_x(dev->pdl, cluster, dev->stream, paged_select_kernel, dim3(cluster * from->n_seq), dim3(kEvictThreads), 0, e));
   dev->launches++;
@@ -248,10 +248,11 @@ WGPT_EXPORT int32_t wgpt_verify_drafts(wgpt_device *dev, int32_t n_seq, int32_t 
   const int rows = a.draft ? 2 * n_draft + 1 : n_draft + 1;
   const size_t places = (size_t)n_seq * (2 * n_draft + 1);
   if (top_k > 0) {
-    TRY(scratch_reserve(dev, places * top_k * 8));
-    a.list_value = static_cast<float *>(dev->scratch);
+    TRY(scratch_reserve(dev, places * (16 + (size_t)top_k * 8)));
+    a.list_sum = static_cast<double2 *>(dev->scratch);
+    a.list_value = reinterpret_cast<float *>(a.list_sum + places);
     a.list_id = reinterpret_cast<int *>(a.list_value + places * top_k);
-    const int cap = top_k * ((V + kListThreads - 1) / kListThreads);
+    const int cap = std::max(kListCap, top_k * ((V + kListThreads - 1) / kListThreads));
     REQUIRE(cap * sizeof(unsigned long long) <= size_t(200) << 10, WGPT_ERR_SHAPE,
             "top_k %d with a vocabulary of %d needs %zu bytes of shared memory for the candidate list", top_k, V,
             cap * sizeof(unsigned long long));
@@ -262,12 +263,17 @@ WGPT_EXPORT int32_t wgpt_verify_drafts(wgpt_device *dev, int32_t n_seq, int32_t 
   }
   TRY(scratch_reserve(dev, places * a.chunks * sizeof(float2)));
   a.partial = static_cast<float2 *>(dev->scratch);
-  LAUNCH_PDL(dev, verify_sums_kernel, dim3(a.chunks, rows, n_seq), dim3(kVerifyThreads), 0, a);
-  const dim3 grid(kDrawCluster * n_seq), block(kDrawThreads);
-  if (V <= 16 * 32 * kDrawWarps * kDrawCluster)
-    CK(launch_ex_x(dev->pdl, kDrawCluster, dev->stream, verify_draw_kernel<16>, grid, block, 0, a));
+  const int warps = kVerifyThreads / 32;
+  LAUNCH_PDL(dev, verify_sums_kernel, dim3((a.chunks + warps - 1) / warps, rows, n_seq), dim3(kVerifyThreads), 0, a);
+  // as many CTAs a sequence as are resident at once: two an SM, and one where a few sequences keep their exponentials
+  int C = kDrawCluster;
+  while (C > 1 && C * n_seq > 2 * dev->sm_count) C /= 2;
+  if (getenv("DRAWC")) C = atoi(getenv("DRAWC"));
+  const dim3 grid(C * n_seq), block(kDrawThreads);
+  if (C == kDrawCluster && C * n_seq <= dev->sm_count && V <= 16 * 32 * kDrawWarps * C)
+    CK(launch_ex_x(dev->pdl, C, dev->stream, verify_draw_kernel<16>, grid, block, 0, a));
   else
-    CK(launch_ex_x(dev->pdl, kDrawCluster, dev->stream, verify_draw_kernel<0>, grid, block, 0, a));
+    CK(launch_ex_x(dev->pdl, C, dev->stream, verify_draw_kernel<0>, grid, block, 0, a));
   dev->launches++;
   return WGPT_OK;
 }

@@ -1,7 +1,7 @@
 // Verification of drafted tokens against the target's probabilities (speculative sampling), from given random numbers.
 #pragma once
 #include "common.cuh"
-#include "paged.cuh"
+#include "paged_attention.cuh"
 #include "sample_key.cuh"
 
 namespace wgpt {
@@ -23,7 +23,8 @@ struct Verify {
   int *n_accepted;
   int *err;
   float2 *partial;   // (largest, sum) of each chunk of each row: [n_seq][2 * n_draft + 1][chunks]
-  float *list_value; // top_k > 0: each row's kept logits, largest first, and their ids, [n_seq][2 * n_draft + 1][top_k]
+  double2 *list_sum; // top_k > 0: each row's sum of exponentials and the drafted id's probability, [n_seq][2 * n_draft + 1]
+  float *list_value; // each row's kept logits, largest first, and their ids, [n_seq][2 * n_draft + 1][top_k]
   int *list_id;
 };
 
@@ -54,45 +55,44 @@ __device__ __forceinline__ double warp_sum64(double v) {
   return v;
 }
 
-// The largest value of each chunk of a row and the sum of exp((x - largest) / temperature) over it; a chunk is in registers
-// between the two. Decides whether drafts are accepted: each exponential is good to 2^-22, their sum to a few 1e-8.
-constexpr int kVerifyThreads = 256, kVerifyVals = 16, kVerifyChunk = kVerifyThreads * kVerifyVals;
+// The largest value of each chunk of a row and the sum of exp((x - largest) / temperature) over it, a warp a chunk: every lane has its
+// own running maximum until the end. Decides whether drafts are accepted: each exponential is good to 2^-22, their sum to a few 1e-8.
+constexpr int kVerifyThreads = 256, kVerifyVals = 16, kVerifyTurns = 4, kVerifyChunk = 32 * kVerifyVals * kVerifyTurns;
 
 __global__ void __launch_bounds__(kVerifyThreads) verify_sums_kernel(const __grid_constant__ Verify a) {
-  __shared__ float red[kVerifyThreads / 32];
-  __shared__ double red64[kVerifyThreads / 32];
   pdl_launch_dependents();
   pdl_wait();
-  const int s = blockIdx.z, r = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int beg = blockIdx.x * kVerifyChunk;
-  if (!row_wanted(a, r, drafted(a, s))) return;
-  const float *x = logits_row(a, s, r) + beg;
-  const int n = min(a.V - beg, kVerifyChunk);
-  float v[kVerifyVals], m = -INFINITY;
-#pragma unroll
-  for (int u = 0; u < kVerifyVals; u++) v[u] = tid + u * kVerifyThreads < n ? __ldcg(x + tid + u * kVerifyThreads) : -INFINITY;
-#pragma unroll
-  for (int u = 0; u < kVerifyVals; u++) m = fmaxf(m, v[u]);  // NaN is passed over
-  m = warp_max(m);
-  if (lane == 0) red[warp] = m;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kVerifyThreads / 32; w++) m = fmaxf(m, red[w]);
+  const int s = blockIdx.z, r = blockIdx.y, lane = threadIdx.x & 31, chunk = blockIdx.x * (kVerifyThreads / 32) + (threadIdx.x >> 5);
+  if (chunk >= a.chunks || !row_wanted(a, r, drafted(a, s))) return;
+  const float *x = logits_row(a, s, r) + (long long)chunk * kVerifyChunk + lane;
+  const int n = min(a.V - chunk * kVerifyChunk, kVerifyChunk) - lane;
   const float c = (float)(1.4426950408889634 / a.temperature);
-  float sum = 0.f;
+  float v[kVerifyVals], next[kVerifyVals], m = -INFINITY, sum = 0.f;
 #pragma unroll
-  for (int u = 0; u < kVerifyVals; u++) {
-    const float e = exp2f((v[u] - m) * c);
-    sum += v[u] > -INFINITY ? e : 0.f;
+  for (int u = 0; u < kVerifyVals; u++) next[u] = 32 * u < n ? __ldcg(x + 32 * u) : -INFINITY;
+#pragma unroll
+  for (int t = 0; t < kVerifyTurns; t++) {
+    if (t * 32 * kVerifyVals >= n + lane) break;  // the same for the warp
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < kVerifyVals; u++) top = fmaxf(top, v[u] = fmaxf(next[u], -INFINITY));  // NaN counts as -infinity
+    if (t + 1 < kVerifyTurns) {
+#pragma unroll
+      for (int u = 0; u < kVerifyVals; u++) {
+        const int i = 32 * (u + (t + 1) * kVerifyVals);
+        next[u] = i < n ? __ldcg(x + i) : -INFINITY;
+      }
+    }
+    if (top == -INFINITY) continue;
+    sum *= exp2_of((m - top) * c);
+    m = top;
+#pragma unroll
+    for (int u = 0; u < kVerifyVals; u++) sum += exp2_of((v[u] - m) * c);
   }
-  double sum64 = warp_sum64((double)sum);
-  if (lane == 0) red64[warp] = sum64;
-  __syncthreads();
-  if (tid == 0) {
-    sum64 = 0.0;
-    for (int w = 0; w < kVerifyThreads / 32; w++) sum64 += red64[w];
-    a.partial[((long long)s * (2 * a.n_draft + 1) + r) * a.chunks + blockIdx.x] = make_float2(m, (float)sum64);
-  }
+  const float top = warp_max(m);
+  double all = m > -INFINITY ? (double)(sum * exp2_of((m - top) * c)) : 0.0;
+  all = warp_sum64(all);
+  if (lane == 0) a.partial[((long long)s * (2 * a.n_draft + 1) + r) * a.chunks + chunk] = make_float2(top, (float)all);
 }
 
 // e^(x / temperature) of x <= 0 in double precision, to about 1e-15: x / temperature = (64 n + j + f) ln 2 / 64 with |f| <= 1/2, so
@@ -113,87 +113,134 @@ __device__ __forceinline__ double exp_of(double x, double scale, const double *t
   return t < -65000.0 ? 0.0 : __hiloint2double(__double2hiint(y) + ((n >> 6) << 20), __double2loint(y));  // 2^-1015 and below: 0
 }
 
-// top_k > 0: the kept logits of a row in descending order, by one CTA. Each thread's largest key (of the value, among equals of the
-// lowest index) is a candidate for the bound: the top_k-th largest of them is a key that at least top_k keys reach, all of them in
-// the top_k threads that hold one. Those read their share again; what reaches the bound is ranked by counting.
-constexpr int kListThreads = 1024;
+// top_k > 0: the kept logits of a row in descending order, their sum of exponentials and the drafted id's probability, by one CTA.
+// The largest values of 128 groups of threads give a bound, the top_k-th largest of them, that at least top_k values reach; what
+// reaches it is mostly little more than that, and is ranked by counting. A row made so that more reach it than the list holds goes
+// by the threads' largest keys (of the value, among equals of the lowest index) instead: what reaches the top_k-th largest of
+// those lies in top_k threads' shares.
+constexpr int kListThreads = 1024, kListGroups = 128, kListCap = 1536, kListVals = 28;
 
 __global__ void __launch_bounds__(kListThreads) verify_list_kernel(const __grid_constant__ Verify a, int cap) {
-  extern __shared__ __align__(16) unsigned long long cand[];  // [cap], cap = top_k * ceil(V / kListThreads)
-  __shared__ int count;
+  extern __shared__ __align__(16) unsigned long long cand[];  // [cap], cap >= kListCap and top_k * ceil(V / kListThreads)
+  __shared__ __align__(16) float group[kListGroups];
+  __shared__ unsigned long long top[128];
+  __shared__ double ev[128];
+  __shared__ int count, n_shares;
+  __shared__ short shares[kListThreads];
+  __shared__ float s_bound;
   pdl_launch_dependents();
   pdl_wait();
-  const int s = blockIdx.y, r = blockIdx.x, tid = threadIdx.x;
+  const int s = blockIdx.y, r = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.top_k;
   if (!row_wanted(a, r, drafted(a, s))) return;
   const float *x = logits_row(a, s, r);
-  unsigned long long best = 0ull;
-  for (int i0 = 0; i0 < a.V; i0 += 16 * kListThreads) {
-    float v[16];
+  float m = -INFINITY;
+  for (int i0 = tid; i0 < a.V; i0 += kListVals * kListThreads) {
+    float v[kListVals];
 #pragma unroll
-    for (int u = 0; u < 16; u++) {
-      const int i = i0 + tid + u * kListThreads;
-      v[u] = i < a.V ? logit(x + i) : 0.f;
-    }
+    for (int u = 0; u < kListVals; u++) v[u] = i0 + u * kListThreads < a.V ? __ldcg(x + i0 + u * kListThreads) : -INFINITY;
 #pragma unroll
-    for (int u = 0; u < 16; u++) {
-      const int i = i0 + tid + u * kListThreads;
-      const unsigned long long k = i < a.V ? sample_key(v[u], i) : 0ull;
-      best = k > best ? k : best;
-    }
+    for (int u = 0; u < kListVals; u++) m = fmaxf(m, v[u]);  // NaN is passed over
   }
-  if (tid == 0) count = 0;
-  // the bound, bit by bit: the value's, and where several threads have that value, the index's
-  const int holders = min(a.V, kListThreads);
-  unsigned long long bound = 1ull;
-  if (holders > a.top_k) {
-    bound = 0ull;
-    for (int bit = 63; bit >= 32; bit--) {
-      const unsigned long long trial = bound | 1ull << bit;
-      if (__syncthreads_count(best >= trial) >= a.top_k) bound = trial;
-    }
-    if (__syncthreads_count(best >= bound) > a.top_k)
-      for (int bit = 31; bit >= 0; bit--) {
-        const unsigned long long trial = bound | 1ull << bit;
-        if (__syncthreads_count(best >= trial) >= a.top_k) bound = trial;
-      }
+  const float own = m;
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((lane & 7) == 0) group[tid >> 3] = m;
+  if (tid == 0) {
+    count = n_shares = 0;
+    s_bound = -INFINITY;
   }
   __syncthreads();
-  if (best >= bound)
-    for (int i0 = tid; i0 < a.V; i0 += 16 * kListThreads) {
-      float v[16];
-#pragma unroll
-      for (int u = 0; u < 16; u++) v[u] = i0 + u * kListThreads < a.V ? logit(x + i0 + u * kListThreads) : 0.f;
-#pragma unroll
-      for (int u = 0; u < 16; u++) {
-        const int i = i0 + u * kListThreads;
-        if (i >= a.V) continue;
-        const unsigned long long k = sample_key(v[u], i);
-        if (k >= bound) {
+  if (tid < kListGroups) {
+    const float mine = group[tid];
+    int above = 0, upto = 0;
+#pragma unroll 8
+    for (int j = 0; j < kListGroups / 4; j++) {
+      const float4 g = reinterpret_cast<const float4 *>(group)[j];
+      above += (g.x > mine ? 1 : 0) + (g.y > mine ? 1 : 0) + (g.z > mine ? 1 : 0) + (g.w > mine ? 1 : 0);
+      upto += (g.x >= mine ? 1 : 0) + (g.y >= mine ? 1 : 0) + (g.z >= mine ? 1 : 0) + (g.w >= mine ? 1 : 0);
+    }
+    if (above < K && K <= upto) s_bound = mine;  // equal ones write the same
+  }
+  __syncthreads();
+  // the threads' shares that something at the bound lies in, a warp a share
+  const float bound = s_bound;
+  if (own >= bound) shares[atomicAdd(&n_shares, 1)] = (short)tid;
+  __syncthreads();
+  const int per_thread = (a.V + kListThreads - 1) / kListThreads;
+  for (int j = warp; j < n_shares; j += kListThreads / 32) {
+    const int share = shares[j];
+#pragma unroll 2
+    for (int u = lane; u < per_thread; u += 32) {
+      const int i = share + u * kListThreads;
+      if (i >= a.V) continue;
+      const float y = logit(x + i);
+      if (y >= bound) {
+        const int at = atomicAdd(&count, 1);
+        if (at < cap) cand[at] = sample_key(y, i);
+      }
+    }
+  }
+  __syncthreads();
+  if (count > cap) {  // the same for all
+    unsigned long long best = 0ull, least = 0ull;
+    for (int i = tid; i < a.V; i += kListThreads) {
+      const unsigned long long k = sample_key(logit(x + i), i);
+      best = k > best ? k : best;
+    }
+    for (int bit = 63; bit >= 0; bit--) {
+      const unsigned long long trial = least | 1ull << bit;
+      if (__syncthreads_count(best >= trial) >= K) least = trial;
+    }
+    __syncthreads();
+    if (tid == 0) count = 0;
+    __syncthreads();
+    if (best >= least)
+      for (int i = tid; i < a.V; i += kListThreads) {
+        const unsigned long long k = sample_key(logit(x + i), i);
+        if (k >= least) {
           const int at = atomicAdd(&count, 1);
           if (at < cap) cand[at] = k;
         }
       }
-    }
-  __syncthreads();
+    __syncthreads();
+  }
   const int n = min(count, cap);
-  const long long to = ((long long)s * (2 * a.n_draft + 1) + r) * a.top_k;
+  const long long row = (long long)s * (2 * a.n_draft + 1) + r, to = row * K;
   for (int i = tid; i < n; i += kListThreads) {
     const unsigned long long mine = cand[i];
     int rank = 0;
+#pragma unroll 4
     for (int j = 0; j < n; j++) rank += cand[j] > mine ? 1 : 0;
-    if (rank < a.top_k) {
+    if (rank < K) {
+      top[rank] = mine;
       a.list_value[to + rank] = sample_key_value(mine);
       a.list_id[to + rank] = sample_key_index(mine);
     }
   }
+  __syncthreads();
+  if (tid < K) ev[tid] = exp(((double)sample_key_value(top[tid]) - (double)sample_key_value(top[0])) / a.temperature);
+  __syncthreads();
+  if (warp == 0) {
+    double z = 0.0, p = 0.0;
+    const int i = r <= a.n_draft ? r : r - a.n_draft - 1;
+    const uint32_t id = i < a.n_draft ? __ldcg(a.draft_ids + (long long)s * a.n_draft + i) : kNoId;
+    for (int j = lane; j < K; j += 32) {
+      z += ev[j];
+      if ((uint32_t)sample_key_index(top[j]) == id) p = ev[j];
+    }
+    z = warp_sum64(z);
+    p = warp_sum64(p);
+    if (lane == 0) a.list_sum[row] = make_double2(z, p / z);
+  }
 }
 
 // ids_out and n_accepted of a sequence, once `accepted` and the drawn id are known.
-__device__ __forceinline__ void write_ids(const Verify &a, int s, int accepted, uint32_t drawn) {
-  for (int i = threadIdx.x; i <= a.n_draft; i += blockDim.x)
+template <int NT>
+__device__ __forceinline__ void write_ids(const Verify &a, int s, int accepted, uint32_t drawn, int tid) {
+  for (int i = tid; i <= a.n_draft; i += NT)
     a.ids_out[(long long)s * (a.n_draft + 1) + i] =
         i < accepted ? __ldcg(a.draft_ids + (long long)s * a.n_draft + i) : i == accepted ? drawn : kNoId;
-  if (threadIdx.x == 0) a.n_accepted[s] = accepted;
+  if (tid == 0) a.n_accepted[s] = accepted;
 }
 
 // The accept step and the draw over the whole vocabulary, a cluster of CTAs per sequence. The draw needs running sums good to
@@ -203,8 +250,8 @@ __device__ __forceinline__ void write_ids(const Verify &a, int s, int accepted, 
 constexpr int kDrawThreads = 512, kDrawWarps = kDrawThreads / 32, kDrawCluster = 8;
 
 template <int kVals>
-__global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const __grid_constant__ Verify a) {
-  __shared__ int first_rejected, hit;
+__global__ void __launch_bounds__(kDrawThreads, kVals > 0 ? 1 : 2) verify_draw_kernel(const __grid_constant__ Verify a) {
+  __shared__ int first_rejected;
   __shared__ float s_max[2 * kMaxDraft + 1];
   __shared__ double s_sum[2 * kMaxDraft + 1];
   __shared__ double table[64];
@@ -212,16 +259,17 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const __grid_
   uint32_t C;
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(C));
   const int rank = (int)cluster_ctarank(), s = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  cluster_arrive_relaxed();
+  for (int i = tid; i < 3 * kDrawCluster * kDrawWarps; i += kDrawThreads) (&sums[0][0][0])[i] = 0.0;  // of CTAs that are not there too
+  cluster_arrive();
   if (tid < 64) table[tid] = exp2(tid / 64.0);
   pdl_launch_dependents();
   pdl_wait();
+  const double u01 = __ldcg(a.uniforms + (long long)s * (a.n_draft + 1) + a.n_draft);
   const int n = drafted(a, s), rows = 2 * a.n_draft + 1;
-  if (tid == 0) {
-    first_rejected = n;
-    hit = a.V;
-  }
+  if (tid == 0) first_rejected = n;
+  __syncthreads();
   // every CTA finds the first draft that is not accepted: (largest, sum) of the rows, a warp each
+  const double scale = 64.0 / (0.6931471805599453 * a.temperature);
   const float2 *part = a.partial + (long long)s * rows * a.chunks;
   for (int r = warp; r < rows; r += kDrawWarps) {
     if (!row_wanted(a, r, n) || (r > a.n_draft && !a.draft)) continue;
@@ -231,7 +279,7 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const __grid_
     double z = 0.0;
     for (int c = lane; c < a.chunks; c += 32) {
       const float2 p = __ldcg(part + r * a.chunks + c);
-      if (p.x > -INFINITY) z += (double)p.y * exp(((double)p.x - (double)m) / a.temperature);
+      if (p.x > -INFINITY) z += (double)p.y * exp_of((double)p.x - (double)m, scale, table);
     }
     z = warp_sum64(z);
     if (lane == 0) {
@@ -247,8 +295,8 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const __grid_
     if (x >= (uint32_t)a.V) {
       *a.err = 1;
     } else if (!isinf(s_max[i]) && !(a.draft && isinf(s_max[rq]))) {
-      const double p = exp(((double)logit(logits_row(a, s, i) + x) - (double)s_max[i]) / a.temperature) / s_sum[i];
-      const double q = a.draft ? exp(((double)logit(logits_row(a, s, rq) + x) - (double)s_max[rq]) / a.temperature) / s_sum[rq] : 1.0;
+      const double p = exp_of((double)logit(logits_row(a, s, i) + x) - (double)s_max[i], scale, table) / s_sum[i];
+      const double q = a.draft ? exp_of((double)logit(logits_row(a, s, rq) + x) - (double)s_max[rq], scale, table) / s_sum[rq] : 1.0;
       ok = __ldcg(a.uniforms + (long long)s * (a.n_draft + 1) + i) * q < p;
     }
     if (!ok) atomicMin(&first_rejected, i);
@@ -256,7 +304,7 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const __grid_
   __syncthreads();
   const int at = first_rejected;
   const float *x = logits_row(a, s, at), *y = nullptr;
-  const double m = s_max[at], scale = 64.0 / (0.6931471805599453 * a.temperature);
+  const double m = s_max[at];
   double mq = 0.0;
   uint32_t only = kNoId;
   bool rest = at < n;
@@ -273,38 +321,64 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const __grid_
   const bool none = isinf(m);
   const int stretch = (a.V + (int)C * kDrawWarps - 1) / ((int)C * kDrawWarps);
   const int beg = min(a.V, (rank * kDrawWarps + warp) * stretch), end = min(a.V, beg + stretch);
-  auto ex = [&](int i) { return exp_of((double)logit(x + i) - m, scale, table); };
-  auto ey = [&](int i) { return exp_of((double)logit(y + i) - mq, scale, table); };
   const bool two = rest && y != nullptr;
+  constexpr int kLook = kVals > 0 ? kVals : 4, kPick = 4;
   double vx[kVals > 0 ? kVals : 1], vy[kVals > 0 ? kVals : 1];
+  // a lane's logits of ids i0, i0 + 32, ...: -infinity, which counts nothing, behind the stretch
+  auto fetch = [&](int i0, float (&lx)[kLook], float (&ly)[kLook]) {
+#pragma unroll
+    for (int u = 0; u < kLook; u++) {
+      const int i = i0 + 32 * u;
+      lx[u] = i < end ? logit(x + i) : -INFINITY;
+      ly[u] = two && i < end ? logit(y + i) : -INFINITY;
+    }
+  };
   // a sum of every warp to every CTA, behind one barrier of the cluster
   auto tell = [&](int which, double v) {
     v = warp_sum64(v);
     if (lane < (int)C) dsmem_st64(dsmem_addr(&sums[which][rank][warp], lane), (unsigned long long)__double_as_longlong(v));
   };
-  auto total_of = [&](int which) {
-    double v = 0.0;
-    for (int q = 0; q < (int)C; q++)
-      for (int w = 0; w < kDrawWarps; w++) v += sums[which][q][w];
-    return v;
+  // of all warps' sums: what lies before each, and their total; every warp for itself, four sums a lane
+  constexpr int kAll = kDrawCluster * kDrawWarps, kPer = kAll / 32;
+  auto prefix_of = [&](int which, double (&upto)[kPer], double &from) {
+    const double *v = &sums[which][0][0] + lane * kPer;
+    double sum = 0.0;
+#pragma unroll
+    for (int u = 0; u < kPer; u++) upto[u] = sum += v[u];
+    from = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double up = __shfl_up_sync(0xffffffffu, from, o);
+      if (lane >= o) from += up;
+    }
+    const double total = __shfl_sync(0xffffffffu, from, 31);
+    from = __shfl_up_sync(0xffffffffu, from, 1);
+    if (lane == 0) from = 0.0;
+    return total;
   };
+  double upto[kPer], from;
   cluster_wait();  // the others run
   double zx = 1.0, zq = 1.0;
   if (!none) {
     double sx = 0.0, sy = 0.0;
     if constexpr (kVals > 0) {
+      float lx[kVals], ly[kVals];
+      fetch(beg + lane, lx, ly);
 #pragma unroll
       for (int u = 0; u < kVals; u++) {
-        const int i = beg + lane + 32 * u;
-        vx[u] = i < end ? ex(i) : 0.0;
-        vy[u] = two && i < end ? ey(i) : 0.0;
-        sx += vx[u];
-        sy += vy[u];
+        if (beg + 32 * u >= end) break;
+        sx += vx[u] = exp_of((double)lx[u] - m, scale, table);
+        if (two) sy += vy[u] = exp_of((double)ly[u] - mq, scale, table);
       }
     } else {
-      for (int i = beg + lane; i < end; i += 32) {
-        sx += ex(i);
-        if (two) sy += ey(i);
+      for (int i0 = beg + lane; i0 < end; i0 += 32 * kLook) {
+        float lx[kLook], ly[kLook];
+        fetch(i0, lx, ly);
+#pragma unroll
+        for (int u = 0; u < kLook; u++) {
+          sx += exp_of((double)lx[u] - m, scale, table);
+          if (two) sy += exp_of((double)ly[u] - mq, scale, table);
+        }
       }
     }
     tell(0, sx);
@@ -312,11 +386,9 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const __grid_
   }
   cluster_arrive();
   cluster_wait();
-  const double u01 = __ldcg(a.uniforms + (long long)s * (a.n_draft + 1) + a.n_draft);
-  int which = 0;
   if (!none) {
-    zx = total_of(0);
-    if (two) zq = total_of(1);
+    if (two) zq = prefix_of(1, upto, from);
+    zx = prefix_of(0, upto, from);
   }
   const double ix = 1.0 / zx, iq = 1.0 / zq;
   // what an id counts: e / sum, less the draft's (or less all of it at the drafted id), none below zero
@@ -324,134 +396,181 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const __grid_
     const double p = e * ix, q = two ? f * iq : (uint32_t)i == only ? 1.0 : 0.0;
     return rest ? fmax(p - q, 0.0) : e;
   };
-  if (rest && !none) {
-    double sr = 0.0;
-    if constexpr (kVals > 0) {
+  if (at < n) {  // the same for the whole cluster, whether or not there is a distribution to take from
+    if (rest && !none) {
+      double sr = 0.0;
+      if constexpr (kVals > 0) {
 #pragma unroll
-      for (int u = 0; u < kVals; u++) {
-        const int i = beg + lane + 32 * u;
-        if (i < end) sr += weight(vx[u], vy[u], i);
+        for (int u = 0; u < kVals; u++) {
+          const int i = beg + lane + 32 * u;
+          if (beg + 32 * u >= end) break;
+          vx[u] = weight(vx[u], vy[u], i);
+          sr += vx[u];
+        }
+      } else {
+        for (int i0 = beg + lane; i0 < end; i0 += 32 * kLook) {
+          float lx[kLook], ly[kLook];
+          fetch(i0, lx, ly);
+#pragma unroll
+          for (int u = 0; u < kLook; u++)
+            sr += weight(exp_of((double)lx[u] - m, scale, table), two ? exp_of((double)ly[u] - mq, scale, table) : 0.0, i0 + 32 * u);
+        }
       }
-    } else {
-      for (int i = beg + lane; i < end; i += 32) sr += weight(ex(i), two ? ey(i) : 0.0, i);
+      tell(2, sr);
     }
-    tell(2, sr);
+    cluster_arrive();
+    cluster_wait();
   }
-  cluster_arrive();
-  cluster_wait();
   double total = zx;
   if (rest && !none) {
-    total = total_of(2);
-    which = 2;
+    total = prefix_of(2, upto, from);
     if (!(total > 0.0)) {  // nothing is left: drawn from the target's row itself
       rest = false;
-      total = zx;
-      which = 0;
+      total = prefix_of(0, upto, from);
+      if constexpr (kVals > 0) {
+        float lx[kVals], ly[kVals];
+        fetch(beg + lane, lx, ly);
+#pragma unroll
+        for (int u = 0; u < kVals; u++) vx[u] = exp_of((double)lx[u] - m, scale, table);
+      }
     }
   }
   if (!none) {
-    const double goal = u01 * total;
-    double before = 0.0;
-    for (int q = 0; q < rank; q++)
-      for (int w = 0; w < kDrawWarps; w++) before += sums[which][q][w];
-    for (int w = 0; w < warp; w++) before += sums[which][rank][w];
-    // the warp in whose stretch the running sum passes the goal; its id goes to the first CTA
-    if (before + sums[which][rank][warp] > goal && before <= goal) {
+    // the last stretch with anything in it that begins at or below the goal has the id (rounding may put the beginning of an empty
+    // one there); one warp adds it up
+    const double goal = u01 * total, *of = &sums[rest ? 2 : 0][0][0] + lane * kPer;
+    int mine = -1;
+#pragma unroll
+    for (int u = 0; u < kPer; u++)
+      if ((u == 0 ? from : from + upto[u - 1]) <= goal && of[u] > 0.0) mine = lane * kPer + u;
+    const int owner = __reduce_max_sync(0xffffffffu, mine);
+    if (owner == rank * kDrawWarps + warp) {
+      double before = 0.0;
+#pragma unroll
+      for (int u = 0; u < kPer; u++)
+        if (mine == owner && owner == lane * kPer + u) before = u == 0 ? from : from + upto[u - 1];
+      before = __shfl_sync(0xffffffffu, before, owner / kPer);
       int last = -1, found = -1;  // the stretch's sum was rounded in another order: it may pass the goal where the running sum does not
-      for (int i0 = beg; i0 < end && found < 0; i0 += 32) {
-        const int i = i0 + lane;
-        const double w = i < end ? weight(ex(i), two ? ey(i) : 0.0, i) : 0.0;
+      auto look = [&](int i0, double w) {  // 32 ids
         double run = w;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const double up = __shfl_up_sync(0xffffffffu, run, o);
           if (lane >= o) run += up;
         }
-        const unsigned past = __ballot_sync(0xffffffffu, i < end && before + run > goal);
-        if (past) found = i0 + __ffs(past) - 1;
-        const unsigned some = __ballot_sync(0xffffffffu, w > 0.0);
-        if (some) last = i0 + 31 - __clz(some);
-        before += __shfl_sync(0xffffffffu, run, 31);
+        const unsigned past = __ballot_sync(0xffffffffu, i0 + lane < end && before + run > goal);
+        found = past ? i0 + __ffs(past) - 1 : last;  // the row's sum, rounded in another order, passed the goal
+      };
+      // 32 ids at a time: first the sums of some such rows, then the one in which the goal is passed, id by id
+      auto rows_of = [&](int i0, double (&w)[kPick]) {
+        double sum[kPick];
+#pragma unroll
+        for (int u = 0; u < kPick; u++) sum[u] = w[u];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+          for (int u = 0; u < kPick; u++) sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], o);
+#pragma unroll
+        for (int u = 0; u < kPick; u++) {
+          if (found >= 0 || sum[u] == 0.0) continue;
+          last = i0 + 32 * u + 31 - __clz(__ballot_sync(0xffffffffu, w[u] > 0.0));
+          if (before + sum[u] > goal) look(i0 + 32 * u, w[u]);
+          before += sum[u];
+        }
+      };
+      if constexpr (kVals > 0) {
+#pragma unroll
+        for (int h = 0; h < kVals; h += kPick) {
+          double w[kPick];
+#pragma unroll
+          for (int u = 0; u < kPick; u++) w[u] = beg + 32 * (h + u) < end ? vx[h + u] : 0.0;
+          if (found < 0) rows_of(beg + 32 * h, w);
+        }
+      } else {
+        for (int i0 = beg; i0 < end && found < 0; i0 += 32 * kPick) {
+          double w[kPick];
+          float lx[kPick], ly[kPick];
+          fetch(i0 + lane, lx, ly);
+#pragma unroll
+          for (int u = 0; u < kPick; u++)
+            w[u] = weight(exp_of((double)lx[u] - m, scale, table), two ? exp_of((double)ly[u] - mq, scale, table) : 0.0, i0 + lane + 32 * u);
+          rows_of(i0, w);
+        }
       }
-      if (found < 0) found = last;
-      if (lane == 0 && found >= 0) dsmem_st(dsmem_addr(&hit, 0), __int_as_float(found));
+      write_ids<32>(a, s, at, (uint32_t)(found < 0 ? last : found), lane);
+    } else if (owner < 0 && rank == 0 && warp == 0) {  // a number that is none
+      write_ids<32>(a, s, at, (uint32_t)(a.V - 1), lane);
     }
+  } else if (rank == 0 && warp == 0) {
+    if (lane == 0) *a.err = kErrRow;
+    write_ids<32>(a, s, at, 0u, lane);
   }
-  cluster_arrive();
-  cluster_wait();
-  if (rank != 0) return;
-  if (none && tid == 0) *a.err = kErrRow;
-  write_ids(a, s, at, none ? 0u : (uint32_t)min(hit, a.V - 1));
 }
 
 // The same over the kept lists, one CTA per sequence.
 __global__ void __launch_bounds__(128) verify_draw_list_kernel(const __grid_constant__ Verify a) {
-  __shared__ int first_rejected;
+  __shared__ int first_rejected, s_pick;
   __shared__ double w_list[128];
+  __shared__ float vq[128];
+  __shared__ int iq[128];
   pdl_launch_dependents();
   pdl_wait();
-  const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.top_k;
+  const int s = blockIdx.x, tid = threadIdx.x, K = a.top_k;
+  const double u01 = __ldcg(a.uniforms + (long long)s * (a.n_draft + 1) + a.n_draft);
   const int n = drafted(a, s);
   if (tid == 0) first_rejected = n;
   __syncthreads();
-  const long long base = (long long)s * (2 * a.n_draft + 1) * K;
-  const float *lv = a.list_value + base;
-  const int *li = a.list_id + base;
-  auto top_of = [&](int r) { return __ldcg(lv + r * K); };
-  // the sum of a row's exponentials, by a warp, in the order of the list
-  auto row_sum = [&](int r) {
-    double z = 0.0;
-    const double m = top_of(r);
-    for (int j0 = 0; j0 < K; j0 += 32) {
-      const double v = j0 + lane < K ? exp(((double)__ldcg(lv + r * K + j0 + lane) - m) / a.temperature) : 0.0;
-      for (int j = 0; j < 32; j++) z += __shfl_sync(0xffffffffu, v, j);
-    }
-    return z;
-  };
-  auto share_of = [&](int r, uint32_t id, double z) {  // an id's probability in row r, by a warp
-    double p = 0.0;
-    for (int j = lane; j < K; j += 32)
-      if ((uint32_t)__ldcg(li + r * K + j) == id) p = exp(((double)__ldcg(lv + r * K + j) - (double)top_of(r)) / a.temperature) / z;
-    return warp_sum64(p);
-  };
-  for (int i = warp; i < n; i += 4) {
+  const long long base = (long long)s * (2 * a.n_draft + 1);
+  auto top_of = [&](int r) { return __ldcg(a.list_value + (base + r) * K); };
+  if (tid < n) {
+    const int i = tid, rq = a.n_draft + 1 + i;
     const uint32_t x = __ldcg(a.draft_ids + (long long)s * a.n_draft + i);
     bool ok = false;
     if (x >= (uint32_t)a.V) {
-      if (lane == 0) *a.err = 1;
-    } else if (!isinf(top_of(i)) && !(a.draft && isinf(top_of(a.n_draft + 1 + i)))) {
-      const double p = share_of(i, x, row_sum(i));
-      const double q = a.draft ? share_of(a.n_draft + 1 + i, x, row_sum(a.n_draft + 1 + i)) : 1.0;
+      *a.err = 1;
+    } else if (!isinf(top_of(i)) && !(a.draft && isinf(top_of(rq)))) {
+      const double p = __ldcg(a.list_sum + base + i).y, q = a.draft ? __ldcg(a.list_sum + base + rq).y : 1.0;
       ok = __ldcg(a.uniforms + (long long)s * (a.n_draft + 1) + i) * q < p;
     }
-    if (!ok && lane == 0) atomicMin(&first_rejected, i);
+    if (!ok) atomicMin(&first_rejected, i);
   }
   __syncthreads();
-  const int at = first_rejected;
+  const int at = first_rejected, rq = a.n_draft + 1 + at;
   const double m = top_of(at);
   if (isinf(m)) {
     if (tid == 0) *a.err = kErrRow;
-    write_ids(a, s, at, 0u);
+    write_ids<128>(a, s, at, 0u, tid);
     return;
   }
   bool rest = at < n;
-  const int rq = a.n_draft + 1 + at;
-  if (rest && a.draft && isinf(top_of(rq))) {
-    if (tid == 0) *a.err = kErrRow;
-    rest = false;
+  double mq = 0.0, zq = 1.0;
+  if (rest && a.draft) {
+    mq = top_of(rq);
+    zq = __ldcg(a.list_sum + base + rq).x;
+    if (isinf(mq)) {
+      if (tid == 0) *a.err = kErrRow;
+      rest = false;
+    }
+    if (tid < K) {
+      vq[tid] = __ldcg(a.list_value + (base + rq) * K + tid);
+      iq[tid] = __ldcg(a.list_id + (base + rq) * K + tid);
+    }
   }
-  const double z = row_sum(at), zq = rest && a.draft ? row_sum(rq) : 1.0;
-  const double u = __ldcg(a.uniforms + (long long)s * (a.n_draft + 1) + a.n_draft);
+  const double z = __ldcg(a.list_sum + base + at).x;
+  const uint32_t id = tid < K ? (uint32_t)__ldcg(a.list_id + (base + at) * K + tid) : kNoId;
   double p = 0.0, w = 0.0;
+  __syncthreads();
   if (tid < K) {
-    const uint32_t id = (uint32_t)__ldcg(li + at * K + tid);
-    p = exp(((double)__ldcg(lv + at * K + tid) - m) / a.temperature) / z;
+    p = exp(((double)__ldcg(a.list_value + (base + at) * K + tid) - m) / a.temperature) / z;
     w = p;
     if (rest) {
       double q = 0.0;
       if (a.draft) {
-        for (int j = 0; j < K; j++)
-          if ((uint32_t)__ldcg(li + rq * K + j) == id) q = exp(((double)__ldcg(lv + rq * K + j) - (double)top_of(rq)) / a.temperature) / zq;
+        int j = -1;
+#pragma unroll 8
+        for (int i = 0; i < K; i++)
+          if ((uint32_t)iq[i] == id) j = i;
+        if (j >= 0) q = exp(((double)vq[j] - mq) / a.temperature) / zq;
       } else {
         q = id == __ldcg(a.draft_ids + (long long)s * a.n_draft + at) ? 1.0 : 0.0;
       }
@@ -463,18 +582,31 @@ __global__ void __launch_bounds__(128) verify_draw_list_kernel(const __grid_cons
     if (tid < K) w_list[tid] = p;
     __syncthreads();
   }
-  // all threads add the list up alike, left to right
-  double total = 0.0, run = 0.0;
-  for (int j = 0; j < K; j++) total += w_list[j];
-  int pick = K - 1;
-  for (int j = 0; j < K; j++) {
-    run += w_list[j];
-    if (run > u * total) {
-      pick = j;
-      break;
+  // the running sums of the list, four entries a lane
+  if (tid < 32) {
+    double run[4], from = 0.0;
+#pragma unroll
+    for (int u = 0; u < 4; u++) run[u] = from += 4 * tid + u < K ? w_list[4 * tid + u] : 0.0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double up = __shfl_up_sync(0xffffffffu, from, o);
+      if (tid >= o) from += up;
     }
+    const double goal = u01 * __shfl_sync(0xffffffffu, from, 31);
+    from = __shfl_up_sync(0xffffffffu, from, 1);
+    if (tid == 0) from = 0.0;
+    int pick = 127, last = -1;
+#pragma unroll
+    for (int u = 3; u >= 0; u--) {
+      if (from + run[u] > goal) pick = 4 * tid + u;
+      if (4 * tid + u < K && w_list[4 * tid + u] > 0.0) last = max(last, 4 * tid + u);
+    }
+    pick = __reduce_min_sync(0xffffffffu, pick);
+    last = __reduce_max_sync(0xffffffffu, last);
+    if (tid == 0) s_pick = min(pick, last);
   }
-  write_ids(a, s, at, (uint32_t)__ldcg(li + at * K + pick));
+  __syncthreads();
+  write_ids<128>(a, s, at, (uint32_t)__ldcg(a.list_id + (base + at) * K + s_pick), tid);
 }
 
 }  // namespace wgpt
