@@ -61,13 +61,6 @@ __device__ __forceinline__ void tma_load_3d_pair(void *dst, const CUtensorMap *m
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(0), "r"(bar_addr)
       : "memory");
 }
-// Low word of umma_desc_sw128 (start address) and its constant high word. One lane issues every MMA of an SM, so what an
-// instruction costs to issue bounds the narrow tiles: the descriptors' low words are sums of a per-stage base and a
-// constant, and the loop around them is run by the whole warp, the lane being elected inside the instruction. Issued
-// from a branch that one lane had taken, an MMA took about 98 cycles whatever its size (operands have to be moved to
-// the uniform registers it reads, one by one); a decode product of 128 x 16 x 832 took 8.4 us, elected 5.5.
-__device__ __forceinline__ uint32_t umma_desc_lo(uint32_t saddr) { return (saddr & 0x3FFFFu) >> 4; }
-constexpr uint32_t kUmmaDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
 __device__ __forceinline__ void umma2_f16(uint32_t tmem_d, uint32_t alo, uint32_t blo, uint32_t idesc,
                                           uint32_t accumulate) {
   asm volatile(
@@ -85,11 +78,6 @@ __device__ __forceinline__ void umma2_commit_elect(uint32_t cluster_addr) {
       "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(cluster_addr)
       : "memory");
 }
-// Instruction descriptor of kind::f16: FP32 accumulate, half A and B, both K-major.
-__host__ __device__ constexpr uint32_t f16_idesc(int m, int n) {
-  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
-}
-
 // gridDim.x = 2 KS x clusters, cluster (2 KS,1,1). Cluster p walks the 256 x bn tiles p, p + clusters, ... (row tile fastest);
 // with KS > 1 there are as many clusters as tiles.
 // map_a: box of 128 rows; map_b: box of bn/2 rows. bn % 32 == 0, bn <= 256.

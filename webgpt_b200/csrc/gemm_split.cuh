@@ -53,16 +53,6 @@ struct SplitArgs {
   int *err;
 };
 
-__device__ __forceinline__ void umma1_f16(uint32_t tmem_d, uint32_t alo, uint32_t blo, uint32_t idesc,
-                                          uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p, e;\n\t.reg .b64 da, db;\n\t"
-      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
-      "setp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(tmem_d),
-      "r"(alo), "r"(blo), "r"(idesc), "r"(accumulate), "r"(kUmmaDescHi)
-      : "memory");
-}
 // Twice 32 lanes x 16 consecutive 32-bit columns, both loads in flight together.
 __device__ __forceinline__ void tmem_ld_2x16(uint32_t t0, uint32_t t1, float (&v)[16], float (&w)[16]) {
   asm volatile(
@@ -74,13 +64,6 @@ __device__ __forceinline__ void tmem_ld_2x16(uint32_t t0, uint32_t t1, float (&v
       : "=&f"(v[0]), "=&f"(v[1]), "=&f"(v[2]), "=&f"(v[3]), "=&f"(v[4]), "=&f"(v[5]), "=&f"(v[6]), "=&f"(v[7]), "=&f"(v[8]), "=&f"(v[9]), "=&f"(v[10]), "=&f"(v[11]), "=&f"(v[12]), "=&f"(v[13]), "=&f"(v[14]), "=&f"(v[15]),
         "=&f"(w[0]), "=&f"(w[1]), "=&f"(w[2]), "=&f"(w[3]), "=&f"(w[4]), "=&f"(w[5]), "=&f"(w[6]), "=&f"(w[7]), "=&f"(w[8]), "=&f"(w[9]), "=&f"(w[10]), "=&f"(w[11]), "=&f"(w[12]), "=&f"(w[13]), "=&f"(w[14]), "=&f"(w[15])
       : "r"(t0), "r"(t1)
-      : "memory");
-}
-// umma_commit by one elected lane of a converged warp.
-__device__ __forceinline__ void umma_commit_elect(uint64_t *bar) {
-  asm volatile(
-      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
-      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar))
       : "memory");
 }
 __device__ __forceinline__ void sts64(uint32_t saddr, uint2 v) {

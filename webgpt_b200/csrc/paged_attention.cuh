@@ -112,6 +112,71 @@ __device__ __forceinline__ void paged_part(const PagedAttention &a, PagedPart &w
   w.n_tiles = max(0, min((int)(w.next - w.begin), (w.g.highest - q.begin + unit - 1) / unit) - w.u0);
 }
 
+// A CTA's units [first, end) of all there are and the part they begin with, by all its threads (behind it a barrier of theirs):
+// false if there are none. sums: a number for each warp.
+__device__ __forceinline__ bool paged_first(const PagedAttention &a, PagedPart &to, int unit, uint32_t *sums, uint32_t &per, uint32_t &end) {
+  const int threads = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_seq = a.c.n_seq;
+  PagedSeq q;
+  auto weight_of = [&](int s) -> uint32_t {
+    if (s >= n_seq) return 0;
+    q = paged_seq(a, s, unit);
+    return paged_work(a, q);
+  };
+  auto scan = [&](uint32_t mine, uint32_t &all) {  // sum over the threads before this one, and over all
+    uint32_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    all = 0;
+    for (int w = 0; w < threads / 32; w++) {
+      if (w < warp) upto += sums[w];
+      all += sums[w];
+    }
+    return upto - mine;
+  };
+  uint32_t total = 0, mine = 0, before = 0;
+  for (int s0 = 0; s0 < n_seq; s0 += threads) {
+    uint32_t all;
+    mine = weight_of(s0 + tid);
+    before = total + scan(mine, all);
+    total += all;
+  }
+  per = max((uint32_t)a.least, (total + gridDim.x - 1) / gridDim.x);
+  const uint32_t x0 = blockIdx.x * per, x1 = min(total, x0 + per);  // the caller sees to it that neither passes 2^32
+  if (x0 >= x1) return false;
+  end = x1;
+  if (n_seq <= threads) {
+    if (before <= x0 && x0 < before + mine) paged_part(a, to, q, tid, before, x0, x1, unit);
+  } else {
+    uint32_t sum = 0;
+    for (int s0 = 0; s0 < n_seq && sum <= x0; s0 += threads) {
+      uint32_t all;
+      mine = weight_of(s0 + tid);
+      before = sum + scan(mine, all);
+      if (before <= x0 && x0 < before + mine) paged_part(a, to, q, s0 + tid, before, x0, x1, unit);
+      sum += all;
+    }
+  }
+  return true;
+}
+
+// The part behind `w`, which ends before unit `end`. May not be `w` itself.
+__device__ __forceinline__ void paged_next(const PagedAttention &a, PagedPart &to, const PagedPart &w, uint32_t end, int unit) {
+  uint32_t seq_begin = w.seq_begin;
+  PagedSeq q = w.q;
+  int s = w.g.s;
+  while (w.next >= seq_begin + paged_work(a, q)) {
+    seq_begin += paged_work(a, q);
+    q = paged_seq(a, ++s, unit);
+  }
+  paged_part(a, to, q, s, seq_begin, w.next, end, unit);
+}
+
 // Copies 16 bytes, or writes zeros where there is nothing to copy.
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t to, const void *from, bool there) {
   const int bytes = there ? 16 : 0;
@@ -336,6 +401,72 @@ __device__ __forceinline__ uint32_t split2(float &x, float &y) {
 }
 
 
+// Joins a group's parts once this CTA's lies in its slot: the CTA that finishes last does, in the order of the positions. By
+// `threads` threads that meet in sync(); red and red_sum: a place for each of them.
+template <typename Sync>
+__device__ __forceinline__ void paged_join(const PagedAttention &a, const PagedPart &w, int first_cta, int parts, int ROWS, int tid,
+                                           int threads, Sync sync, float4 *red, float *red_sum, int *is_last) {
+  const int hs = a.c.hs, quads = hs / 4, items = w.g.rows * quads, slot_floats = paged_slot(ROWS, hs);
+  __threadfence();
+  sync();
+  if (tid == 0) {
+    const unsigned int done = atomicAdd(a.join + first_cta, 1u);
+    *is_last = done == (unsigned)parts - 1;
+    if (*is_last) a.join[first_cta] = 0;
+  }
+  sync();
+  if (!*is_last) return;
+  __threadfence();
+  // where a row tile has few values, several threads share a quad and take every so many parts
+  auto part_of = [&](int k) { return a.partial + (2ll * (first_cta + k) + (k == 0 ? 1 : 0)) * slot_floats; };
+  const int share = items >= threads ? 1 : threads / items;
+  for (int i0 = 0; i0 < items; i0 += threads) {
+    const int i = share > 1 ? tid % items : i0 + tid, sh = share > 1 ? tid / items : 0;
+    const bool live = i < items && sh < share;
+    const int r = live ? i / quads : 0;
+    float top = -INFINITY, sum = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (live) {
+#pragma unroll 8
+      for (int k = 0; k < parts; k++) top = fmaxf(top, __ldcg(part_of(k) + ROWS * hs + r));
+#pragma unroll 8
+      for (int k = sh; k < parts; k += share) {
+        const float *part = part_of(k);
+        const float m = __ldcg(part + ROWS * hs + r), l = __ldcg(part + ROWS * hs + ROWS + r);
+        const float4 o = __ldcg(reinterpret_cast<const float4 *>(part) + i);
+        const float f = m == -INFINITY && l == 0.f ? 0.f : exp2f(m - top);
+        sum += f * l;
+        v.x += f * o.x;
+        v.y += f * o.y;
+        v.z += f * o.z;
+        v.w += f * o.w;
+      }
+    }
+    if (share > 1) {
+      red[tid] = v;
+      red_sum[tid] = sum;
+      sync();
+      if (tid < items)
+        for (int y = 1; y < share; y++) {
+          const float4 o = red[y * items + tid];
+          v.x += o.x;
+          v.y += o.y;
+          v.z += o.z;
+          v.w += o.w;
+          sum += red_sum[y * items + tid];
+        }
+    }
+    if (live && sh == 0) {
+      if (sum != 0.f) {
+        const float inv = 1.f / sum;
+        v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+      }
+      reinterpret_cast<float4 *>(a.out + row_offset(a, w, r, a.ld_out))[i - r * quads] = v;
+      if (a.stats && i == r * quads) a.stats[row_index(a, w, r)] = top + log2f(sum);
+    }
+  }
+}
+
 template <typename T, int HSP, int RT, int STAGES>
 __global__ void __launch_bounds__(sizeof(T) == 4 ? 128 : 32 * kPagedWarps, sizeof(T) == 4 ? (HSP <= 64 ? 3 : HSP <= 128 ? 2 : 1) : HSP <= 128 ? 2 : 1)
 paged_attention_kernel(const __grid_constant__ PagedAttention a) {
@@ -377,52 +508,9 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
   if (padded) clear(ring_smem, S::kRing);
   pdl_wait();
 
-  // ---- this CTA's units: [x0, x1)
-  PagedSeq q;
-  auto weight_of = [&](int s) -> uint32_t {
-    if (s >= c.n_seq) return 0;
-    q = paged_seq(a, s, unit);
-    return paged_work(a, q);
-  };
-  auto scan = [&](uint32_t mine, uint32_t &all) {  // sum over the threads before this one, and over all
-    uint32_t upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += x;
-    }
-    __syncthreads();
-    if (lane == 31) s_sum[warp] = upto;
-    __syncthreads();
-    all = 0;
-    for (int w = 0; w < threads / 32; w++) {
-      if (w < warp) upto += s_sum[w];
-      all += s_sum[w];
-    }
-    return upto - mine;
-  };
-  uint32_t total = 0, mine = 0, before = 0;
-  for (int s0 = 0; s0 < c.n_seq; s0 += threads) {
-    uint32_t all;
-    mine = weight_of(s0 + tid);
-    before = total + scan(mine, all);
-    total += all;
-  }
-  const uint32_t per = max((uint32_t)a.least, (total + gridDim.x - 1) / gridDim.x);
-  const uint32_t x0 = blockIdx.x * per, x1 = min(total, x0 + per);  // the caller sees to it that neither passes 2^32
-  if (x0 >= x1) return;
-  if (c.n_seq <= threads) {
-    if (before <= x0 && x0 < before + mine) paged_part(a, s_part[0], q, tid, before, x0, x1, unit);
-  } else {
-    uint32_t sum = 0;
-    for (int s0 = 0; s0 < c.n_seq && sum <= x0; s0 += threads) {
-      uint32_t all;
-      mine = weight_of(s0 + tid);
-      before = sum + scan(mine, all);
-      if (before <= x0 && x0 < before + mine) paged_part(a, s_part[0], q, s0 + tid, before, x0, x1, unit);
-      sum += all;
-    }
-  }
+  // ---- this CTA's units: [.., x1)
+  uint32_t per, x1;
+  if (!paged_first(a, s_part[0], unit, s_sum, per, x1)) return;
   __syncthreads();
 
   PagedRing<T, HSP, RT, STAGES> ring(c, smem_addr(ring_smem), s_ok[kg], lane, unit, rw, RW);
@@ -433,17 +521,8 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
     const PagedGroup &g = w.g;
     // ---- the next part, by a thread that has no query to load first
     if (tid == threads - 1) {
-      uint32_t x = w.next, seq_begin = w.seq_begin;
-      s_more = x < x1;
-      if (x < x1) {
-        PagedSeq nq = w.q;
-        int s = g.s;
-        while (x >= seq_begin + paged_work(a, nq)) {
-          seq_begin += paged_work(a, nq);
-          nq = paged_seq(a, ++s, unit);
-        }
-        paged_part(a, s_part[turn ^ 1], nq, s, seq_begin, x, x1, unit);
-      }
+      s_more = w.next < x1;
+      if (w.next < x1) paged_next(a, s_part[turn ^ 1], w, x1, unit);
     }
     // ---- the queries
     if constexpr (S::kWide) {
@@ -826,67 +905,8 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
         }
       }
     }
-    if (parts > 1) {
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) {
-        const unsigned int done = atomicAdd(a.join + first_cta, 1u);
-        s_last = done == (unsigned)parts - 1;
-        if (s_last) a.join[first_cta] = 0;
-      }
-      __syncthreads();
-      if (s_last) {
-        __threadfence();
-        // where a row tile has few values, several threads share a quad and take every so many parts
-        auto part_of = [&](int k) { return a.partial + (2ll * (first_cta + k) + (k == 0 ? 1 : 0)) * slot_floats; };
-        const int share = items >= threads ? 1 : threads / items;
-        for (int i0 = 0; i0 < items; i0 += threads) {
-          const int i = share > 1 ? tid % items : i0 + tid, sh = share > 1 ? tid / items : 0;
-          const bool live = i < items && sh < share;
-          const int r = live ? i / quads : 0;
-          float top = -INFINITY, sum = 0.f;
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (live) {
-#pragma unroll 8
-            for (int k = 0; k < parts; k++) top = fmaxf(top, __ldcg(part_of(k) + ROWS * hs + r));
-#pragma unroll 8
-            for (int k = sh; k < parts; k += share) {
-              const float *part = part_of(k);
-              const float m = __ldcg(part + ROWS * hs + r), l = __ldcg(part + ROWS * hs + ROWS + r);
-              const float4 o = __ldcg(reinterpret_cast<const float4 *>(part) + i);
-              const float f = m == -INFINITY && l == 0.f ? 0.f : exp2f(m - top);
-              sum += f * l;
-              v.x += f * o.x;
-              v.y += f * o.y;
-              v.z += f * o.z;
-              v.w += f * o.w;
-            }
-          }
-          if (share > 1) {
-            s_red[tid] = v;
-            s_red_sum[tid] = sum;
-            __syncthreads();
-            if (tid < items)
-              for (int y = 1; y < share; y++) {
-                const float4 o = s_red[y * items + tid];
-                v.x += o.x;
-                v.y += o.y;
-                v.z += o.z;
-                v.w += o.w;
-                sum += s_red_sum[y * items + tid];
-              }
-          }
-          if (live && sh == 0) {
-            if (sum != 0.f) {
-              const float inv = 1.f / sum;
-              v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-            }
-            reinterpret_cast<float4 *>(a.out + row_offset(a, w, r, a.ld_out))[i - r * quads] = v;
-            if (a.stats && i == r * quads) a.stats[row_index(a, w, r)] = top + log2f(sum);
-          }
-        }
-      }
-    }
+    if (parts > 1)
+      paged_join(a, w, first_cta, parts, ROWS, tid, threads, [] { __syncthreads(); }, s_red, s_red_sum, &s_last);
     __syncthreads();
     if (!more) break;
     if (padded) clear(reinterpret_cast<unsigned char *>(o_smem), a.ahead ? S::kTileBytes : S::kRing);

@@ -1,0 +1,470 @@
+// Attention over a paged cache of half-precision values for more than eight rows that share a head of the cache (grouped heads,
+// drafts, prompts), head sizes up to 128, on tcgen05: the mathematics, the equal shares and the joining of
+// paged_attention_kernel. There every warp's path of loading fragments, eight rows at a time, is what bounds such calls.
+//
+// Keys are the instruction's 128 lanes and query rows its columns: S^T = K Q^T from shared memory (the key tile as it lies, the
+// queries as the sum of two half or three bfloat16 values), so that a thread of the four softmax warps has one key and all the
+// rows. Its probabilities, split the same way, go back to shared memory as the second operand of O^T = V^T P^T, whose first is
+// the value tile as it lies, MN-major; there a thread has one dimension and all the rows. A tile's O is added to f32 sums in
+// registers, so that nothing is accumulated across tiles in tensor memory, whose additions cut off.
+//
+// A row's maximum would have to be found across the lanes. The exponents are taken relative to a reference instead, a whole
+// number at or above the first tile's maximum, that is raised only when some score of a tile is more than 2^kSlack above it: one vote
+// a tile, and the maxima across lanes only then.
+//   warps 0-3   softmax and sums;
+//   warp 4      issues the MMAs: the next tile's scores before this tile's values;
+//   warps 5-8   fill a ring of tiles by cp.async, 32 rows each, in the order in which they are used up: K0 K1 V0 K2 V1 ...
+// Every wait is bounded; on expiry *err = 3 and the result is void.
+#pragma once
+#include "paged_attention.cuh"
+#include "tcgen05.cuh"
+
+namespace wgpt {
+
+constexpr int kTcKeys = 128, kTcThreads = 288, kTcBlock = kTcKeys * 128;  // positions of a tile; bytes of 64 dimensions of one
+constexpr float kSlack = 8.f;
+
+// HB: blocks of 64 dimensions; N: rows of a row tile
+template <typename T, int HB, int N>
+struct TcShape {
+  static constexpr int kTerms = std::is_same<T, __half>::value ? 2 : 3;
+  static constexpr int kStage = HB * kTcBlock;
+  static constexpr int kP = kTerms * kTcBlock, kQ = kTerms * HB * N * 128;
+  static constexpr int kFit = (int)(((220 << 10) - kP - kQ) / kStage);
+  static constexpr int kStages = kFit < 8 ? kFit : 8;
+  static constexpr int kLag = kStages - 2;  // tiles whose copies are in flight behind the one that is waited for
+  static constexpr int kSmem = 1024 + kStages * kStage + kP + kQ;
+  static_assert(kStages >= 4, "");
+};
+
+template <int N>
+__device__ __forceinline__ void tmem_ld_rows(uint32_t taddr, float (&v)[N]) {
+  if constexpr (N == 32) {
+    tmem_ld_32x32(taddr, v);
+  } else {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int j = 0; j < 16; j++) v[j] = __uint_as_float(r[j]);
+  }
+}
+
+template <typename T, int HB, int N>
+__global__ void __launch_bounds__(kTcThreads, 1) paged_attention_tc_kernel(const __grid_constant__ PagedAttention a) {
+  using S = TcShape<T, HB, N>;
+  constexpr int TERMS = S::kTerms, NS = S::kStages;
+  constexpr float kLift = TERMS == 2 ? 7.f : 0.f;  // probabilities up to 2^(kSlack + kLift), in a half's range
+  extern __shared__ uint8_t tc_raw[];
+  uint8_t *stages = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(tc_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t *Ps = stages + NS * S::kStage, *Qs = Ps + S::kP;
+  __shared__ uint64_t full[NS], empty[NS], q_ready, s_done[2], p_ready, o_done, drained;
+  __shared__ uint32_t tmem_slot, s_sum[kTcThreads / 32];
+  __shared__ int abort_word, s_last;
+  __shared__ PagedPart s_part;
+  __shared__ __align__(16) float s_qscale[N], s_max[4][N], s_l[N], s_m[N];
+  __shared__ int s_lo[N], s_hi[N];
+  __shared__ long long s_row[N];
+  __shared__ float4 s_red[128];
+  __shared__ float s_red_sum[128];
+  volatile int *abort_flag = &abort_word;
+  const PagedView &c = a.c;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, hs = c.hs;
+  if (tid == 0) {
+    for (int i = 0; i < NS; i++) {
+      mbar_init(&full[i], 4);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(&q_ready, 4);
+    mbar_init(&s_done[0], 1);
+    mbar_init(&s_done[1], 1);
+    mbar_init(&p_ready, 4);
+    mbar_init(&o_done, 1);
+    mbar_init(&drained, 1);
+    abort_word = 0;
+    fence_async_smem();
+  }
+  if (warp == 4) tmem_alloc(&tmem_slot, 128);  // scores of two tiles at 0 and 32, values at 64
+  if (hs & 63)  // what lies behind a row's end takes part in products: zeros
+    for (int i = tid; i < NS * S::kStage / 16; i += kTcThreads) reinterpret_cast<uint4 *>(stages)[i] = make_uint4(0, 0, 0, 0);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  pdl_launch_dependents();  // behind the allocation: the next kernel's CTAs may want tensor memory too
+  pdl_wait();
+
+  uint32_t per = 1, x1 = 0;
+  const bool any = paged_first(a, s_part, kTcKeys, s_sum, per, x1);
+  __syncthreads();
+  // A wait that has run out makes all others return at once: every role runs to its end.
+  auto wait = [&](uint64_t *bar, uint32_t parity) {
+    if (!*abort_flag && !mbar_wait(bar, parity & 1, TC_POLLS)) *abort_flag = 1;
+    __syncwarp();
+  };
+
+  if (any && warp < 4) {
+    // ------------------------------------------------------------------ softmax and sums
+    PagedPart w = s_part;
+    const uint32_t lanes = tmem + ((uint32_t)(32 * warp) << 16);
+    const int key = tid;  // of a tile, and the dimension whose sums this thread has
+    uint32_t tile = 0;    // of all parts
+    auto meet = [] { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); };
+    auto some = [&](bool x) -> bool {  // in any thread of the four warps
+      int r;
+      asm volatile(
+          "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+          : "=r"(r)
+          : "r"((int)x)
+          : "memory");
+      return r != 0;
+    };
+    for (;;) {
+      const int rows = w.g.rows, n_tiles = w.n_tiles;
+      // ---- the queries: K-major rows of 128 bytes, 16-byte pieces swizzled
+      if (n_tiles > 0) {
+        for (int r = warp; r < N; r += 4) {
+          float v[2 * HB], top = 0.f;
+          const float *row = r < rows ? a.q + row_offset(a, w, r, a.ld_q) : nullptr;
+#pragma unroll
+          for (int i = 0; i < HB; i++) {
+            const int d = 2 * lane + 64 * i;
+            const float2 f = row && d < hs ? __ldcg(reinterpret_cast<const float2 *>(row + d)) : make_float2(0.f, 0.f);
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+          int e = 0;
+          if constexpr (TERMS == 2) {  // a power of two that brings the row's largest value near 2^13
+            top = warp_max(top);
+            e = top > 0.f && top < INFINITY ? ilogbf(top) - 13 : 0;
+          }
+#pragma unroll
+          for (int i = 0; i < HB; i++) {
+            float f0 = scalbnf(v[2 * i], -e), f1 = scalbnf(v[2 * i + 1], -e);
+#pragma unroll
+            for (int t = 0; t < TERMS; t++)
+              *reinterpret_cast<uint32_t *>(Qs + ((t * HB + i) * N + r) * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) =
+                  split2<T>(f0, f1);
+          }
+          if (lane == 0) s_qscale[r] = scalbnf(a.scale2, e);
+        }
+      }
+      if (tid < N) {
+        int lo = 0, hi = 0;
+        if (tid < rows) row_range(a, w.q, (w.g.r0 + tid) / a.group, lo, hi);
+        s_lo[tid] = lo;
+        s_hi[tid] = hi;
+        if (a.scores) s_row[tid] = row_index(a, w, tid) * c.max_length;
+      }
+      fence_async_smem();
+      meet();
+      if (n_tiles > 0 && lane == 0) mbar_arrive(&q_ready);
+      float m[N], l[N], o[N];
+#pragma unroll
+      for (int r = 0; r < N; r++) {
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+        o[r] = 0.f;
+      }
+      int pos = w.q.begin + w.u0 * kTcKeys + key;
+      const uint32_t *table = c.table + (size_t)w.g.s * c.table_stride;
+      auto page_of = [&](int p) -> uint32_t {  // asked for a tile ahead
+        if (p < w.g.lowest || p >= w.g.highest) return 0xFFFFFFFFu;
+        return __ldcg(table + (c.page_shift >= 0 ? (uint32_t)p >> c.page_shift : (uint32_t)p / c.page_size));
+      };
+      uint32_t page = n_tiles > 0 ? page_of(pos) : 0u;
+      auto add_values = [&](uint32_t i) {  // of tile i
+        wait(&o_done, i);
+        tc_fence_after();
+        float v[N];
+        tmem_ld_rows<N>(lanes + 64, v);
+#pragma unroll
+        for (int r = 0; r < N; r++) o[r] += v[r];
+      };
+      for (int t = 0; t < n_tiles; t++, tile++, pos += kTcKeys) {
+        const bool there = page < c.n_pages;
+        page = t + 1 < n_tiles ? page_of(pos + kTcKeys) : 0u;
+        wait(&s_done[tile & 1], tile >> 1);
+        tc_fence_after();
+        float x[N];
+        tmem_ld_rows<N>(lanes + 32 * (tile & 1), x);
+        const int pos0 = pos - key;
+        const bool whole = pos0 >= w.g.inner_low && pos0 + kTcKeys <= w.g.inner_high;
+#pragma unroll
+        for (int r = 0; r < N; r += 4) {
+          const float4 qs = *reinterpret_cast<const float4 *>(s_qscale + r);
+          x[r] *= qs.x;
+          x[r + 1] *= qs.y;
+          x[r + 2] *= qs.z;
+          x[r + 3] *= qs.w;
+        }
+        if (!whole || !there) {
+#pragma unroll
+          for (int r = 0; r < N; r++)
+            if (!(there && pos >= s_lo[r] && pos < s_hi[r])) x[r] = -INFINITY;
+        }
+        if (a.scores) {
+#pragma unroll
+          for (int r = 0; r < N; r++)
+            if (r < rows && pos >= s_lo[r] && pos < s_hi[r]) a.scores[s_row[r] + pos] = x[r];
+        }
+        bool far = false;
+#pragma unroll
+        for (int r = 0; r < N; r++) far |= x[r] > m[r] + kSlack;
+        if (t > 0) add_values(tile - 1);
+        tc_fence_before();
+        __syncwarp();
+        if (some(far)) {  // raise the references of the rows that need it
+#pragma unroll
+          for (int r = 0; r < N; r++) {
+            float top = x[r];
+#pragma unroll
+            for (int y = 16; y > 0; y >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, y));
+            if (lane == 0) s_max[warp][r] = top;
+          }
+          meet();
+#pragma unroll
+          for (int r = 0; r < N; r++) {
+            const float top = ceilf(fmaxf(fmaxf(s_max[0][r], s_max[1][r]), fmaxf(s_max[2][r], s_max[3][r])));
+            if (top > m[r]) {
+              const float f = exp2f(m[r] - top);
+              l[r] *= f;
+              o[r] *= f;
+              m[r] = top;
+            }
+          }
+          meet();  // before the maxima are written again
+        }
+        // ---- probabilities: MN-major rows of 128 bytes, a key each, 16-byte pieces of eight rows swizzled
+#pragma unroll
+        for (int g = 0; g < N / 8; g++) {
+          uint32_t words[TERMS][4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int r = 8 * g + 2 * i;
+            float p0 = x[r] == -INFINITY ? 0.f : exp2_of(x[r] - (m[r] - kLift));
+            float p1 = x[r + 1] == -INFINITY ? 0.f : exp2_of(x[r + 1] - (m[r + 1] - kLift));
+            l[r] += p0;
+            l[r + 1] += p1;
+#pragma unroll
+            for (int u = 0; u < TERMS; u++) words[u][i] = split2<T>(p0, p1);
+          }
+#pragma unroll
+          for (int u = 0; u < TERMS; u++)
+            *reinterpret_cast<uint4 *>(Ps + u * kTcBlock + key * 128 + ((g ^ (key & 7)) << 4)) =
+                make_uint4(words[u][0], words[u][1], words[u][2], words[u][3]);
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready);
+      }
+      if (n_tiles > 0) add_values(tile - 1);
+      tc_fence_before();
+      // ---- the rows' sums over the keys
+      const float down = kLift != 0.f ? 1.f / 128.f : 1.f;
+      bool finite = true;
+#pragma unroll
+      for (int r = 0; r < N; r++) {
+        const float sum = warp_sum(l[r]);
+        if (lane == 0) s_max[warp][r] = sum;
+        o[r] *= down;
+        finite = finite && (r >= rows || key >= hs || fabsf(o[r]) < INFINITY);
+      }
+      meet();
+      if (tid < N) {
+        s_l[tid] = ((s_max[0][tid] + s_max[1][tid]) + (s_max[2][tid] + s_max[3][tid])) * down;
+        finite = finite && (tid >= rows || fabsf(s_l[tid]) < INFINITY);
+      }
+#pragma unroll
+      for (int r = 0; r < N; r++)
+        if (tid == r) s_m[r] = m[r];
+      if (some(!finite)) {  // each row from what it sees alone, in the probabilities' place
+        float *values = reinterpret_cast<float *>(Ps);
+        const int share = (rows + 3) / 4;
+        paged_rows_apart<T, kTcKeys>(a, w, 0, 1, warp * share, min(rows, warp * share + share), lane, values, s_m, s_l);
+        meet();
+#pragma unroll
+        for (int r = 0; r < N; r++)
+          if (r < rows && key < hs) o[r] = values[r * hs + key];
+        meet();
+      }
+      // ---- the result, or this part of it
+      const int first_cta = (int)(w.begin / per), last_cta = (int)((w.end - 1) / per), parts = last_cta - first_cta + 1;
+      float *slot = a.partial + (2ll * blockIdx.x + ((int)blockIdx.x == first_cta ? 1 : 0)) * paged_slot(N, hs);
+#pragma unroll
+      for (int r = 0; r < N; r++) {
+        if (r < rows && key < hs) {
+          if (parts == 1)
+            a.out[row_offset(a, w, r, a.ld_out) + key] = s_l[r] != 0.f ? o[r] / s_l[r] : 0.f;
+          else
+            __stcg(slot + r * hs + key, o[r]);
+        }
+      }
+      if (tid < rows) {
+        if (parts > 1) {
+          __stcg(slot + N * hs + tid, s_m[tid]);
+          __stcg(slot + N * hs + N + tid, s_l[tid]);
+        } else if (a.stats) {
+          a.stats[row_index(a, w, tid)] = s_m[tid] + log2f(s_l[tid]);
+        }
+      }
+      if (parts > 1) paged_join(a, w, first_cta, parts, N, tid, 128, meet, s_red, s_red_sum, &s_last);
+      if (w.next >= x1) break;
+      meet();
+      const PagedPart before = w;
+      paged_next(a, w, before, x1, kTcKeys);
+    }
+  } else if (any && warp == 4) {
+    // ------------------------------------------------------------------ products: the whole warp runs this, one lane issues
+    PagedPart w = s_part;
+    constexpr uint32_t kType = TERMS == 2 ? 0u : (1u << 7) | (1u << 10);
+    constexpr uint32_t idesc_s = f16_idesc(128, N) | kType, idesc_o = idesc_s | (1u << 15) | (1u << 16);  // values and probabilities: MN-major
+    const uint32_t st0 = umma_desc_lo(smem_addr(stages)), p0 = umma_desc_lo(smem_addr(Ps)), q0 = umma_desc_lo(smem_addr(Qs));
+    uint32_t tile = 0, use = 0, part = 0;  // of all parts: tiles, stages used up, parts with tiles
+    auto scores = [&](uint32_t i) {
+      const uint32_t st = use % NS;
+      wait(&full[st], use / NS);
+      tc_fence_after();
+      const uint32_t d = tmem + 32 * (i & 1), k = st0 + st * (S::kStage >> 4);
+#pragma unroll
+      for (int u = TERMS - 1; u >= 0; u--)  // the smallest terms first
+#pragma unroll
+        for (int b = 0; b < HB; b++)
+#pragma unroll
+          for (int s = 0; s < 4; s++)
+            umma1_f16(d, k + b * (kTcBlock >> 4) + 2 * s, q0 + (u * HB + b) * (N * 128 >> 4) + 2 * s, idesc_s,
+                      u < TERMS - 1 || b > 0 || s > 0 ? 1u : 0u);
+      umma_commit_elect(&s_done[i & 1]);
+      umma_commit_elect(&empty[st]);
+      use++;
+    };
+    for (;;) {
+      const int n_tiles = w.n_tiles;
+      if (n_tiles > 0) {
+        wait(&q_ready, part++);
+        scores(tile);
+        for (int t = 0; t < n_tiles; t++, tile++) {
+          if (t + 1 < n_tiles) scores(tile + 1);
+          const uint32_t st = use % NS;
+          wait(&full[st], use / NS);
+          wait(&p_ready, tile);
+          tc_fence_after();
+          // 16 keys a step; the block of dimensions from 64 on lies kTcBlock further (with one block, the same once more)
+          const uint32_t v = (st0 + st * (S::kStage >> 4)) | (HB > 1 ? (uint32_t)(kTcBlock >> 4) << 16 : 0u);
+#pragma unroll
+          for (int u = TERMS - 1; u >= 0; u--)
+#pragma unroll
+            for (int s = 0; s < kTcKeys / 16; s++)
+              umma1_f16(tmem + 64, v + s * (2048 >> 4), p0 + u * (kTcBlock >> 4) + s * (2048 >> 4), idesc_o, u < TERMS - 1 || s > 0 ? 1u : 0u);
+          umma_commit_elect(&o_done);
+          umma_commit_elect(&empty[st]);
+          use++;
+        }
+      }
+      if (w.next >= x1) break;
+      const PagedPart before = w;
+      paged_next(a, w, before, x1, kTcKeys);
+    }
+    if (*abort_flag) {  // what has been issued ends before its operands go
+      umma_commit_elect(&drained);
+      mbar_wait(&drained, 0, TC_POLLS);
+    }
+  } else if (any) {
+    // ------------------------------------------------------------------ copies
+    PagedPart w = s_part;
+    constexpr int kLanes = 8 * HB, kAtOnce = 32 / kLanes;  // lanes that share a row
+    const int lw = warp - 5, piece = lane % kLanes, sub = lane / kLanes;
+    const bool mine = piece * 8 < hs;  // 8 values a piece
+    const uint32_t st0 = smem_addr(stages) + (piece >> 3) * kTcBlock + (32 * lw + sub) * 128;
+    uint32_t fills = 0, arrived = 0;
+    auto arrive = [&]() {  // a stage whose copies have landed
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[arrived % NS]);
+      arrived++;
+    };
+    auto fill = [&](const T *from, long long at, bool plain) {
+      const uint32_t st = fills % NS;
+      wait(&empty[st], fills / NS + 1);  // the first use of a stage waits for nothing
+      const uint32_t to = st0 + st * S::kStage;
+      const char *base = reinterpret_cast<const char *>(from + (long long)sub * c.position_stride) + piece * 16;
+      const long long step = (long long)kAtOnce * c.position_stride * 2;
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+        const char *p = base + __shfl_sync(0xffffffffu, at, 16 * b) * 2;
+#pragma unroll
+        for (int i = 0; i < 16 / kAtOnce; i++) {
+          const int row = 16 * b + i * kAtOnce;  // and sub
+          const uint32_t dst = to + row * 128 + (((piece & 7) ^ ((row + sub) & 7)) << 4);
+          if (plain) {
+            if (mine) cp_async16(dst, p);
+            p += step;
+          } else {
+            const long long x = __shfl_sync(0xffffffffu, at, row + sub);
+            if (mine) cp_async16_or_zero(dst, reinterpret_cast<const char *>(from + (x < 0 ? 0 : x)) + piece * 16, x >= 0);
+          }
+        }
+      }
+      cp_async_commit();
+      fills++;
+      if (fills > S::kLag) {
+        cp_async_wait<S::kLag>();
+        arrive();
+      }
+    };
+    for (;;) {
+      const T *k = static_cast<const T *>(c.k) + w.g.kvh * c.head_stride, *v = static_cast<const T *>(c.v) + w.g.kvh * c.head_stride;
+      const uint32_t *table = c.table + (size_t)w.g.s * c.table_stride;
+      int pos = w.q.begin + w.u0 * kTcKeys + 32 * lw + lane;
+      uint32_t page = 0xFFFFFFFFu, slot = 0;
+      auto look_up = [&]() {
+        page = 0xFFFFFFFFu;
+        if (pos >= w.g.lowest && pos < w.g.highest) {
+          const uint32_t index = c.page_shift >= 0 ? (uint32_t)pos >> c.page_shift : (uint32_t)pos / c.page_size;
+          slot = (uint32_t)pos - index * c.page_size;
+          page = __ldcg(table + index);
+        }
+      };
+      if (w.n_tiles > 0) look_up();
+      long long before_at = -1;
+      bool before_plain = false;
+      for (int t = 0; t <= w.n_tiles; t++) {
+        long long at = -1;
+        bool plain = false;
+        if (t < w.n_tiles) {
+          if (page < c.n_pages)
+            at = (long long)page * c.page_stride + (long long)slot * c.position_stride;
+          else if (pos >= w.g.lowest && pos < w.g.highest)
+            *c.err = kErrCache;
+          plain = c.page_size % 16 == 0 && __all_sync(0xffffffffu, at >= 0);
+          pos += kTcKeys;
+          if (t + 1 < w.n_tiles) look_up();
+          fill(k, at, plain);
+        }
+        if (t > 0) fill(v, before_at, before_plain);
+        before_at = at;
+        before_plain = plain;
+      }
+      if (w.next >= x1) break;
+      const PagedPart before = w;
+      paged_next(a, w, before, x1, kTcKeys);
+    }
+    cp_async_wait<0>();
+    while (arrived < fills) arrive();
+  }
+  __syncthreads();
+  if (tid == 0 && *abort_flag) atomicExch(c.err, 3);
+  if (warp == 4) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 128);
+  }
+}
+
+}  // namespace wgpt

@@ -7,6 +7,7 @@
 #include "host.cuh"
 #include "paged.cuh"
 #include "paged_attention.cuh"
+#include "paged_tc.cuh"
 #include "verify.cuh"
 
 using namespace wgpt;
@@ -73,6 +74,25 @@ WGPT_EXPORT int32_t wgpt_paged_append(wgpt_device *dev, const wgpt_paged_cache *
   return WGPT_OK;
 }
 
+// What an attention kernel of this grid and unit takes of the workspace.
+static int32_t paged_workspace(wgpt_device *dev, PagedAttention &a, int grid, int unit) {
+  // units and rows are counted in 32 bits
+  REQUIRE((int64_t)a.r.n_rows * a.group < (int64_t)1 << 30 &&
+              ((int64_t)a.r.n_rows * a.group / a.rows + a.c.n_seq) * (a.c.max_length / unit + 2) <
+                  (((int64_t)1 << 32) - ((int64_t)1 << 20)) / a.c.n_kv,
+          WGPT_ERR_SHAPE, "%d rows over up to %d positions of %d heads: split the call", a.r.n_rows, a.c.max_length, a.c.n_kv);
+  const size_t rows = a.stats ? (size_t)a.r.n_rows * a.n_head : 0, scores = rows * (size_t)a.c.max_length;
+  const size_t partial = (size_t)2 * grid * paged_slot(a.rows, a.c.hs);
+  TRY(scratch_reserve(dev, (partial + rows + scores) * 4));
+  a.partial = static_cast<float *>(dev->scratch);
+  if (a.stats) {
+    a.stats = a.partial + partial;
+    a.scores = a.stats + rows;
+  }
+  a.join = dev->d_join;
+  return WGPT_OK;
+}
+
 template <typename T, int HSP, int RT, int STAGES>
 static int32_t launch_paged_attention(wgpt_device *dev, PagedAttention &a) {
   using S = PagedShape<T, HSP, RT, STAGES>;
@@ -90,22 +110,21 @@ static int32_t launch_paged_attention(wgpt_device *dev, PagedAttention &a) {
   }
   const int grid = std::min(per_sm * dev->sm_count, kJoinCounters);
   REQUIRE(S::fits(a.rows, a.c.hs), WGPT_ERR_UNSUPPORTED, "%d rows of %d do not fit the ring", a.rows, a.c.hs);
-  // units and rows are counted in 32 bits
-  REQUIRE((int64_t)a.r.n_rows * a.group < (int64_t)1 << 30 &&
-              ((int64_t)a.r.n_rows * a.group / a.rows + a.c.n_seq) * (a.c.max_length / unit + 2) < (((int64_t)1 << 32) - ((int64_t)1 << 20)) / a.c.n_kv,
-          WGPT_ERR_SHAPE, "%d rows over up to %d positions of %d heads: split the call", a.r.n_rows, a.c.max_length, a.c.n_kv);
-  const size_t rows = a.stats ? (size_t)a.r.n_rows * a.n_head : 0, scores = rows * (size_t)a.c.max_length;
-  const size_t partial = (size_t)2 * grid * paged_slot(a.rows, a.c.hs);
-  TRY(scratch_reserve(dev, (partial + rows + scores) * 4));
-  a.partial = static_cast<float *>(dev->scratch);
-  if (a.stats) {
-    a.stats = a.partial + partial;
-    a.scores = a.stats + rows;
-  }
-  a.join = dev->d_join;
+  TRY(paged_workspace(dev, a, grid, unit));
   a.ahead = S::ahead(a.rows, a.c.hs);
   a.least = 2;
   LAUNCH_PDL(dev, kernel, grid, threads, smem, a);
+  return WGPT_OK;
+}
+
+template <typename T, int HB, int N>
+static int32_t launch_paged_tc(wgpt_device *dev, PagedAttention &a) {
+  using S = TcShape<T, HB, N>;
+  a.rows = N;
+  TRY(paged_workspace(dev, a, std::min(dev->sm_count, kJoinCounters), kTcKeys));
+  a.least = 1;
+  CK(allow_smem(dev, paged_attention_tc_kernel<T, HB, N>, true));
+  LAUNCH_PDL(dev, (paged_attention_tc_kernel<T, HB, N>), std::min(dev->sm_count, kJoinCounters), kTcThreads, S::kSmem, a);
   return WGPT_OK;
 }
 
@@ -122,6 +141,10 @@ static int32_t launch_paged_rows(wgpt_device *dev, PagedAttention &a, long long 
     if (rows <= 4) return launch_paged_attention<T, HSP, 4, 3>(dev, a);
     return launch_paged_attention<T, HSP, 8, 3>(dev, a);
   } else {
+    if constexpr (HSP <= 128) {
+      if (rows > (getenv("TCROWS") ? atoi(getenv("TCROWS")) : 8))
+        return rows <= 16 ? launch_paged_tc<T, HSP / 64, 16>(dev, a) : launch_paged_tc<T, HSP / 64, 32>(dev, a);
+    }
     const int most = HSP <= 128 ? 4 : 3;
     const long long eights = (rows + 7) / 8, tiles = (eights + most - 1) / most;
     a.row_warps = (int)((eights + tiles - 1) / tiles);
