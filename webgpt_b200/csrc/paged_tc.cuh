@@ -3,17 +3,17 @@
 // paged_attention_kernel. There every warp's path of loading fragments, eight rows at a time, is what bounds such calls.
 //
 // Keys are the instruction's 128 lanes and query rows its columns: S^T = K Q^T from shared memory (the key tile as it lies, the
-// queries as the sum of two half or three bfloat16 values), so that a thread of the four softmax warps has one key and all the
+// queries as the sum of two half or three bfloat16 values), so that a softmax thread has one key and up to 16
 // rows. Its probabilities, split the same way, go back to shared memory as the second operand of O^T = V^T P^T, whose first is
-// the value tile as it lies, MN-major; there a thread has one dimension and all the rows. A tile's O is added to f32 sums in
+// the value tile as it lies, MN-major; there a thread has one dimension and those rows. A tile's O is added to f32 sums in
 // registers, so that nothing is accumulated across tiles in tensor memory, whose additions cut off.
 //
 // A row's maximum would have to be found across the lanes. The exponents are taken relative to a reference instead, a whole
 // number at or above the first tile's maximum, that is raised only when some score of a tile is more than 2^kSlack above it: one vote
 // a tile, and the maxima across lanes only then.
-//   warps 0-3   softmax and sums;
-//   warp 4      issues the MMAs: the next tile's scores before this tile's values;
-//   warps 5-8   fill a ring of tiles by cp.async, 32 rows each, in the order in which they are used up: K0 K1 V0 K2 V1 ...
+//   four warps for every 16 rows: softmax and sums;
+//   one warp    issues the MMAs: the next tile's scores before this tile's values;
+//   four warps  fill a ring of tiles by cp.async, 32 rows each, in the order in which they are used up: K0 K1 V0 K2 V1 ...
 // Every wait is bounded; on expiry *err = 3 and the result is void.
 #pragma once
 #include "paged_attention.cuh"
@@ -21,78 +21,74 @@
 
 namespace wgpt {
 
-constexpr int kTcKeys = 128, kTcThreads = 288, kTcBlock = kTcKeys * 128;  // positions of a tile; bytes of 64 dimensions of one
+constexpr int kTcKeys = 128, kTcBlock = kTcKeys * 128, kTcRows = 16;  // positions of a tile; bytes of 64 dimensions of one; rows of a softmax thread
 constexpr float kSlack = 8.f;
 
 // HB: blocks of 64 dimensions; N: rows of a row tile
 template <typename T, int HB, int N>
 struct TcShape {
   static constexpr int kTerms = std::is_same<T, __half>::value ? 2 : 3;
+  static constexpr int kGroups = N / kTcRows, kSoft = 128 * kGroups, kThreads = kSoft + 32 + 128;
   static constexpr int kStage = HB * kTcBlock;
   static constexpr int kP = kTerms * kTcBlock, kQ = kTerms * HB * N * 128;
   static constexpr int kFit = (int)(((220 << 10) - kP - kQ) / kStage);
   static constexpr int kStages = kFit < 8 ? kFit : 8;
-  static constexpr int kLag = kStages - 2;  // tiles whose copies are in flight behind the one that is waited for
   static constexpr int kSmem = 1024 + kStages * kStage + kP + kQ;
   static_assert(kStages >= 4, "");
 };
 
-template <int N>
-__device__ __forceinline__ void tmem_ld_rows(uint32_t taddr, float (&v)[N]) {
-  if constexpr (N == 32) {
-    tmem_ld_32x32(taddr, v);
-  } else {
-    uint32_t r[16];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr)
-        : "memory");
+// 32 lanes x 16 consecutive 32-bit columns.
+__device__ __forceinline__ void tmem_ld_16(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
 #pragma unroll
-    for (int j = 0; j < 16; j++) v[j] = __uint_as_float(r[j]);
-  }
+  for (int j = 0; j < 16; j++) v[j] = __uint_as_float(r[j]);
 }
 
 template <typename T, int HB, int N>
-__global__ void __launch_bounds__(kTcThreads, 1) paged_attention_tc_kernel(const __grid_constant__ PagedAttention a) {
+__global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attention_tc_kernel(const __grid_constant__ PagedAttention a) {
   using S = TcShape<T, HB, N>;
-  constexpr int TERMS = S::kTerms, NS = S::kStages;
+  constexpr int TERMS = S::kTerms, NS = S::kStages, R = kTcRows, SOFT = S::kSoft, WARPS = SOFT / 32;
   constexpr float kLift = TERMS == 2 ? 7.f : 0.f;  // probabilities up to 2^(kSlack + kLift), in a half's range
   extern __shared__ uint8_t tc_raw[];
   uint8_t *stages = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(tc_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *Ps = stages + NS * S::kStage, *Qs = Ps + S::kP;
   __shared__ uint64_t full[NS], empty[NS], q_ready, s_done[2], p_ready, o_done, drained;
-  __shared__ uint32_t tmem_slot, s_sum[kTcThreads / 32];
+  __shared__ uint32_t tmem_slot, s_sum[S::kThreads / 32];
   __shared__ int abort_word, s_last;
   __shared__ PagedPart s_part;
   __shared__ __align__(16) float s_qscale[N], s_max[4][N], s_l[N], s_m[N];
   __shared__ int s_lo[N], s_hi[N];
   __shared__ long long s_row[N];
-  __shared__ float4 s_red[128];
-  __shared__ float s_red_sum[128];
+  __shared__ float4 s_red[SOFT];
+  __shared__ float s_red_sum[SOFT];
   volatile int *abort_flag = &abort_word;
   const PagedView &c = a.c;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, hs = c.hs;
   if (tid == 0) {
     for (int i = 0; i < NS; i++) {
-      mbar_init(&full[i], 4);
+      mbar_init(&full[i], 128);
       mbar_init(&empty[i], 1);
     }
-    mbar_init(&q_ready, 4);
+    mbar_init(&q_ready, WARPS);
     mbar_init(&s_done[0], 1);
     mbar_init(&s_done[1], 1);
-    mbar_init(&p_ready, 4);
+    mbar_init(&p_ready, WARPS);
     mbar_init(&o_done, 1);
     mbar_init(&drained, 1);
     abort_word = 0;
     fence_async_smem();
   }
-  if (warp == 4) tmem_alloc(&tmem_slot, 128);  // scores of two tiles at 0 and 32, values at 64
+  if (warp == WARPS) tmem_alloc(&tmem_slot, 128);  // scores of two tiles at 0 and 32, values at 64
   if (hs & 63)  // what lies behind a row's end takes part in products: zeros
-    for (int i = tid; i < NS * S::kStage / 16; i += kTcThreads) reinterpret_cast<uint4 *>(stages)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < NS * S::kStage / 16; i += S::kThreads) reinterpret_cast<uint4 *>(stages)[i] = make_uint4(0, 0, 0, 0);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -109,19 +105,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attention_tc_kernel(const
     __syncwarp();
   };
 
-  if (any && warp < 4) {
+  if (any && warp < WARPS) {
     // ------------------------------------------------------------------ softmax and sums
     PagedPart w = s_part;
-    const uint32_t lanes = tmem + ((uint32_t)(32 * warp) << 16);
-    const int key = tid;  // of a tile, and the dimension whose sums this thread has
+    const int quad = warp & 3, r0 = (warp >> 2) * R;  // of the tensor memory's lanes; this thread's rows
+    const uint32_t lanes = tmem + ((uint32_t)(32 * quad) << 16) + r0;
+    const int key = tid & 127;  // of a tile, and the dimension whose sums this thread has
     uint32_t tile = 0;    // of all parts
-    auto meet = [] { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); };
+    auto meet = [] { asm volatile("barrier.cta.sync 1, %0;" ::"n"(SOFT) : "memory"); };
     auto some = [&](bool x) -> bool {  // in any thread of the four warps
       int r;
       asm volatile(
-          "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+          "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, %2, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
           : "=r"(r)
-          : "r"((int)x)
+          : "r"((int)x), "n"(SOFT)
           : "memory");
       return r != 0;
     };
@@ -129,7 +126,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attention_tc_kernel(const
       const int rows = w.g.rows, n_tiles = w.n_tiles;
       // ---- the queries: K-major rows of 128 bytes, 16-byte pieces swizzled
       if (n_tiles > 0) {
-        for (int r = warp; r < N; r += 4) {
+        for (int r = warp; r < N; r += WARPS) {
           float v[2 * HB], top = 0.f;
           const float *row = r < rows ? a.q + row_offset(a, w, r, a.ld_q) : nullptr;
 #pragma unroll
@@ -166,9 +163,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attention_tc_kernel(const
       fence_async_smem();
       meet();
       if (n_tiles > 0 && lane == 0) mbar_arrive(&q_ready);
-      float m[N], l[N], o[N];
+      float m[R], l[R], o[R];
 #pragma unroll
-      for (int r = 0; r < N; r++) {
+      for (int r = 0; r < R; r++) {
         m[r] = -INFINITY;
         l[r] = 0.f;
         o[r] = 0.f;
@@ -183,23 +180,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attention_tc_kernel(const
       auto add_values = [&](uint32_t i) {  // of tile i
         wait(&o_done, i);
         tc_fence_after();
-        float v[N];
-        tmem_ld_rows<N>(lanes + 64, v);
+        float v[R];
+        tmem_ld_16(lanes + 64, v);
 #pragma unroll
-        for (int r = 0; r < N; r++) o[r] += v[r];
+        for (int r = 0; r < R; r++) o[r] += v[r];
       };
       for (int t = 0; t < n_tiles; t++, tile++, pos += kTcKeys) {
         const bool there = page < c.n_pages;
-        page = t + 1 < n_tiles ? page_of(pos + kTcKeys) : 0u;
         wait(&s_done[tile & 1], tile >> 1);
         tc_fence_after();
-        float x[N];
-        tmem_ld_rows<N>(lanes + 32 * (tile & 1), x);
+        float x[R];
+        tmem_ld_16(lanes + 32 * (tile & 1), x);
         const int pos0 = pos - key;
         const bool whole = pos0 >= w.g.inner_low && pos0 + kTcKeys <= w.g.inner_high;
 #pragma unroll
-        for (int r = 0; r < N; r += 4) {
-          const float4 qs = *reinterpret_cast<const float4 *>(s_qscale + r);
+        for (int r = 0; r < R; r += 4) {
+          const float4 qs = *reinterpret_cast<const float4 *>(s_qscale + r0 + r);
           x[r] *= qs.x;
           x[r + 1] *= qs.y;
           x[r + 2] *= qs.z;
@@ -207,32 +203,30 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attention_tc_kernel(const
         }
         if (!whole || !there) {
 #pragma unroll
-          for (int r = 0; r < N; r++)
-            if (!(there && pos >= s_lo[r] && pos < s_hi[r])) x[r] = -INFINITY;
+          for (int r = 0; r < R; r++)
+            if (!(there && pos >= s_lo[r0 + r] && pos < s_hi[r0 + r])) x[r] = -INFINITY;
         }
         if (a.scores) {
 #pragma unroll
-          for (int r = 0; r < N; r++)
-            if (r < rows && pos >= s_lo[r] && pos < s_hi[r]) a.scores[s_row[r] + pos] = x[r];
+          for (int r = 0; r < R; r++)
+            if (r0 + r < rows && pos >= s_lo[r0 + r] && pos < s_hi[r0 + r]) a.scores[s_row[r0 + r] + pos] = x[r];
         }
         bool far = false;
 #pragma unroll
-        for (int r = 0; r < N; r++) far |= x[r] > m[r] + kSlack;
+        for (int r = 0; r < R; r++) far |= x[r] > m[r] + kSlack;
         if (t > 0) add_values(tile - 1);
         tc_fence_before();
         __syncwarp();
         if (some(far)) {  // raise the references of the rows that need it
 #pragma unroll
-          for (int r = 0; r < N; r++) {
-            float top = x[r];
-#pragma unroll
-            for (int y = 16; y > 0; y >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, y));
-            if (lane == 0) s_max[warp][r] = top;
+          for (int r = 0; r < R; r++) {
+            const float top = warp_max(x[r]);
+            if (lane == 0) s_max[quad][r0 + r] = top;
           }
           meet();
 #pragma unroll
-          for (int r = 0; r < N; r++) {
-            const float top = ceilf(fmaxf(fmaxf(s_max[0][r], s_max[1][r]), fmaxf(s_max[2][r], s_max[3][r])));
+          for (int r = 0; r < R; r++) {
+            const float top = ceilf(fmaxf(fmaxf(s_max[0][r0 + r], s_max[1][r0 + r]), fmaxf(s_max[2][r0 + r], s_max[3][r0 + r])));
             if (top > m[r]) {
               const float f = exp2f(m[r] - top);
               l[r] *= f;
@@ -244,7 +238,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attention_tc_kernel(const
         }
         // ---- probabilities: MN-major rows of 128 bytes, a key each, 16-byte pieces of eight rows swizzled
 #pragma unroll
-        for (int g = 0; g < N / 8; g++) {
+        for (int g = 0; g < R / 8; g++) {
           uint32_t words[TERMS][4];
 #pragma unroll
           for (int i = 0; i < 4; i++) {
@@ -258,12 +252,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attention_tc_kernel(const
           }
 #pragma unroll
           for (int u = 0; u < TERMS; u++)
-            *reinterpret_cast<uint4 *>(Ps + u * kTcBlock + key * 128 + ((g ^ (key & 7)) << 4)) =
+            *reinterpret_cast<uint4 *>(Ps + u * kTcBlock + key * 128 + (((r0 / 8 + g) ^ (key & 7)) << 4)) =
                 make_uint4(words[u][0], words[u][1], words[u][2], words[u][3]);
         }
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_ready);
+        page = t + 1 < n_tiles ? page_of(pos + kTcKeys) : 0u;
       }
       if (n_tiles > 0) add_values(tile - 1);
       tc_fence_before();
@@ -271,40 +266,39 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attention_tc_kernel(const
       const float down = kLift != 0.f ? 1.f / 128.f : 1.f;
       bool finite = true;
 #pragma unroll
-      for (int r = 0; r < N; r++) {
+      for (int r = 0; r < R; r++) {
         const float sum = warp_sum(l[r]);
-        if (lane == 0) s_max[warp][r] = sum;
+        if (lane == 0) s_max[quad][r0 + r] = sum;
         o[r] *= down;
-        finite = finite && (r >= rows || key >= hs || fabsf(o[r]) < INFINITY);
+        finite = finite && (r0 + r >= rows || key >= hs || fabsf(o[r]) < INFINITY);
+        if (key == r) s_m[r0 + r] = m[r];
       }
       meet();
       if (tid < N) {
         s_l[tid] = ((s_max[0][tid] + s_max[1][tid]) + (s_max[2][tid] + s_max[3][tid])) * down;
         finite = finite && (tid >= rows || fabsf(s_l[tid]) < INFINITY);
       }
-#pragma unroll
-      for (int r = 0; r < N; r++)
-        if (tid == r) s_m[r] = m[r];
+      __syncwarp();
       if (some(!finite)) {  // each row from what it sees alone, in the probabilities' place
         float *values = reinterpret_cast<float *>(Ps);
-        const int share = (rows + 3) / 4;
+        const int share = (rows + WARPS - 1) / WARPS;
         paged_rows_apart<T, kTcKeys>(a, w, 0, 1, warp * share, min(rows, warp * share + share), lane, values, s_m, s_l);
         meet();
 #pragma unroll
-        for (int r = 0; r < N; r++)
-          if (r < rows && key < hs) o[r] = values[r * hs + key];
+        for (int r = 0; r < R; r++)
+          if (r0 + r < rows && key < hs) o[r] = values[(r0 + r) * hs + key];
         meet();
       }
       // ---- the result, or this part of it
       const int first_cta = (int)(w.begin / per), last_cta = (int)((w.end - 1) / per), parts = last_cta - first_cta + 1;
       float *slot = a.partial + (2ll * blockIdx.x + ((int)blockIdx.x == first_cta ? 1 : 0)) * paged_slot(N, hs);
 #pragma unroll
-      for (int r = 0; r < N; r++) {
-        if (r < rows && key < hs) {
+      for (int r = 0; r < R; r++) {
+        if (r0 + r < rows && key < hs) {
           if (parts == 1)
-            a.out[row_offset(a, w, r, a.ld_out) + key] = s_l[r] != 0.f ? o[r] / s_l[r] : 0.f;
+            a.out[row_offset(a, w, r0 + r, a.ld_out) + key] = s_l[r0 + r] != 0.f ? o[r] / s_l[r0 + r] : 0.f;
           else
-            __stcg(slot + r * hs + key, o[r]);
+            __stcg(slot + (r0 + r) * hs + key, o[r]);
         }
       }
       if (tid < rows) {
@@ -315,13 +309,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attention_tc_kernel(const
           a.stats[row_index(a, w, tid)] = s_m[tid] + log2f(s_l[tid]);
         }
       }
-      if (parts > 1) paged_join(a, w, first_cta, parts, N, tid, 128, meet, s_red, s_red_sum, &s_last);
+      if (parts > 1) paged_join(a, w, first_cta, parts, N, tid, SOFT, meet, s_red, s_red_sum, &s_last);
       if (w.next >= x1) break;
       meet();
       const PagedPart before = w;
       paged_next(a, w, before, x1, kTcKeys);
     }
-  } else if (any && warp == 4) {
+  } else if (any && warp == WARPS) {
     // ------------------------------------------------------------------ products: the whole warp runs this, one lane issues
     PagedPart w = s_part;
     constexpr uint32_t kType = TERMS == 2 ? 0u : (1u << 7) | (1u << 10);
@@ -331,6 +325,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attention_tc_kernel(const
     auto scores = [&](uint32_t i) {
       const uint32_t st = use % NS;
       wait(&full[st], use / NS);
+      fence_async_smem();
       tc_fence_after();
       const uint32_t d = tmem + 32 * (i & 1), k = st0 + st * (S::kStage >> 4);
 #pragma unroll
@@ -355,6 +350,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attention_tc_kernel(const
           const uint32_t st = use % NS;
           wait(&full[st], use / NS);
           wait(&p_ready, tile);
+          fence_async_smem();
           tc_fence_after();
           // 16 keys a step; the block of dimensions from 64 on lies kTcBlock further (with one block, the same once more)
           const uint32_t v = (st0 + st * (S::kStage >> 4)) | (HB > 1 ? (uint32_t)(kTcBlock >> 4) << 16 : 0u);
@@ -380,16 +376,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attention_tc_kernel(const
     // ------------------------------------------------------------------ copies
     PagedPart w = s_part;
     constexpr int kLanes = 8 * HB, kAtOnce = 32 / kLanes;  // lanes that share a row
-    const int lw = warp - 5, piece = lane % kLanes, sub = lane / kLanes;
+    const int lw = warp - WARPS - 1, piece = lane % kLanes, sub = lane / kLanes;
     const bool mine = piece * 8 < hs;  // 8 values a piece
     const uint32_t st0 = smem_addr(stages) + (piece >> 3) * kTcBlock + (32 * lw + sub) * 128;
-    uint32_t fills = 0, arrived = 0;
-    auto arrive = [&]() {  // a stage whose copies have landed
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&full[arrived % NS]);
-      arrived++;
-    };
+    uint32_t fills = 0;
     auto fill = [&](const T *from, long long at, bool plain) {
       const uint32_t st = fills % NS;
       wait(&empty[st], fills / NS + 1);  // the first use of a stage waits for nothing
@@ -412,12 +402,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attention_tc_kernel(const
           }
         }
       }
-      cp_async_commit();
+      // arrives when this thread's copies have landed; the warp that issues the products fences them for the async proxy (a fence
+      // here would wait for every copy in flight)
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(&full[st])) : "memory");
       fills++;
-      if (fills > S::kLag) {
-        cp_async_wait<S::kLag>();
-        arrive();
-      }
     };
     for (;;) {
       const T *k = static_cast<const T *>(c.k) + w.g.kvh * c.head_stride, *v = static_cast<const T *>(c.v) + w.g.kvh * c.head_stride;
@@ -456,12 +444,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attention_tc_kernel(const
       const PagedPart before = w;
       paged_next(a, w, before, x1, kTcKeys);
     }
-    cp_async_wait<0>();
-    while (arrived < fills) arrive();
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
   __syncthreads();
   if (tid == 0 && *abort_flag) atomicExch(c.err, 3);
-  if (warp == 4) {
+  if (warp == WARPS) {
     tc_fence_after();
     tmem_dealloc(tmem, 128);
   }

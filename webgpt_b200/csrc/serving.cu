@@ -124,7 +124,7 @@ static int32_t launch_paged_tc(wgpt_device *dev, PagedAttention &a) {
   TRY(paged_workspace(dev, a, std::min(dev->sm_count, kJoinCounters), kTcKeys));
   a.least = 1;
   CK(allow_smem(dev, paged_attention_tc_kernel<T, HB, N>, true));
-  LAUNCH_PDL(dev, (paged_attention_tc_kernel<T, HB, N>), std::min(dev->sm_count, kJoinCounters), kTcThreads, S::kSmem, a);
+  LAUNCH_PDL(dev, (paged_attention_tc_kernel<T, HB, N>), std::min(dev->sm_count, kJoinCounters), S::kThreads, S::kSmem, a);
   return WGPT_OK;
 }
 
