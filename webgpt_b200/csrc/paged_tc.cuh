@@ -379,27 +379,36 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
     const int lw = warp - WARPS - 1, piece = lane % kLanes, sub = lane / kLanes;
     const bool mine = piece * 8 < hs;  // 8 values a piece
     const uint32_t st0 = smem_addr(stages) + (piece >> 3) * kTcBlock + (32 * lw + sub) * 128;
-    uint32_t fills = 0;
+    uint32_t fills = 0, swizzle[8 / kAtOnce];
+#pragma unroll
+    for (int i = 0; i < 8 / kAtOnce; i++) swizzle[i] = ((piece & 7) ^ ((i * kAtOnce + sub) & 7)) << 4;
     auto fill = [&](const T *from, long long at, bool plain) {
       const uint32_t st = fills % NS;
       wait(&empty[st], fills / NS + 1);  // the first use of a stage waits for nothing
       const uint32_t to = st0 + st * S::kStage;
-      const char *base = reinterpret_cast<const char *>(from + (long long)sub * c.position_stride) + piece * 16;
-      const long long step = (long long)kAtOnce * c.position_stride * 2;
+      if (plain) {  // one address per 16 positions, the others at a fixed distance
+        uint32_t dst[8 / kAtOnce];  // the swizzle repeats every eight rows
 #pragma unroll
-      for (int b = 0; b < 2; b++) {
-        const char *p = base + __shfl_sync(0xffffffffu, at, 16 * b) * 2;
+        for (int i = 0; i < 8 / kAtOnce; i++) dst[i] = to + swizzle[i];
+        const long long step = (long long)kAtOnce * c.position_stride * 2;
 #pragma unroll
-        for (int i = 0; i < 16 / kAtOnce; i++) {
-          const int row = 16 * b + i * kAtOnce;  // and sub
-          const uint32_t dst = to + row * 128 + (((piece & 7) ^ ((row + sub) & 7)) << 4);
-          if (plain) {
-            if (mine) cp_async16(dst, p);
-            p += step;
-          } else {
-            const long long x = __shfl_sync(0xffffffffu, at, row + sub);
-            if (mine) cp_async16_or_zero(dst, reinterpret_cast<const char *>(from + (x < 0 ? 0 : x)) + piece * 16, x >= 0);
+        for (int b = 0; b < 2; b++) {
+          const char *p = reinterpret_cast<const char *>(from + __shfl_sync(0xffffffffu, at, 16 * b) + (long long)sub * c.position_stride) + piece * 16;
+          if (mine) {
+#pragma unroll
+            for (int i = 0; i < 16 / kAtOnce; i++) {
+              cp_async16(dst[i % (8 / kAtOnce)] + (16 * b + i * kAtOnce) * 128, p);
+              p += step;
+            }
           }
+        }
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < 32 / kAtOnce; i++) {
+          const long long x = __shfl_sync(0xffffffffu, at, i * kAtOnce + sub);
+          if (mine)
+            cp_async16_or_zero(to + i * kAtOnce * 128 + (((piece & 7) ^ ((i * kAtOnce + sub) & 7)) << 4),
+                               reinterpret_cast<const char *>(from + (x < 0 ? 0 : x)) + piece * 16, x >= 0);
         }
       }
       // arrives when this thread's copies have landed; the warp that issues the products fences them for the async proxy (a fence
