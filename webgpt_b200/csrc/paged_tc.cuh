@@ -3,7 +3,8 @@
 // paged_attention_kernel. There every warp's path of loading fragments, eight rows at a time, is what bounds such calls.
 //
 // Keys are the instruction's 128 lanes and query rows its columns: S^T = K Q^T from shared memory (the key tile as it lies, the
-// queries as the sum of two half or three bfloat16 values), so that a softmax thread has one key and up to 16
+// queries as the sum of two half or three bfloat16 values, whose columns lie beside one another: the tile's bytes, which every
+// instruction reads again, are what an instruction of few columns takes), so that a softmax thread has one key and up to 16
 // rows. Its probabilities, split the same way, go back to shared memory as the second operand of O^T = V^T P^T, whose first is
 // the value tile as it lies, MN-major; there a thread has one dimension and those rows. A tile's O is added to f32 sums in
 // registers, so that nothing is accumulated across tiles in tensor memory, whose additions cut off.
@@ -30,26 +31,45 @@ struct TcShape {
   static constexpr int kTerms = std::is_same<T, __half>::value ? 2 : 3;
   static constexpr int kGroups = N / kTcRows, kSoft = 128 * kGroups, kThreads = kSoft + 32 + 128;
   static constexpr int kStage = HB * kTcBlock;
-  static constexpr int kP = kTerms * kTcBlock, kQ = kTerms * HB * N * 128;
+  static constexpr int kCols = kTerms * N;  // columns of an instruction: the rows' terms beside one another, so that the tile is read once
+  static constexpr int kP = (kCols + 63) / 64 * kTcBlock, kQ = HB * kCols * 128;
+  static constexpr uint32_t kTmem = 3 * kCols <= 128 ? 128 : 3 * kCols <= 256 ? 256 : 512;  // scores of two tiles, values
   static constexpr int kFit = (int)(((220 << 10) - kP - kQ) / kStage);
   static constexpr int kStages = kFit < 8 ? kFit : 8;
   static constexpr int kSmem = 1024 + kStages * kStage + kP + kQ;
   static_assert(kStages >= 4, "");
 };
 
-// 32 lanes x 16 consecutive 32-bit columns.
-__device__ __forceinline__ void tmem_ld_16(uint32_t taddr, float (&v)[16]) {
-  uint32_t r[16];
+// 16 consecutive 32-bit columns of each term, the terms `apart` columns from one another, added up, the last term first.
+template <int TERMS>
+__device__ __forceinline__ void tmem_ld_terms(uint32_t taddr, uint32_t apart, float (&v)[16]) {
+  uint32_t a[16], b[16];
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%32];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%33];\n\t"
       "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
+      : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]),
+        "=r"(a[8]), "=r"(a[9]), "=r"(a[10]), "=r"(a[11]), "=r"(a[12]), "=r"(a[13]), "=r"(a[14]), "=r"(a[15]),
+        "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3]), "=r"(b[4]), "=r"(b[5]), "=r"(b[6]), "=r"(b[7]),
+        "=r"(b[8]), "=r"(b[9]), "=r"(b[10]), "=r"(b[11]), "=r"(b[12]), "=r"(b[13]), "=r"(b[14]), "=r"(b[15])
+      : "r"(taddr + (TERMS - 1) * apart), "r"(taddr + (TERMS - 2) * apart)
       : "memory");
 #pragma unroll
-  for (int j = 0; j < 16; j++) v[j] = __uint_as_float(r[j]);
+  for (int j = 0; j < 16; j++) v[j] = __uint_as_float(a[j]) + __uint_as_float(b[j]);
+  if constexpr (TERMS == 3) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]),
+          "=r"(a[8]), "=r"(a[9]), "=r"(a[10]), "=r"(a[11]), "=r"(a[12]), "=r"(a[13]), "=r"(a[14]), "=r"(a[15])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int j = 0; j < 16; j++) v[j] += __uint_as_float(a[j]);
+  }
 }
 
 template <typename T, int HB, int N>
@@ -86,7 +106,7 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
     abort_word = 0;
     fence_async_smem();
   }
-  if (warp == WARPS) tmem_alloc(&tmem_slot, 128);  // scores of two tiles at 0 and 32, values at 64
+  if (warp == WARPS) tmem_alloc(&tmem_slot, S::kTmem);
   if (hs & 63)  // what lies behind a row's end takes part in products: zeros
     for (int i = tid; i < NS * S::kStage / 16; i += S::kThreads) reinterpret_cast<uint4 *>(stages)[i] = make_uint4(0, 0, 0, 0);
   tc_fence_before();
@@ -147,7 +167,7 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
             float f0 = scalbnf(v[2 * i], -e), f1 = scalbnf(v[2 * i + 1], -e);
 #pragma unroll
             for (int t = 0; t < TERMS; t++)
-              *reinterpret_cast<uint32_t *>(Qs + ((t * HB + i) * N + r) * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) =
+              *reinterpret_cast<uint32_t *>(Qs + ((i * TERMS + t) * N + r) * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) =
                   split2<T>(f0, f1);
           }
           if (lane == 0) s_qscale[r] = scalbnf(a.scale2, e);
@@ -181,7 +201,7 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
         wait(&o_done, i);
         tc_fence_after();
         float v[R];
-        tmem_ld_16(lanes + 64, v);
+        tmem_ld_terms<TERMS>(lanes + 2 * S::kCols, N, v);
 #pragma unroll
         for (int r = 0; r < R; r++) o[r] += v[r];
       };
@@ -190,7 +210,7 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
         wait(&s_done[tile & 1], tile >> 1);
         tc_fence_after();
         float x[R];
-        tmem_ld_16(lanes + 32 * (tile & 1), x);
+        tmem_ld_terms<TERMS>(lanes + S::kCols * (tile & 1), N, x);
         const int pos0 = pos - key;
         const bool whole = pos0 >= w.g.inner_low && pos0 + kTcKeys <= w.g.inner_high;
 #pragma unroll
@@ -251,9 +271,11 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
             for (int u = 0; u < TERMS; u++) words[u][i] = split2<T>(p0, p1);
           }
 #pragma unroll
-          for (int u = 0; u < TERMS; u++)
-            *reinterpret_cast<uint4 *>(Ps + u * kTcBlock + key * 128 + (((r0 / 8 + g) ^ (key & 7)) << 4)) =
+          for (int u = 0; u < TERMS; u++) {
+            const int at = (u * N + r0) / 8 + g;  // of the row's 16-byte pieces
+            *reinterpret_cast<uint4 *>(Ps + at / 8 * kTcBlock + key * 128 + (((at & 7) ^ (key & 7)) << 4)) =
                 make_uint4(words[u][0], words[u][1], words[u][2], words[u][3]);
+          }
         }
         fence_async_smem();
         __syncwarp();
@@ -319,7 +341,7 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
     // ------------------------------------------------------------------ products: the whole warp runs this, one lane issues
     PagedPart w = s_part;
     constexpr uint32_t kType = TERMS == 2 ? 0u : (1u << 7) | (1u << 10);
-    constexpr uint32_t idesc_s = f16_idesc(128, N) | kType, idesc_o = idesc_s | (1u << 15) | (1u << 16);  // values and probabilities: MN-major
+    constexpr uint32_t idesc_s = f16_idesc(128, S::kCols) | kType, idesc_o = idesc_s | (1u << 15) | (1u << 16);  // values and probabilities: MN-major
     const uint32_t st0 = umma_desc_lo(smem_addr(stages)), p0 = umma_desc_lo(smem_addr(Ps)), q0 = umma_desc_lo(smem_addr(Qs));
     uint32_t tile = 0, use = 0, part = 0;  // of all parts: tiles, stages used up, parts with tiles
     auto scores = [&](uint32_t i) {
@@ -327,15 +349,12 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
       wait(&full[st], use / NS);
       fence_async_smem();
       tc_fence_after();
-      const uint32_t d = tmem + 32 * (i & 1), k = st0 + st * (S::kStage >> 4);
+      const uint32_t d = tmem + S::kCols * (i & 1), k = st0 + st * (S::kStage >> 4);
 #pragma unroll
-      for (int u = TERMS - 1; u >= 0; u--)  // the smallest terms first
+      for (int b = 0; b < HB; b++)
 #pragma unroll
-        for (int b = 0; b < HB; b++)
-#pragma unroll
-          for (int s = 0; s < 4; s++)
-            umma1_f16(d, k + b * (kTcBlock >> 4) + 2 * s, q0 + (u * HB + b) * (N * 128 >> 4) + 2 * s, idesc_s,
-                      u < TERMS - 1 || b > 0 || s > 0 ? 1u : 0u);
+        for (int s = 0; s < 4; s++)
+          umma1_f16(d, k + b * (kTcBlock >> 4) + 2 * s, q0 + b * (S::kCols * 128 >> 4) + 2 * s, idesc_s, b > 0 || s > 0 ? 1u : 0u);
       umma_commit_elect(&s_done[i & 1]);
       umma_commit_elect(&empty[st]);
       use++;
@@ -352,13 +371,13 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
           wait(&p_ready, tile);
           fence_async_smem();
           tc_fence_after();
-          // 16 keys a step; the block of dimensions from 64 on lies kTcBlock further (with one block, the same once more)
+          // 16 keys a step; the block of dimensions from 64 on, and that of columns from 64 on, lie kTcBlock further (with one
+          // block of dimensions, it is taken twice)
           const uint32_t v = (st0 + st * (S::kStage >> 4)) | (HB > 1 ? (uint32_t)(kTcBlock >> 4) << 16 : 0u);
+          const uint32_t p = p0 | (S::kCols > 64 ? (uint32_t)(kTcBlock >> 4) << 16 : 0u);
 #pragma unroll
-          for (int u = TERMS - 1; u >= 0; u--)
-#pragma unroll
-            for (int s = 0; s < kTcKeys / 16; s++)
-              umma1_f16(tmem + 64, v + s * (2048 >> 4), p0 + u * (kTcBlock >> 4) + s * (2048 >> 4), idesc_o, u < TERMS - 1 || s > 0 ? 1u : 0u);
+          for (int s = 0; s < kTcKeys / 16; s++)
+            umma1_f16(tmem + 2 * S::kCols, v + s * (2048 >> 4), p + s * (2048 >> 4), idesc_o, s > 0 ? 1u : 0u);
           umma_commit_elect(&o_done);
           umma_commit_elect(&empty[st]);
           use++;
@@ -459,7 +478,7 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
   if (tid == 0 && *abort_flag) atomicExch(c.err, 3);
   if (warp == WARPS) {
     tc_fence_after();
-    tmem_dealloc(tmem, 128);
+    tmem_dealloc(tmem, S::kTmem);
   }
 }
 
