@@ -32,8 +32,8 @@ struct TcShape {
   static constexpr int kGroups = N / kTcRows, kSoft = 128 * kGroups, kThreads = kSoft + 32 + 128;
   static constexpr int kStage = HB * kTcBlock;
   static constexpr int kCols = kTerms * N;  // columns of an instruction: the rows' terms beside one another, so that the tile is read once
-  static constexpr int kP = (kCols + 63) / 64 * kTcBlock, kQ = HB * kCols * 128;
-  static constexpr uint32_t kTmem = 3 * kCols <= 128 ? 128 : 3 * kCols <= 256 ? 256 : 512;  // scores of two tiles, values
+  static constexpr int kPTile = (kCols + 63) / 64 * kTcBlock, kP = 2 * kPTile, kQ = HB * kCols * 128;
+  static constexpr uint32_t kTmem = 4 * kCols <= 128 ? 128 : 4 * kCols <= 256 ? 256 : 512;  // scores and values of two tiles each
   static constexpr int kFit = (int)(((220 << 10) - kP - kQ) / kStage);
   static constexpr int kStages = kFit < 8 ? kFit : 8;
   static constexpr int kSmem = 1024 + kStages * kStage + kP + kQ;
@@ -80,7 +80,7 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
   extern __shared__ uint8_t tc_raw[];
   uint8_t *stages = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(tc_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *Ps = stages + NS * S::kStage, *Qs = Ps + S::kP;
-  __shared__ uint64_t full[NS], empty[NS], q_ready, s_done[2], p_ready, o_done, drained;
+  __shared__ uint64_t full[NS], empty[NS], q_ready, s_done[2], p_ready[2], o_done[2], drained;
   __shared__ uint32_t tmem_slot, s_sum[S::kThreads / 32];
   __shared__ int abort_word, s_last;
   __shared__ PagedPart s_part;
@@ -98,10 +98,11 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
       mbar_init(&empty[i], 1);
     }
     mbar_init(&q_ready, WARPS);
-    mbar_init(&s_done[0], 1);
-    mbar_init(&s_done[1], 1);
-    mbar_init(&p_ready, WARPS);
-    mbar_init(&o_done, 1);
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&s_done[i], 1);
+      mbar_init(&p_ready[i], WARPS);
+      mbar_init(&o_done[i], 1);
+    }
     mbar_init(&drained, 1);
     abort_word = 0;
     fence_async_smem();
@@ -198,10 +199,10 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
       };
       uint32_t page = n_tiles > 0 ? page_of(pos) : 0u;
       auto add_values = [&](uint32_t i) {  // of tile i
-        wait(&o_done, i);
+        wait(&o_done[i & 1], i >> 1);
         tc_fence_after();
         float v[R];
-        tmem_ld_terms<TERMS>(lanes + 2 * S::kCols, N, v);
+        tmem_ld_terms<TERMS>(lanes + S::kCols * (2 + (i & 1)), N, v);
 #pragma unroll
         for (int r = 0; r < R; r++) o[r] += v[r];
       };
@@ -234,10 +235,11 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
         bool far = false;
 #pragma unroll
         for (int r = 0; r < R; r++) far |= x[r] > m[r] + kSlack;
-        if (t > 0) add_values(tile - 1);
-        tc_fence_before();
         __syncwarp();
+        bool added = t == 0;  // the last tile's values
         if (some(far)) {  // raise the references of the rows that need it
+          if (!added) add_values(tile - 1);
+          added = true;
 #pragma unroll
           for (int r = 0; r < R; r++) {
             const float top = warp_max(x[r]);
@@ -273,13 +275,15 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
 #pragma unroll
           for (int u = 0; u < TERMS; u++) {
             const int at = (u * N + r0) / 8 + g;  // of the row's 16-byte pieces
-            *reinterpret_cast<uint4 *>(Ps + at / 8 * kTcBlock + key * 128 + (((at & 7) ^ (key & 7)) << 4)) =
+            *reinterpret_cast<uint4 *>(Ps + (tile & 1) * S::kPTile + at / 8 * kTcBlock + key * 128 + (((at & 7) ^ (key & 7)) << 4)) =
                 make_uint4(words[u][0], words[u][1], words[u][2], words[u][3]);
           }
         }
         fence_async_smem();
+        tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_ready);
+        if (lane == 0) mbar_arrive(&p_ready[tile & 1]);
+        if (!added) add_values(tile - 1);  // while this tile's are made
         page = t + 1 < n_tiles ? page_of(pos + kTcKeys) : 0u;
       }
       if (n_tiles > 0) add_values(tile - 1);
@@ -368,17 +372,17 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
           if (t + 1 < n_tiles) scores(tile + 1);
           const uint32_t st = use % NS;
           wait(&full[st], use / NS);
-          wait(&p_ready, tile);
+          wait(&p_ready[tile & 1], tile >> 1);
           fence_async_smem();
           tc_fence_after();
           // 16 keys a step; the block of dimensions from 64 on, and that of columns from 64 on, lie kTcBlock further (with one
           // block of dimensions, it is taken twice)
           const uint32_t v = (st0 + st * (S::kStage >> 4)) | (HB > 1 ? (uint32_t)(kTcBlock >> 4) << 16 : 0u);
-          const uint32_t p = p0 | (S::kCols > 64 ? (uint32_t)(kTcBlock >> 4) << 16 : 0u);
+          const uint32_t p = (p0 + (tile & 1) * (S::kPTile >> 4)) | (S::kCols > 64 ? (uint32_t)(kTcBlock >> 4) << 16 : 0u);
 #pragma unroll
           for (int s = 0; s < kTcKeys / 16; s++)
-            umma1_f16(tmem + 2 * S::kCols, v + s * (2048 >> 4), p + s * (2048 >> 4), idesc_o, s > 0 ? 1u : 0u);
-          umma_commit_elect(&o_done);
+            umma1_f16(tmem + S::kCols * (2 + (tile & 1)), v + s * (2048 >> 4), p + s * (2048 >> 4), idesc_o, s > 0 ? 1u : 0u);
+          umma_commit_elect(&o_done[tile & 1]);
           umma_commit_elect(&empty[st]);
           use++;
         }
