@@ -23,6 +23,7 @@ __device__ __forceinline__ float paged_value(const float *p) { return __ldcg(p);
 __device__ __forceinline__ float paged_value(const __half *p) { return __half2float(__ldcg(p)); }
 __device__ __forceinline__ float paged_value(const __nv_bfloat16 *p) { return __bfloat162float(__ldcg(p)); }
 
+constexpr int kJoinFactors = 256;
 constexpr int kPagedKeyGroups = 4, kPagedWarps = 8, kPagedRows = 32;  // at most, in a CTA
 
 struct PagedAttention {
@@ -112,9 +113,10 @@ __device__ __forceinline__ void paged_part(const PagedAttention &a, PagedPart &w
   w.n_tiles = max(0, min((int)(w.next - w.begin), (w.g.highest - q.begin + unit - 1) / unit) - w.u0);
 }
 
-// A CTA's units [first, end) of all there are and the part they begin with, by all its threads (behind it a barrier of theirs):
-// false if there are none. sums: a number for each warp.
-__device__ __forceinline__ bool paged_first(const PagedAttention &a, PagedPart &to, int unit, uint32_t *sums, uint32_t &per, uint32_t &end) {
+// A CTA's units [.., end) of all there are and the part they begin with, by all its threads, every one of which gets it: false if
+// there are none. sums: a number for each warp; place: a part.
+__device__ __forceinline__ bool paged_first(const PagedAttention &a, PagedPart &to, int unit, uint32_t *sums, PagedPart *place, uint32_t &per,
+                                            uint32_t &end) {
   const int threads = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_seq = a.c.n_seq;
   PagedSeq q;
   auto weight_of = [&](int s) -> uint32_t {
@@ -122,22 +124,39 @@ __device__ __forceinline__ bool paged_first(const PagedAttention &a, PagedPart &
     q = paged_seq(a, s, unit);
     return paged_work(a, q);
   };
-  auto scan = [&](uint32_t mine, uint32_t &all) {  // sum over the threads before this one, and over all
-    uint32_t upto = mine;
+  auto before_lane = [&](uint32_t mine) {  // sum over the lanes up to this one
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += x;
+      const uint32_t x = __shfl_up_sync(0xffffffffu, mine, o);
+      if (lane >= o) mine += x;
     }
+    return mine;
+  };
+  if (n_seq <= 32) {  // every warp for itself, a sequence a lane
+    const uint32_t mine = weight_of(lane), upto = before_lane(mine), total = __shfl_sync(0xffffffffu, upto, 31);
+    per = max((uint32_t)a.least, (total + gridDim.x - 1) / gridDim.x);
+    const uint32_t x0 = blockIdx.x * per;  // the caller sees to it that it does not pass 2^32
+    end = min(total, x0 + per);
+    if (x0 >= end) return false;
+    const int s = __ffs(__ballot_sync(0xffffffffu, x0 < upto)) - 1;
+    PagedSeq of;
+    of.first = __shfl_sync(0xffffffffu, q.first, s);
+    of.n = __shfl_sync(0xffffffffu, q.n, s);
+    of.L = __shfl_sync(0xffffffffu, q.L, s);
+    of.begin = __shfl_sync(0xffffffffu, q.begin, s);
+    of.tiles = __shfl_sync(0xffffffffu, q.tiles, s);
+    of.units = __shfl_sync(0xffffffffu, q.units, s);
+    paged_part(a, to, of, s, __shfl_sync(0xffffffffu, upto - mine, s), x0, end, unit);
+    return true;
+  }
+  auto scan = [&](uint32_t mine, uint32_t &all) {  // sum over the threads before this one, and over all
+    const uint32_t upto = before_lane(mine);
     __syncthreads();
     if (lane == 31) sums[warp] = upto;
     __syncthreads();
-    all = 0;
-    for (int w = 0; w < threads / 32; w++) {
-      if (w < warp) upto += sums[w];
-      all += sums[w];
-    }
-    return upto - mine;
+    const uint32_t of = lane < threads / 32 ? sums[lane] : 0u;
+    all = __reduce_add_sync(0xffffffffu, of);
+    return upto - mine + __reduce_add_sync(0xffffffffu, lane < warp ? of : 0u);
   };
   uint32_t total = 0, mine = 0, before = 0;
   for (int s0 = 0; s0 < n_seq; s0 += threads) {
@@ -150,18 +169,16 @@ __device__ __forceinline__ bool paged_first(const PagedAttention &a, PagedPart &
   const uint32_t x0 = blockIdx.x * per, x1 = min(total, x0 + per);  // the caller sees to it that neither passes 2^32
   if (x0 >= x1) return false;
   end = x1;
-  if (n_seq <= threads) {
-    if (before <= x0 && x0 < before + mine) paged_part(a, to, q, tid, before, x0, x1, unit);
-  } else {
-    uint32_t sum = 0;
-    for (int s0 = 0; s0 < n_seq && sum <= x0; s0 += threads) {
-      uint32_t all;
-      mine = weight_of(s0 + tid);
-      before = sum + scan(mine, all);
-      if (before <= x0 && x0 < before + mine) paged_part(a, to, q, s0 + tid, before, x0, x1, unit);
-      sum += all;
-    }
+  uint32_t sum = 0;
+  for (int s0 = 0; s0 < n_seq && sum <= x0; s0 += threads) {
+    uint32_t all;
+    mine = weight_of(s0 + tid);
+    before = sum + scan(mine, all);
+    if (before <= x0 && x0 < before + mine) paged_part(a, *place, q, s0 + tid, before, x0, x1, unit);
+    sum += all;
   }
+  __syncthreads();
+  to = *place;
   return true;
 }
 
@@ -402,10 +419,10 @@ __device__ __forceinline__ uint32_t split2(float &x, float &y) {
 
 
 // Joins a group's parts once this CTA's lies in its slot: the CTA that finishes last does, in the order of the positions. By
-// `threads` threads that meet in sync(); red and red_sum: a place for each of them.
+// `threads` threads that meet in sync(); red and red_sum: a place for each of them; factor and sums: kJoinFactors places.
 template <typename Sync>
 __device__ __forceinline__ void paged_join(const PagedAttention &a, const PagedPart &w, int first_cta, int parts, int ROWS, int tid,
-                                           int threads, Sync sync, float4 *red, float *red_sum, int *is_last) {
+                                           int threads, Sync sync, float4 *red, float *red_sum, float *factor, float *sums, int *is_last) {
   const int hs = a.c.hs, quads = hs / 4, items = w.g.rows * quads, slot_floats = paged_slot(ROWS, hs);
   __threadfence();
   sync();
@@ -417,8 +434,30 @@ __device__ __forceinline__ void paged_join(const PagedAttention &a, const PagedP
   sync();
   if (!*is_last) return;
   __threadfence();
-  // where a row tile has few values, several threads share a quad and take every so many parts
   auto part_of = [&](int k) { return a.partial + (2ll * (first_cta + k) + (k == 0 ? 1 : 0)) * slot_floats; };
+  const int rows = w.g.rows, n = parts * rows;
+  const bool table = n <= kJoinFactors;  // else every thread computes the factors that it needs
+  if (table) {
+    for (int i = tid; i < n; i += threads) {
+      const int k = i / rows, r = i - k * rows;
+      factor[i] = __ldcg(part_of(k) + ROWS * hs + r);
+      sums[i] = __ldcg(part_of(k) + ROWS * hs + ROWS + r);
+    }
+    sync();
+    for (int r = tid; r < rows; r += threads) {
+      float top = -INFINITY, sum = 0.f;
+      for (int k = 0; k < parts; k++) top = fmaxf(top, factor[k * rows + r]);
+      for (int k = 0; k < parts; k++) {
+        const float m = factor[k * rows + r], l = sums[k * rows + r], f = m == -INFINITY && l == 0.f ? 0.f : exp2f(m - top);
+        factor[k * rows + r] = f;
+        sum += f * l;
+      }
+      sums[r] = sum != 0.f ? 1.f / sum : 0.f;  // the first part's places: read already
+      if (a.stats) a.stats[row_index(a, w, r)] = top + log2f(sum);
+    }
+    sync();
+  }
+  // where a row tile has few values, several threads share a quad and take every so many parts
   const int share = items >= threads ? 1 : threads / items;
   for (int i0 = 0; i0 < items; i0 += threads) {
     const int i = share > 1 ? tid % items : i0 + tid, sh = share > 1 ? tid / items : 0;
@@ -427,15 +466,20 @@ __device__ __forceinline__ void paged_join(const PagedAttention &a, const PagedP
     float top = -INFINITY, sum = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (live) {
-#pragma unroll 8
-      for (int k = 0; k < parts; k++) top = fmaxf(top, __ldcg(part_of(k) + ROWS * hs + r));
+      if (!table)
+        for (int k = 0; k < parts; k++) top = fmaxf(top, __ldcg(part_of(k) + ROWS * hs + r));
 #pragma unroll 8
       for (int k = sh; k < parts; k += share) {
         const float *part = part_of(k);
-        const float m = __ldcg(part + ROWS * hs + r), l = __ldcg(part + ROWS * hs + ROWS + r);
         const float4 o = __ldcg(reinterpret_cast<const float4 *>(part) + i);
-        const float f = m == -INFINITY && l == 0.f ? 0.f : exp2f(m - top);
-        sum += f * l;
+        float f;
+        if (table) {
+          f = factor[k * rows + r];
+        } else {
+          const float m = __ldcg(part + ROWS * hs + r), l = __ldcg(part + ROWS * hs + ROWS + r);
+          f = m == -INFINITY && l == 0.f ? 0.f : exp2f(m - top);
+          sum += f * l;
+        }
         v.x += f * o.x;
         v.y += f * o.y;
         v.z += f * o.z;
@@ -457,12 +501,10 @@ __device__ __forceinline__ void paged_join(const PagedAttention &a, const PagedP
         }
     }
     if (live && sh == 0) {
-      if (sum != 0.f) {
-        const float inv = 1.f / sum;
-        v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-      }
+      const float inv = table ? sums[r] : sum != 0.f ? 1.f / sum : 0.f;
+      if (table || sum != 0.f) v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
       reinterpret_cast<float4 *>(a.out + row_offset(a, w, r, a.ld_out))[i - r * quads] = v;
-      if (a.stats && i == r * quads) a.stats[row_index(a, w, r)] = top + log2f(sum);
+      if (a.stats && !table && i == r * quads) a.stats[row_index(a, w, r)] = top + log2f(sum);
     }
   }
 }
@@ -484,8 +526,8 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
   __shared__ uint32_t s_sum[kPagedWarps];
   __shared__ PagedPart s_part[2];
   __shared__ int s_last, s_more;
-  __shared__ float4 s_red[32 * kPagedWarps];
-  __shared__ float s_red_sum[32 * kPagedWarps];
+  __shared__ float4 s_red[S::kWide ? 128 : 32 * kPagedWarps];
+  __shared__ float s_red_sum[S::kWide ? 128 : 32 * kPagedWarps], s_factor[kJoinFactors], s_sums[kJoinFactors];
   const PagedView &c = a.c;
   const int KG = a.key_groups, RW = S::kWide ? 1 : a.row_warps, ROWS = S::kWide ? RT : a.rows, threads = blockDim.x;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hs = c.hs, unit = KG * kTile;
@@ -510,7 +552,11 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
 
   // ---- this CTA's units: [.., x1)
   uint32_t per, x1;
-  if (!paged_first(a, s_part[0], unit, s_sum, per, x1)) return;
+  {
+    PagedPart first;
+    if (!paged_first(a, first, unit, s_sum, &s_part[1], per, x1)) return;
+    if (tid == 0) s_part[0] = first;
+  }
   __syncthreads();
 
   PagedRing<T, HSP, RT, STAGES> ring(c, smem_addr(ring_smem), s_ok[kg], lane, unit, rw, RW);
@@ -534,30 +580,42 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
         q4[i] = v;
       }
     } else {
-      for (int r = warp; r < ROWS; r += threads / 32) {
-        float v[HSP / 32], top = 0.f;
-        const float *row = r < g.rows ? a.q + row_offset(a, w, r, a.ld_q) : nullptr;
+      constexpr int kAtOnce = 2;  // rows of a warp whose loads are in flight together: eight rows a row warp, two key groups or more
+      for (int rr = warp; rr < ROWS; rr += threads / 32 * kAtOnce) {
+        float v[kAtOnce][HSP / 32];
 #pragma unroll
-        for (int i = 0; i < HSP / 64; i++) {
-          const int d = 2 * lane + 64 * i;
-          const float2 f = row && d < hs ? __ldcg(reinterpret_cast<const float2 *>(row + d)) : make_float2(0.f, 0.f);
-          v[2 * i] = f.x;
-          v[2 * i + 1] = f.y;
-          top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-        }
-        int e = 0;
-        if constexpr (TERMS == 2) {  // a power of two that brings the row's largest value near 2^13
-          top = warp_max(top);
-          e = top > 0.f && top < INFINITY ? ilogbf(top) - 13 : 0;
+        for (int y = 0; y < kAtOnce; y++) {
+          const int r = rr + y * (threads / 32);
+          const float *row = r < g.rows ? a.q + row_offset(a, w, r, a.ld_q) : nullptr;
+#pragma unroll
+          for (int i = 0; i < HSP / 64; i++) {
+            const int d = 2 * lane + 64 * i;
+            const float2 f = row && d < hs ? __ldcg(reinterpret_cast<const float2 *>(row + d)) : make_float2(0.f, 0.f);
+            v[y][2 * i] = f.x;
+            v[y][2 * i + 1] = f.y;
+          }
         }
 #pragma unroll
-        for (int i = 0; i < HSP / 64; i++) {
-          float f0 = scalbnf(v[2 * i], -e), f1 = scalbnf(v[2 * i + 1], -e);
+        for (int y = 0; y < kAtOnce; y++) {
+          const int r = rr + y * (threads / 32);
+          if (r >= ROWS) break;
+          int e = 0;
+          if constexpr (TERMS == 2) {  // a power of two that brings the row's largest value near 2^13
+            float top = 0.f;
 #pragma unroll
-          for (int t = 0; t < TERMS; t++)
-            *reinterpret_cast<uint32_t *>(q_smem + (t * ROWS + r) * S::kQPitch + (2 * lane + 64 * i) * 2) = split2<T>(f0, f1);
+            for (int i = 0; i < HSP / 32; i++) top = fmaxf(top, fabsf(v[y][i]));
+            top = warp_max(top);
+            e = top > 0.f && top < INFINITY ? ilogbf(top) - 13 : 0;
+          }
+#pragma unroll
+          for (int i = 0; i < HSP / 64; i++) {
+            float f0 = scalbnf(v[y][2 * i], -e), f1 = scalbnf(v[y][2 * i + 1], -e);
+#pragma unroll
+            for (int t = 0; t < TERMS; t++)
+              *reinterpret_cast<uint32_t *>(q_smem + (t * ROWS + r) * S::kQPitch + (2 * lane + 64 * i) * 2) = split2<T>(f0, f1);
+          }
+          if (lane == 0) s_qscale[r] = scalbnf(a.scale2, e);
         }
-        if (lane == 0) s_qscale[r] = scalbnf(a.scale2, e);
       }
     }
     if (tid < ROWS) {
@@ -906,7 +964,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
       }
     }
     if (parts > 1)
-      paged_join(a, w, first_cta, parts, ROWS, tid, threads, [] { __syncthreads(); }, s_red, s_red_sum, &s_last);
+      paged_join(a, w, first_cta, parts, ROWS, tid, threads, [] { __syncthreads(); }, s_red, s_red_sum, s_factor, s_sums, &s_last);
     __syncthreads();
     if (!more) break;
     if (padded) clear(reinterpret_cast<unsigned char *>(o_smem), a.ahead ? S::kTileBytes : S::kRing);

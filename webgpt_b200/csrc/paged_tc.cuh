@@ -25,6 +25,22 @@ namespace wgpt {
 constexpr int kTcKeys = 128, kTcBlock = kTcKeys * 128, kTcRows = 16;  // positions of a tile; bytes of 64 dimensions of one; rows of a softmax thread
 constexpr float kSlack = 8.f;
 
+// For each of 16 values the warp's result of f: lanes 2 r and 2 r + 1 get that of value r. Halves of what is left are exchanged, so
+// that 16 shuffles do what 80 would.
+template <typename F>
+__device__ __forceinline__ float warp_each16(const float (&x)[16], int lane, F f) {
+  float a[8], b[4], c[2];
+  const bool h16 = lane & 16, h8 = lane & 8, h4 = lane & 4, h2 = lane & 2;
+#pragma unroll
+  for (int i = 0; i < 8; i++) a[i] = f(h16 ? x[i + 8] : x[i], __shfl_xor_sync(0xffffffffu, h16 ? x[i] : x[i + 8], 16));
+#pragma unroll
+  for (int i = 0; i < 4; i++) b[i] = f(h8 ? a[i + 4] : a[i], __shfl_xor_sync(0xffffffffu, h8 ? a[i] : a[i + 4], 8));
+#pragma unroll
+  for (int i = 0; i < 2; i++) c[i] = f(h4 ? b[i + 2] : b[i], __shfl_xor_sync(0xffffffffu, h4 ? b[i] : b[i + 2], 4));
+  const float d = f(h2 ? c[1] : c[0], __shfl_xor_sync(0xffffffffu, h2 ? c[0] : c[1], 2));
+  return f(d, __shfl_xor_sync(0xffffffffu, d, 1));
+}
+
 // HB: blocks of 64 dimensions; N: rows of a row tile
 template <typename T, int HB, int N>
 struct TcShape {
@@ -34,7 +50,7 @@ struct TcShape {
   static constexpr int kCols = kTerms * N;  // columns of an instruction: the rows' terms beside one another, so that the tile is read once
   static constexpr int kPTile = (kCols + 63) / 64 * kTcBlock, kP = 2 * kPTile, kQ = HB * kCols * 128;
   static constexpr uint32_t kTmem = 4 * kCols <= 128 ? 128 : 4 * kCols <= 256 ? 256 : 512;  // scores and values of two tiles each
-  static constexpr int kFit = (int)(((220 << 10) - kP - kQ) / kStage);
+  static constexpr int kFit = (int)(((216 << 10) - kP - kQ) / kStage);
   static constexpr int kStages = kFit < 8 ? kFit : 8;
   static constexpr int kSmem = 1024 + kStages * kStage + kP + kQ;
   static_assert(kStages >= 4, "");
@@ -88,7 +104,7 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
   __shared__ int s_lo[N], s_hi[N];
   __shared__ long long s_row[N];
   __shared__ float4 s_red[SOFT];
-  __shared__ float s_red_sum[SOFT];
+  __shared__ float s_red_sum[SOFT], s_factor[kJoinFactors], s_sums[kJoinFactors];
   volatile int *abort_flag = &abort_word;
   const PagedView &c = a.c;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, hs = c.hs;
@@ -118,8 +134,8 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
   pdl_wait();
 
   uint32_t per = 1, x1 = 0;
-  const bool any = paged_first(a, s_part, kTcKeys, s_sum, per, x1);
-  __syncthreads();
+  PagedPart w;
+  const bool any = paged_first(a, w, kTcKeys, s_sum, &s_part, per, x1);
   // A wait that has run out makes all others return at once: every role runs to its end.
   auto wait = [&](uint64_t *bar, uint32_t parity) {
     if (!*abort_flag && !mbar_wait(bar, parity & 1, TC_POLLS)) *abort_flag = 1;
@@ -128,7 +144,6 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
 
   if (any && warp < WARPS) {
     // ------------------------------------------------------------------ softmax and sums
-    PagedPart w = s_part;
     const int quad = warp & 3, r0 = (warp >> 2) * R;  // of the tensor memory's lanes; this thread's rows
     const uint32_t lanes = tmem + ((uint32_t)(32 * quad) << 16) + r0;
     const int key = tid & 127;  // of a tile, and the dimension whose sums this thread has
@@ -147,25 +162,34 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
       const int rows = w.g.rows, n_tiles = w.n_tiles;
       // ---- the queries: K-major rows of 128 bytes, 16-byte pieces swizzled
       if (n_tiles > 0) {
-        for (int r = warp; r < N; r += WARPS) {
-          float v[2 * HB], top = 0.f;
+        constexpr int kMine = N / WARPS;  // rows of a warp, their loads in flight together
+        float v[kMine][2 * HB];
+#pragma unroll
+        for (int y = 0; y < kMine; y++) {
+          const int r = warp + y * WARPS;
           const float *row = r < rows ? a.q + row_offset(a, w, r, a.ld_q) : nullptr;
 #pragma unroll
           for (int i = 0; i < HB; i++) {
             const int d = 2 * lane + 64 * i;
             const float2 f = row && d < hs ? __ldcg(reinterpret_cast<const float2 *>(row + d)) : make_float2(0.f, 0.f);
-            v[2 * i] = f.x;
-            v[2 * i + 1] = f.y;
-            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+            v[y][2 * i] = f.x;
+            v[y][2 * i + 1] = f.y;
           }
+        }
+#pragma unroll
+        for (int y = 0; y < kMine; y++) {
+          const int r = warp + y * WARPS;
           int e = 0;
           if constexpr (TERMS == 2) {  // a power of two that brings the row's largest value near 2^13
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2 * HB; i++) top = fmaxf(top, fabsf(v[y][i]));
             top = warp_max(top);
             e = top > 0.f && top < INFINITY ? ilogbf(top) - 13 : 0;
           }
 #pragma unroll
           for (int i = 0; i < HB; i++) {
-            float f0 = scalbnf(v[2 * i], -e), f1 = scalbnf(v[2 * i + 1], -e);
+            float f0 = scalbnf(v[y][2 * i], -e), f1 = scalbnf(v[y][2 * i + 1], -e);
 #pragma unroll
             for (int t = 0; t < TERMS; t++)
               *reinterpret_cast<uint32_t *>(Qs + ((i * TERMS + t) * N + r) * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) =
@@ -240,11 +264,8 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
         if (some(far)) {  // raise the references of the rows that need it
           if (!added) add_values(tile - 1);
           added = true;
-#pragma unroll
-          for (int r = 0; r < R; r++) {
-            const float top = warp_max(x[r]);
-            if (lane == 0) s_max[quad][r0 + r] = top;
-          }
+          const float most = warp_each16(x, lane, [](float u, float v) { return fmaxf(u, v); });
+          if ((lane & 1) == 0) s_max[quad][r0 + lane / 2] = most;
           meet();
 #pragma unroll
           for (int r = 0; r < R; r++) {
@@ -291,10 +312,10 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
       // ---- the rows' sums over the keys
       const float down = kLift != 0.f ? 1.f / 128.f : 1.f;
       bool finite = true;
+      const float mine_sum = warp_each16(l, lane, [](float u, float v) { return u + v; });
+      if ((lane & 1) == 0) s_max[quad][r0 + lane / 2] = mine_sum;
 #pragma unroll
       for (int r = 0; r < R; r++) {
-        const float sum = warp_sum(l[r]);
-        if (lane == 0) s_max[quad][r0 + r] = sum;
         o[r] *= down;
         finite = finite && (r0 + r >= rows || key >= hs || fabsf(o[r]) < INFINITY);
         if (key == r) s_m[r0 + r] = m[r];
@@ -335,7 +356,7 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
           a.stats[row_index(a, w, tid)] = s_m[tid] + log2f(s_l[tid]);
         }
       }
-      if (parts > 1) paged_join(a, w, first_cta, parts, N, tid, SOFT, meet, s_red, s_red_sum, &s_last);
+      if (parts > 1) paged_join(a, w, first_cta, parts, N, tid, SOFT, meet, s_red, s_red_sum, s_factor, s_sums, &s_last);
       if (w.next >= x1) break;
       meet();
       const PagedPart before = w;
@@ -343,7 +364,6 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
     }
   } else if (any && warp == WARPS) {
     // ------------------------------------------------------------------ products: the whole warp runs this, one lane issues
-    PagedPart w = s_part;
     constexpr uint32_t kType = TERMS == 2 ? 0u : (1u << 7) | (1u << 10);
     constexpr uint32_t idesc_s = f16_idesc(128, S::kCols) | kType, idesc_o = idesc_s | (1u << 15) | (1u << 16);  // values and probabilities: MN-major
     const uint32_t st0 = umma_desc_lo(smem_addr(stages)), p0 = umma_desc_lo(smem_addr(Ps)), q0 = umma_desc_lo(smem_addr(Qs));
@@ -397,7 +417,6 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
     }
   } else if (any) {
     // ------------------------------------------------------------------ copies
-    PagedPart w = s_part;
     constexpr int kLanes = 8 * HB, kAtOnce = 32 / kLanes;  // lanes that share a row
     const int lw = warp - WARPS - 1, piece = lane % kLanes, sub = lane / kLanes;
     const bool mine = piece * 8 < hs;  // 8 values a piece
@@ -426,7 +445,7 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
           }
         }
       } else {
-#pragma unroll 1
+#pragma unroll 4
         for (int i = 0; i < 32 / kAtOnce; i++) {
           const long long x = __shfl_sync(0xffffffffu, at, i * kAtOnce + sub);
           if (mine)
