@@ -42,6 +42,9 @@ struct PagedAttention {
   float *scores, *stats; // [n_rows * n_head][max_length] and [n_rows * n_head], in units of log 2, or NULL
 };
 
+// Quotients that the chain ahead of the first copy waits for: mostly by one.
+__device__ __forceinline__ uint32_t quotient(uint32_t x, uint32_t by) { return by == 1 ? x : x / by; }
+
 // A sequence's share of the work.
 struct PagedSeq {
   int first, n, L, begin;  // rows, length, position of the first unit
@@ -54,8 +57,8 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedAttention &a, int s, in
   q.L = paged_length(a.c, s);
   const int lowest = a.window > 0 ? max(0, q.L - q.n + 1 - a.window) : 0;
   q.begin = min(lowest, q.L) & ~(unit - 1);
-  q.tiles = (q.n * a.group + a.rows - 1) / a.rows;
-  q.units = max(1, (q.L - q.begin + unit - 1) / unit);  // one even if there is nothing to see: the rows are set to zero
+  q.tiles = q.n * a.group <= a.rows ? (q.n > 0 ? 1 : 0) : (q.n * a.group + a.rows - 1) / a.rows;
+  q.units = max(1, (q.L - q.begin + unit - 1) >> (__ffs(unit) - 1));  // one even if there is nothing to see: the rows are set to zero
   return q;
 }
 __device__ __forceinline__ uint32_t paged_work(const PagedAttention &a, const PagedSeq &q) {
@@ -85,32 +88,34 @@ __device__ __forceinline__ void row_range(const PagedAttention &a, const PagedSe
   lo = a.window > 0 ? max(0, hi - a.window) : 0;
 }
 __device__ __forceinline__ long long row_offset(const PagedAttention &a, const PagedPart &w, int r, long long ld) {
-  const int token = (w.g.r0 + r) / a.group, head = w.g.kvh * a.group + (w.g.r0 + r) - token * a.group;
+  const int token = (int)quotient(w.g.r0 + r, a.group), head = w.g.kvh * a.group + (w.g.r0 + r) - token * a.group;
   return (long long)(w.q.first + token) * ld + (long long)head * a.c.hs;
 }
 __device__ __forceinline__ long long row_index(const PagedAttention &a, const PagedPart &w, int r) {
-  const int token = (w.g.r0 + r) / a.group, head = w.g.kvh * a.group + (w.g.r0 + r) - token * a.group;
+  const int token = (int)quotient(w.g.r0 + r, a.group), head = w.g.kvh * a.group + (w.g.r0 + r) - token * a.group;
   return (long long)(w.q.first + token) * a.n_head + head;
 }
 
 // The part that begins at unit x of sequence s, up to unit end at most; q and seq_begin are the sequence's.
 __device__ __forceinline__ void paged_part(const PagedAttention &a, PagedPart &w, const PagedSeq &q, int s, uint32_t seq_begin, uint32_t x,
                                            uint32_t end, int unit) {
-  const uint32_t gi = (x - seq_begin) / (uint32_t)q.units;
+  const uint32_t gi = quotient(x - seq_begin, (uint32_t)q.units);
   w.q = q;
   w.seq_begin = seq_begin;
   w.begin = seq_begin + gi * (uint32_t)q.units;
   w.end = w.begin + (uint32_t)q.units;
   w.next = min(end, w.end);
   w.g.s = s;
-  w.g.kvh = (int)(gi / (uint32_t)q.tiles);
+  w.g.kvh = (int)quotient(gi, (uint32_t)q.tiles);
   w.g.r0 = (int)(gi - (uint32_t)w.g.kvh * (uint32_t)q.tiles) * a.rows;
   w.g.rows = min(a.rows, q.n * a.group - w.g.r0);
-  row_range(a, q, w.g.r0 / a.group, w.g.lowest, w.g.inner_high);
-  row_range(a, q, (w.g.r0 + w.g.rows - 1) / a.group, w.g.inner_low, w.g.highest);
+  const int first = q.n == 1 ? 0 : (int)quotient(w.g.r0, a.group), last = q.n == 1 ? 0 : (int)quotient(w.g.r0 + w.g.rows - 1, a.group);
+  row_range(a, q, first, w.g.lowest, w.g.inner_high);
+  row_range(a, q, last, w.g.inner_low, w.g.highest);
   // units that no row of the tile sees are left out
-  w.u0 = max((int)(x - w.begin), (w.g.lowest - q.begin) / unit);
-  w.n_tiles = max(0, min((int)(w.next - w.begin), (w.g.highest - q.begin + unit - 1) / unit) - w.u0);
+  const int shift = __ffs(unit) - 1;
+  w.u0 = max((int)(x - w.begin), (w.g.lowest - q.begin) >> shift);
+  w.n_tiles = max(0, min((int)(w.next - w.begin), (w.g.highest - q.begin + unit - 1) >> shift) - w.u0);
 }
 
 // A CTA's units [.., end) of all there are and the part they begin with, by all its threads, every one of which gets it: false if
@@ -199,6 +204,14 @@ __device__ __forceinline__ void cp_async16_or_zero(uint32_t to, const void *from
   const int bytes = there ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
+
+// The power of two that brings a row's largest magnitude near 2^13, the middle of a half's range, as its exponent; a row that has an
+// infinity or no value but zero stays.
+__device__ __forceinline__ int row_exponent(float top) {
+  const int e = (__float_as_int(top) >> 23) - 127 - 13;  // top >= 0
+  return top > 0.f && top < INFINITY ? max(e, -126) : 0;
+}
+__device__ __forceinline__ float pow2_of(int e) { return __int_as_float((127 + e) << 23); }  // |e| <= 126
 
 __device__ __forceinline__ float exp2_of(float x) {
   float y;
@@ -600,21 +613,21 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
           const int r = rr + y * (threads / 32);
           if (r >= ROWS) break;
           int e = 0;
-          if constexpr (TERMS == 2) {  // a power of two that brings the row's largest value near 2^13
+          if constexpr (TERMS == 2) {
             float top = 0.f;
 #pragma unroll
             for (int i = 0; i < HSP / 32; i++) top = fmaxf(top, fabsf(v[y][i]));
             top = warp_max(top);
-            e = top > 0.f && top < INFINITY ? ilogbf(top) - 13 : 0;
+            e = row_exponent(top);
           }
 #pragma unroll
           for (int i = 0; i < HSP / 64; i++) {
-            float f0 = scalbnf(v[y][2 * i], -e), f1 = scalbnf(v[y][2 * i + 1], -e);
+            float f0 = v[y][2 * i] * pow2_of(-e), f1 = v[y][2 * i + 1] * pow2_of(-e);
 #pragma unroll
             for (int t = 0; t < TERMS; t++)
               *reinterpret_cast<uint32_t *>(q_smem + (t * ROWS + r) * S::kQPitch + (2 * lane + 64 * i) * 2) = split2<T>(f0, f1);
           }
-          if (lane == 0) s_qscale[r] = scalbnf(a.scale2, e);
+          if (lane == 0) s_qscale[r] = a.scale2 * pow2_of(e);
         }
       }
     }
@@ -934,7 +947,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
     const int slot_floats = paged_slot(ROWS, hs);
     float *slot = a.partial + (2ll * blockIdx.x + ((int)blockIdx.x == first_cta ? 1 : 0)) * slot_floats;
     for (int i = tid; i < items; i += threads) {
-      const int r = i / quads, d = i - r * quads;
+      const int r = g_rows == 1 ? 0 : i / quads, d = i - r * quads;
       float top = s_m[0][r], sum = 0.f;
       for (int y = 1; y < KG; y++) top = fmaxf(top, s_m[y][r]);
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -972,9 +985,10 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
   }
 }
 
-// weights[s][j] += sum over the sequence's rows and heads, in their order, of 2^(score - log2 of the sum).
+// weights[s][j] += sum over the sequence's rows and heads, in their order, of 2^(score - log2 of the sum). A thread has a position;
+// the scores of eight heads are asked for together.
 __global__ void __launch_bounds__(256)
-paged_weights_kernel(PagedAttention a, float *__restrict__ weights, long long ld) {
+paged_weights_kernel(const __grid_constant__ PagedAttention a, float *__restrict__ weights, long long ld) {
   pdl_launch_dependents();
   pdl_wait();
   const PagedView &c = a.c;
@@ -984,16 +998,24 @@ paged_weights_kernel(PagedAttention a, float *__restrict__ weights, long long ld
   const int L = paged_length(c, s);
   for (int j = blockIdx.x * 256 + threadIdx.x; j < L; j += gridDim.x * 256) {
     float w = 0.f;
+    const float old = weights[s * ld + j];
     for (int t = 0; t < n; t++) {
       const int end = L - n + t + 1, begin = a.window > 0 ? max(0, end - a.window) : 0;
       if (j < begin || j >= end) continue;
-      for (int h = 0; h < a.n_head; h++) {
-        const long long rh = (long long)(first + t) * a.n_head + h;
-        const float sc = __ldcg(a.scores + rh * c.max_length + j);
-        if (sc != -INFINITY) w += exp2f(sc - __ldcg(a.stats + rh));
+      const long long row = (long long)(first + t) * a.n_head;
+      for (int h0 = 0; h0 < a.n_head; h0 += 8) {
+        float sc[8], lse[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+          const bool in = h0 + u < a.n_head;
+          sc[u] = in ? __ldcg(a.scores + (row + h0 + u) * c.max_length + j) : -INFINITY;
+          lse[u] = in ? __ldcg(a.stats + row + h0 + u) : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < 8; u++) w += sc[u] != -INFINITY ? exp2_of(sc[u] - lse[u]) : 0.f;
       }
     }
-    weights[s * ld + j] += w;
+    weights[s * ld + j] = old + w;
   }
 }
 

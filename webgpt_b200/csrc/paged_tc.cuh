@@ -180,22 +180,22 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
         for (int y = 0; y < kMine; y++) {
           const int r = warp + y * WARPS;
           int e = 0;
-          if constexpr (TERMS == 2) {  // a power of two that brings the row's largest value near 2^13
+          if constexpr (TERMS == 2) {
             float top = 0.f;
 #pragma unroll
             for (int i = 0; i < 2 * HB; i++) top = fmaxf(top, fabsf(v[y][i]));
             top = warp_max(top);
-            e = top > 0.f && top < INFINITY ? ilogbf(top) - 13 : 0;
+            e = row_exponent(top);
           }
 #pragma unroll
           for (int i = 0; i < HB; i++) {
-            float f0 = scalbnf(v[y][2 * i], -e), f1 = scalbnf(v[y][2 * i + 1], -e);
+            float f0 = v[y][2 * i] * pow2_of(-e), f1 = v[y][2 * i + 1] * pow2_of(-e);
 #pragma unroll
             for (int t = 0; t < TERMS; t++)
               *reinterpret_cast<uint32_t *>(Qs + ((i * TERMS + t) * N + r) * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) =
                   split2<T>(f0, f1);
           }
-          if (lane == 0) s_qscale[r] = scalbnf(a.scale2, e);
+          if (lane == 0) s_qscale[r] = a.scale2 * pow2_of(e);
         }
       }
       if (tid < N) {

@@ -2,7 +2,6 @@
 // verification of drafted tokens, behind the C ABI of include/webgpt_b200.h.
 #include <algorithm>
 #include <atomic>
-#include <cstdlib>
 
 #include "host.cuh"
 #include "paged.cuh"
@@ -128,6 +127,13 @@ static int32_t launch_paged_tc(wgpt_device *dev, PagedAttention &a) {
   return WGPT_OK;
 }
 
+// Whether no CTA can get more than a few units: such calls are a chain of latencies, and the form with all of them in flight,
+// one CTA an SM, is shorter than that with more CTAs an SM and fewer tiles in each one's rings. One sequence with a new token:
+// 12 heads of 64 in f32, 200 positions, 7.3 us against 8.7; 8 heads of 128 in f16, 4000 positions, 18.1 us against 19.6.
+static bool paged_few(const wgpt_device *dev, const PagedAttention &a, int unit) {
+  return ((int64_t)a.c.max_length / unit + 1) * a.c.n_seq * a.c.n_kv <= 4 * (int64_t)dev->sm_count;
+}
+
 // How many of the rows that share a head of the cache a CTA takes at once: what a sequence has of them on average. More row
 // tiles read the cache again, fewer rows leave room for more keys in flight.
 template <typename T, int HSP>
@@ -136,22 +142,27 @@ static int32_t launch_paged_rows(wgpt_device *dev, PagedAttention &a, long long 
     a.key_groups = 4;
     a.row_warps = 1;
     a.rows = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;
-    if (rows <= 1) return launch_paged_attention<T, HSP, 1, HSP <= 64 ? 2 : 3>(dev, a);
+    if (rows <= 1) {
+      if constexpr (HSP == 64)
+        if (paged_few(dev, a, 128)) return launch_paged_attention<T, HSP, 1, 4>(dev, a);
+      return launch_paged_attention<T, HSP, 1, HSP == 64 ? 2 : 3>(dev, a);
+    }
     if (rows <= 2) return launch_paged_attention<T, HSP, 2, 3>(dev, a);
     if (rows <= 4) return launch_paged_attention<T, HSP, 4, 3>(dev, a);
     return launch_paged_attention<T, HSP, 8, 3>(dev, a);
   } else {
     if constexpr (HSP <= 128) {
-      if (rows > (getenv("TCROWS") ? atoi(getenv("TCROWS")) : 8))
+      if (rows > 8)
         return rows <= 16 ? launch_paged_tc<T, HSP / 64, 16>(dev, a) : launch_paged_tc<T, HSP / 64, 32>(dev, a);
     }
-    const int most = HSP <= 128 ? 4 : 3;
-    const long long eights = (rows + 7) / 8, tiles = (eights + most - 1) / most;
+    // up to eight rows, or head sizes above 128: a key group of one warp for every eight rows, up to 24
+    const long long eights = HSP <= 128 ? 1 : (rows + 7) / 8, tiles = (eights + 2) / 3;
     a.row_warps = (int)((eights + tiles - 1) / tiles);
     a.key_groups = a.row_warps == 1 ? 4 : 2;
     a.rows = 8 * a.row_warps;
-    if (HSP == 128 && a.row_warps == 1) return launch_paged_attention<T, HSP, 1, 2>(dev, a);
-    return launch_paged_attention<T, HSP, 1, 3>(dev, a);
+    if constexpr (HSP == 128)
+      if (paged_few(dev, a, 128)) return launch_paged_attention<T, HSP, 1, 4>(dev, a);
+    return launch_paged_attention<T, HSP, 1, HSP == 128 ? 2 : 3>(dev, a);
   }
 }
 
@@ -288,10 +299,10 @@ WGPT_EXPORT int32_t wgpt_verify_drafts(wgpt_device *dev, int32_t n_seq, int32_t 
   a.partial = static_cast<float2 *>(dev->scratch);
   const int warps = kVerifyThreads / 32;
   LAUNCH_PDL(dev, verify_sums_kernel, dim3((a.chunks + warps - 1) / warps, rows, n_seq), dim3(kVerifyThreads), 0, a);
-  // as many CTAs a sequence as are resident at once: two an SM, and one where a few sequences keep their exponentials
+  // as many CTAs a sequence as are resident at once: two an SM, and one where a few sequences keep their exponentials. 64 sequences
+  // of 4 drafts over 50257 ids take 64 us with four CTAs each, 71 with eight (two waves), 88 with two and 136 with one.
   int C = kDrawCluster;
   while (C > 1 && C * n_seq > 2 * dev->sm_count) C /= 2;
-  if (getenv("DRAWC")) C = atoi(getenv("DRAWC"));
   const dim3 grid(C * n_seq), block(kDrawThreads);
   if (C == kDrawCluster && C * n_seq <= dev->sm_count && V <= 16 * 32 * kDrawWarps * C)
     CK(launch_ex_x(dev->pdl, C, dev->stream, verify_draw_kernel<16>, grid, block, 0, a));
