@@ -46,7 +46,6 @@ class PagedCache:
         self._lengths = [device.buffer(n_seq * 4) for _ in range(2)]
         self._pools = [(device.buffer(nbytes), device.buffer(nbytes)) for _ in range(n_layer)]
         self._weights = [device.buffer(n_seq * self.max_length * 4) for _ in range(n_layer)] if weights else None
-        self._kept = None
         for b in self._weights or []:
             b.write(np.zeros(n_seq * self.max_length, np.float32))
         self._upload()
@@ -108,11 +107,13 @@ class PagedCache:
     # ------------------------------------------------------------------ eviction
     def evict(self, keep, recent):
         """Thins out the sequences that hold more than keep positions, in every layer by its own weights; returns the
-        positions that stayed, [n_layer, n_seq, keep], -1 behind them. Needs as many free pages as what stays fills in the
-        sequences that are thinned out."""
+        positions that stayed, [n_layer, n_seq, keep], -1 behind them. Sequences of up to keep positions are copied whole:
+        needs as many free pages as all that stays fills."""
         if self._weights is None:
             raise ValueError("the cache keeps no weights: create it with weights=True")
-        keep = min(int(keep), self.max_length)
+        keep, recent = min(int(keep), self.max_length), int(recent)
+        if keep < 1 or not 0 <= recent <= keep:
+            raise ValueError(f"keep {keep} and recent {recent}: 0 <= recent <= keep, keep >= 1")
         after = np.minimum(self.lengths, keep)
         need = [-(-int(L) // self.page_size) for L in after]
         if sum(need) > len(self.free):
@@ -121,23 +122,22 @@ class PagedCache:
         self._tables[1].write(self._table_of(pages))
         kept = self.device.buffer(self.n_seq * keep * 4)
         moved = self.device.buffer(self.n_seq * keep * 4)
-        out = []
+        out, rows = [], np.zeros((self.n_layer, self.n_seq, self.max_length), np.float32)
         try:
             for i in range(self.n_layer):
-                w = self._weights[i]
-                _lib.call("wgpt_paged_evict", self.device.handle, self.layer(i).ptr, self.layer(i, 1).ptr, keep, int(recent), w.ptr,
-                          self.max_length, moved.ptr, keep, kept.ptr)
+                _lib.call("wgpt_paged_evict", self.device.handle, self.layer(i).ptr, self.layer(i, 1).ptr, keep, recent,
+                          self._weights[i].ptr, self.max_length, moved.ptr, keep, kept.ptr)
                 out.append(kept.read(np.int32, self.n_seq * keep).reshape(self.n_seq, keep))
-                rows = np.zeros((self.n_seq, self.max_length), np.float32)
-                rows[:, :keep] = moved.read(np.float32, self.n_seq * keep).reshape(self.n_seq, keep)
-                w.write(rows)
-        except Exception:
+                rows[i, :, :keep] = moved.read(np.float32, self.n_seq * keep).reshape(self.n_seq, keep)
+        except Exception:  # nothing that the cache goes by has changed yet
             for p in pages:
                 self.free += p
             raise
         finally:
             kept.destroy()
             moved.destroy()
+        for w, r in zip(self._weights, rows):
+            w.write(r)
         for s in range(self.n_seq):
             self.free += self.pages[s]
         self.pages = pages
