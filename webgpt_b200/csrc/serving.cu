@@ -300,7 +300,7 @@ WGPT_EXPORT int32_t wgpt_verify_drafts(wgpt_device *dev, int32_t n_seq, int32_t 
   const int warps = kVerifyThreads / 32;
   LAUNCH_PDL(dev, verify_sums_kernel, dim3((a.chunks + warps - 1) / warps, rows, n_seq), dim3(kVerifyThreads), 0, a);
   // as many CTAs a sequence as are resident at once: two an SM, and one where a few sequences keep their exponentials. 64 sequences
-  // of 4 drafts over 50257 ids take 64 us with four CTAs each, 71 with eight (two waves), 88 with two and 136 with one.
+  // of 4 drafts over 50257 ids take 51 us with four CTAs each, 55 with eight (two waves) and 71 with two.
   int C = kDrawCluster;
   while (C > 1 && C * n_seq > 2 * dev->sm_count) C /= 2;
   const dim3 grid(C * n_seq), block(kDrawThreads);

@@ -245,7 +245,8 @@ __device__ __forceinline__ void write_ids(const Verify &a, int s, int accepted, 
 
 // The accept step and the draw over the whole vocabulary, a cluster of CTAs per sequence. The draw needs running sums good to
 // far below the smallest probability, so its exponentials are in double precision: those of the target's row, and of the draft's if a
-// draft was not accepted. Every warp takes a stretch of ids; the sums of the stretches say in which one the running sum passes the
+// draft was not accepted, each by its row's sum, which the accept step has (good to a few 1e-8; the same for rows that are the same,
+// so that nothing is left of them). Every warp takes a stretch of ids; the sums of the stretches say in which one the running sum passes the
 // number, and that warp adds its stretch up id by id. A lane keeps its exponentials where they fit kVals registers.
 constexpr int kDrawThreads = 512, kDrawWarps = kDrawThreads / 32, kDrawCluster = 8;
 
@@ -255,11 +256,11 @@ __global__ void __launch_bounds__(kDrawThreads, kVals > 0 ? 1 : 2) verify_draw_k
   __shared__ float s_max[2 * kMaxDraft + 1];
   __shared__ double s_sum[2 * kMaxDraft + 1];
   __shared__ double table[64];
-  __shared__ double sums[3][kDrawCluster][kDrawWarps];  // of every warp of the cluster: the target's, the draft's, what is drawn from
+  __shared__ double sums[2][kDrawCluster][kDrawWarps];  // of every warp of the cluster: the target's, what a draft leaves of it
   uint32_t C;
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(C));
   const int rank = (int)cluster_ctarank(), s = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  for (int i = tid; i < 3 * kDrawCluster * kDrawWarps; i += kDrawThreads) (&sums[0][0][0])[i] = 0.0;  // of CTAs that are not there too
+  for (int i = tid; i < 2 * kDrawCluster * kDrawWarps; i += kDrawThreads) (&sums[0][0][0])[i] = 0.0;  // of CTAs that are not there too
   cluster_arrive();
   if (tid < 64) table[tid] = exp2(tid / 64.0);
   pdl_launch_dependents();
@@ -323,25 +324,57 @@ __global__ void __launch_bounds__(kDrawThreads, kVals > 0 ? 1 : 2) verify_draw_k
   const int beg = min(a.V, (rank * kDrawWarps + warp) * stretch), end = min(a.V, beg + stretch);
   const bool two = rest && y != nullptr;
   constexpr int kLook = kVals > 0 ? kVals : 4, kPick = 4;
-  double vx[kVals > 0 ? kVals : 1], vy[kVals > 0 ? kVals : 1];
+  double vx[kVals > 0 ? kVals : 1];
   // a lane's logits of ids i0, i0 + 32, ...: -infinity, which counts nothing, behind the stretch
-  auto fetch = [&](int i0, float (&lx)[kLook], float (&ly)[kLook]) {
+  auto fetch = [&](int i0, auto &lx, auto &ly) {
 #pragma unroll
-    for (int u = 0; u < kLook; u++) {
+    for (int u = 0; u < (int)(sizeof(lx) / sizeof(float)); u++) {
       const int i = i0 + 32 * u;
       lx[u] = i < end ? logit(x + i) : -INFINITY;
-      ly[u] = two && i < end ? logit(y + i) : -INFINITY;
+      ly[u] = two && rest && i < end ? logit(y + i) : -INFINITY;
     }
   };
-  // a sum of every warp to every CTA, behind one barrier of the cluster
-  auto tell = [&](int which, double v) {
-    v = warp_sum64(v);
-    if (lane < (int)C) dsmem_st64(dsmem_addr(&sums[which][rank][warp], lane), (unsigned long long)__double_as_longlong(v));
+  // what an id counts: its exponential; where a draft was turned down that by its row's sum, less the draft's (or less all of it
+  // at the drafted id), none below zero
+  const double ix = none ? 0.0 : 1.0 / s_sum[at], iq = two ? 1.0 / s_sum[a.n_draft + 1 + at] : 0.0;
+  auto weight = [&](float lx, float ly, int i) {
+    const double e = exp_of((double)lx - m, scale, table);
+    if (!rest) return e;
+    const double q = two ? __dmul_rn(exp_of((double)ly - mq, scale, table), iq) : (uint32_t)i == only ? 1.0 : 0.0;
+    return fmax(__dmul_rn(e, ix) - q, 0.0);  // rounded alike, so that equal rows leave zeros
+  };
+  // every warp's sum over its stretch, told to every CTA, behind one barrier of the cluster
+  auto add_up = [&]() {
+    double sum = 0.0;
+    if (!none) {
+      if constexpr (kVals > 0) {
+        float lx[kVals], ly[kVals];
+        fetch(beg + lane, lx, ly);
+#pragma unroll
+        for (int u = 0; u < kVals; u++) {
+          if (beg + 32 * u >= end) break;
+          sum += vx[u] = weight(lx[u], ly[u], beg + lane + 32 * u);
+        }
+      } else {
+        for (int i0 = beg + lane; i0 < end; i0 += 32 * kLook) {
+          float lx[kLook], ly[kLook];
+          fetch(i0, lx, ly);
+#pragma unroll
+          for (int u = 0; u < kLook; u++) sum += weight(lx[u], ly[u], i0 + 32 * u);
+        }
+      }
+      sum = warp_sum64(sum);
+      if (lane < (int)C)
+        dsmem_st64(dsmem_addr(&sums[rest ? 1 : 0][rank][warp], lane), (unsigned long long)__double_as_longlong(sum));
+    }
+    cluster_arrive();
+    cluster_wait();
   };
   // of all warps' sums: what lies before each, and their total; every warp for itself, four sums a lane
   constexpr int kAll = kDrawCluster * kDrawWarps, kPer = kAll / 32;
-  auto prefix_of = [&](int which, double (&upto)[kPer], double &from) {
-    const double *v = &sums[which][0][0] + lane * kPer;
+  double upto[kPer], from;
+  auto prefixes = [&]() {
+    const double *v = &sums[rest ? 1 : 0][0][0] + lane * kPer;
     double sum = 0.0;
 #pragma unroll
     for (int u = 0; u < kPer; u++) upto[u] = sum += v[u];
@@ -356,89 +389,18 @@ __global__ void __launch_bounds__(kDrawThreads, kVals > 0 ? 1 : 2) verify_draw_k
     if (lane == 0) from = 0.0;
     return total;
   };
-  double upto[kPer], from;
   cluster_wait();  // the others run
-  double zx = 1.0, zq = 1.0;
-  if (!none) {
-    double sx = 0.0, sy = 0.0;
-    if constexpr (kVals > 0) {
-      float lx[kVals], ly[kVals];
-      fetch(beg + lane, lx, ly);
-#pragma unroll
-      for (int u = 0; u < kVals; u++) {
-        if (beg + 32 * u >= end) break;
-        sx += vx[u] = exp_of((double)lx[u] - m, scale, table);
-        if (two) sy += vy[u] = exp_of((double)ly[u] - mq, scale, table);
-      }
-    } else {
-      for (int i0 = beg + lane; i0 < end; i0 += 32 * kLook) {
-        float lx[kLook], ly[kLook];
-        fetch(i0, lx, ly);
-#pragma unroll
-        for (int u = 0; u < kLook; u++) {
-          sx += exp_of((double)lx[u] - m, scale, table);
-          if (two) sy += exp_of((double)ly[u] - mq, scale, table);
-        }
-      }
-    }
-    tell(0, sx);
-    if (two) tell(1, sy);
-  }
-  cluster_arrive();
-  cluster_wait();
-  if (!none) {
-    if (two) zq = prefix_of(1, upto, from);
-    zx = prefix_of(0, upto, from);
-  }
-  const double ix = 1.0 / zx, iq = 1.0 / zq;
-  // what an id counts: e / sum, less the draft's (or less all of it at the drafted id), none below zero
-  auto weight = [&](double e, double f, int i) {
-    const double p = e * ix, q = two ? f * iq : (uint32_t)i == only ? 1.0 : 0.0;
-    return rest ? fmax(p - q, 0.0) : e;
-  };
-  if (at < n) {  // the same for the whole cluster, whether or not there is a distribution to take from
-    if (rest && !none) {
-      double sr = 0.0;
-      if constexpr (kVals > 0) {
-#pragma unroll
-        for (int u = 0; u < kVals; u++) {
-          const int i = beg + lane + 32 * u;
-          if (beg + 32 * u >= end) break;
-          vx[u] = weight(vx[u], vy[u], i);
-          sr += vx[u];
-        }
-      } else {
-        for (int i0 = beg + lane; i0 < end; i0 += 32 * kLook) {
-          float lx[kLook], ly[kLook];
-          fetch(i0, lx, ly);
-#pragma unroll
-          for (int u = 0; u < kLook; u++)
-            sr += weight(exp_of((double)lx[u] - m, scale, table), two ? exp_of((double)ly[u] - mq, scale, table) : 0.0, i0 + 32 * u);
-        }
-      }
-      tell(2, sr);
-    }
-    cluster_arrive();
-    cluster_wait();
-  }
-  double total = zx;
-  if (rest && !none) {
-    total = prefix_of(2, upto, from);
-    if (!(total > 0.0)) {  // nothing is left: drawn from the target's row itself
-      rest = false;
-      total = prefix_of(0, upto, from);
-      if constexpr (kVals > 0) {
-        float lx[kVals], ly[kVals];
-        fetch(beg + lane, lx, ly);
-#pragma unroll
-        for (int u = 0; u < kVals; u++) vx[u] = exp_of((double)lx[u] - m, scale, table);
-      }
-    }
+  add_up();
+  double total = prefixes();
+  if (rest && !(total > 0.0)) {  // nothing is left, in the whole cluster's eyes: drawn from the target's row itself
+    rest = false;
+    add_up();
+    total = prefixes();
   }
   if (!none) {
     // the last stretch with anything in it that begins at or below the goal has the id (rounding may put the beginning of an empty
     // one there); one warp adds it up
-    const double goal = u01 * total, *of = &sums[rest ? 2 : 0][0][0] + lane * kPer;
+    const double goal = u01 * total, *of = &sums[rest ? 1 : 0][0][0] + lane * kPer;
     int mine = -1;
 #pragma unroll
     for (int u = 0; u < kPer; u++)
@@ -492,8 +454,7 @@ __global__ void __launch_bounds__(kDrawThreads, kVals > 0 ? 1 : 2) verify_draw_k
           float lx[kPick], ly[kPick];
           fetch(i0 + lane, lx, ly);
 #pragma unroll
-          for (int u = 0; u < kPick; u++)
-            w[u] = weight(exp_of((double)lx[u] - m, scale, table), two ? exp_of((double)ly[u] - mq, scale, table) : 0.0, i0 + lane + 32 * u);
+          for (int u = 0; u < kPick; u++) w[u] = weight(lx[u], ly[u], i0 + lane + 32 * u);
           rows_of(i0, w);
         }
       }
