@@ -36,6 +36,7 @@ struct PagedAttention {
   long long ld_q, ld_out;
   int key_groups, row_warps, rows;  // of a CTA: key groups of row_warps warps; rows of a row tile
   int least;             // fewest units a CTA takes
+  int extra;             // units that the beginning and end of a group count as
   int ahead;             // whether the results of a group leave room for the next one's first tiles
   float *partial;        // [2 * CTAs][paged_slot(rows, hs)]
   unsigned int *join;    // a counter per CTA, zero on entry and left zero
@@ -48,7 +49,7 @@ __device__ __forceinline__ uint32_t quotient(uint32_t x, uint32_t by) { return b
 // A sequence's share of the work.
 struct PagedSeq {
   int first, n, L, begin;  // rows, length, position of the first unit
-  int tiles, units;        // row tiles, units of each
+  int tiles, units;        // row tiles, units of each and what is added to them
 };
 
 __device__ __forceinline__ PagedSeq paged_seq(const PagedAttention &a, int s, int unit) {
@@ -58,7 +59,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedAttention &a, int s, in
   const int lowest = a.window > 0 ? max(0, q.L - q.n + 1 - a.window) : 0;
   q.begin = min(lowest, q.L) & ~(unit - 1);
   q.tiles = q.n * a.group <= a.rows ? (q.n > 0 ? 1 : 0) : (q.n * a.group + a.rows - 1) / a.rows;
-  q.units = max(1, (q.L - q.begin + unit - 1) >> (__ffs(unit) - 1));  // one even if there is nothing to see: the rows are set to zero
+  q.units = a.extra + max(1, (q.L - q.begin + unit - 1) >> (__ffs(unit) - 1));  // one even if there is nothing to see: the rows are set to zero
   return q;
 }
 __device__ __forceinline__ uint32_t paged_work(const PagedAttention &a, const PagedSeq &q) {
@@ -96,6 +97,14 @@ __device__ __forceinline__ long long row_index(const PagedAttention &a, const Pa
   return (long long)(w.q.first + token) * a.n_head + head;
 }
 
+// Every group begins with a.extra units that have no positions: what it takes to load its queries and to put its results together,
+// which a CTA with the end of one group and the beginning of another does twice. A share that ends among them leaves the group to
+// the next CTA.
+__device__ __forceinline__ bool paged_more(const PagedAttention &a, const PagedPart &w, uint32_t end) { return w.next + a.extra < end; }
+__device__ __forceinline__ int paged_first_cta(const PagedAttention &a, const PagedPart &w, uint32_t per) {
+  return (int)((w.begin + a.extra) / per);
+}
+
 // The part that begins at unit x of sequence s, up to unit end at most; q and seq_begin are the sequence's.
 __device__ __forceinline__ void paged_part(const PagedAttention &a, PagedPart &w, const PagedSeq &q, int s, uint32_t seq_begin, uint32_t x,
                                            uint32_t end, int unit) {
@@ -114,8 +123,8 @@ __device__ __forceinline__ void paged_part(const PagedAttention &a, PagedPart &w
   row_range(a, q, last, w.g.inner_low, w.g.highest);
   // units that no row of the tile sees are left out
   const int shift = __ffs(unit) - 1;
-  w.u0 = max((int)(x - w.begin), (w.g.lowest - q.begin) >> shift);
-  w.n_tiles = max(0, min((int)(w.next - w.begin), (w.g.highest - q.begin + unit - 1) >> shift) - w.u0);
+  w.u0 = max(max(0, (int)(x - w.begin) - a.extra), (w.g.lowest - q.begin) >> shift);
+  w.n_tiles = max(0, min((int)(w.next - w.begin) - a.extra, (w.g.highest - q.begin + unit - 1) >> shift) - w.u0);
 }
 
 // A CTA's units [.., end) of all there are and the part they begin with, by all its threads, every one of which gets it: false if
@@ -152,7 +161,7 @@ __device__ __forceinline__ bool paged_first(const PagedAttention &a, PagedPart &
     of.tiles = __shfl_sync(0xffffffffu, q.tiles, s);
     of.units = __shfl_sync(0xffffffffu, q.units, s);
     paged_part(a, to, of, s, __shfl_sync(0xffffffffu, upto - mine, s), x0, end, unit);
-    return true;
+    return end > to.begin + a.extra;
   }
   auto scan = [&](uint32_t mine, uint32_t &all) {  // sum over the threads before this one, and over all
     const uint32_t upto = before_lane(mine);
@@ -184,7 +193,7 @@ __device__ __forceinline__ bool paged_first(const PagedAttention &a, PagedPart &
   }
   __syncthreads();
   to = *place;
-  return true;
+  return end > to.begin + a.extra;
 }
 
 // The part behind `w`, which ends before unit `end`. May not be `w` itself.
@@ -432,10 +441,11 @@ __device__ __forceinline__ uint32_t split2(float &x, float &y) {
 
 
 // Joins a group's parts once this CTA's lies in its slot: the CTA that finishes last does, in the order of the positions. By
-// `threads` threads that meet in sync(); red and red_sum: a place for each of them; factor and sums: kJoinFactors places.
+// `threads` threads that meet in sync(); red and red_sum: a place for each of them; factor and sums: kJoinFactors places; out_at:
+// where the rows' results go.
 template <typename Sync>
 __device__ __forceinline__ void paged_join(const PagedAttention &a, const PagedPart &w, int first_cta, int parts, int ROWS, int tid,
-                                           int threads, Sync sync, float4 *red, float *red_sum, float *factor, float *sums, int *is_last) {
+                                           int threads, Sync sync, float4 *red, float *red_sum, float *factor, float *sums, const long long *out_at, int *is_last) {
   const int hs = a.c.hs, quads = hs / 4, items = w.g.rows * quads, slot_floats = paged_slot(ROWS, hs);
   __threadfence();
   sync();
@@ -516,7 +526,7 @@ __device__ __forceinline__ void paged_join(const PagedAttention &a, const PagedP
     if (live && sh == 0) {
       const float inv = table ? sums[r] : sum != 0.f ? 1.f / sum : 0.f;
       if (table || sum != 0.f) v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-      reinterpret_cast<float4 *>(a.out + row_offset(a, w, r, a.ld_out))[i - r * quads] = v;
+      reinterpret_cast<float4 *>(a.out + out_at[r])[i - r * quads] = v;
       if (a.stats && !table && i == r * quads) a.stats[row_index(a, w, r)] = top + log2f(sum);
     }
   }
@@ -534,7 +544,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
   extern __shared__ __align__(16) unsigned char paged_smem[];
   __shared__ float s_m[kPagedKeyGroups][MAXROWS], s_l[kPagedKeyGroups][MAXROWS], s_qscale[MAXROWS];
   __shared__ int s_lo[MAXROWS], s_hi[MAXROWS];
-  __shared__ long long s_row[MAXROWS];
+  __shared__ long long s_row[MAXROWS], s_out[MAXROWS];  // where the rows' scores and results begin
   __shared__ uint32_t s_ok[kPagedKeyGroups][D];
   __shared__ uint32_t s_sum[kPagedWarps];
   __shared__ PagedPart s_part[2];
@@ -580,8 +590,8 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
     const PagedGroup &g = w.g;
     // ---- the next part, by a thread that has no query to load first
     if (tid == threads - 1) {
-      s_more = w.next < x1;
-      if (w.next < x1) paged_next(a, s_part[turn ^ 1], w, x1, unit);
+      s_more = paged_more(a, w, x1);
+      if (s_more) paged_next(a, s_part[turn ^ 1], w, x1, unit);
     }
     // ---- the queries
     if constexpr (S::kWide) {
@@ -633,7 +643,10 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
     }
     if (tid < ROWS) {
       int lo = 0, hi = 0;
-      if (tid < g.rows) row_range(a, w.q, (g.r0 + tid) / a.group, lo, hi);
+      if (tid < g.rows) {
+        row_range(a, w.q, (g.r0 + tid) / a.group, lo, hi);
+        s_out[tid] = row_offset(a, w, tid, a.ld_out);
+      }
       s_lo[tid] = lo;
       s_hi[tid] = hi;
       if (a.scores) s_row[tid] = row_index(a, w, tid) * c.max_length;
@@ -942,7 +955,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
     __syncthreads();
 
     // ---- the key groups' results, and the group's if other CTAs have a part of it
-    const int first_cta = (int)(w.begin / per), last_cta = (int)((w.end - 1) / per), parts = last_cta - first_cta + 1;
+    const int first_cta = paged_first_cta(a, w, per), last_cta = (int)((w.end - 1) / per), parts = last_cta - first_cta + 1;
     const int quads = hs / 4, items = g_rows * quads;
     const int slot_floats = paged_slot(ROWS, hs);
     float *slot = a.partial + (2ll * blockIdx.x + ((int)blockIdx.x == first_cta ? 1 : 0)) * slot_floats;
@@ -966,7 +979,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
           const float inv = 1.f / sum;
           v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
         }
-        reinterpret_cast<float4 *>(a.out + row_offset(a, w, r, a.ld_out))[d] = v;
+        reinterpret_cast<float4 *>(a.out + s_out[r])[d] = v;
         if (a.stats && d == 0) a.stats[row_index(a, w, r)] = top + log2f(sum);
       } else {
         __stcg(reinterpret_cast<float4 *>(slot) + i, v);
@@ -977,7 +990,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
       }
     }
     if (parts > 1)
-      paged_join(a, w, first_cta, parts, ROWS, tid, threads, [] { __syncthreads(); }, s_red, s_red_sum, s_factor, s_sums, &s_last);
+      paged_join(a, w, first_cta, parts, ROWS, tid, threads, [] { __syncthreads(); }, s_red, s_red_sum, s_factor, s_sums, s_out, &s_last);
     __syncthreads();
     if (!more) break;
     if (padded) clear(reinterpret_cast<unsigned char *>(o_smem), a.ahead ? S::kTileBytes : S::kRing);

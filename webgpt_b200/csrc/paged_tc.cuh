@@ -99,10 +99,10 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
   __shared__ uint64_t full[NS], empty[NS], q_ready, s_done[2], p_ready[2], o_done[2], drained;
   __shared__ uint32_t tmem_slot, s_sum[S::kThreads / 32];
   __shared__ int abort_word, s_last;
-  __shared__ PagedPart s_part;
+  __shared__ PagedPart s_part[3];  // the softmax warps' part and the next, and a place for the first
   __shared__ __align__(16) float s_qscale[N], s_max[4][N], s_l[N], s_m[N];
   __shared__ int s_lo[N], s_hi[N];
-  __shared__ long long s_row[N];
+  __shared__ long long s_row[N], s_out[N];  // where the rows' scores and results begin
   __shared__ float4 s_red[SOFT];
   __shared__ float s_red_sum[SOFT], s_factor[kJoinFactors], s_sums[kJoinFactors];
   volatile int *abort_flag = &abort_word;
@@ -134,8 +134,8 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
   pdl_wait();
 
   uint32_t per = 1, x1 = 0;
-  PagedPart w;
-  const bool any = paged_first(a, w, kTcKeys, s_sum, &s_part, per, x1);
+  PagedPart first;
+  const bool any = paged_first(a, first, kTcKeys, s_sum, &s_part[2], per, x1);
   // A wait that has run out makes all others return at once: every role runs to its end.
   auto wait = [&](uint64_t *bar, uint32_t parity) {
     if (!*abort_flag && !mbar_wait(bar, parity & 1, TC_POLLS)) *abort_flag = 1;
@@ -158,8 +158,12 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
           : "memory");
       return r != 0;
     };
-    for (;;) {
+    if (tid == 0) s_part[0] = first;
+    meet();
+    for (int turn = 0;; turn ^= 1) {
+      const PagedPart &w = s_part[turn];
       const int rows = w.g.rows, n_tiles = w.n_tiles;
+      const long long q_at = lane < rows ? row_offset(a, w, lane, a.ld_q) : -1;  // of the row that is this lane's number
       // ---- the queries: K-major rows of 128 bytes, 16-byte pieces swizzled
       if (n_tiles > 0) {
         constexpr int kMine = N / WARPS;  // rows of a warp, their loads in flight together
@@ -167,11 +171,11 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
 #pragma unroll
         for (int y = 0; y < kMine; y++) {
           const int r = warp + y * WARPS;
-          const float *row = r < rows ? a.q + row_offset(a, w, r, a.ld_q) : nullptr;
+          const long long at = __shfl_sync(0xffffffffu, q_at, r);
 #pragma unroll
           for (int i = 0; i < HB; i++) {
             const int d = 2 * lane + 64 * i;
-            const float2 f = row && d < hs ? __ldcg(reinterpret_cast<const float2 *>(row + d)) : make_float2(0.f, 0.f);
+            const float2 f = at >= 0 && d < hs ? __ldcg(reinterpret_cast<const float2 *>(a.q + at + d)) : make_float2(0.f, 0.f);
             v[y][2 * i] = f.x;
             v[y][2 * i + 1] = f.y;
           }
@@ -200,7 +204,10 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
       }
       if (tid < N) {
         int lo = 0, hi = 0;
-        if (tid < rows) row_range(a, w.q, (w.g.r0 + tid) / a.group, lo, hi);
+        if (tid < rows) {
+          row_range(a, w.q, (w.g.r0 + tid) / a.group, lo, hi);
+          s_out[tid] = row_offset(a, w, tid, a.ld_out);
+        }
         s_lo[tid] = lo;
         s_hi[tid] = hi;
         if (a.scores) s_row[tid] = row_index(a, w, tid) * c.max_length;
@@ -208,6 +215,10 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
       fence_async_smem();
       meet();
       if (n_tiles > 0 && lane == 0) mbar_arrive(&q_ready);
+      // the next part, by one thread while the first scores are on their way
+      const bool more = paged_more(a, w, x1);
+      if (more && tid == SOFT - 1) paged_next(a, s_part[turn ^ 1], w, x1, kTcKeys);
+      __syncwarp();
       float m[R], l[R], o[R];
 #pragma unroll
       for (int r = 0; r < R; r++) {
@@ -221,7 +232,7 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
         if (p < w.g.lowest || p >= w.g.highest) return 0xFFFFFFFFu;
         return __ldcg(table + (c.page_shift >= 0 ? (uint32_t)p >> c.page_shift : (uint32_t)p / c.page_size));
       };
-      uint32_t page = n_tiles > 0 ? page_of(pos) : 0u;
+      uint32_t page = 0u, page_next = n_tiles > 0 ? page_of(pos) : 0u;
       auto add_values = [&](uint32_t i) {  // of tile i
         wait(&o_done[i & 1], i >> 1);
         tc_fence_after();
@@ -231,7 +242,8 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
         for (int r = 0; r < R; r++) o[r] += v[r];
       };
       for (int t = 0; t < n_tiles; t++, tile++, pos += kTcKeys) {
-        const bool there = page < c.n_pages;
+        page = page_next;
+        page_next = t + 1 < n_tiles ? page_of(pos + kTcKeys) : 0u;
         wait(&s_done[tile & 1], tile >> 1);
         tc_fence_after();
         float x[R];
@@ -246,6 +258,7 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
           x[r + 2] *= qs.z;
           x[r + 3] *= qs.w;
         }
+        const bool there = page < c.n_pages;
         if (!whole || !there) {
 #pragma unroll
           for (int r = 0; r < R; r++)
@@ -305,7 +318,6 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_ready[tile & 1]);
         if (!added) add_values(tile - 1);  // while this tile's are made
-        page = t + 1 < n_tiles ? page_of(pos + kTcKeys) : 0u;
       }
       if (n_tiles > 0) add_values(tile - 1);
       tc_fence_before();
@@ -337,16 +349,19 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
         meet();
       }
       // ---- the result, or this part of it
-      const int first_cta = (int)(w.begin / per), last_cta = (int)((w.end - 1) / per), parts = last_cta - first_cta + 1;
+      const int first_cta = paged_first_cta(a, w, per), last_cta = (int)((w.end - 1) / per), parts = last_cta - first_cta + 1;
       float *slot = a.partial + (2ll * blockIdx.x + ((int)blockIdx.x == first_cta ? 1 : 0)) * paged_slot(N, hs);
+      if (parts == 1) {
+        if (tid < N) s_max[0][tid] = s_l[tid] != 0.f ? 1.f / s_l[tid] : 0.f;
+        meet();
 #pragma unroll
-      for (int r = 0; r < R; r++) {
-        if (r0 + r < rows && key < hs) {
-          if (parts == 1)
-            a.out[row_offset(a, w, r0 + r, a.ld_out) + key] = s_l[r0 + r] != 0.f ? o[r] / s_l[r0 + r] : 0.f;
-          else
-            __stcg(slot + (r0 + r) * hs + key, o[r]);
-        }
+        for (int r = 0; r < R; r++)
+          if (r0 + r < rows && key < hs) a.out[s_out[r0 + r] + key] = o[r] * s_max[0][r0 + r];
+      } else {
+        float *to = slot + r0 * hs + key;
+#pragma unroll
+        for (int r = 0; r < R; r++, to += hs)
+          if (r0 + r < rows && key < hs) __stcg(to, o[r]);
       }
       if (tid < rows) {
         if (parts > 1) {
@@ -356,11 +371,9 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
           a.stats[row_index(a, w, tid)] = s_m[tid] + log2f(s_l[tid]);
         }
       }
-      if (parts > 1) paged_join(a, w, first_cta, parts, N, tid, SOFT, meet, s_red, s_red_sum, s_factor, s_sums, &s_last);
-      if (w.next >= x1) break;
+      if (parts > 1) paged_join(a, w, first_cta, parts, N, tid, SOFT, meet, s_red, s_red_sum, s_factor, s_sums, s_out, &s_last);
+      if (!more) break;
       meet();
-      const PagedPart before = w;
-      paged_next(a, w, before, x1, kTcKeys);
     }
   } else if (any && warp == WARPS) {
     // ------------------------------------------------------------------ products: the whole warp runs this, one lane issues
@@ -383,6 +396,7 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
       umma_commit_elect(&empty[st]);
       use++;
     };
+    PagedPart w = first;
     for (;;) {
       const int n_tiles = w.n_tiles;
       if (n_tiles > 0) {
@@ -407,7 +421,7 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
           use++;
         }
       }
-      if (w.next >= x1) break;
+      if (!paged_more(a, w, x1)) break;
       const PagedPart before = w;
       paged_next(a, w, before, x1, kTcKeys);
     }
@@ -458,6 +472,7 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(&full[st])) : "memory");
       fills++;
     };
+    PagedPart w = first;
     for (;;) {
       const T *k = static_cast<const T *>(c.k) + w.g.kvh * c.head_stride, *v = static_cast<const T *>(c.v) + w.g.kvh * c.head_stride;
       const uint32_t *table = c.table + (size_t)w.g.s * c.table_stride;
@@ -491,7 +506,7 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
         before_at = at;
         before_plain = plain;
       }
-      if (w.next >= x1) break;
+      if (!paged_more(a, w, x1)) break;
       const PagedPart before = w;
       paged_next(a, w, before, x1, kTcKeys);
     }
