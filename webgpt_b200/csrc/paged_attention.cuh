@@ -447,16 +447,16 @@ template <typename Sync>
 __device__ __forceinline__ void paged_join(const PagedAttention &a, const PagedPart &w, int first_cta, int parts, int ROWS, int tid,
                                            int threads, Sync sync, float4 *red, float *red_sum, float *factor, float *sums, const long long *out_at, int *is_last) {
   const int hs = a.c.hs, quads = hs / 4, items = w.g.rows * quads, slot_floats = paged_slot(ROWS, hs);
-  __threadfence();
   sync();
-  if (tid == 0) {
+  if (tid == 0) {  // its fences stand for all threads', on their side of the barriers
+    __threadfence();
     const unsigned int done = atomicAdd(a.join + first_cta, 1u);
     *is_last = done == (unsigned)parts - 1;
     if (*is_last) a.join[first_cta] = 0;
+    __threadfence();
   }
   sync();
   if (!*is_last) return;
-  __threadfence();
   auto part_of = [&](int k) { return a.partial + (2ll * (first_cta + k) + (k == 0 ? 1 : 0)) * slot_floats; };
   const int rows = w.g.rows, n = parts * rows;
   const bool table = n <= kJoinFactors;  // else every thread computes the factors that it needs
@@ -480,8 +480,35 @@ __device__ __forceinline__ void paged_join(const PagedAttention &a, const PagedP
     }
     sync();
   }
-  // where a row tile has few values, several threads share a quad and take every so many parts
+  // where a row tile has few values, several threads share a quad and take every so many parts; where it has many, the loads of two
+  // quads are in flight together
   const int share = items >= threads ? 1 : threads / items;
+  if (table && share == 1) {
+    for (int i = tid; i < items; i += 2 * threads) {
+      const int at[2] = {i, min(i + threads, items - 1)}, r[2] = {at[0] / quads, at[1] / quads};
+      float4 v[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll 4
+      for (int k = 0; k < parts; k++) {
+        const float4 *part = reinterpret_cast<const float4 *>(part_of(k));
+        const float4 o[2] = {__ldcg(part + at[0]), __ldcg(part + at[1])};
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+          const float f = factor[k * rows + r[y]];
+          v[y].x += f * o[y].x;
+          v[y].y += f * o[y].y;
+          v[y].z += f * o[y].z;
+          v[y].w += f * o[y].w;
+        }
+      }
+#pragma unroll
+      for (int y = 0; y < 2; y++) {
+        const float inv = sums[r[y]];
+        if (i + y * threads < items)
+          reinterpret_cast<float4 *>(a.out + out_at[r[y]])[at[y] - r[y] * quads] = make_float4(v[y].x * inv, v[y].y * inv, v[y].z * inv, v[y].w * inv);
+      }
+    }
+    return;
+  }
   for (int i0 = 0; i0 < items; i0 += threads) {
     const int i = share > 1 ? tid % items : i0 + tid, sh = share > 1 ? tid / items : 0;
     const bool live = i < items && sh < share;
