@@ -320,8 +320,8 @@ enum { WGPT_TYPE_F32 = 0, WGPT_TYPE_F16 = 1, WGPT_TYPE_BF16 = 2 };
  * elements, so that pools [page][position][head][head_size] and [page][head][position][head_size] both fit). Several layers
  * may share table and lengths; sequences may share pages that are only read. The descriptor is read during the call; the
  * arrays it names are read when the kernels run. Requirements, otherwise WGPT_ERR_SHAPE / WGPT_ERR_ALIGN: head_size a
- * multiple of 8 up to 256, table_stride * page_size >= max_length, k and v 16-byte aligned, strides that are not negative and multiples of
- * 16 bytes. Of what lies in the pages, only positions below a sequence's length are read. */
+ * multiple of 8 up to 256, table_stride * page_size >= max_length, at most 65535 sequences of at most 2^30 positions, k and v
+ * 16-byte aligned, strides that are not negative and multiples of 16 bytes. Of what lies in the pages, only positions below a sequence's length are read. */
 typedef struct wgpt_paged_cache {
   void *k, *v;              /* pools of n_pages pages, elements of `type` */
   const uint32_t *table;    /* [n_seq, table_stride] page ids; entries behind a sequence's last page are not read */
@@ -346,8 +346,10 @@ int32_t wgpt_paged_append(wgpt_device *dev, const wgpt_paged_cache *cache, int32
  * head_size f32 values, rows ld_q apart; head h reads the cache's head h / (n_head / n_kv_head). The row of position t sees
  * the positions j <= t, and of these j > t - window where window > 0:
  *   out = sum_j softmax_j(scale * q . k_j) v_j,
- * f32 throughout (half-precision caches go through the tensor cores as they are, q and the probabilities as sums of half-precision values). A row
- * that belongs to a token but sees nothing (it has no position, or a page id of its is out of range throughout) is set to zeros; positions in a page whose id is out of range are not seen. Rows that belong to no sequence are left as they were.
+ * f32 throughout (half-precision caches go through the tensor cores as they are, q and the probabilities as sums of
+ * half-precision values). Positions in a page whose id is out of range are not seen; a row that belongs to a token but sees
+ * nothing is set to zeros; rows that belong to no sequence are left as they were. q and out may be one array. ld_q and ld_out
+ * multiples of 4. The row tiles of a call times its tiles of positions have to stay below 2^32 (WGPT_ERR_SHAPE: split the call).
  * weights, or NULL: [n_seq, ld_weights] f32, ld_weights >= max_length; the attention weight that each position got, summed
  * over the heads and new tokens of its sequence, is added to weights[s * ld_weights + j]. The order of all sums is fixed:
  * the same call gives the same bits. */
@@ -358,11 +360,11 @@ int32_t wgpt_paged_attention(wgpt_device *dev, const wgpt_paged_cache *cache, in
 /* Thins out every sequence that holds more than `keep` positions: the `recent` newest stay and, of the older ones, the
  * keep - recent with the largest accumulated weight (the lowest position among equals; NaN counts as the largest). What
  * stays keeps its order and goes to the positions 0, 1, ... of the cache `to`, which has the shape and type of `from` and
- * pages, a table and lengths of its own; its lengths are set to min(length, keep). Sequences of up to `keep` positions are copied
- * whole. The pages of `to` must not overlap the pages of `from` (slots that are read may be shared by sequences, so
+ * pages and a table of its own; its lengths (which may be from's array) are set to min(length, keep). Sequences of up to `keep`
+ * positions are copied whole. The pages of `to` must not overlap the pages of `from` (slots that are read may be shared by sequences, so
  * nothing is moved in place): hand over free pages and take back the old ones. Key and value rows are copied as they are.
  * weights [n_seq, ld_weights] as above; weights_to [n_seq, ld_weights_to >= keep], or NULL: the weights of what stays, zeros
- * behind it; kept [n_seq, keep]: the positions in `from` that stayed, -1 behind them. 0 <= recent <= keep, keep >= 1,
+ * behind it, not overlapping weights; kept [n_seq, keep]: the positions in `from` that stayed, -1 behind them. 0 <= recent <= keep, keep >= 1,
  * to->max_length >= min(keep, from->max_length). A position whose page id is out of range, on either side, is not copied. */
 int32_t wgpt_paged_evict(wgpt_device *dev, const wgpt_paged_cache *from, const wgpt_paged_cache *to, int32_t keep,
                          int32_t recent, const float *weights, int64_t ld_weights, float *weights_to,
@@ -376,11 +378,12 @@ int32_t wgpt_paged_evict(wgpt_device *dev, const wgpt_paged_cache *from, const w
  * next token is drawn from max(p_i - q_i, 0), or from p_i if that is zero everywhere; behind the last accepted one from
  * p_i. Drawn: with the number uniforms[s * (n_draft + 1) + n_draft] in [0,1), the first id whose running sum exceeds number * total, in
  * the order of the ids, or of descending logits where top_k > 0 (so that no drafts and a top_k give wgpt_sample_topk's
- * pick). Probabilities that decide are in double precision. NaN logits count as -infinity; a row with no finite value or with +infinity has no distribution:
- * as a target it accepts nothing and draws id 0, as a draft it accepts nothing and counts as q = 0, and both are reported. A drafted id >= V is not
- * accepted and reported.
+ * pick). Probabilities are in double precision; a row's sum over the whole vocabulary, by which they are divided, is good to a
+ * few 1e-8. NaN logits count as -infinity; a row with no finite value or with +infinity has no distribution: as a target it
+ * accepts nothing and draws id 0, as a draft it accepts nothing and counts as q = 0, and both are reported. A drafted id >= V
+ * is not accepted and reported. ld_target and ld_draft >= V, in any alignment.
  * ids_out [n_seq, n_draft + 1]: the accepted drafts, the drawn token, WGPT_NO_ID behind it; n_accepted [n_seq].
- * 0 <= n_draft <= WGPT_MAX_DRAFT, 0 <= top_k <= min(WGPT_MAX_TOP_K, V). */
+ * 0 <= n_draft <= WGPT_MAX_DRAFT, 0 <= top_k <= min(WGPT_MAX_TOP_K, V), n_seq <= 65535; top_k * V up to 26 million. */
 #define WGPT_MAX_DRAFT 64
 #define WGPT_NO_ID 0xFFFFFFFFu
 int32_t wgpt_verify_drafts(wgpt_device *dev, int32_t n_seq, int32_t n_draft, int32_t V, const float *target,

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 import serving_reference as ref
-from test_gpu_paged import cast
+from test_gpu_paged import OnDevice, cast, make
 from webgpt_b200 import _lib
 
 pytestmark = pytest.mark.gpu
@@ -178,6 +178,72 @@ def test_steps_of_several_users(blocks, type, n_head, n_kv, hs, window, replayed
     for b in g.operations:
         b.clearBufferCache()
     cache.destroy()
+
+
+def test_eviction_replayed(blocks):
+    """A recorded eviction goes by the lengths and weights of the time it is replayed, and may share the lengths of its two caches."""
+    dev, g = blocks
+    rng = np.random.default_rng(5)
+    pages = make(rng, [40, 25, 5000], 8, 2, 16, "f16")
+    src, dst = OnDevice(dev, pages, "f16"), OnDevice(dev, make(rng, [5000] * 3, 8, 2, 16, "f16", fill=-7.0), "f16")
+    src.d.lengths = dst.d.lengths  # one array
+    lengths = dst.lengths
+    lengths.write(np.array([40, 25, 5000], np.int32))
+    w = rng.random((3, 5000)).astype(np.float32)
+    wb = dev.tensor(w)
+    wt = dev.buffer(3 * 30 * 4)
+    graph = C.c_void_p()
+    passes = g.PagedEvictBlock.newInstance(Described(src), Described(dst), 30, 7, wb, wt)
+    _lib.call("wgpt_graph_begin", dev.handle)
+    run(passes["passes"])
+    _lib.call("wgpt_graph_end", dev.handle, C.byref(graph))
+    for L in ([40, 25, 5000], [31, 0, 4096], [30, 29, 31]):
+        L = [min(a, b) for a, b in zip(L, [40, 25, 5000])]
+        lengths.write(np.array(L, np.int32))
+        w = rng.integers(0, 50, w.shape).astype(np.float32)  # many equal ones
+        wb.write(w)
+        _lib.call("wgpt_graph_launch", dev.handle, graph)
+        kept, moved = passes["resultBuffer"].read(np.int32, 90).reshape(3, 30), wt.read(np.float32, 90).reshape(3, 30)
+        for s in range(3):
+            want = ref.keep(w[s], L[s], 30, 7)
+            assert list(kept[s]) == want + [-1] * (30 - len(want))
+            assert list(moved[s]) == list(w[s, want]) + [0] * (30 - len(want))
+            assert lengths.read(np.int32, 3)[s] == len(want)
+    _lib.call("wgpt_graph_destroy", dev.handle, graph)
+
+
+def test_limits(blocks):
+    """Counts past what the kernels' grids and positions hold, and evictions that would write what they read, are refused."""
+    dev, _ = blocks
+    pages = make(np.random.default_rng(0), [20, 10], 16, 2, 64, "f32")
+    x = dev.buffer(1 << 16)
+
+    def refused(code, name, *args):
+        with pytest.raises(_lib.WgptError) as e:
+            _lib.call(name, dev.handle, *args)
+        assert e.value.code == code, e.value
+
+    for change in (dict(n_seq=65536), dict(max_length=(1 << 30) + 1, page_size=1 << 30)):
+        c = OnDevice(dev, pages, "f32")
+        for name, value in change.items():
+            setattr(c.d, name, value)
+        refused(_lib.ERR_SHAPE, "wgpt_paged_append", c.ptr, 65536, None, x.ptr, x.ptr, 128)
+        refused(_lib.ERR_SHAPE, "wgpt_paged_attention", c.ptr, 65536, None, 2, 0.125, 0, x.ptr, 128, x.ptr, 128, None, 0)
+        refused(_lib.ERR_SHAPE, "wgpt_paged_evict", c.ptr, c.ptr, 4, 1, x.ptr, 1 << 30, None, 0, x.ptr)
+    c, to = OnDevice(dev, pages, "f32"), OnDevice(dev, pages, "f32")
+    refused(_lib.ERR_ARG, "wgpt_paged_evict", c.ptr, c.ptr, 4, 1, x.ptr, 20, None, 0, x.ptr + 4096)
+    for at in (0, 39 * 4, -4 * 7):  # weights are 20 + 20 values, weights_to 4 + 4
+        refused(_lib.ERR_ARG, "wgpt_paged_evict", c.ptr, to.ptr, 4, 1, x.ptr + 2048, 20, x.ptr + 2048 + at, 4, x.ptr + 4096)
+    _lib.call("wgpt_paged_evict", dev.handle, c.ptr, to.ptr, 4, 1, x.ptr + 2048, 20, x.ptr + 2048 + 160, 4, x.ptr + 4096)
+    _lib.call("wgpt_paged_evict", dev.handle, c.ptr, to.ptr, 4, 1, x.ptr + 2048, 20, x.ptr + 2048 - 32, 4, x.ptr + 4096)
+    dev.synchronize()
+
+
+class Described:
+    """A test cache as a pass takes it."""
+
+    def __init__(self, cache):
+        self.ptr, self.n_seq, self.max_length = cache.ptr, cache.d.n_seq, cache.d.max_length
 
 
 class Part:

@@ -167,3 +167,34 @@ def test_reference_eviction():
     assert ref.keep(w, 7, 3, 3) == [4, 5, 6]
     assert ref.keep(w, 7, 2, 0) == [2, 6]
     assert ref.keep(w, 3, 3, 0) == [0, 1, 2]
+
+
+def test_eviction_that_fails_changes_nothing(monkeypatch):
+    """A call that fails in a later layer leaves pages, lengths and every layer's weights as they were."""
+    class Readable(FakeBuffer):
+        def read(self, dtype, count):
+            return self.data.view(dtype)[:count]
+
+    monkeypatch.setattr(FakeDevice, "buffer", lambda self, nbytes, dims=None: Readable(nbytes))
+    c = PagedCache(FakeDevice(), 2, 1, 8, n_pages=12, page_size=4, max_length=16, n_layer=2, weights=True)
+    c.advance([13, 5])
+    for i in range(2):
+        c.weights(i).write(np.arange(32, dtype=np.float32))
+    calls = []
+
+    def call(name, *args):
+        calls.append(name)
+        if len(calls) == 2:
+            raise _lib.WgptError(_lib.ERR_SHAPE, "no")
+
+    monkeypatch.setattr(_lib, "call", call)
+    pages, weights = [list(p) for p in c.pages], [w.data.copy() for w in c._weights]
+    with pytest.raises(_lib.WgptError):
+        c.evict(4, 2)
+    assert c.pages == pages and list(c.lengths) == [13, 5] and len(calls) == 2
+    assert all(np.array_equal(w.data, before) for w, before in zip(c._weights, weights))
+    check(c)
+    for keep, recent in ((0, 0), (4, 5), (4, -1)):
+        with pytest.raises(ValueError):
+            c.evict(keep, recent)
+    check(c)

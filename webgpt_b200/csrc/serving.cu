@@ -21,6 +21,9 @@ static int32_t check_cache(wgpt_device *dev, const wgpt_paged_cache *c, PagedVie
               c->max_length >= 1,
           WGPT_ERR_SHAPE, "empty cache: %d pages of %d, %d heads, %d sequences of up to %d positions, %d pages a table row",
           c->n_pages, c->page_size, c->n_kv_head, c->n_seq, c->max_length, c->table_stride);
+  // positions are counted in 32 bits, with room for the tiles that are asked for ahead
+  REQUIRE(c->n_seq <= 65535 && c->max_length <= 1 << 30, WGPT_ERR_SHAPE, "%d sequences of up to %d positions: at most 65535 of 2^30",
+          c->n_seq, c->max_length);
   REQUIRE(c->head_size >= 8 && c->head_size <= 256 && c->head_size % 8 == 0, WGPT_ERR_SHAPE,
           "head_size %d is not a multiple of 8 up to 256", c->head_size);
   REQUIRE((int64_t)c->table_stride * c->page_size >= c->max_length, WGPT_ERR_SHAPE,
@@ -234,6 +237,10 @@ WGPT_EXPORT int32_t wgpt_paged_evict(wgpt_device *dev, const wgpt_paged_cache *f
           to->max_length, std::min(keep, from->max_length));
   REQUIRE(ld_weights >= from->max_length && (!weights_to || ld_weights_to >= keep), WGPT_ERR_SHAPE,
           "rows of weights are shorter than their sequences");
+  REQUIRE(from->table != to->table, WGPT_ERR_ARG, "the two caches have one table: nothing is moved in place");
+  const float *weights_end = weights + (from->n_seq - 1) * ld_weights + from->max_length;
+  REQUIRE(!weights_to || weights_to >= weights_end || weights_to + (from->n_seq - 1) * ld_weights_to + keep <= weights, WGPT_ERR_ARG,
+          "weights_to overlaps weights");
   e.keep = keep;
   e.recent = recent;
   e.weights = weights;
