@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 import serving_reference as ref
-from test_gpu_paged import OnDevice, cast, make
+from test_gpu_paged import OnDevice, cast, check_attention, make
 from webgpt_b200 import _lib
 
 pytestmark = pytest.mark.gpu
@@ -178,6 +178,15 @@ def test_steps_of_several_users(blocks, type, n_head, n_kv, hs, window, replayed
     for b in g.operations:
         b.clearBufferCache()
     cache.destroy()
+
+
+@pytest.mark.parametrize("type,group,new,hs,L", [("f16", 8, 4, 64, 17920), ("f16", 8, 4, 64, 9000), ("bf16", 4, 1, 128, 9000), ("f16", 8, 1, 64, 70000),
+                                                 ("f32", 8, 1, 40, 50000)])
+def test_one_sequence_over_all_ctas(blocks, type, group, new, hs, L):
+    """One head's positions spread over the GPU: joins of many parts, also of more than their factors have places for."""
+    dev, _ = blocks
+    pages = make(np.random.default_rng(L), [L], 64, 1, hs, type)
+    check_attention(dev, pages, type, "positions", [new], group, weights=True)
 
 
 def test_eviction_replayed(blocks):

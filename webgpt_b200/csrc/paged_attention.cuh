@@ -23,7 +23,6 @@ __device__ __forceinline__ float paged_value(const float *p) { return __ldcg(p);
 __device__ __forceinline__ float paged_value(const __half *p) { return __half2float(__ldcg(p)); }
 __device__ __forceinline__ float paged_value(const __nv_bfloat16 *p) { return __bfloat162float(__ldcg(p)); }
 
-constexpr int kJoinFactors = 256;
 constexpr int kPagedKeyGroups = 4, kPagedWarps = 8, kPagedRows = 32;  // at most, in a CTA
 
 struct PagedAttention {
@@ -441,11 +440,11 @@ __device__ __forceinline__ uint32_t split2(float &x, float &y) {
 
 
 // Joins a group's parts once this CTA's lies in its slot: the CTA that finishes last does, in the order of the positions. By
-// `threads` threads that meet in sync(); red and red_sum: a place for each of them; factor and sums: kJoinFactors places; out_at:
+// `threads` threads that meet in sync(); red and red_sum: a place for each of them; factor: twice `places` values; out_at:
 // where the rows' results go.
 template <typename Sync>
 __device__ __forceinline__ void paged_join(const PagedAttention &a, const PagedPart &w, int first_cta, int parts, int ROWS, int tid,
-                                           int threads, Sync sync, float4 *red, float *red_sum, float *factor, float *sums, const long long *out_at, int *is_last) {
+                                           int threads, Sync sync, float4 *red, float *red_sum, float *factor, int places, const long long *out_at, int *is_last) {
   const int hs = a.c.hs, quads = hs / 4, items = w.g.rows * quads, slot_floats = paged_slot(ROWS, hs);
   sync();
   if (tid == 0) {  // its fences stand for all threads', on their side of the barriers
@@ -459,7 +458,8 @@ __device__ __forceinline__ void paged_join(const PagedAttention &a, const PagedP
   if (!*is_last) return;
   auto part_of = [&](int k) { return a.partial + (2ll * (first_cta + k) + (k == 0 ? 1 : 0)) * slot_floats; };
   const int rows = w.g.rows, n = parts * rows;
-  const bool table = n <= kJoinFactors;  // else every thread computes the factors that it needs
+  const bool table = n <= places;  // else every thread computes the factors that it needs
+  float *sums = factor + places;
   if (table) {
     for (int i = tid; i < n; i += threads) {
       const int k = i / rows, r = i - k * rows;
@@ -467,38 +467,52 @@ __device__ __forceinline__ void paged_join(const PagedAttention &a, const PagedP
       sums[i] = __ldcg(part_of(k) + ROWS * hs + ROWS + r);
     }
     sync();
-    for (int r = tid; r < rows; r += threads) {
+    // a warp a row, or a thread where there are few parts
+    const int of = parts > 8 ? 32 : 1, lane = parts > 8 ? tid & 31 : 0;
+    for (int r = tid / of; r < rows; r += threads / of) {
       float top = -INFINITY, sum = 0.f;
-      for (int k = 0; k < parts; k++) top = fmaxf(top, factor[k * rows + r]);
-      for (int k = 0; k < parts; k++) {
+      for (int k = lane; k < parts; k += of) top = fmaxf(top, factor[k * rows + r]);
+      if (of > 1) top = warp_max(top);
+      for (int k = lane; k < parts; k += of) {
         const float m = factor[k * rows + r], l = sums[k * rows + r], f = m == -INFINITY && l == 0.f ? 0.f : exp2f(m - top);
         factor[k * rows + r] = f;
         sum += f * l;
       }
-      sums[r] = sum != 0.f ? 1.f / sum : 0.f;  // the first part's places: read already
-      if (a.stats) a.stats[row_index(a, w, r)] = top + log2f(sum);
+      if (of > 1) sum = warp_sum(sum);
+      if (lane == 0) {
+        sums[r] = sum != 0.f ? 1.f / sum : 0.f;  // the first part's places: this row's, read already
+        if (a.stats) a.stats[row_index(a, w, r)] = top + log2f(sum);
+      }
     }
     sync();
   }
-  // where a row tile has few values, several threads share a quad and take every so many parts; where it has many, the loads of two
-  // quads are in flight together
+  // Where a row tile has few values, several threads share a quad and take every so many parts. A part's values are a round trip
+  // away, so that what counts is how many are asked for at once: eight, or four of two quads.
   const int share = items >= threads ? 1 : threads / items;
-  if (table && share == 1) {
+  if (table && items > threads) {
     for (int i = tid; i < items; i += 2 * threads) {
       const int at[2] = {i, min(i + threads, items - 1)}, r[2] = {at[0] / quads, at[1] / quads};
       float4 v[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-#pragma unroll 4
-      for (int k = 0; k < parts; k++) {
-        const float4 *part = reinterpret_cast<const float4 *>(part_of(k));
-        const float4 o[2] = {__ldcg(part + at[0]), __ldcg(part + at[1])};
+      for (int k0 = 0; k0 < parts; k0 += 4) {
+        float4 o[4][2];
 #pragma unroll
-        for (int y = 0; y < 2; y++) {
-          const float f = factor[k * rows + r[y]];
-          v[y].x += f * o[y].x;
-          v[y].y += f * o[y].y;
-          v[y].z += f * o[y].z;
-          v[y].w += f * o[y].w;
+        for (int x = 0; x < 4; x++) {
+          const float4 *part = reinterpret_cast<const float4 *>(part_of(min(k0 + x, parts - 1)));
+          o[x][0] = __ldcg(part + at[0]);
+          o[x][1] = __ldcg(part + at[1]);
         }
+#pragma unroll
+        for (int x = 0; x < 4; x++)
+          if (k0 + x < parts) {
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+              const float f = factor[(k0 + x) * rows + r[y]];
+              v[y].x += f * o[x][y].x;
+              v[y].y += f * o[x][y].y;
+              v[y].z += f * o[x][y].z;
+              v[y].w += f * o[x][y].w;
+            }
+          }
       }
 #pragma unroll
       for (int y = 0; y < 2; y++) {
@@ -518,22 +532,30 @@ __device__ __forceinline__ void paged_join(const PagedAttention &a, const PagedP
     if (live) {
       if (!table)
         for (int k = 0; k < parts; k++) top = fmaxf(top, __ldcg(part_of(k) + ROWS * hs + r));
-#pragma unroll 8
-      for (int k = sh; k < parts; k += share) {
-        const float *part = part_of(k);
-        const float4 o = __ldcg(reinterpret_cast<const float4 *>(part) + i);
-        float f;
-        if (table) {
-          f = factor[k * rows + r];
-        } else {
-          const float m = __ldcg(part + ROWS * hs + r), l = __ldcg(part + ROWS * hs + ROWS + r);
-          f = m == -INFINITY && l == 0.f ? 0.f : exp2f(m - top);
-          sum += f * l;
+      for (int k0 = sh; k0 < parts; k0 += 8 * share) {
+        float4 o[8];
+        float fs[8];
+#pragma unroll
+        for (int x = 0; x < 8; x++) {
+          const int k = min(k0 + x * share, parts - 1);
+          const float *part = part_of(k);
+          o[x] = __ldcg(reinterpret_cast<const float4 *>(part) + i);
+          if (table) {
+            fs[x] = factor[k * rows + r];
+          } else {
+            const float m = __ldcg(part + ROWS * hs + r), l = __ldcg(part + ROWS * hs + ROWS + r);
+            fs[x] = m == -INFINITY && l == 0.f ? 0.f : exp2f(m - top);
+            if (k0 + x * share < parts) sum += fs[x] * l;
+          }
         }
-        v.x += f * o.x;
-        v.y += f * o.y;
-        v.z += f * o.z;
-        v.w += f * o.w;
+#pragma unroll
+        for (int x = 0; x < 8; x++)
+          if (k0 + x * share < parts) {
+            v.x += fs[x] * o[x].x;
+            v.y += fs[x] * o[x].y;
+            v.z += fs[x] * o[x].z;
+            v.w += fs[x] * o[x].w;
+          }
       }
     }
     if (share > 1) {
@@ -577,7 +599,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
   __shared__ PagedPart s_part[2];
   __shared__ int s_last, s_more;
   __shared__ float4 s_red[S::kWide ? 128 : 32 * kPagedWarps];
-  __shared__ float s_red_sum[S::kWide ? 128 : 32 * kPagedWarps], s_factor[kJoinFactors], s_sums[kJoinFactors];
+  __shared__ float s_red_sum[S::kWide ? 128 : 32 * kPagedWarps];
   const PagedView &c = a.c;
   const int KG = a.key_groups, RW = S::kWide ? 1 : a.row_warps, ROWS = S::kWide ? RT : a.rows, threads = blockDim.x;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hs = c.hs, unit = KG * kTile;
@@ -1016,8 +1038,10 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
         }
       }
     }
-    if (parts > 1)
-      paged_join(a, w, first_cta, parts, ROWS, tid, threads, [] { __syncthreads(); }, s_red, s_red_sum, s_factor, s_sums, s_out, &s_last);
+    if (parts > 1) {  // the factors take the place of the first key group's results, or of all rings once they are done with
+      paged_join(a, w, first_cta, parts, ROWS, tid, threads, [] { __syncthreads(); }, s_red, s_red_sum,
+                 reinterpret_cast<float *>(more ? rings + o_at : rings), (more ? S::kTileBytes : KG * S::kRing) / 8, s_out, &s_last);
+    }
     __syncthreads();
     if (!more) break;
     if (padded) clear(reinterpret_cast<unsigned char *>(o_smem), a.ahead ? S::kTileBytes : S::kRing);

@@ -104,7 +104,7 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
   __shared__ int s_lo[N], s_hi[N];
   __shared__ long long s_row[N], s_out[N];  // where the rows' scores and results begin
   __shared__ float4 s_red[SOFT];
-  __shared__ float s_red_sum[SOFT], s_factor[kJoinFactors], s_sums[kJoinFactors];
+  __shared__ float s_red_sum[SOFT];
   volatile int *abort_flag = &abort_word;
   const PagedView &c = a.c;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, hs = c.hs;
@@ -338,8 +338,8 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
         finite = finite && (tid >= rows || fabsf(s_l[tid]) < INFINITY);
       }
       __syncwarp();
-      if (some(!finite)) {  // each row from what it sees alone, in the probabilities' place
-        float *values = reinterpret_cast<float *>(Ps);
+      float *values = reinterpret_cast<float *>(Ps);  // the probabilities' place: the products that read them are done
+      if (some(!finite)) {  // each row from what it sees alone
         const int share = (rows + WARPS - 1) / WARPS;
         paged_rows_apart<T, kTcKeys>(a, w, 0, 1, warp * share, min(rows, warp * share + share), lane, values, s_m, s_l);
         meet();
@@ -371,7 +371,7 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
           a.stats[row_index(a, w, tid)] = s_m[tid] + log2f(s_l[tid]);
         }
       }
-      if (parts > 1) paged_join(a, w, first_cta, parts, N, tid, SOFT, meet, s_red, s_red_sum, s_factor, s_sums, s_out, &s_last);
+      if (parts > 1) paged_join(a, w, first_cta, parts, N, tid, SOFT, meet, s_red, s_red_sum, values, S::kP / 8, s_out, &s_last);
       if (!more) break;
       meet();
     }
