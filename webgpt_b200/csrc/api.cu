@@ -1,3 +1,4 @@
+// C ABI of webgpt_b200 (declared in include/webgpt_b200.h): device/buffer management, the per-operator entry
 // points mirroring the reference's instruction classes, and the model/session level that mirrors class GPT.
 
 #include <cuda_runtime.h>

@@ -119,8 +119,8 @@ __device__ __forceinline__ uint4 ldg_stream4u(const uint4 *p) {
 // Development aid, compiled in only with -DWGPT_TRACE: thread 0 of the first and last CTA of a kernel append
 // (globaltimer, kernel id, phase) records to a device buffer that a debug entry point reads back.
 #ifdef WGPT_TRACE
-__device__ unsigned long long g_trace_buf[1 << 17];
-__device__ unsigned int g_trace_n;
+static __device__ unsigned long long g_trace_buf[1 << 17];
+static __device__ unsigned int g_trace_n;
 // One atomic per kernel (at entry, ahead of the dependency wait) reserves 32 record slots; later phases only read
 // the timer and store, so they do not stall the traced thread.
 __device__ __forceinline__ unsigned int trace_begin(int kid) {
