@@ -189,6 +189,19 @@ def test_one_sequence_over_all_ctas(blocks, type, group, new, hs, L):
     check_attention(dev, pages, type, "positions", [new], group, weights=True)
 
 
+@pytest.mark.parametrize("type,group,hs,window", [("f16", 6, 64, 0), ("bf16", 6, 128, 50), ("f16", 1, 128, 0), ("f32", 2, 64, 50), ("f16", 12, 256, 0)])
+def test_seventy_sequences_of_all_lengths(blocks, type, group, hs, window):
+    """More sequences than a warp has lanes, some empty, some without new tokens, for each of the kernels."""
+    dev, _ = blocks
+    rng = np.random.default_rng(group * hs)
+    lengths = [int(x) for x in rng.integers(0, 400, 70)]
+    lengths[3], lengths[40], lengths[41], lengths[69] = 0, 1, 0, 1500
+    new = [int(min(L, n)) for L, n in zip(lengths, rng.integers(0, 5, 70))]
+    new[69] = 4
+    pages = make(rng, lengths, 16, 2, hs, type)
+    check_attention(dev, pages, type, "heads", new, 2 * group, window=window, weights=True, before=1, behind=2)
+
+
 def test_eviction_replayed(blocks):
     """A recorded eviction goes by the lengths and weights of the time it is replayed, and may share the lengths of its two caches."""
     dev, g = blocks
@@ -239,6 +252,8 @@ def test_limits(blocks):
         refused(_lib.ERR_SHAPE, "wgpt_paged_append", c.ptr, 65536, None, x.ptr, x.ptr, 128)
         refused(_lib.ERR_SHAPE, "wgpt_paged_attention", c.ptr, 65536, None, 2, 0.125, 0, x.ptr, 128, x.ptr, 128, None, 0)
         refused(_lib.ERR_SHAPE, "wgpt_paged_evict", c.ptr, c.ptr, 4, 1, x.ptr, 1 << 30, None, 0, x.ptr)
+    refused(_lib.ERR_SHAPE, "wgpt_verify_drafts", 1, 0, (1 << 30) + 1, x.ptr, (1 << 30) + 1, None, 0, None, None, 0, 1.0, x.ptr, x.ptr, x.ptr)
+    refused(_lib.ERR_SHAPE, "wgpt_verify_drafts", 65536, 0, 8, x.ptr, 8, None, 0, None, None, 0, 1.0, x.ptr, x.ptr, x.ptr)
     c, to = OnDevice(dev, pages, "f32"), OnDevice(dev, pages, "f32")
     refused(_lib.ERR_ARG, "wgpt_paged_evict", c.ptr, c.ptr, 4, 1, x.ptr, 20, None, 0, x.ptr + 4096)
     for at in (0, 39 * 4, -4 * 7):  # weights are 20 + 20 values, weights_to 4 + 4
