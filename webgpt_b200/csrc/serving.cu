@@ -143,7 +143,10 @@ static bool paged_few(const wgpt_device *dev, const PagedAttention &a, int unit)
 // tiles read the cache again, fewer rows leave room for more keys in flight. 16-bit types, head sizes up to 128: up to eight rows
 // are one tile of mma.sync, more go to tcgen05. Measured with both, f16, 4 heads of the cache, one new token, tcgen05 first: head size
 // 128, 8 users of 8192 positions, 8 rows 27.4 / 30.8 us, 12 rows 28.3 / 41.7; 64 users of 1000, 35.4 / 33.1 and 36.4 / 50.9; head
-// size 64, 24.2 / 21.0 and 23.7 / 26.7, 32.2 / 24.6 and 32.1 / 31.0.
+// size 64, 24.2 / 21.0 and 23.7 / 26.7, 32.2 / 24.6 and 32.1 / 31.0. 12 rows in tiles of 16 and of 32: 28.4 / 30.9 and 32.0 / 34.8.
+// f32, 8 users of 8192, 4 heads of 64, 2 rows in tiles of two and of four: 27.2 / 31.4, 4 rows in tiles of four and of eight: 31.5 / 41.7.
+// Tiles of a ring: as many as leave room for another CTA on the SM. f32, head size 64, one row (16 users of 25 heads), two and three:
+// 29.7 / 30.7; f16, head size 128, 8 users of 8 heads, 8192 positions, two and three: 43.6 / 59.7, where only one CTA is left.
 template <typename T, int HSP>
 static int32_t launch_paged_rows(wgpt_device *dev, PagedAttention &a, long long rows) {
   if constexpr (sizeof(T) == 4) {
