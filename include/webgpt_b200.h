@@ -378,10 +378,9 @@ int32_t wgpt_paged_evict(wgpt_device *dev, const wgpt_paged_cache *from, const w
  * next token is drawn from max(p_i - q_i, 0), or from p_i if that is zero everywhere; behind the last accepted one from
  * p_i. Drawn: with the number uniforms[s * (n_draft + 1) + n_draft] in [0,1), the first id whose running sum exceeds number * total, in
  * the order of the ids, or of descending logits where top_k > 0 (so that no drafts and a top_k give wgpt_sample_topk's
- * pick). Probabilities are in double precision; a row's sum over the whole vocabulary, by which they are divided, is good to a
- * few 1e-8. NaN logits count as -infinity; a row with no finite value or with +infinity has no distribution: as a target it
- * accepts nothing and draws id 0, as a draft it accepts nothing and counts as q = 0, and both are reported. A drafted id >= V
- * is not accepted and reported. ld_target and ld_draft >= V, in any alignment.
+ * pick). Probabilities, sums and comparisons are in double precision. NaN logits count as -infinity; a row with no finite value
+ * or with +infinity has no distribution: as a target it accepts nothing and draws id 0, as a draft it accepts nothing and counts
+ * as q = 0, and both are reported. A drafted id >= V is not accepted and reported. ld_target and ld_draft >= V, in any alignment.
  * ids_out [n_seq, n_draft + 1]: the accepted drafts, the drawn token, WGPT_NO_ID behind it; n_accepted [n_seq].
  * 0 <= n_draft <= WGPT_MAX_DRAFT, 0 <= top_k <= min(WGPT_MAX_TOP_K, V), n_seq <= 65535, V <= 2^30; top_k * V up to 26 million. */
 #define WGPT_MAX_DRAFT 64

@@ -315,16 +315,16 @@ WGPT_EXPORT int32_t wgpt_verify_drafts(wgpt_device *dev, int32_t n_seq, int32_t 
   a.partial = static_cast<float2 *>(dev->scratch);
   const int warps = kVerifyThreads / 32;
   LAUNCH_PDL(dev, verify_sums_kernel, dim3((a.chunks + warps - 1) / warps, rows, n_seq), dim3(kVerifyThreads), 0, a);
-  // as many CTAs a sequence as are resident at once: two an SM, and one where a few sequences keep their exponentials. 64 sequences
-  // of 4 drafts over 50257 ids take 51 us with four CTAs each, 55 with eight (two waves) and 71 with two. With the exponentials kept and
-  // computed again: 1 sequence 15.2 / 19.1 us, 8 18.5 / 22.6, 16 27.3 / 26.6.
+  // As many CTAs a sequence as are resident at once, two an SM: 64 sequences of 4 drafts over 50257 ids take 45.4 us with four CTAs each,
+  // 55.4 with eight (two waves), 57.2 with two. Where a few sequences leave half of the SMs empty anyway, a CTA may take all the registers:
+  // five logits of each row at once and one CTA an SM, against two and two: 1 sequence 15.6 / 16.1 us, 8 20.0 / 22.2, 16 30.0 / 26.8.
   int C = kDrawCluster;
   while (C > 1 && C * n_seq > 2 * dev->sm_count) C /= 2;
   const dim3 grid(C * n_seq), block(kDrawThreads);
-  if (C == kDrawCluster && C * n_seq <= dev->sm_count && V <= 16 * 32 * kDrawWarps * C)
-    CK(launch_ex_x(dev->pdl, C, dev->stream, verify_draw_kernel<16>, grid, block, 0, a));
+  if (C == kDrawCluster && 2 * C * n_seq <= dev->sm_count)
+    CK(launch_ex_x(dev->pdl, C, dev->stream, verify_draw_kernel<5, 1>, grid, block, 0, a));
   else
-    CK(launch_ex_x(dev->pdl, C, dev->stream, verify_draw_kernel<0>, grid, block, 0, a));
+    CK(launch_ex_x(dev->pdl, C, dev->stream, verify_draw_kernel<2, 2>, grid, block, 0, a));
   dev->launches++;
   return WGPT_OK;
 }

@@ -56,7 +56,7 @@ __device__ __forceinline__ double warp_sum64(double v) {
 }
 
 // The largest value of each chunk of a row and the sum of exp((x - largest) / temperature) over it, a warp a chunk: every lane has its
-// own running maximum until the end. Decides whether drafts are accepted: each exponential is good to 2^-22, their sum to a few 1e-8.
+// own running maximum until the end. Tells whether a draft is accepted wherever the answer is not close (kUnsure).
 // Bound by bytes: 64 users with up to 4 drafts over 50257 ids (85 MB) 20 us, 4.3 TB/s, launch and ragged ends included.
 constexpr int kVerifyThreads = 256, kVerifyVals = 16, kVerifyTurns = 4, kVerifyChunk = 32 * kVerifyVals * kVerifyTurns;
 
@@ -245,26 +245,60 @@ __device__ __forceinline__ void write_ids(const Verify &a, int s, int accepted, 
   if (tid == 0) a.n_accepted[s] = accepted;
 }
 
-// The accept step and the draw over the whole vocabulary, a cluster of CTAs per sequence. The draw needs running sums good to
-// far below the smallest probability, so its exponentials are in double precision: those of the target's row, and of the draft's if a
-// draft was not accepted, each by its row's sum, which the accept step has (good to a few 1e-8; the same for rows that are the same,
-// so that nothing is left of them). Every warp takes a stretch of ids; the sums of the stretches say in which one the running sum passes the
-// number, and that warp adds its stretch up id by id. A lane keeps its exponentials where they fit kVals registers. Bound by latency
-// (logits, exponentials, two barriers of the cluster): one user with 4 drafts 15 us with the sums, 64 users 51; the FP64 pipe is
-// busy a fifth of the time. Going over the rows a second time for their own sums took 64.
+// The accept step and the draw over the whole vocabulary, a cluster of CTAs per sequence, in double precision.
+// Accepting: u q < p is decided by the sums in f32 unless the two sides are within kUnsure of one another; both rows are
+// added up in double precision by the cluster then, for one in some 30 000 drafts.
+// The draw needs running sums good to far below the smallest probability: those of e_p where all drafts were accepted, else of
+// max(e_p / Z_p - e_q / Z_q, 0), here times Z_p Z_q. The rows' sums Z would have to be known first; but they hardly change which ids
+// count. So the ids are told apart by the f32 sums (a difference of two logits against a border), and the same round adds up both
+// rows and, over the ids that count, both rows again: Z_q sum e_p - Z_p sum e_q of a stretch is off by the ids on the wrong side alone, which are
+// few and whose terms are within the f32 sums' error of zero. Where little is left (kLeft) that might still be seen, and a second round
+// tells them apart by the good sums. Equal rows have equal sums and leave zeros.
+// Every warp takes a stretch of ids; the sums of the stretches say in which one the running sum passes the number, and the warps of
+// its CTA add that stretch up id by id, a row of 32 ids each.
+// Bound by latency (logits, exponentials, three barriers of the cluster): one user with 4 drafts over 50257 ids 14.1 us with the sums, 64 users
+// 45.5.
 constexpr int kDrawThreads = 512, kDrawWarps = kDrawThreads / 32, kDrawCluster = 8;
+// A row's sum in f32 is off by less than 1e-5 of itself: 70 roundings of a lane's additions and of its five rescalings (2^-24 each), six
+// exponentials (2^-22), and three roundings in each exponent's argument, (largest - logit) / temperature, whose mean over the
+// distribution is below ln V <= 21. Both sums of a draft's two rows: 2e-5.
+constexpr double kUnsure = 1.0 / 32768;
+constexpr double kLeft = 1.0 / 16;
+constexpr double kNoise = 1.5e-14;  // a difference below this much of its terms is their rounding: nothing
 
-template <int kVals>
-__global__ void __launch_bounds__(kDrawThreads, kVals > 0 ? 1 : 2) verify_draw_kernel(const __grid_constant__ Verify a) {
-  __shared__ int first_rejected;
+// A row's sum of exponentials in double precision, by the whole cluster of C CTAs; every thread gets it. A lane has the ids i0, i0 + 32,
+// ... below end; places: a number for each warp of the cluster, the same in every CTA, those of CTAs that are not there zero.
+__device__ __noinline__ double draw_row_sum(const float *x, float top, int i0, int end, double scale, const double *table, double *places,
+                                            int place, int C, int lane) {
+  double sum = 0.0;
+  for (int i = i0; i < end; i += 32) sum += exp_of((double)logit(x + i) - (double)top, scale, table);
+  sum = warp_sum64(sum);
+  if (lane < C) dsmem_st64(dsmem_addr(places + place, lane), (unsigned long long)__double_as_longlong(sum));
+  cluster_arrive();
+  cluster_wait();
+  sum = 0.0;
+  for (int i = lane; i < kDrawCluster * kDrawWarps; i += 32) sum += places[i];
+  sum = warp_sum64(sum);
+  cluster_arrive();  // before the places are written again
+  cluster_wait();
+  return sum;
+}
+
+// kLook: logits of a row that a lane asks for at once.
+template <int kLook, int kCtas>
+__global__ void __launch_bounds__(kDrawThreads, kCtas) verify_draw_kernel(const __grid_constant__ Verify a) {
+  __shared__ int first_rejected, s_last;
+  __shared__ unsigned s_unsure[2];  // drafts that the sums in f32 do not decide
   __shared__ float s_max[2 * kMaxDraft + 1];
   __shared__ double s_sum[2 * kMaxDraft + 1];
   __shared__ double table[64];
-  __shared__ double sums[2][kDrawCluster][kDrawWarps];  // of every warp of the cluster: the target's, what a draft leaves of it
+  // of every warp of the cluster, for each round: the target's row, the draft's, and both over the ids that count
+  __shared__ double sums[2][4][kDrawCluster][kDrawWarps];
+  __shared__ double s_row[2][32];  // sums of rows of 32 ids
   uint32_t C;
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(C));
   const int rank = (int)cluster_ctarank(), s = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  for (int i = tid; i < 2 * kDrawCluster * kDrawWarps; i += kDrawThreads) (&sums[0][0][0])[i] = 0.0;  // of CTAs that are not there too
+  for (int i = tid; i < 8 * kDrawCluster * kDrawWarps; i += kDrawThreads) (&sums[0][0][0][0])[i] = 0.0;  // of CTAs that are not there too
   cluster_arrive();
   if (tid < 64) table[tid] = exp2(tid / 64.0);
   pdl_launch_dependents();
@@ -273,6 +307,8 @@ __global__ void __launch_bounds__(kDrawThreads, kVals > 0 ? 1 : 2) verify_draw_k
   const int n = drafted(a, s), rows = 2 * a.n_draft + 1;
   if (tid == 0) first_rejected = n;
   __syncthreads();
+  const int stretch = (a.V + (int)C * kDrawWarps - 1) / ((int)C * kDrawWarps);
+  const int beg = min(a.V, (rank * kDrawWarps + warp) * stretch), end = min(a.V, beg + stretch);
   // every CTA finds the first draft that is not accepted: (largest, sum) of the rows, a warp each
   const double scale = 64.0 / (0.6931471805599453 * a.temperature);
   const float2 *part = a.partial + (long long)s * rows * a.chunks;
@@ -293,21 +329,42 @@ __global__ void __launch_bounds__(kDrawThreads, kVals > 0 ? 1 : 2) verify_draw_k
     }
   }
   __syncthreads();
-  if (tid < n) {
+  auto weight_of = [&](int r, uint32_t id) { return exp_of((double)logit(logits_row(a, s, r) + id) - (double)s_max[r], scale, table); };
+  if (tid < 64) {
     const int i = tid, rq = a.n_draft + 1 + i;
-    const uint32_t x = __ldcg(a.draft_ids + (long long)s * a.n_draft + i);
-    bool ok = false;
-    if (x >= (uint32_t)a.V) {
-      *a.err = 1;
-    } else if (!isinf(s_max[i]) && !(a.draft && isinf(s_max[rq]))) {
-      const double p = exp_of((double)logit(logits_row(a, s, i) + x) - (double)s_max[i], scale, table) / s_sum[i];
-      const double q = a.draft ? exp_of((double)logit(logits_row(a, s, rq) + x) - (double)s_max[rq], scale, table) / s_sum[rq] : 1.0;
-      ok = __ldcg(a.uniforms + (long long)s * (a.n_draft + 1) + i) * q < p;
+    bool open = false;
+    if (i < n) {
+      const uint32_t x = __ldcg(a.draft_ids + (long long)s * a.n_draft + i);
+      bool ok = false;
+      if (x >= (uint32_t)a.V) {
+        *a.err = 1;
+      } else if (!isinf(s_max[i]) && !(a.draft && isinf(s_max[rq]))) {
+        // u q < p with both sides times Z_p Z_q
+        const double p = weight_of(i, x) * (a.draft ? s_sum[rq] : 1.0),
+                     uq = __ldcg(a.uniforms + (long long)s * (a.n_draft + 1) + i) * (a.draft ? weight_of(rq, x) : 1.0) * s_sum[i];
+        ok = uq < p;
+        open = p > 0.0 && fabs(uq - p) <= kUnsure * p;
+      }
+      if (!ok && !open) atomicMin(&first_rejected, i);
     }
-    if (!ok) atomicMin(&first_rejected, i);
+    const unsigned all = __ballot_sync(0xffffffffu, open);
+    if (lane == 0) s_unsure[warp] = all;
   }
   __syncthreads();
-  const int at = first_rejected;
+  int at = first_rejected;
+  cluster_wait();  // the others run
+  auto row_sum = [&](int r) {
+    return draw_row_sum(logits_row(a, s, r), s_max[r], beg + lane, end, scale, table, &sums[0][0][0][0], rank * kDrawWarps + warp, (int)C, lane);
+  };
+  unsigned long long unsure = (unsigned long long)s_unsure[1] << 32 | s_unsure[0];
+  for (; unsure != 0; unsure &= unsure - 1) {  // the same for the whole cluster
+    const int i = __ffsll((long long)unsure) - 1;
+    if (i >= at) break;
+    const uint32_t x = __ldcg(a.draft_ids + (long long)s * a.n_draft + i);
+    const int rq = a.n_draft + 1 + i;
+    const double p = weight_of(i, x) * (a.draft ? row_sum(rq) : 1.0), q = (a.draft ? weight_of(rq, x) : 1.0) * row_sum(i);
+    if (!(__ldcg(a.uniforms + (long long)s * (a.n_draft + 1) + i) * q < p)) at = i;
+  }
   const float *x = logits_row(a, s, at), *y = nullptr;
   const double m = s_max[at];
   double mq = 0.0;
@@ -323,153 +380,237 @@ __global__ void __launch_bounds__(kDrawThreads, kVals > 0 ? 1 : 2) verify_draw_k
   } else if (rest) {
     only = __ldcg(a.draft_ids + (long long)s * a.n_draft + at);
   }
-  const bool none = isinf(m);
-  const int stretch = (a.V + (int)C * kDrawWarps - 1) / ((int)C * kDrawWarps);
-  const int beg = min(a.V, (rank * kDrawWarps + warp) * stretch), end = min(a.V, beg + stretch);
-  const bool two = rest && y != nullptr;
-  constexpr int kLook = kVals > 0 ? kVals : 4, kPick = 4;
-  double vx[kVals > 0 ? kVals : 1];
-  // a lane's logits of ids i0, i0 + 32, ...: -infinity, which counts nothing, behind the stretch
-  auto fetch = [&](int i0, auto &lx, auto &ly) {
-#pragma unroll
-    for (int u = 0; u < (int)(sizeof(lx) / sizeof(float)); u++) {
-      const int i = i0 + 32 * u;
-      lx[u] = i < end ? logit(x + i) : -INFINITY;
-      ly[u] = two && rest && i < end ? logit(y + i) : -INFINITY;
-    }
-  };
-  // what an id counts: its exponential; where a draft was turned down that by its row's sum, less the draft's (or less all of it
-  // at the drafted id), none below zero
-  const double ix = none ? 0.0 : 1.0 / s_sum[at], iq = two ? 1.0 / s_sum[a.n_draft + 1 + at] : 0.0;
-  auto weight = [&](float lx, float ly, int i) {
-    const double e = exp_of((double)lx - m, scale, table);
-    if (!rest) return e;
-    const double q = two ? __dmul_rn(exp_of((double)ly - mq, scale, table), iq) : (uint32_t)i == only ? 1.0 : 0.0;
-    return fmax(__dmul_rn(e, ix) - q, 0.0);  // rounded alike, so that equal rows leave zeros
-  };
-  // every warp's sum over its stretch, told to every CTA, behind one barrier of the cluster
+  const bool none = isinf(m), two = rest && y != nullptr;
+  auto exp_x = [&](float l) { return exp_of((double)l - m, scale, table); };
+  auto exp_y = [&](float l) { return exp_of((double)l - mq, scale, table); };
+  double zp = none ? 1.0 : s_sum[at], zq = two ? s_sum[a.n_draft + 1 + at] : 1.0;
+  // an id counts where its target's logit is further above its draft's than this: e_p z_q > e_q z_p
+  const float border = two && !none ? (float)(m - mq + a.temperature * (double)logf((float)zp / (float)zq)) : 0.f;
+  // every warp's sums over its stretch, told to every CTA, behind one barrier of the cluster
+  int round = 0;
   auto add_up = [&]() {
-    double sum = 0.0;
+    double sum[4] = {0.0, 0.0, 0.0, 0.0};
     if (!none) {
-      if constexpr (kVals > 0) {
-        float lx[kVals], ly[kVals];
-        fetch(beg + lane, lx, ly);
+      float lx[kLook], ly[kLook], next_x[kLook], next_y[kLook];
+      auto fetch = [&](int i0) {  // -infinity, which counts nothing, behind the stretch
 #pragma unroll
-        for (int u = 0; u < kVals; u++) {
-          if (beg + 32 * u >= end) break;
-          sum += vx[u] = weight(lx[u], ly[u], beg + lane + 32 * u);
+        for (int u = 0; u < kLook; u++) {
+          const int i = i0 + 32 * u;
+          next_x[u] = i < end ? logit(x + i) : -INFINITY;
+          next_y[u] = two && i < end ? logit(y + i) : -INFINITY;
         }
-      } else {
-        for (int i0 = beg + lane; i0 < end; i0 += 32 * kLook) {
-          float lx[kLook], ly[kLook];
-          fetch(i0, lx, ly);
+      };
+      fetch(beg + lane);
+      for (int i0 = beg + lane; i0 - lane < end; i0 += 32 * kLook) {
 #pragma unroll
-          for (int u = 0; u < kLook; u++) sum += weight(lx[u], ly[u], i0 + 32 * u);
+        for (int u = 0; u < kLook; u++) {
+          lx[u] = next_x[u];
+          ly[u] = next_y[u];
+        }
+        fetch(i0 + 32 * kLook);
+        double e[kLook], f[kLook];
+#pragma unroll
+        for (int u = 0; u < kLook; u++) sum[0] += e[u] = exp_x(lx[u]);
+        if (two) {
+#pragma unroll
+          for (int u = 0; u < kLook; u++) sum[1] += f[u] = exp_y(ly[u]);
+#pragma unroll
+          for (int u = 0; u < kLook; u++) {
+            const bool in = round == 0 ? lx[u] - ly[u] > border : __dmul_rn(e[u], zq) > __dmul_rn(f[u], zp);
+            sum[2] += in ? e[u] : 0.0;
+            sum[3] += in ? f[u] : 0.0;
+          }
+        } else if (rest) {
+#pragma unroll
+          for (int u = 0; u < kLook; u++) sum[2] += (uint32_t)(i0 + 32 * u) == only ? 0.0 : e[u];
         }
       }
-      sum = warp_sum64(sum);
-      if (lane < (int)C)
-        dsmem_st64(dsmem_addr(&sums[rest ? 1 : 0][rank][warp], lane), (unsigned long long)__double_as_longlong(sum));
+      if (two) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+          for (int k = 0; k < 4; k++) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], o);
+      } else {
+        sum[0] = warp_sum64(sum[0]);
+        if (rest) sum[2] = warp_sum64(sum[2]);
+      }
+      if (lane < (int)C) {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          if (k == 0 || two || (rest && k == 2))
+            dsmem_st64(dsmem_addr(&sums[round][k][rank][warp], lane), (unsigned long long)__double_as_longlong(sum[k]));
+      }
     }
     cluster_arrive();
     cluster_wait();
   };
-  // of all warps' sums: what lies before each, and their total; every warp for itself, four sums a lane
+  // of all warps' sums: what each counts and what lies before it, and their total; every warp for itself, four sums a lane
   constexpr int kAll = kDrawCluster * kDrawWarps, kPer = kAll / 32;
-  double upto[kPer], from;
+  double of[kPer], ahead[kPer];
+  auto before_lane = [&](double upto) {  // no difference: a tiny sum ahead of a large one is not to be lost
+    const double x = __shfl_up_sync(0xffffffffu, upto, 1);
+    return lane > 0 ? x : 0.0;
+  };
   auto prefixes = [&]() {
-    const double *v = &sums[rest ? 1 : 0][0][0] + lane * kPer;
-    double sum = 0.0;
+    const double *v = &sums[round][0][0][0] + lane * kPer;
+    const double *v2 = v + (rest ? 2 * kAll : 0);
+    double up2[kPer], up3[kPer], run2 = 0.0, run3 = 0.0;
 #pragma unroll
-    for (int u = 0; u < kPer; u++) upto[u] = sum += v[u];
-    from = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double up = __shfl_up_sync(0xffffffffu, from, o);
-      if (lane >= o) from += up;
+    for (int u = 0; u < kPer; u++) {
+      up2[u] = run2;
+      run2 += v2[u];
     }
-    const double total = __shfl_sync(0xffffffffu, from, 31);
-    from = __shfl_up_sync(0xffffffffu, from, 1);
-    if (lane == 0) from = 0.0;
+    double before2 = run2, before3 = 0.0, total;
+    if (two && rest) {
+      zp = zq = 0.0;
+#pragma unroll
+      for (int u = 0; u < kPer; u++) {
+        up3[u] = run3;
+        run3 += v[3 * kAll + u];
+        zp += v[u];
+        zq += v[kAll + u];
+      }
+      before3 = run3;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double a2 = __shfl_up_sync(0xffffffffu, before2, o), a3 = __shfl_up_sync(0xffffffffu, before3, o);
+        if (lane >= o) {
+          before2 += a2;
+          before3 += a3;
+        }
+        zp += __shfl_xor_sync(0xffffffffu, zp, o);
+        zq += __shfl_xor_sync(0xffffffffu, zq, o);
+      }
+      total = __shfl_sync(0xffffffffu, before2, 31) * zq - __shfl_sync(0xffffffffu, before3, 31) * zp;
+      before2 = before_lane(before2);
+      before3 = before_lane(before3);
+#pragma unroll
+      for (int u = 0; u < kPer; u++) {
+        const double p = v2[u] * zq, w = p - v[3 * kAll + u] * zp;
+        of[u] = w > kNoise * p ? w : 0.0;
+        ahead[u] = (before2 + up2[u]) * zq - (before3 + up3[u]) * zp;
+      }
+      if (!__any_sync(0xffffffffu, of[0] + of[1] + of[2] + of[3] > 0.0)) total = 0.0;
+    } else {
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double a2 = __shfl_up_sync(0xffffffffu, before2, o);
+        if (lane >= o) before2 += a2;
+      }
+      total = __shfl_sync(0xffffffffu, before2, 31);
+      before2 = before_lane(before2);
+#pragma unroll
+      for (int u = 0; u < kPer; u++) {
+        of[u] = v2[u];
+        ahead[u] = before2 + up2[u];
+      }
+    }
     return total;
   };
-  cluster_wait();  // the others run
-  add_up();
-  double total = prefixes();
-  if (rest && !(total > 0.0)) {  // nothing is left, in the whole cluster's eyes: drawn from the target's row itself
-    rest = false;
-    add_up();
+  static_assert(kPer == 4, "");
+  double total;
+  for (bool added = false;;) {  // the same for the whole cluster
+    if (!added) add_up();
+    added = true;
     total = prefixes();
+    if (two && rest && !none && round == 0 && total < kLeft * zp * zq) {  // again, with the good sums
+      round = 1;
+      added = false;
+    } else if (rest && !(total > 0.0)) {  // nothing is left: drawn from the target's row itself
+      rest = false;
+    } else {
+      break;
+    }
   }
-  if (!none) {
-    // the last stretch with anything in it that begins at or below the goal has the id (rounding may put the beginning of an empty
-    // one there); one warp adds it up
-    const double goal = u01 * total, *of = &sums[rest ? 1 : 0][0][0] + lane * kPer;
-    int mine = -1;
+  if (none) {
+    if (rank == 0 && warp == 0) {
+      if (lane == 0) *a.err = kErrRow;
+      write_ids<32>(a, s, at, 0u, lane);
+    }
+    return;
+  }
+  // the last stretch with anything in it that begins at or below the goal has the id (rounding may put the beginning of an empty
+  // one there)
+  const double goal = u01 * total;
+  int mine = -1;
 #pragma unroll
-    for (int u = 0; u < kPer; u++)
-      if ((u == 0 ? from : from + upto[u - 1]) <= goal && of[u] > 0.0) mine = lane * kPer + u;
-    const int owner = __reduce_max_sync(0xffffffffu, mine);
-    if (owner == rank * kDrawWarps + warp) {
-      double before = 0.0;
+  for (int u = 0; u < kPer; u++)
+    if (ahead[u] <= goal && of[u] > 0.0) mine = lane * kPer + u;
+  const int owner = __reduce_max_sync(0xffffffffu, mine);
+  if (owner < 0) {  // a number that is none
+    if (rank == 0 && warp == 0) write_ids<32>(a, s, at, (uint32_t)(a.V - 1), lane);
+    return;
+  }
+  if (owner / kDrawWarps != rank) return;
+  double before = 0.0;
 #pragma unroll
-      for (int u = 0; u < kPer; u++)
-        if (mine == owner && owner == lane * kPer + u) before = u == 0 ? from : from + upto[u - 1];
-      before = __shfl_sync(0xffffffffu, before, owner / kPer);
-      int last = -1, found = -1;  // the stretch's sum was rounded in another order: it may pass the goal where the running sum does not
-      auto look = [&](int i0, double w) {  // 32 ids
-        double run = w;
+  for (int u = 0; u < kPer; u++)
+    if (owner == lane * kPer + u) before = ahead[u];
+  before = __shfl_sync(0xffffffffu, before, owner / kPer);
+  // The stretch's rows of 32 ids, two a warp at a time: their sums, then, in the first whose running sum passes the goal, id by
+  // id. The stretch's sum was rounded in another order and may pass the goal where the running sum does not: the last id that counts then.
+  constexpr int kRows = 2;
+  static_assert(kRows * kDrawWarps == 32, "a lane a row");
+  const int own_end = min(a.V, (owner + 1) * stretch);
+  for (int i0 = owner * stretch, turn = 0; i0 < own_end; i0 += 32 * 32, turn ^= 1) {
+    double w[kRows], sum[kRows];
+    float lx[kRows], ly[kRows];
+#pragma unroll
+    for (int u = 0; u < kRows; u++) {
+      const int i = i0 + 32 * (u * kDrawWarps + warp) + lane;
+      lx[u] = i < own_end ? logit(x + i) : -INFINITY;
+      ly[u] = two && i < own_end ? logit(y + i) : -INFINITY;
+    }
+#pragma unroll
+    for (int u = 0; u < kRows; u++) {
+      w[u] = exp_x(lx[u]);
+      if (rest && two)
+        w[u] = fmax(__dmul_rn(w[u], zq) - __dmul_rn(exp_y(ly[u]), zp), 0.0);
+      else if (rest && (uint32_t)(i0 + 32 * (u * kDrawWarps + warp) + lane) == only)
+        w[u] = 0.0;
+      sum[u] = w[u];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+      for (int u = 0; u < kRows; u++) sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], o);
+    if (lane == 0)
+      for (int u = 0; u < kRows; u++) s_row[turn][u * kDrawWarps + warp] = sum[u];
+    __syncthreads();
+    const double row = s_row[turn][lane];
+    double run = row;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double up = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += up;
+    }
+    const unsigned full = __ballot_sync(0xffffffffu, row > 0.0), past = __ballot_sync(0xffffffffu, row > 0.0 && before + run > goal);
+    const int hit = past ? __ffs(past) - 1 : 31 - __clz(full);  // a row; -1: all are empty
+    const double above = __shfl_sync(0xffffffffu, run - row, hit & 31);
+#pragma unroll
+    for (int u = 0; u < kRows; u++) {
+      if (hit != u * kDrawWarps + warp) continue;
+      const int first = i0 + 32 * hit;
+      int id = first + 31 - __clz(__ballot_sync(0xffffffffu, w[u] > 0.0));
+      if (past) {
+        double r = w[u];
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-          const double up = __shfl_up_sync(0xffffffffu, run, o);
-          if (lane >= o) run += up;
+          const double up = __shfl_up_sync(0xffffffffu, r, o);
+          if (lane >= o) r += up;
         }
-        const unsigned past = __ballot_sync(0xffffffffu, i0 + lane < end && before + run > goal);
-        found = past ? i0 + __ffs(past) - 1 : last;  // the row's sum, rounded in another order, passed the goal
-      };
-      // 32 ids at a time: first the sums of some such rows, then the one in which the goal is passed, id by id
-      auto rows_of = [&](int i0, double (&w)[kPick]) {
-        double sum[kPick];
-#pragma unroll
-        for (int u = 0; u < kPick; u++) sum[u] = w[u];
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-          for (int u = 0; u < kPick; u++) sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], o);
-#pragma unroll
-        for (int u = 0; u < kPick; u++) {
-          if (found >= 0 || sum[u] == 0.0) continue;
-          last = i0 + 32 * u + 31 - __clz(__ballot_sync(0xffffffffu, w[u] > 0.0));
-          if (before + sum[u] > goal) look(i0 + 32 * u, w[u]);
-          before += sum[u];
-        }
-      };
-      if constexpr (kVals > 0) {
-#pragma unroll
-        for (int h = 0; h < kVals; h += kPick) {
-          double w[kPick];
-#pragma unroll
-          for (int u = 0; u < kPick; u++) w[u] = beg + 32 * (h + u) < end ? vx[h + u] : 0.0;
-          if (found < 0) rows_of(beg + 32 * h, w);
-        }
-      } else {
-        for (int i0 = beg; i0 < end && found < 0; i0 += 32 * kPick) {
-          double w[kPick];
-          float lx[kPick], ly[kPick];
-          fetch(i0 + lane, lx, ly);
-#pragma unroll
-          for (int u = 0; u < kPick; u++) w[u] = weight(lx[u], ly[u], i0 + lane + 32 * u);
-          rows_of(i0, w);
-        }
+        const unsigned in = __ballot_sync(0xffffffffu, w[u] > 0.0 && before + above + r > goal);
+        if (in) id = first + __ffs(in) - 1;
+        write_ids<32>(a, s, at, (uint32_t)id, lane);
+      } else if (lane == 0) {
+        s_last = id;
       }
-      write_ids<32>(a, s, at, (uint32_t)(found < 0 ? last : found), lane);
-    } else if (owner < 0 && rank == 0 && warp == 0) {  // a number that is none
-      write_ids<32>(a, s, at, (uint32_t)(a.V - 1), lane);
     }
-  } else if (rank == 0 && warp == 0) {
-    if (lane == 0) *a.err = kErrRow;
-    write_ids<32>(a, s, at, 0u, lane);
+    if (past) return;  // the same for the whole CTA
+    before += __shfl_sync(0xffffffffu, run, 31);
   }
+  __syncthreads();
+  if (warp == 0) write_ids<32>(a, s, at, (uint32_t)s_last, lane);
 }
 
 // The same over the kept lists, one CTA per sequence.
