@@ -69,3 +69,20 @@ def test_numbers_next_to_acceptance(dev, V, n_seq, temperature, drawn):  # noqa:
             u[s, i] = min(p[x] / q[x] * (1 + near), np.nextafter(1.0, 0.0))
     accepted = check(dev, t, d if drawn else None, ids, None, 0, temperature, u)[1]
     assert (accepted >= n_draft - 1).all() and (n_seq < 20 or len(set(accepted)) == 2)
+
+
+@pytest.mark.parametrize("top_k", [0, 6])
+@pytest.mark.parametrize("temperature", [5e-324, 1e-300, 1e-39, 3e-39, 1e-20, 1e30, 1e39, 1e300, np.inf])
+def test_temperatures_at_the_ends(dev, temperature, top_k):  # noqa: F811
+    """Every positive temperature is one: a tiny one leaves the largest logits alone, a huge one makes all finite ones alike."""
+    rng = np.random.default_rng(3)
+    V = 3000
+    t = np.round(rng.standard_normal((6, 3, V)) * 4).astype(np.float32)  # several largest ones
+    d = np.round(rng.standard_normal((6, 2, V)) * 4).astype(np.float32)
+    if temperature < np.inf:
+        t[1, :, ::3], d[2, :, 5:] = -np.inf, -np.inf
+    ids = np.stack([np.argmax(t[:, i], axis=1) for i in range(2)], 1).astype(np.uint32)
+    ids[4:, 1] = 17
+    with np.errstate(over="ignore"):
+        check(dev, t, d, ids, None, top_k, temperature, rng.random((6, 3)))
+        check(dev, t, None, ids, None, top_k, temperature, rng.random((6, 3)))

@@ -290,7 +290,7 @@ WGPT_EXPORT int32_t wgpt_verify_drafts(wgpt_device *dev, int32_t n_seq, int32_t 
   a.ld_draft = ld_draft;
   a.draft_ids = draft_ids;
   a.n_drafted = n_drafted;
-  a.temperature = temperature;
+  a.temperature = std::min(temperature, 1e37);  // its reciprocal is no zero in f32, so that -infinity stays what it is; beyond it all is flat
   a.uniforms = uniforms;
   a.ids_out = ids_out;
   a.n_accepted = n_accepted;

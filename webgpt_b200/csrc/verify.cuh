@@ -1,5 +1,7 @@
 // Verification of drafted tokens against the target's probabilities (speculative sampling), from given random numbers.
 #pragma once
+#include <cfloat>
+
 #include "common.cuh"
 #include "paged_attention.cuh"
 #include "sample_key.cuh"
@@ -67,7 +69,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_sums_kernel(const __gri
   if (chunk >= a.chunks || !row_wanted(a, r, drafted(a, s))) return;
   const float *x = logits_row(a, s, r) + (long long)chunk * kVerifyChunk + lane;
   const int n = min(a.V - chunk * kVerifyChunk, kVerifyChunk) - lane;
-  const float c = (float)(1.4426950408889634 / a.temperature);
+  const float c = (float)fmin(1.4426950408889634 / a.temperature, (double)FLT_MAX);  // finite: zero times it is zero
   float v[kVerifyVals], next[kVerifyVals], m = -INFINITY, sum = 0.f;
 #pragma unroll
   for (int u = 0; u < kVerifyVals; u++) next[u] = 32 * u < n ? __ldcg(x + 32 * u) : -INFINITY;
@@ -310,7 +312,7 @@ __global__ void __launch_bounds__(kDrawThreads, kCtas) verify_draw_kernel(const 
   const int stretch = (a.V + (int)C * kDrawWarps - 1) / ((int)C * kDrawWarps);
   const int beg = min(a.V, (rank * kDrawWarps + warp) * stretch), end = min(a.V, beg + stretch);
   // every CTA finds the first draft that is not accepted: (largest, sum) of the rows, a warp each
-  const double scale = 64.0 / (0.6931471805599453 * a.temperature);
+  const double scale = fmin(64.0 / (0.6931471805599453 * a.temperature), DBL_MAX);
   const float2 *part = a.partial + (long long)s * rows * a.chunks;
   for (int r = warp; r < rows; r += kDrawWarps) {
     if (!row_wanted(a, r, n) || (r > a.n_draft && !a.draft)) continue;
