@@ -67,9 +67,7 @@ class PagedCache:
     def advance(self, new):
         """Makes room for new[s] more tokens of each sequence (a number: as many for each). Changes nothing if a sequence
         would grow past max_length or there are too few pages."""
-        new = np.broadcast_to(np.asarray(new, np.int64), (self.n_seq,))
-        if (new < 0).any():
-            raise ValueError("a sequence cannot advance by a negative number of tokens: use retreat()")
+        new = self._each(new)
         want = self.lengths + new
         if (want > self.max_length).any():
             raise ValueError(f"a sequence would hold {int(want.max())} positions, more than max_length {self.max_length}")
@@ -101,8 +99,8 @@ class PagedCache:
         self.retreat(by)
 
     def starts(self, new):
-        """The starts array of a step of new[s] tokens per sequence, on the device."""
-        return self.device.tensor(np.concatenate([[0], np.cumsum(new)]).astype(np.int32))
+        """The starts array of a step of new[s] tokens per sequence (a number: as many for each), on the device."""
+        return self.device.tensor(np.concatenate([[0], np.cumsum(self._each(new))]).astype(np.int32))
 
     # ------------------------------------------------------------------ eviction
     def evict(self, keep, recent):
@@ -146,6 +144,12 @@ class PagedCache:
         return np.stack(out)
 
     # ------------------------------------------------------------------ inside
+    def _each(self, new):
+        new = np.broadcast_to(np.asarray(new, np.int64), (self.n_seq,))
+        if (new < 0).any():
+            raise ValueError("a sequence cannot advance by a negative number of tokens: use retreat()")
+        return new
+
     def _cut(self, s, length):
         n = -(-length // self.page_size)
         self.free += self.pages[s][n:]
