@@ -48,7 +48,7 @@ class PagedCache:
         self._weights = [device.buffer(n_seq * self.max_length * 4) for _ in range(n_layer)] if weights else None
         for b in self._weights or []:
             b.write(np.zeros(n_seq * self.max_length, np.float32))
-        self._upload()
+        self._take_over(self.pages, self.lengths)
 
     # ------------------------------------------------------------------ what the calls take
     def layer(self, i=0, which=0):
@@ -74,23 +74,24 @@ class PagedCache:
         need = [-(-int(L) // self.page_size) - len(p) for L, p in zip(want, self.pages)]
         if sum(need) > len(self.free):
             raise MemoryError(f"{sum(need)} pages are needed, {len(self.free)} are free")
-        for s, n in enumerate(need):
-            self.pages[s] += [self.free.pop() for _ in range(n)]
-        self.lengths[:] = want
-        self._upload()
+        free = list(self.free)
+        self._take_over([p + [free.pop() for _ in range(n)] for p, n in zip(self.pages, need)], want)
+        self.free = free
 
     def retreat(self, by):
         """Drops the by[s] newest positions of each sequence (a number: as many of each)."""
         by = np.broadcast_to(np.asarray(by, np.int64), (self.n_seq,))
         if (by < 0).any() or (by > self.lengths).any():
             raise ValueError("a sequence cannot retreat by a negative number of positions or past its beginning")
-        for s in range(self.n_seq):
-            L = int(self.lengths[s] - by[s])
-            if self._weights and by[s]:
-                for w in self._weights:
-                    w.write(np.zeros(int(by[s]), np.float32), offset=(s * self.max_length + L) * 4)
-            self._cut(s, L)
-        self._upload()
+        want = self.lengths - by
+        for s in np.flatnonzero(by):
+            for w in self._weights or []:
+                w.write(np.zeros(int(by[s]), np.float32), offset=int(s * self.max_length + want[s]) * 4)
+        held = [-(-int(L) // self.page_size) for L in want]
+        gone = [x for p, n in zip(self.pages, held) for x in p[n:]]
+        # the table stays: what lies behind a sequence's last page is not read
+        self._take_over([p[:n] for p, n in zip(self.pages, held)], want, table=False)
+        self.free += gone
 
     def release(self, s):
         """Ends sequence s: its pages are free again."""
@@ -136,11 +137,9 @@ class PagedCache:
             moved.destroy()
         for w, r in zip(self._weights, rows):
             w.write(r)
-        for s in range(self.n_seq):
-            self.free += self.pages[s]
-        self.pages = pages
-        self.lengths[:] = after
-        self._upload()
+        old = [x for p in self.pages for x in p]
+        self._take_over(pages, after)
+        self.free += old
         return np.stack(out)
 
     # ------------------------------------------------------------------ inside
@@ -150,21 +149,25 @@ class PagedCache:
             raise ValueError("a sequence cannot advance by a negative number of tokens: use retreat()")
         return new
 
-    def _cut(self, s, length):
-        n = -(-length // self.page_size)
-        self.free += self.pages[s][n:]
-        self.pages[s] = self.pages[s][:n]
-        self.lengths[s] = length
-
     def _table_of(self, pages):
         table = np.zeros((self.n_seq, self.width), np.uint32)
         for s, p in enumerate(pages):
             table[s, :len(p)] = p
         return table
 
-    def _upload(self):
-        self._tables[0].write(self._table_of(self.pages))
-        self._lengths[0].write(self.lengths)
+    def _take_over(self, pages, lengths, table=True):
+        """Makes these the cache's pages and lengths, on the device and here; a write that fails leaves the old ones."""
+        lengths = np.asarray(lengths, np.int32)
+        try:
+            if table:
+                self._tables[0].write(self._table_of(pages))
+            self._lengths[0].write(lengths)
+        except Exception:
+            if table:
+                self._tables[0].write(self._table_of(self.pages))
+            raise
+        self.pages = pages
+        self.lengths[:] = lengths
 
     def destroy(self):
         for b in self._tables + self._lengths + [x for p in self._pools for x in p] + (self._weights or []):
