@@ -70,3 +70,65 @@ def test_steps_that_fail_change_nothing():
     assert attempts(c, lambda: c.retreat([0, 1, 9]), lambda: None) >= 2
     assert attempts(c, lambda: c.release(0), lambda: None) >= 2
     assert list(c.lengths) == [0, 0, 8]
+
+
+def keeper(monkeypatch, c, calls=None):
+    """Stands in for wgpt_paged_evict on the fake device: the first keep - recent positions and the newest stay."""
+    from webgpt_b200 import _lib
+    buffers = lambda: {b.ptr: b for b in c.device.made}  # noqa: E731
+
+    def find(ptr):
+        for base, b in buffers().items():
+            if base <= ptr < base + max(1, b.data.size):
+                return b.data[ptr - base:]
+        raise AssertionError("an address of no buffer")
+
+    def call(name, handle, src, dst, keep, recent, w, ld, wt, ld_to, kept):
+        c.device.step()
+        assert name == "wgpt_paged_evict"
+        a, b = src._obj, dst._obj
+        if calls is not None:
+            calls.append((a.n_seq, a.k))
+        assert (a.max_length, a.table_stride, a.page_size, a.k) == (b.max_length, b.table_stride, b.page_size, b.k) and a.table != b.table
+        lengths, to = find(a.lengths).view(np.int32)[:a.n_seq], find(b.lengths).view(np.int32)[:a.n_seq]
+        pages = [find(x.table).view(np.uint32)[:a.n_seq * x.table_stride].reshape(a.n_seq, -1) for x in (a, b)]
+        old, new = set(), set()
+        for s, L in enumerate(lengths):
+            n = min(L, keep)
+            stay = list(range(L)) if L <= keep else list(range(keep - recent)) + list(range(L - recent, L))
+            row = find(kept).view(np.int32)[s * keep:(s + 1) * keep]
+            row[:n], row[n:] = stay, -1
+            x, y = find(w).view(np.float32)[s * ld:], find(wt).view(np.float32)[s * ld_to:]
+            y[:n], y[n:keep] = x[stay], 0
+            old |= set(pages[0][s, :-(-int(L) // a.page_size)])
+            new |= set(pages[1][s, :-(-int(n) // a.page_size)])
+            to[s] = n
+        assert not old & new and new <= set(c.free) and max(new) < c.n_pages  # nothing is moved in place
+
+    monkeypatch.setattr(_lib, "call", call)
+
+
+class Addresses(Failing):
+    """Buffers with addresses far apart."""
+
+    def buffer(self, nbytes, dims=None):
+        b = super().buffer(nbytes, dims)
+        b.ptr = len(self.made) << 32
+        return b
+
+
+def test_eviction_that_fails_anywhere_loses_no_page(monkeypatch):
+    c = PagedCache(Addresses(), 3, 1, 8, n_pages=30, page_size=4, max_length=30, n_layer=2, weights=True)
+    keeper(monkeypatch, c)
+    c.advance([25, 3, 18])
+    for i in range(2):
+        c.weights(i).write(np.arange(90, dtype=np.float32) + i)
+    made = len(c.device.made)
+    assert attempts(c, lambda: c.evict(8, 3), lambda: None) >= 7
+    assert all(b.gone for b in c.device.made[made:])  # what the call allocated is given back, failed or not
+    assert list(c.lengths) == [8, 3, 8] and len(c.free) == 30 - 5
+    for i in range(2):
+        w = c.weights(i).data.view(np.float32).reshape(3, 30)
+        assert list(w[0]) == [x + i for x in (0, 1, 2, 3, 4, 22, 23, 24)] + [0] * 22
+        assert list(w[1][:3]) == [30 + i, 31 + i, 32 + i]
+        assert list(w[2]) == [60 + x + i for x in (0, 1, 2, 3, 4, 15, 16, 17)] + [0] * 22

@@ -117,29 +117,27 @@ class PagedCache:
         need = [-(-int(L) // self.page_size) for L in after]
         if sum(need) > len(self.free):
             raise MemoryError(f"{sum(need)} pages are needed, {len(self.free)} are free")
-        pages = [[self.free.pop() for _ in range(n)] for n in need]
-        self._tables[1].write(self._table_of(pages))
-        kept = self.device.buffer(self.n_seq * keep * 4)
-        moved = self.device.buffer(self.n_seq * keep * 4)
-        out, rows = [], np.zeros((self.n_layer, self.n_seq, self.max_length), np.float32)
+        free = list(self.free)  # nothing that the cache goes by changes before all layers have been thinned out
+        pages = [[free.pop() for _ in range(n)] for n in need]
+        held, out, rows = [], [], np.zeros((self.n_layer, self.n_seq, self.max_length), np.float32)
         try:
+            for _ in range(2):
+                held.append(self.device.buffer(self.n_seq * keep * 4))
+            kept, moved = held
+            self._tables[1].write(self._table_of(pages))
             for i in range(self.n_layer):
                 _lib.call("wgpt_paged_evict", self.device.handle, self.layer(i).ptr, self.layer(i, 1).ptr, keep, recent,
                           self._weights[i].ptr, self.max_length, moved.ptr, keep, kept.ptr)
                 out.append(kept.read(np.int32, self.n_seq * keep).reshape(self.n_seq, keep))
                 rows[i, :, :keep] = moved.read(np.float32, self.n_seq * keep).reshape(self.n_seq, keep)
-        except Exception:  # nothing that the cache goes by has changed yet
-            for p in pages:
-                self.free += p
-            raise
         finally:
-            kept.destroy()
-            moved.destroy()
+            for b in held:
+                b.destroy()
         for w, r in zip(self._weights, rows):
             w.write(r)
         old = [x for p in self.pages for x in p]
         self._take_over(pages, after)
-        self.free += old
+        self.free = free + old
         return np.stack(out)
 
     # ------------------------------------------------------------------ inside
