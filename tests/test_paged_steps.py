@@ -19,13 +19,14 @@ def test_starts_has_a_number_for_every_sequence():
 
 
 class Failing(FakeDevice):
-    """A device whose n-th allocation or write from now on fails."""
+    """A device whose n-th allocation or write from now on fails, and no other."""
     left = None
 
     def step(self):
         if self.left is not None:
             self.left -= 1
             if self.left < 0:
+                self.left = None
                 raise OSError("no")
 
     def buffer(self, nbytes, dims=None):
@@ -41,8 +42,14 @@ class Failing(FakeDevice):
                 return self.data[offset:offset + count * np.dtype(dtype).itemsize].view(dtype).copy()
 
         b = Buffer(nbytes)
+        b.nbytes = nbytes
         self.made = getattr(self, "made", []) + [b]
         return b
+
+
+    def copy(self, src, src_offset, dst, dst_offset, size):  # only enqueues
+        assert not src.gone and not dst.gone
+        dst.data[dst_offset:dst_offset + size] = src.data[src_offset:src_offset + size]
 
 
 def attempts(c, call, untouched):
@@ -124,7 +131,12 @@ def test_eviction_that_fails_anywhere_loses_no_page(monkeypatch):
     for i in range(2):
         c.weights(i).write(np.arange(90, dtype=np.float32) + i)
     made = len(c.device.made)
-    assert attempts(c, lambda: c.evict(8, 3), lambda: None) >= 7
+    before = [w.data.copy() for w in c._weights]
+
+    def untouched():
+        assert all(np.array_equal(w.data, x) for w, x in zip(c._weights, before))
+
+    assert attempts(c, lambda: c.evict(8, 3), untouched) >= 7
     assert all(b.gone for b in c.device.made[made:])  # what the call allocated is given back, failed or not
     assert list(c.lengths) == [8, 3, 8] and len(c.free) == 30 - 5
     for i in range(2):

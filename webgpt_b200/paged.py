@@ -119,25 +119,25 @@ class PagedCache:
             raise MemoryError(f"{sum(need)} pages are needed, {len(self.free)} are free")
         free = list(self.free)  # nothing that the cache goes by changes before all layers have been thinned out
         pages = [[free.pop() for _ in range(n)] for n in need]
-        held, out, rows = [], [], np.zeros((self.n_layer, self.n_seq, self.max_length), np.float32)
+        out, moved, kept = [], [], None
         try:
-            for _ in range(2):
-                held.append(self.device.buffer(self.n_seq * keep * 4))
-            kept, moved = held
+            kept = self.device.buffer(self.n_seq * keep * 4)
+            for _ in range(self.n_layer):  # the weights that stay, zeros behind them
+                moved.append(self.device.buffer(self.n_seq * self.max_length * 4))
+                moved[-1].write(np.zeros(self.n_seq * self.max_length, np.float32))
             self._tables[1].write(self._table_of(pages))
             for i in range(self.n_layer):
                 _lib.call("wgpt_paged_evict", self.device.handle, self.layer(i).ptr, self.layer(i, 1).ptr, keep, recent,
-                          self._weights[i].ptr, self.max_length, moved.ptr, keep, kept.ptr)
+                          self._weights[i].ptr, self.max_length, moved[i].ptr, self.max_length, kept.ptr)
                 out.append(kept.read(np.int32, self.n_seq * keep).reshape(self.n_seq, keep))
-                rows[i, :, :keep] = moved.read(np.float32, self.n_seq * keep).reshape(self.n_seq, keep)
+            old = [x for p in self.pages for x in p]
+            self._take_over(pages, after)
+            self.free = free + old
+            for w, m in zip(self._weights, moved):
+                self.device.copy(m, 0, w, 0, m.nbytes)
         finally:
-            for b in held:
+            for b in [kept] * (kept is not None) + moved:
                 b.destroy()
-        for w, r in zip(self._weights, rows):
-            w.write(r)
-        old = [x for p in self.pages for x in p]
-        self._take_over(pages, after)
-        self.free = free + old
         return np.stack(out)
 
     # ------------------------------------------------------------------ inside
