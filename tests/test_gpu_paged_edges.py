@@ -1,0 +1,53 @@
+"""The paged cache's operators where the other tests do not look: full pools, offsets that make no sense, row tiles beside one another,
+values that are not finite in long sequences, workspaces larger than memory."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+import serving_reference as ref
+from test_gpu_paged import OnDevice, attend, cast, check_attention, dev, make, reported, to_bits, to_f32  # noqa: F401 (dev: a fixture)
+from webgpt_b200 import _lib
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("type", ["f32", "f16"])
+def test_a_full_cache_is_thinned_out(dev, type):  # noqa: F811
+    """One free page: the long sequences go one after the other, those that stay whole keep their pages."""
+    from webgpt_b200.paged import PagedCache
+    rng = np.random.default_rng(1)
+    lengths, n_kv, hs, page, keep, recent = [5, 40, 37, 8, 64, 23, 8], 2, 16, 8, 8, 3
+    used = sum(-(-L // page) for L in lengths)
+    cache = PagedCache(dev, 7, n_kv, hs, n_pages=used + 1, page_size=page, type=type, n_layer=2, max_length=70, weights=True)
+    cache.advance(lengths)
+    width = n_kv * hs
+    rows = [rng.standard_normal((sum(lengths), 2 * width)).astype(np.float32) for _ in range(2)]
+    w = rng.integers(0, 30, (2, 7, 70)).astype(np.float32)
+    for s, L in enumerate(lengths):
+        w[:, s, L:] = 0
+    starts = cache.starts(lengths)
+    for i in range(2):
+        b = dev.tensor(rows[i])
+        _lib.call("wgpt_paged_append", dev.handle, cache.layer(i).ptr, sum(lengths), starts.ptr, b.ptr, b.ptr + 4 * width, 2 * width)
+        cache.weights(i).write(w[i])
+        dev.synchronize()
+    kept = cache.evict(keep, recent)
+    assert list(cache.lengths) == [min(L, keep) for L in lengths] and len(cache.free) == used + 1 - 7
+    table = cache._tables[0].read(np.uint32).reshape(7, -1)
+    assert list(cache._lengths[0].read(np.int32)) == list(cache.lengths)
+    first = np.cumsum([0] + lengths)
+    for i in range(2):
+        pools = [to_f32(b.read(np.uint32 if type == "f32" else np.uint16), type).reshape(-1, page, width) for b in cache._pools[i]]
+        got = cache.weights(i).read().reshape(7, 70)
+        for s, L in enumerate(lengths):
+            stay = ref.keep(w[i, s], L, keep, recent)
+            assert list(kept[i, s]) == stay + [-1] * (keep - len(stay))
+            assert list(got[s]) == list(w[i, s, stay]) + [0] * (70 - len(stay))
+            at = np.arange(len(stay))
+            for x, pool in enumerate(pools):
+                want = cast(type)(rows[i][first[s] + np.array(stay), x * width:(x + 1) * width])
+                assert np.array_equal(pool[table[s, at // page], at % page], want)
+    _lib.call("wgpt_device_check", dev.handle)
+    cache.destroy()

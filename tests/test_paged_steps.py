@@ -144,3 +144,37 @@ def test_eviction_that_fails_anywhere_loses_no_page(monkeypatch):
         assert list(w[0]) == [x + i for x in (0, 1, 2, 3, 4, 22, 23, 24)] + [0] * 22
         assert list(w[1][:3]) == [30 + i, 31 + i, 32 + i]
         assert list(w[2]) == [60 + x + i for x in (0, 1, 2, 3, 4, 15, 16, 17)] + [0] * 22
+
+
+def test_a_full_cache_is_thinned_out(monkeypatch):
+    """Sequences that stay whole keep their pages and are not copied; the others go some at a time where few pages are free."""
+    calls = []
+    c = PagedCache(Addresses(), 6, 1, 8, n_pages=40, page_size=4, max_length=60, n_layer=2, weights=True)
+    keeper(monkeypatch, c, calls)
+    c.advance([7, 40, 33, 8, 28, 29])  # 2 + 10 + 9 + 2 + 7 + 8 pages: two are free
+    for i in range(2):
+        c.weights(i).write(np.arange(360, dtype=np.float32) + 1000 * i)
+    assert len(c.free) == 2
+    short = [list(c.pages[0]), list(c.pages[3])]
+    kept = c.evict(8, 2)
+    check(c)
+    assert list(c.lengths) == [7, 8, 8, 8, 8, 8] and [c.pages[0], c.pages[3]] == short and len(c.free) == 40 - 12
+    assert [n for n, _ in calls] == [1, 1, 1, 2, 1, 2]  # in both layers one sequence at first, then all that is left, run by run
+    assert kept.shape == (2, 6, 8)
+    for i in range(2):
+        assert kept[i].tolist() == [[0, 1, 2, 3, 4, 5, 6, -1], [0, 1, 2, 3, 4, 5, 38, 39], [0, 1, 2, 3, 4, 5, 31, 32], list(range(8)),
+                                    [0, 1, 2, 3, 4, 5, 26, 27], [0, 1, 2, 3, 4, 5, 27, 28]]
+        w = c.weights(i).data.view(np.float32).reshape(6, 60)
+        assert list(w[0]) == list(np.arange(60) + 1000 * i)  # untouched
+        assert list(w[5]) == [300 + x + 1000 * i for x in kept[i, 5]] + [0] * 52
+    # nothing longer than keep: no call, no page needed
+    c.advance([0, 0, 0, 0, 0, 52])
+    c.advance([0, 0, 52, 0, 0, 0])
+    del calls[:]
+    assert len(c.free) == 2
+    assert c.evict(60, 0).shape == (2, 6, 60) and not calls
+    # no room for a single one
+    with pytest.raises(MemoryError):
+        c.evict(12, 0)
+    check(c)
+    assert not calls and list(c.lengths) == [7, 8, 60, 8, 8, 60]

@@ -51,13 +51,14 @@ class PagedCache:
         self._take_over(self.pages, self.lengths)
 
     # ------------------------------------------------------------------ what the calls take
-    def layer(self, i=0, which=0):
-        """The descriptor of layer i's cache (which = 1: the one that evict() writes to)."""
+    def layer(self, i=0, which=0, first=0, count=None):
+        """The descriptor of layer i's cache (which = 1: the one that evict() writes to), of `count` sequences from `first` on."""
         k, v = self._pools[i]
         n_kv, hs = self._shape
-        return Layer(self, _lib.PagedCache(k.ptr, v.ptr, self._tables[which].ptr, self._lengths[which].ptr,
-                                           self.page_size * n_kv * hs, n_kv * hs, hs, self.type, self.n_pages, self.page_size,
-                                           n_kv, hs, self.n_seq, self.width, self.max_length))
+        count = self.n_seq - first if count is None else count
+        return Layer(self, _lib.PagedCache(k.ptr, v.ptr, self._tables[which].ptr + first * self.width * 4,
+                                           self._lengths[which].ptr + first * 4, self.page_size * n_kv * hs, n_kv * hs, hs,
+                                           self.type, self.n_pages, self.page_size, n_kv, hs, count, self.width, self.max_length))
 
     def weights(self, i=0):
         """Layer i's accumulated weights, [n_seq, max_length]."""
@@ -106,39 +107,65 @@ class PagedCache:
     # ------------------------------------------------------------------ eviction
     def evict(self, keep, recent):
         """Thins out the sequences that hold more than keep positions, in every layer by its own weights; returns the
-        positions that stayed, [n_layer, n_seq, keep], -1 behind them. Sequences of up to keep positions are copied whole:
-        needs as many free pages as all that stays fills."""
+        positions that stayed, [n_layer, n_seq, keep], -1 behind them. Sequences of up to keep positions stay as they are.
+        What stays of the others goes to free pages: needs as many as one sequence of keep positions has. As many sequences
+        as there are pages for are thinned out together; a failure leaves those whole that had not come to it."""
         if self._weights is None:
             raise ValueError("the cache keeps no weights: create it with weights=True")
         keep, recent = min(int(keep), self.max_length), int(recent)
         if keep < 1 or not 0 <= recent <= keep:
             raise ValueError(f"keep {keep} and recent {recent}: 0 <= recent <= keep, keep >= 1")
-        after = np.minimum(self.lengths, keep)
-        need = [-(-int(L) // self.page_size) for L in after]
-        if sum(need) > len(self.free):
-            raise MemoryError(f"{sum(need)} pages are needed, {len(self.free)} are free")
-        free = list(self.free)  # nothing that the cache goes by changes before all layers have been thinned out
-        pages = [[free.pop() for _ in range(n)] for n in need]
-        out, moved, kept = [], [], None
+        each = -(-keep // self.page_size)
+        long = [int(s) for s in np.flatnonzero(self.lengths > keep)]
+        if long and each > len(self.free):
+            raise MemoryError(f"{each} pages are needed, {len(self.free)} are free")
+        stayed = np.where(np.arange(keep) < self.lengths[:, None], np.arange(keep), -1).astype(np.int32)
+        stayed = np.tile(stayed, (self.n_layer, 1, 1))
+        while long:  # each sequence gives back as many pages as it takes, or more
+            n = len(self.free) // each
+            self._thin_out(long[:n], keep, recent, stayed)
+            long = long[n:]
+        return stayed
+
+    def _thin_out(self, sequences, keep, recent, stayed):
+        """evict() of these, all longer than keep; free pages are enough. Nothing changes unless all layers' calls go through."""
+        free = list(self.free)
+        pages = [list(p) for p in self.pages]
+        for s in sequences:
+            pages[s] = [free.pop() for _ in range(-(-keep // self.page_size))]
+        # consecutive sequences share a call: (where they begin among `sequences`, the first, how many)
+        runs = []
+        for at, s in enumerate(sequences):
+            if runs and s == runs[-1][1] + runs[-1][2]:
+                runs[-1][2] += 1
+            else:
+                runs.append([at, s, 1])
+        row = self.max_length * 4
+        got, moved, kept = [], [], None
         try:
-            kept = self.device.buffer(self.n_seq * keep * 4)
+            kept = self.device.buffer(len(sequences) * keep * 4)
             for _ in range(self.n_layer):  # the weights that stay, zeros behind them
-                moved.append(self.device.buffer(self.n_seq * self.max_length * 4))
-                moved[-1].write(np.zeros(self.n_seq * self.max_length, np.float32))
+                moved.append(self.device.buffer(len(sequences) * row))
+                moved[-1].write(np.zeros(len(sequences) * self.max_length, np.float32))
             self._tables[1].write(self._table_of(pages))
             for i in range(self.n_layer):
-                _lib.call("wgpt_paged_evict", self.device.handle, self.layer(i).ptr, self.layer(i, 1).ptr, keep, recent,
-                          self._weights[i].ptr, self.max_length, moved[i].ptr, self.max_length, kept.ptr)
-                out.append(kept.read(np.int32, self.n_seq * keep).reshape(self.n_seq, keep))
-            old = [x for p in self.pages for x in p]
-            self._take_over(pages, after)
+                for at, s, n in runs:
+                    _lib.call("wgpt_paged_evict", self.device.handle, self.layer(i, 0, s, n).ptr, self.layer(i, 1, s, n).ptr, keep, recent,
+                              self._weights[i].ptr + s * row, self.max_length, moved[i].ptr + at * row, self.max_length,
+                              kept.ptr + at * keep * 4)
+                got.append(kept.read(np.int32, len(sequences) * keep).reshape(-1, keep))
+            lengths = self.lengths.copy()
+            lengths[sequences] = keep
+            old = [x for s in sequences for x in self.pages[s]]
+            self._take_over(pages, lengths)
             self.free = free + old
+            stayed[:, sequences] = np.stack(got)
             for w, m in zip(self._weights, moved):
-                self.device.copy(m, 0, w, 0, m.nbytes)
+                for at, s, n in runs:
+                    self.device.copy(m, at * row, w, s * row, n * row)
         finally:
             for b in [kept] * (kept is not None) + moved:
                 b.destroy()
-        return np.stack(out)
 
     # ------------------------------------------------------------------ inside
     def _each(self, new):
