@@ -178,3 +178,15 @@ def test_a_full_cache_is_thinned_out(monkeypatch):
         c.evict(12, 0)
     check(c)
     assert not calls and list(c.lengths) == [7, 8, 60, 8, 8, 60]
+
+
+def test_keep_past_the_longest_sequence(monkeypatch):
+    """0 <= recent <= keep is all that is asked: a keep that no sequence can pass thins nothing out, whatever recent is."""
+    c = PagedCache(Addresses(), 2, 1, 8, n_pages=8, page_size=4, max_length=16, weights=True)
+    c.advance([9, 3])
+    for keep, recent in ((100, 100), (100, 17), (17, 16), (16, 16)):
+        kept = c.evict(keep, recent)
+        assert kept.shape == (1, 2, 16) and kept[0].tolist() == [list(range(9)) + [-1] * 7, list(range(3)) + [-1] * 13]
+    for keep, recent in ((100, 101), (0, 0), (5, -1)):
+        with pytest.raises(ValueError):
+            c.evict(keep, recent)

@@ -107,14 +107,15 @@ class PagedCache:
     # ------------------------------------------------------------------ eviction
     def evict(self, keep, recent):
         """Thins out the sequences that hold more than keep positions, in every layer by its own weights; returns the
-        positions that stayed, [n_layer, n_seq, keep], -1 behind them. Sequences of up to keep positions stay as they are.
+        positions that stayed, [n_layer, n_seq, min(keep, max_length)], -1 behind them. Sequences of up to keep positions stay as they are.
         What stays of the others goes to free pages: needs as many as one sequence of keep positions has. As many sequences
         as there are pages for are thinned out together; a failure leaves those whole that had not come to it."""
         if self._weights is None:
             raise ValueError("the cache keeps no weights: create it with weights=True")
-        keep, recent = min(int(keep), self.max_length), int(recent)
+        keep, recent = int(keep), int(recent)
         if keep < 1 or not 0 <= recent <= keep:
             raise ValueError(f"keep {keep} and recent {recent}: 0 <= recent <= keep, keep >= 1")
+        keep = min(keep, self.max_length)  # no sequence is longer
         each = -(-keep // self.page_size)
         long = [int(s) for s in np.flatnonzero(self.lengths > keep)]
         if long and each > len(self.free):
