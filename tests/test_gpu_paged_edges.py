@@ -51,3 +51,12 @@ def test_a_full_cache_is_thinned_out(dev, type):  # noqa: F811
                 assert np.array_equal(pool[table[s, at // page], at % page], want)
     _lib.call("wgpt_device_check", dev.handle)
     cache.destroy()
+
+
+@pytest.mark.parametrize("type,n_head", [("f32", 1), ("f16", 1), ("bf16", 12)])
+def test_windows_past_every_length(dev, type, n_head):  # noqa: F811
+    """A window that no sequence fills is none, up to the largest number, also for sequences shorter than their new tokens."""
+    rng = np.random.default_rng(2)
+    pages = make(rng, [300, 200, 3], 16, 1, 64, type)
+    for window in (301, 1 << 30, (1 << 31) - 1):
+        check_attention(dev, pages, type, "positions", [303, 205, 9], n_head, window=window, weights=True)

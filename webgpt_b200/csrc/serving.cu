@@ -205,7 +205,7 @@ WGPT_EXPORT int32_t wgpt_paged_attention(wgpt_device *dev, const wgpt_paged_cach
           (long long)ld_weights, cache->max_length);
   a.n_head = n_head;
   a.group = n_head / cache->n_kv_head;
-  a.window = window;
+  a.window = window < cache->max_length ? window : 0;  // one that no sequence fills is none; differences of it stay in 32 bits
   a.scale2 = scale * 1.44269504088896f;
   a.q = q;
   a.out = out;
