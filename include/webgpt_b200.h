@@ -348,7 +348,7 @@ int32_t wgpt_paged_append(wgpt_device *dev, const wgpt_paged_cache *cache, int32
  *   out = sum_j softmax_j(scale * q . k_j) v_j,
  * f32 throughout (half-precision caches go through the tensor cores as they are, q and the probabilities as sums of
  * half-precision values). Positions in a page whose id is out of range are not seen; a row that belongs to a token but sees
- * nothing is set to zeros; rows that belong to no sequence are left as they were. q and out may be one array. ld_q and ld_out
+ * nothing is set to zeros; rows that belong to no sequence are left as they were, all rows and weights where starts decreases. q and out may be one array. ld_q and ld_out
  * multiples of 4. The row tiles of a call times its tiles of positions have to stay below 2^32 (WGPT_ERR_SHAPE: split the call).
  * weights, or NULL: [n_seq, ld_weights] f32, ld_weights >= max_length; the attention weight that each position got, summed
  * over the heads and new tokens of its sequence, is added to weights[s * ld_weights + j]. The order of all sums is fixed:

@@ -60,3 +60,26 @@ def test_windows_past_every_length(dev, type, n_head):  # noqa: F811
     pages = make(rng, [300, 200, 3], 16, 1, 64, type)
     for window in (301, 1 << 30, (1 << 31) - 1):
         check_attention(dev, pages, type, "positions", [303, 205, 9], n_head, window=window, weights=True)
+
+
+@pytest.mark.parametrize("type,n_head,n_seq", [("f32", 1, 3), ("f16", 1, 20), ("f16", 12, 20), ("f32", 1, 1024), ("f16", 1, 1024), ("bf16", 16, 1024)])
+def test_offsets_that_decrease(dev, type, n_head, n_seq):  # noqa: F811
+    """Sequences that would share rows: nothing is computed, nothing out of range is touched, and the call is reported. The rows
+    of all of them together times their tiles do not fit 32 bits at 1024 sequences: 512 x 1024 rows of 8192 units and more."""
+    rng = np.random.default_rng(3)
+    pages = make(rng, [17] * n_seq, 16, 1, 64, type, max_length=1 << 20)
+    c = OnDevice(dev, pages, type)
+    c.lengths.write(np.full(n_seq, 1 << 20, np.int32))  # pages that are not there are not seen
+    q = rng.standard_normal((n_seq, n_head, 64)).astype(np.float32)
+    alternating = [0, n_seq] * (n_seq // 2 + 1)
+    for starts in (alternating[:n_seq + 1], [n_seq - i for i in range(n_seq + 1)], list(range(n_seq)) + [n_seq - 2]):
+        got, _ = attend(dev, c, starts, n_seq, n_head, 0.125, 0, q)
+        assert (got == 7.0).all()
+        reported(dev)
+    small = OnDevice(dev, make(rng, [9] * n_seq, 16, 1, 64, type), type)
+    w0 = rng.random((n_seq, 9)).astype(np.float32)
+    got, w = attend(dev, small, alternating[:n_seq + 1], n_seq, n_head, 0.125, 0, q, w0)
+    assert (got == 7.0).all() and np.array_equal(w, w0)
+    reported(dev)
+    attend(dev, small, list(range(n_seq + 1)), n_seq, n_head, 0.125, 0, q, w0)
+    _lib.call("wgpt_device_check", dev.handle)

@@ -34,17 +34,19 @@ __device__ __forceinline__ int paged_length(const PagedView &c, int s) {
   return L < 0 ? 0 : c.max_length;
 }
 
-// Rows [first, first + n) of sequence s, inside [0, n_rows) whatever starts says.
-__device__ __forceinline__ void new_rows(const PagedView &c, const NewRows &r, int s, int &first, int &n) {
+// Rows [first, first + n) of sequence s, inside [0, n_rows) whatever starts says. Whether starts goes on from s to s + 1: sequences
+// share no rows where it always does.
+__device__ __forceinline__ bool new_rows(const PagedView &c, const NewRows &r, int s, int &first, int &n) {
   if (r.starts == nullptr) {
     first = s * r.per;
     n = r.per;
-    return;
+    return true;
   }
   const int a = __ldcg(r.starts + s), b = __ldcg(r.starts + s + 1);
   first = min(max(a, 0), r.n_rows);
   n = min(max(b, first), r.n_rows) - first;
   if (a != first || b != first + n) *c.err = kErrCache;
+  return a <= b;
 }
 
 // Where a position's rows begin (elements into a pool), or -1 and the error word.

@@ -43,6 +43,7 @@ struct PagedAttention {
   float *partial;        // [2 * CTAs][paged_slot(rows, hs)]
   unsigned int *join;    // a counter per CTA, zero on entry and left zero
   float *scores, *stats; // [n_rows * n_head][max_length] and [n_rows * n_head], in units of log 2, or NULL
+  unsigned int *skip;    // whether the call does nothing, for the kernel that adds the weights up; or NULL
 };
 
 // Quotients that the chain ahead of the first copy waits for: mostly by one.
@@ -54,9 +55,10 @@ struct PagedSeq {
   int tiles, units;        // row tiles, units of each and what is added to them
 };
 
-__device__ __forceinline__ PagedSeq paged_seq(const PagedAttention &a, int s, int unit) {
+__device__ __forceinline__ PagedSeq paged_seq(const PagedAttention &a, int s, int unit, bool *in_order = nullptr) {
   PagedSeq q;
-  new_rows(a.c, a.r, s, q.first, q.n);
+  const bool on = new_rows(a.c, a.r, s, q.first, q.n);
+  if (in_order) *in_order = on;
   q.L = paged_length(a.c, s);
   const int lowest = a.window > 0 ? max(0, q.L - q.n + 1 - a.window) : 0;
   q.begin = min(lowest, q.L) & ~(unit - 1);
@@ -130,15 +132,23 @@ __device__ __forceinline__ void paged_part(const PagedAttention &a, PagedPart &w
 }
 
 // A CTA's units [.., end) of all there are and the part they begin with, by all its threads, every one of which gets it: false if
-// there are none. sums: a number for each warp; place: a part.
+// there are none. Nor are there any where the row offsets decrease somewhere: rows would be counted for several sequences, more of them
+// than the caller's bound on the units allows for. sums: a number for each warp; place: a part.
 __device__ __forceinline__ bool paged_first(const PagedAttention &a, PagedPart &to, int unit, uint32_t *sums, PagedPart *place, uint32_t &per,
                                             uint32_t &end) {
   const int threads = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_seq = a.c.n_seq;
   PagedSeq q;
+  bool bad = false;
   auto weight_of = [&](int s) -> uint32_t {
     if (s >= n_seq) return 0;
-    q = paged_seq(a, s, unit);
+    bool in_order;
+    q = paged_seq(a, s, unit, &in_order);
+    bad = bad || !in_order;
     return paged_work(a, q);
+  };
+  auto skipped = [&](bool skip) {
+    if (a.skip && blockIdx.x == 0 && tid == 0) *a.skip = skip ? 1u : 0u;
+    return skip;
   };
   auto before_lane = [&](uint32_t mine) {  // sum over the lanes up to this one
 #pragma unroll
@@ -150,6 +160,7 @@ __device__ __forceinline__ bool paged_first(const PagedAttention &a, PagedPart &
   };
   if (n_seq <= 32) {  // every warp for itself, a sequence a lane
     const uint32_t mine = weight_of(lane), upto = before_lane(mine), total = __shfl_sync(0xffffffffu, upto, 31);
+    if (skipped(__any_sync(0xffffffffu, bad))) return false;
     per = max((uint32_t)a.least, (total + gridDim.x - 1) / gridDim.x);
     const uint32_t x0 = blockIdx.x * per;  // the caller sees to it that it does not pass 2^32
     end = min(total, x0 + per);
@@ -181,6 +192,7 @@ __device__ __forceinline__ bool paged_first(const PagedAttention &a, PagedPart &
     before = total + scan(mine, all);
     total += all;
   }
+  if (skipped(__syncthreads_or(bad))) return false;
   per = max((uint32_t)a.least, (total + gridDim.x - 1) / gridDim.x);
   const uint32_t x0 = blockIdx.x * per, x1 = min(total, x0 + per);  // the caller sees to it that neither passes 2^32
   if (x0 >= x1) return false;
@@ -1064,6 +1076,7 @@ paged_weights_kernel(const __grid_constant__ PagedAttention a, float *__restrict
   pdl_wait();
   const PagedView &c = a.c;
   const int s = blockIdx.y;
+  if (__ldcg(a.skip) != 0) return;
   int first, n;
   new_rows(c, a.r, s, first, n);
   const int L = paged_length(c, s);

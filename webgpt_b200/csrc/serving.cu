@@ -85,10 +85,12 @@ static int32_t paged_workspace(wgpt_device *dev, PagedAttention &a, int grid, in
           WGPT_ERR_SHAPE, "%d rows over up to %d positions of %d heads: split the call", a.r.n_rows, a.c.max_length, a.c.n_kv);
   const size_t rows = a.stats ? (size_t)a.r.n_rows * a.n_head : 0, scores = rows * (size_t)a.c.max_length;
   const size_t partial = (size_t)2 * grid * paged_slot(a.rows, a.c.hs);
-  TRY(scratch_reserve(dev, (partial + rows + scores) * 4));
+  TRY(scratch_reserve(dev, (partial + 1 + rows + scores) * 4));
   a.partial = static_cast<float *>(dev->scratch);
+  a.skip = nullptr;
   if (a.stats) {
-    a.stats = a.partial + partial;
+    a.skip = reinterpret_cast<unsigned int *>(a.partial + partial);
+    a.stats = a.partial + partial + 1;
     a.scores = a.stats + rows;
   }
   a.join = dev->d_join;
