@@ -83,3 +83,53 @@ def test_offsets_that_decrease(dev, type, n_head, n_seq):  # noqa: F811
     reported(dev)
     attend(dev, small, list(range(n_seq + 1)), n_seq, n_head, 0.125, 0, q, w0)
     _lib.call("wgpt_device_check", dev.handle)
+
+
+@pytest.mark.parametrize("type,n_kv,group,hs,new", [("f16", 2, 12, 64, 1), ("f16", 2, 4, 128, 6), ("bf16", 2, 16, 64, 1), ("bf16", 1, 3, 128, 9), ("f16", 2, 1, 64, 1),
+                                                    ("bf16", 1, 8, 128, 1), ("f32", 2, 2, 64, 1), ("f16", 1, 4, 256, 2)])
+def test_values_that_are_not_finite_in_long_sequences(dev, type, n_kv, group, hs, new):  # noqa: F811
+    """Sequences of thousands of positions beside many short ones, each of the long ones with a value that is not finite: rows that
+    see it get it, rows that do not and other sequences stay as good as ever, and no wait runs out meanwhile."""
+    rng = np.random.default_rng(4)
+    lengths = [6000, 9000] + [int(x) for x in rng.integers(new, 300, 90)] + [7001]
+    pages = make(rng, lengths, 16, n_kv, hs, type)
+    n_head = n_kv * group
+    starts = [new * s for s in range(len(lengths) + 1)]
+    q = (rng.standard_normal((starts[-1], n_head, hs)) * 1.5).astype(np.float32)
+    want, _, size, top = ref.attend(pages, starts, n_head, 0.125, 2500, q)
+    pages.v[pages.place(0, 5990)][0, 3] = np.inf        # in every row's window
+    pages.v[pages.place(1, 100)] = np.nan               # in no row's window nor tiles
+    pages.v[pages.place(1, 9000 - 2500 - new)] = -np.inf  # just before the first row's
+    pages.k[pages.place(92, 7001 - 2500 + 1 - new)] = np.nan  # in the first row's alone
+    cache = OnDevice(dev, pages, type)
+    got, _ = attend(dev, cache, starts, starts[-1], n_head, 0.125, 2500, q)
+    _lib.call("wgpt_device_check", dev.handle)
+    assert (got[:new, :group, 3] == np.inf).all()
+    got[:new, :group, 3] = want[:new, :group, 3]
+    first = starts[92]
+    assert np.isnan(got[first]).all()
+    got[first] = want[first]
+    assert (np.abs(got - want) <= ref.attend_tolerance(pages, size, top)).all()
+
+
+@pytest.mark.parametrize("type,group", [("f16", 12), ("f16", 1), ("f32", 1)])
+def test_many_sequences_without_new_tokens(dev, type, group):  # noqa: F811
+    """Two sequences with new tokens and tens of thousands without between them: a CTA that has a part of both looks for its next one
+    for a long time."""
+    n_seq, hs = 65535, 64
+    rng = np.random.default_rng(5)
+    lengths = [150] + [0] * (n_seq - 2) + [170]
+    pages = make(rng, lengths, 16, 1, hs, type)
+    starts = [0] + [1] * (n_seq - 1) + [2]
+    q = rng.standard_normal((2, group, hs)).astype(np.float32)
+    c = OnDevice(dev, pages, type)
+    for _ in range(2):
+        got, _ = attend(dev, c, starts, 2, group, 0.125, 0, q)
+    few = ref.Pages(rng, [150, 170], 16, 1, hs)
+    for which in ("k", "v"):
+        for at, s in enumerate((0, n_seq - 1)):
+            for j in range(lengths[s]):
+                getattr(few, which)[few.place(at, j)] = getattr(pages, which)[pages.place(s, j)]
+    want, _, size, top = ref.attend(few, [0, 1, 2], group, 0.125, 0, q)
+    assert (np.abs(got - want) <= ref.attend_tolerance(few, size, top)).all()
+    _lib.call("wgpt_device_check", dev.handle)

@@ -210,14 +210,16 @@ __device__ __forceinline__ bool paged_first(const PagedAttention &a, PagedPart &
   return end > to.begin + a.extra;
 }
 
-// The part behind `w`, which ends before unit `end`. May not be `w` itself.
-__device__ __forceinline__ void paged_next(const PagedAttention &a, PagedPart &to, const PagedPart &w, uint32_t end, int unit) {
+// The part behind `w`, which ends before unit `end`. May not be `w` itself. progress, or NULL: goes on with every sequence passed over.
+__device__ __forceinline__ void paged_next(const PagedAttention &a, PagedPart &to, const PagedPart &w, uint32_t end, int unit,
+                                           unsigned int *progress = nullptr) {
   uint32_t seq_begin = w.seq_begin;
   PagedSeq q = w.q;
   int s = w.g.s;
   while (w.next >= seq_begin + paged_work(a, q)) {
     seq_begin += paged_work(a, q);
     q = paged_seq(a, ++s, unit);
+    if (progress) atomicAdd(progress, 1u);
   }
   paged_part(a, to, q, s, seq_begin, w.next, end, unit);
 }
@@ -261,51 +263,80 @@ struct PagedShape {
   __host__ __device__ static constexpr bool fits(int rows, int hs) { return rows * hs * 4 <= kRing; }
 };
 
-// Rows of a tile that a warp saw something non-finite in (an infinity or NaN in V, in a key, in q, also where a row's mask
-// leaves it out: zero times infinity): the same again one position at a time, each row from what it sees alone. Leaves the row's
-// maximum, sum and values as the fast path does.
-template <typename T, int TILE>
-__device__ __noinline__ void paged_rows_apart(const PagedAttention &a, const PagedPart &w, int key_group, int key_groups,
-                                              int row0, int row1, int lane, float *o_out, float *m_out, float *l_out) {
+// Rows of a tile that came out non-finite (an infinity or NaN in V, in a key, in q, also where a row's mask leaves it out: zero times
+// infinity), a bit each: the same again by one warp, each row from what it sees alone, in the order of the positions. Leaves the row's
+// maximum, sum and values as the fast path does. The pages of 32 positions are looked up at once, and some positions' keys and
+// values are on their way together. progress, or NULL: goes on with every 32 positions, for those who wait.
+// PIECES: of 32 dimensions.
+template <typename T, int TILE, int PIECES>
+__device__ __noinline__ void paged_rows_apart(const PagedAttention &a, const PagedPart &w, int key_group, int key_groups, uint32_t rows,
+                                              int lane, float *o_out, float *m_out, float *l_out, unsigned int *progress) {
+  constexpr int kAtOnce = PIECES <= 2 ? 4 : PIECES <= 4 ? 3 : 2, kBlock = TILE < 32 ? TILE : 32;
   const PagedView &c = a.c;
   const PagedSeq &q = w.q;
   const PagedGroup &g = w.g;
-  for (int r = row0; r < row1; r++) {
+  const T *ck = static_cast<const T *>(c.k) + g.kvh * c.head_stride + lane, *cv = static_cast<const T *>(c.v) + g.kvh * c.head_stride + lane;
+  for (; rows != 0; rows &= rows - 1) {
+    const int r = __ffs(rows) - 1;
     int lo, hi;
     row_range(a, q, (g.r0 + r) / a.group, lo, hi);
     const float *x = a.q + row_offset(a, w, r, a.ld_q);
-    float qv[8], o[8], m = -INFINITY, l = 0.f;
+    float qv[PIECES], o[PIECES], m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
+    for (int i = 0; i < PIECES; i++) {
       qv[i] = lane + 32 * i < c.hs ? __ldcg(x + lane + 32 * i) : 0.f;
       o[i] = 0.f;
     }
     for (int u = w.u0; u < w.u0 + w.n_tiles; u++) {
       const int base = q.begin + (u * key_groups + key_group) * TILE;
-      for (int j = max(base, lo); j < min(base + TILE, hi); j++) {
-        const long long at = paged_offset(c, g.s, j);
-        float sc = -INFINITY;
-        if (at >= 0) {
-          const T *k = static_cast<const T *>(c.k) + at + g.kvh * c.head_stride, *v = static_cast<const T *>(c.v) + at + g.kvh * c.head_stride;
-          float d = 0.f;
+      for (int b = base; b < base + TILE; b += kBlock) {
+        const int first = max(b, lo), last = min(b + kBlock, hi);
+        if (first >= last) continue;
+        const long long mine = b + lane >= first && b + lane < last ? paged_offset(c, g.s, b + lane) : -1;
+        for (int j = first; j < last; j += kAtOnce) {
+          long long at[kAtOnce];
+          float kk[kAtOnce][PIECES], vv[kAtOnce][PIECES], d[kAtOnce];
 #pragma unroll
-          for (int i = 0; i < 8; i++)
-            if (lane + 32 * i < c.hs) d += qv[i] * paged_value(k + lane + 32 * i);
-          sc = warp_sum(d) * a.scale2;
-          if (sc != -INFINITY) {
-            const float nm = fmaxf(m, sc), f = exp2f(m - nm), p = exp2f(sc - nm);
-            l = l * f + p;
+          for (int y = 0; y < kAtOnce; y++) {
+            at[y] = __shfl_sync(0xffffffffu, mine, (j + y - b) & 31);
+            if (j + y >= last) at[y] = -1;
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-              if (lane + 32 * i < c.hs) o[i] = o[i] * f + p * paged_value(v + lane + 32 * i);
-            m = nm;
+            for (int i = 0; i < PIECES; i++) {
+              const bool in = at[y] >= 0 && lane + 32 * i < c.hs;
+              kk[y][i] = in ? paged_value(ck + at[y] + 32 * i) : 0.f;
+              vv[y][i] = in ? paged_value(cv + at[y] + 32 * i) : 0.f;
+            }
+          }
+#pragma unroll
+          for (int y = 0; y < kAtOnce; y++) {
+            d[y] = 0.f;
+#pragma unroll
+            for (int i = 0; i < PIECES; i++)
+              if (lane + 32 * i < c.hs) d[y] += qv[i] * kk[y][i];
+          }
+#pragma unroll
+          for (int o2 = 16; o2 > 0; o2 >>= 1)
+#pragma unroll
+            for (int y = 0; y < kAtOnce; y++) d[y] += __shfl_xor_sync(0xffffffffu, d[y], o2);
+#pragma unroll
+          for (int y = 0; y < kAtOnce; y++) {
+            const float sc = at[y] >= 0 ? d[y] * a.scale2 : -INFINITY;
+            if (sc != -INFINITY) {
+              const float nm = fmaxf(m, sc), f = exp2f(m - nm), p = exp2f(sc - nm);
+              l = l * f + p;
+#pragma unroll
+              for (int i = 0; i < PIECES; i++)
+                if (lane + 32 * i < c.hs) o[i] = o[i] * f + p * vv[y][i];
+              m = nm;
+            }
+            if (a.scores && lane == 0 && j + y < last) a.scores[row_index(a, w, r) * c.max_length + j + y] = sc;
           }
         }
-        if (a.scores && lane == 0) a.scores[row_index(a, w, r) * c.max_length + j] = sc;
+        if (progress && lane == 0) atomicAdd(progress, 1u);
       }
     }
 #pragma unroll
-    for (int i = 0; i < 8; i++)
+    for (int i = 0; i < PIECES; i++)
       if (lane + 32 * i < c.hs) o_out[r * c.hs + lane + 32 * i] = o[i];
     if (lane == 0) {
       m_out[r] = m;
@@ -723,7 +754,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
     const int n_tiles = w.n_tiles, inner_low = g.inner_low, inner_high = g.inner_high, g_rows = g.rows;
     const bool more = s_more != 0;
     int pos0 = w.q.begin + (w.u0 * KG + kg) * kTile, now = 0;  // of the tile at hand; the stage that is next to be used up
-    bool finite = true;
+    uint32_t odd = 0;  // rows that came out non-finite
     if constexpr (S::kWide) {
       constexpr int kShare = 32 / kTile;  // lanes that share a key
       const int key = lane % kTile, share = lane / kTile, half = lane >> 4, dim = lane & 15;
@@ -840,11 +871,11 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
           }
           const int d = (kHalves == 2 ? dim : lane) + 32 * i;
           if (r < g_rows && 4 * d < hs) {
-            finite = finite && fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) < INFINITY;
+            if (!(fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) < INFINITY)) odd |= 1u << r;
             if (kHalves == 1 || half == 0) *reinterpret_cast<float4 *>(o_smem + r * hs + 4 * d) = v;
           }
         }
-        finite = finite && (r >= g_rows || fabsf(l[r]) < INFINITY);
+        if (r < g_rows && !(fabsf(l[r]) < INFINITY)) odd |= 1u << r;
         if (lane == 0) {
           s_m[kg][r] = m[r];
           s_l[kg][r] = l[r];
@@ -1000,7 +1031,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
           s_l[kg][r] = l[e] * down;
         }
         if (r < g_rows) {
-          finite = finite && fabsf(l[e]) < INFINITY;
+          bool finite = fabsf(l[e]) < INFINITY;
 #pragma unroll
           for (int i = 0; i < KS; i++)
 #pragma unroll
@@ -1012,13 +1043,12 @@ paged_attention_kernel(const __grid_constant__ PagedAttention a) {
                 o_smem[r * hs + d] = v;
               }
             }
+          if (!finite) odd |= 1u << r;
         }
       }
     }
-    if (!__all_sync(0xffffffffu, finite)) {
-      __syncwarp();
-      paged_rows_apart<T, kTile>(a, w, kg, KG, S::kWide ? 0 : 8 * rw, S::kWide ? g_rows : min(g_rows, 8 * rw + 8), lane, o_smem, s_m[kg], s_l[kg]);
-    }
+    odd = __reduce_or_sync(0xffffffffu, odd);
+    if (odd != 0) paged_rows_apart<T, kTile, HSP / 32>(a, w, kg, KG, odd, lane, o_smem, s_m[kg], s_l[kg], nullptr);
     __syncthreads();
 
     // ---- the key groups' results, and the group's if other CTAs have a part of it

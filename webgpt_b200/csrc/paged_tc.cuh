@@ -15,7 +15,8 @@
 //   four warps for every 16 rows: softmax and sums;
 //   one warp    issues the MMAs: the next tile's scores before this tile's values;
 //   four warps  fill a ring of tiles by cp.async, 32 rows each, in the order in which they are used up: K0 K1 V0 K2 V1 ...
-// Every wait is bounded; on expiry *err = 3 and the result is void.
+// Every wait is bounded; on expiry *err = 3 and the result is void. A row that meets an infinity or NaN is computed again by a warp,
+// which may take longer than a wait's polls: a wait begins anew as long as such a warp, or one that looks for its next sequence, gets on.
 // Measured, 8 heads of 128, f16, 8 users with up to 5 tokens of 4 rows each: up to 8192 positions (192 MB) 48 us, 4.0 TB/s, of which
 // some 25 are the beginning (7), the change from one group to the next and the joins; up to 32768 (663 MB) 117 us, 5.7 TB/s. A tile of
 // 64 KB takes a CTA 1.4 us then, which is its share of the copy rate.
@@ -102,6 +103,7 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
   __shared__ uint64_t full[NS], empty[NS], q_ready, s_done[2], p_ready[2], o_done[2], drained;
   __shared__ uint32_t tmem_slot, s_sum[S::kThreads / 32];
   __shared__ int abort_word, s_last;
+  __shared__ unsigned int s_progress, s_odd;  // how far work has come that the others cannot see; rows that came out non-finite
   __shared__ PagedPart s_part[3];  // the softmax warps' part and the next, and a place for the first
   __shared__ __align__(16) float s_qscale[N], s_max[4][N], s_l[N], s_m[N];
   __shared__ int s_lo[N], s_hi[N];
@@ -109,6 +111,7 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
   __shared__ float4 s_red[SOFT];
   __shared__ float s_red_sum[SOFT];
   volatile int *abort_flag = &abort_word;
+  volatile unsigned int *progress = &s_progress;
   const PagedView &c = a.c;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, hs = c.hs;
   if (tid == 0) {
@@ -124,6 +127,7 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
     }
     mbar_init(&drained, 1);
     abort_word = 0;
+    s_progress = s_odd = 0;
     fence_async_smem();
   }
   if (warp == WARPS) tmem_alloc(&tmem_slot, S::kTmem);
@@ -141,7 +145,13 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
   const bool any = paged_first(a, first, kTcKeys, s_sum, &s_part[2], per, x1);
   // A wait that has run out makes all others return at once: every role runs to its end.
   auto wait = [&](uint64_t *bar, uint32_t parity) {
-    if (!*abort_flag && !mbar_wait(bar, parity & 1, TC_POLLS)) *abort_flag = 1;
+    if (!*abort_flag && !mbar_wait(bar, parity & 1, TC_POLLS)) {
+      unsigned int seen;
+      do {
+        seen = *progress;
+      } while (!*abort_flag && !mbar_wait(bar, parity & 1, TC_POLLS) && *progress != seen);
+      if (!mbar_wait(bar, parity & 1, 1)) *abort_flag = 1;
+    }
     __syncwarp();
   };
 
@@ -220,7 +230,7 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
       if (n_tiles > 0 && lane == 0) mbar_arrive(&q_ready);
       // the next part, by one thread while the first scores are on their way
       const bool more = paged_more(a, w, x1);
-      if (more && tid == SOFT - 1) paged_next(a, s_part[turn ^ 1], w, x1, kTcKeys);
+      if (more && tid == SOFT - 1) paged_next(a, s_part[turn ^ 1], w, x1, kTcKeys, &s_progress);
       __syncwarp();
       float m[R], l[R], o[R];
 #pragma unroll
@@ -326,29 +336,35 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
       tc_fence_before();
       // ---- the rows' sums over the keys
       const float down = kLift != 0.f ? 1.f / 128.f : 1.f;
-      bool finite = true;
+      uint32_t odd = 0;
       const float mine_sum = warp_each16(l, lane, [](float u, float v) { return u + v; });
       if ((lane & 1) == 0) s_max[quad][r0 + lane / 2] = mine_sum;
 #pragma unroll
       for (int r = 0; r < R; r++) {
         o[r] *= down;
-        finite = finite && (r0 + r >= rows || key >= hs || fabsf(o[r]) < INFINITY);
+        if (r0 + r < rows && key < hs && !(fabsf(o[r]) < INFINITY)) odd |= 1u << (r0 + r);
         if (key == r) s_m[r0 + r] = m[r];
       }
       meet();
       if (tid < N) {
         s_l[tid] = ((s_max[0][tid] + s_max[1][tid]) + (s_max[2][tid] + s_max[3][tid])) * down;
-        finite = finite && (tid >= rows || fabsf(s_l[tid]) < INFINITY);
+        if (tid < rows && !(fabsf(s_l[tid]) < INFINITY)) odd |= 1u << tid;
       }
       __syncwarp();
       float *values = reinterpret_cast<float *>(Ps);  // the probabilities' place: the products that read them are done
-      if (some(!finite)) {  // each row from what it sees alone
-        const int share = (rows + WARPS - 1) / WARPS;
-        paged_rows_apart<T, kTcKeys>(a, w, 0, 1, warp * share, min(rows, warp * share + share), lane, values, s_m, s_l);
+      if (odd != 0) atomicOr(&s_odd, odd);
+      if (some(odd != 0)) {  // each such row from what it sees alone, a warp a row
+        odd = s_odd;
+        uint32_t mine = 0;
+        int turn_of = 0;
+        for (uint32_t left = odd; left != 0; left &= left - 1)
+          if (turn_of++ % WARPS == warp) mine |= left & -left;
+        paged_rows_apart<T, kTcKeys, 2 * HB>(a, w, 0, 1, mine, lane, values, s_m, s_l, &s_progress);
         meet();
 #pragma unroll
         for (int r = 0; r < R; r++)
-          if (r0 + r < rows && key < hs) o[r] = values[(r0 + r) * hs + key];
+          if ((odd >> (r0 + r) & 1u) && key < hs) o[r] = values[(r0 + r) * hs + key];
+        if (tid == 0) s_odd = 0;
         meet();
       }
       // ---- the result, or this part of it
@@ -426,7 +442,7 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
       }
       if (!paged_more(a, w, x1)) break;
       const PagedPart before = w;
-      paged_next(a, w, before, x1, kTcKeys);
+      paged_next(a, w, before, x1, kTcKeys, lane == 0 ? &s_progress : nullptr);
     }
     if (*abort_flag) {  // what has been issued ends before its operands go
       umma_commit_elect(&drained);
@@ -511,7 +527,7 @@ __global__ void __launch_bounds__((TcShape<T, HB, N>::kThreads), 1) paged_attent
       }
       if (!paged_more(a, w, x1)) break;
       const PagedPart before = w;
-      paged_next(a, w, before, x1, kTcKeys);
+      paged_next(a, w, before, x1, kTcKeys, lane == 0 ? &s_progress : nullptr);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   }
