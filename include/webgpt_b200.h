@@ -309,7 +309,8 @@ int32_t wgpt_sample_topk(wgpt_device *dev, const float *logits, int32_t n_rows, 
 /* ---- serving sequences of different lengths: a paged key-value cache, attention over it, its eviction, and the
  *      verification of drafted tokens. No counterpart in the reference, which recomputes one window per token
  *      (model.js:69,104-268); the attention is that of instructions.js:1101-1214 and the softmax and pick are those of
- *      globals.js:47-74. All of these calls only enqueue; what a kernel finds wrong in device memory (a page id, a length,
+ *      globals.js:47-74. All of these calls only enqueue (but for the workspace, which the first or a larger call makes grow: not
+ *      while a pass list is being recorded); what a kernel finds wrong in device memory (a page id, a length,
  *      row offsets, a token id out of range, a row of logits without a distribution) is skipped as said below and reported
  *      by the next wgpt_device_check as WGPT_ERR_ARG. Nothing of a captured call depends on host memory. */
 
@@ -351,8 +352,11 @@ int32_t wgpt_paged_append(wgpt_device *dev, const wgpt_paged_cache *cache, int32
  * nothing is set to zeros; rows that belong to no sequence are left as they were, all rows and weights where starts decreases. q and out may be one array. ld_q and ld_out
  * multiples of 4. The row tiles of a call times its tiles of positions have to stay below 2^32 (WGPT_ERR_SHAPE: split the call).
  * weights, or NULL: [n_seq, ld_weights] f32, ld_weights >= max_length; the attention weight that each position got, summed
- * over the heads and new tokens of its sequence, is added to weights[s * ld_weights + j]. The order of all sums is fixed:
- * the same call gives the same bits. */
+ * over the heads and new tokens of its sequence, is added to weights[s * ld_weights + j]. Drafts that are not accepted later have
+ * added theirs all the same. The order of all sums is fixed: the same call gives the same bits.
+ * Workspace: with weights, max_length f32 scores for every head of as many rows as take up to 1 GiB (of one row at least; more rows
+ * are done so many at a time, by two launches each), WGPT_ERR_OOM where that is not to be had; else some MB. The call that makes it
+ * grow waits for the device. */
 int32_t wgpt_paged_attention(wgpt_device *dev, const wgpt_paged_cache *cache, int32_t n_rows, const int32_t *starts,
                              int32_t n_head, float scale, int32_t window, const float *q, int64_t ld_q, float *out,
                              int64_t ld_out, float *weights, int64_t ld_weights);

@@ -133,3 +133,16 @@ def test_many_sequences_without_new_tokens(dev, type, group):  # noqa: F811
     want, _, size, top = ref.attend(few, [0, 1, 2], group, 0.125, 0, q)
     assert (np.abs(got - want) <= ref.attend_tolerance(few, size, top)).all()
     _lib.call("wgpt_device_check", dev.handle)
+
+
+@pytest.mark.parametrize("type,n_kv,group,hs,window", [("f32", 8, 1, 64, 0), ("f16", 2, 4, 64, 30), ("bf16", 1, 12, 128, 0), ("f16", 1, 8, 256, 0), ("f16", 1, 16, 64, 17)])
+def test_scores_of_more_than_the_workspace_holds(dev, type, n_kv, group, hs, window):  # noqa: F811
+    """2^20 positions a sequence at most: 32 rows of eight heads take a gigabyte. A call of more rows is cut, inside sequences too."""
+    rng = np.random.default_rng(6)
+    lengths, new = [40, 3, 90, 0, 300, 61], [20, 9, 1, 2, 33, 30]
+    pages = make(rng, lengths, 16, n_kv, hs, type, max_length=1 << 20)
+    free = dev.mem_info()[0]
+    check_attention(dev, pages, type, "positions", new, n_kv * group, window=window, weights=True, before=1, behind=3)
+    assert free - dev.mem_info()[0] < 3 << 29  # 95 rows whole: 3 GB
+    check_attention(dev, pages, type, "positions", [1, 1, 1, 0, 1, 1], n_kv * group, window=window, weights=True)
+    _lib.call("wgpt_device_check", dev.handle)

@@ -42,7 +42,8 @@ struct PagedAttention {
   int ahead;             // whether the results of a group leave room for the next one's first tiles
   float *partial;        // [2 * CTAs][paged_slot(rows, hs)]
   unsigned int *join;    // a counter per CTA, zero on entry and left zero
-  float *scores, *stats; // [n_rows * n_head][max_length] and [n_rows * n_head], in units of log 2, or NULL
+  int row0, row1;        // the rows of this launch: [row0, row1)
+  float *scores, *stats; // [(row1 - row0) * n_head][max_length] and [(row1 - row0) * n_head], in units of log 2, or NULL
   unsigned int *skip;    // whether the call does nothing, for the kernel that adds the weights up; or NULL
 };
 
@@ -55,11 +56,21 @@ struct PagedSeq {
   int tiles, units;        // row tiles, units of each and what is added to them
 };
 
+// A sequence's rows in this launch, and how many positions there are up to the last of them: one whose last rows come later is as much
+// shorter. Returns what new_rows does.
+__device__ __forceinline__ bool launch_rows(const PagedAttention &a, int s, int &first, int &n, int &L) {
+  const bool on = new_rows(a.c, a.r, s, first, n);
+  const int end = first + n, to = min(end, a.row1);
+  L = max(0, paged_length(a.c, s) - (end - to));
+  first = max(first, a.row0);
+  n = max(0, to - first);
+  return on;
+}
+
 __device__ __forceinline__ PagedSeq paged_seq(const PagedAttention &a, int s, int unit, bool *in_order = nullptr) {
   PagedSeq q;
-  const bool on = new_rows(a.c, a.r, s, q.first, q.n);
+  const bool on = launch_rows(a, s, q.first, q.n, q.L);
   if (in_order) *in_order = on;
-  q.L = paged_length(a.c, s);
   const int lowest = a.window > 0 ? max(0, q.L - q.n + 1 - a.window) : 0;
   q.begin = min(lowest, q.L) & ~(unit - 1);
   q.tiles = q.n * a.group <= a.rows ? (q.n > 0 ? 1 : 0) : (q.n * a.group + a.rows - 1) / a.rows;
@@ -98,7 +109,7 @@ __device__ __forceinline__ long long row_offset(const PagedAttention &a, const P
 }
 __device__ __forceinline__ long long row_index(const PagedAttention &a, const PagedPart &w, int r) {
   const int token = (int)quotient(w.g.r0 + r, a.group), head = w.g.kvh * a.group + (w.g.r0 + r) - token * a.group;
-  return (long long)(w.q.first + token) * a.n_head + head;
+  return (long long)(w.q.first - a.row0 + token) * a.n_head + head;
 }
 
 // Every group begins with a.extra units that have no positions: what it takes to load its queries and to put its results together,
@@ -1130,17 +1141,17 @@ paged_weights_kernel(const __grid_constant__ PagedAttention a, float *__restrict
   pdl_wait();
   const PagedView &c = a.c;
   const int s = blockIdx.y;
-  if (__ldcg(a.skip) != 0) return;
-  int first, n;
-  new_rows(c, a.r, s, first, n);
-  const int L = paged_length(c, s);
+  const unsigned int skip = __ldcg(a.skip);
+  int first, n, L;
+  launch_rows(a, s, first, n, L);
+  if (n == 0 || skip != 0) return;
   for (int j = blockIdx.x * 256 + threadIdx.x; j < L; j += gridDim.x * 256) {
     float w = 0.f;
     const float old = weights[s * ld + j];
     for (int t = 0; t < n; t++) {
       const int end = L - n + t + 1, begin = a.window > 0 ? max(0, end - a.window) : 0;
       if (j < begin || j >= end) continue;
-      const long long row = (long long)(first + t) * a.n_head;
+      const long long row = (long long)(first - a.row0 + t) * a.n_head;
       for (int h0 = 0; h0 < a.n_head; h0 += 8) {
         float sc[8], lse[8];
 #pragma unroll

@@ -83,7 +83,7 @@ static int32_t paged_workspace(wgpt_device *dev, PagedAttention &a, int grid, in
               ((int64_t)a.r.n_rows * a.group / a.rows + a.c.n_seq) * (a.c.max_length / unit + 2 + a.extra) <
                   (((int64_t)1 << 32) - ((int64_t)1 << 20)) / a.c.n_kv,
           WGPT_ERR_SHAPE, "%d rows over up to %d positions of %d heads: split the call", a.r.n_rows, a.c.max_length, a.c.n_kv);
-  const size_t rows = a.stats ? (size_t)a.r.n_rows * a.n_head : 0, scores = rows * (size_t)a.c.max_length;
+  const size_t rows = a.stats ? (size_t)(a.row1 - a.row0) * a.n_head : 0, scores = rows * (size_t)a.c.max_length;
   const size_t partial = (size_t)2 * grid * paged_slot(a.rows, a.c.hs);
   TRY(scratch_reserve(dev, (partial + 1 + rows + scores) * 4));
   a.partial = static_cast<float *>(dev->scratch);
@@ -213,17 +213,24 @@ WGPT_EXPORT int32_t wgpt_paged_attention(wgpt_device *dev, const wgpt_paged_cach
   a.out = out;
   a.ld_q = ld_q;
   a.ld_out = ld_out;
-  a.scores = nullptr;
-  a.stats = weights;  // that there are any; their place is found with the rest of the workspace
-  if (cache->type == WGPT_TYPE_F32)
-    TRY(launch_paged_type<float>(dev, a));
-  else if (cache->type == WGPT_TYPE_F16)
-    TRY(launch_paged_type<__half>(dev, a));
-  else
-    TRY(launch_paged_type<__nv_bfloat16>(dev, a));
-  if (weights) {
-    const int blocks = std::min((cache->max_length + 255) / 256, std::max(1, 8 * dev->sm_count / cache->n_seq));
-    LAUNCH_PDL(dev, paged_weights_kernel, dim3(blocks, cache->n_seq), dim3(256), 0, a, weights, (long long)ld_weights);
+  // Scores are kept for the kernel that adds them up: as many rows at a time as take no more than this of the workspace, or one
+  const size_t per_row = (size_t)n_head * cache->max_length * sizeof(float), most = (size_t)1 << 30;
+  const int64_t slice = weights ? std::max<int64_t>(1, (int64_t)(most / per_row)) : n_rows;
+  for (int64_t row = 0; row < n_rows; row += slice) {
+    a.row0 = (int)row;
+    a.row1 = (int)std::min<int64_t>(n_rows, row + slice);
+    a.scores = nullptr;
+    a.stats = weights;  // that there are any; their place is found with the rest of the workspace
+    if (cache->type == WGPT_TYPE_F32)
+      TRY(launch_paged_type<float>(dev, a));
+    else if (cache->type == WGPT_TYPE_F16)
+      TRY(launch_paged_type<__half>(dev, a));
+    else
+      TRY(launch_paged_type<__nv_bfloat16>(dev, a));
+    if (weights) {
+      const int blocks = std::min((cache->max_length + 255) / 256, std::max(1, 8 * dev->sm_count / cache->n_seq));
+      LAUNCH_PDL(dev, paged_weights_kernel, dim3(blocks, cache->n_seq), dim3(256), 0, a, weights, (long long)ld_weights);
+    }
   }
   return WGPT_OK;
 }
