@@ -146,3 +146,60 @@ def test_scores_of_more_than_the_workspace_holds(dev, type, n_kv, group, hs, win
     assert free - dev.mem_info()[0] < 3 << 29  # 95 rows whole: 3 GB
     check_attention(dev, pages, type, "positions", [1, 1, 1, 0, 1, 1], n_kv * group, window=window, weights=True)
     _lib.call("wgpt_device_check", dev.handle)
+
+
+@pytest.mark.parametrize("type,n_kv,group,hs", [("f16", 2, 3, 64), ("bf16", 1, 5, 128), ("f16", 1, 20, 40), ("bf16", 2, 1, 72), ("f32", 1, 3, 64), ("f16", 1, 2, 256)])
+@pytest.mark.parametrize("window", [0, 200])
+def test_prompts_behind_contexts(dev, type, n_kv, group, hs, window):  # noqa: F811
+    """Many row tiles over many key tiles each: tiles that begin and end at different units, parts without any, joins of unequal parts."""
+    rng = np.random.default_rng(7)
+    pages = make(rng, [1500, 260, 700, 129], 32, n_kv, hs, type)
+    check_attention(dev, pages, type, "heads", [170, 260, 90, 1], n_kv * group, window=window, weights=True, before=1, behind=1)
+
+
+@pytest.mark.parametrize("type,group,hs", [("f32", 1, 64), ("f32", 8, 64), ("f16", 1, 64), ("f16", 8, 128), ("f16", 12, 64), ("f16", 20, 128), ("bf16", 1, 64),
+                                           ("bf16", 8, 128), ("bf16", 12, 64), ("bf16", 20, 128), ("f16", 9, 256), ("bf16", 9, 256)])
+def test_queries_and_probabilities_are_as_good_as_f32(dev, type, group, hs):  # noqa: F811
+    """Keys and values of the unit vectors and a scale of one: the output is the softmax of the query itself, whose products and
+    sums of values are exact. What is left, in halves of an f32 step: a score s is the query's value times log2 e in f32 (two roundings), the
+    difference to a maximum (one), all times s; an exponential (four: 2^-22); a probability and the sum it is divided by have these
+    (twice); additions of the sum over lanes, tiles and key groups, rescalings, the quotient: up to 28. Half-precision queries are two
+    values, good to 2^-22 of the row's largest, four steps of it. Third terms of bfloat16 queries that are left out are 2^-18 of the query:
+    64 steps times s; of probabilities likewise 64, on average 37, of which the root of the mean square shows more than a tenth."""
+    rng = np.random.default_rng(8)
+    pages = ref.Pages(rng, [hs], 16, 1, hs)
+    for j in range(hs):
+        for pool in (pages.k, pages.v):
+            pool[pages.place(0, j)] = np.eye(hs, dtype=np.float32)[j]
+    cache = OnDevice(dev, pages, type)
+    for low, high in ((12.0, 16.0), (-1.0, 1.0)):
+        q = rng.uniform(low, high, (1, group, hs)).astype(np.float32)
+        got, _ = attend(dev, cache, None, 1, group, 1.0, 0, q)
+        e = np.exp(q.astype(np.float64) - q.max(-1, keepdims=True))
+        want = e / e.sum(-1, keepdims=True)
+        off = np.abs(got / want - 1) / ref.U32
+        most = 2 * (6 * max(abs(low), high) + 4) + 28 + (2 * 4 * 16 if type == "f16" and high > 2 else 8 if type == "f16" else 0)
+        assert off.max() <= most
+        if high < 2:
+            # some 50 roundings, each of a mean square of a third of a half step's: four steps, three times over
+            assert math.sqrt((off ** 2).mean()) <= 12
+
+
+def test_a_step_while_a_pass_list_is_recorded(dev):  # noqa: F811
+    """What waits for the device is refused there, and the cache stays as it was."""
+    from webgpt_b200.paged import PagedCache
+    cache = PagedCache(dev, 2, 1, 8, n_pages=8, page_size=4, n_layer=1, weights=True)
+    cache.advance([5, 9])
+    before = [list(p) for p in cache.pages], list(cache.free), list(cache.lengths)
+    g = C.c_void_p()
+    _lib.call("wgpt_graph_begin", dev.handle)
+    for step in (lambda: cache.advance(1), lambda: cache.retreat([1, 0]), lambda: cache.release(1), lambda: cache.evict(4, 1)):
+        with pytest.raises(_lib.WgptError) as e:
+            step()
+        assert e.value.code == _lib.ERR_STATE
+        assert (cache.pages, cache.free, list(cache.lengths)) == before
+    _lib.call("wgpt_graph_end", dev.handle, C.byref(g))
+    _lib.call("wgpt_graph_destroy", dev.handle, g)
+    cache.retreat([1, 2])
+    assert list(cache._lengths[0].read(np.int32)) == [4, 7]
+    cache.destroy()

@@ -6,6 +6,7 @@ import pytest
 
 import serving_reference as ref
 from test_gpu_verify import check, dev  # noqa: F401 (a fixture)
+from webgpt_b200 import _lib
 
 NEAR = 1e-10
 
@@ -86,3 +87,33 @@ def test_temperatures_at_the_ends(dev, temperature, top_k):  # noqa: F811
     with np.errstate(over="ignore"):
         check(dev, t, d, ids, None, top_k, temperature, rng.random((6, 3)))
         check(dev, t, None, ids, None, top_k, temperature, rng.random((6, 3)))
+
+
+@pytest.mark.parametrize("top_k", [0, 7])
+@pytest.mark.parametrize("value", [np.nan, -np.inf, np.inf])
+@pytest.mark.parametrize("of_draft", [False, True])
+def test_rows_without_a_distribution_are_reported(dev, top_k, value, of_draft):  # noqa: F811
+    """Each such row by itself, where it decides something: rows of nothing but NaN or -infinity, rows with one +infinity."""
+    rng = np.random.default_rng(9)
+    V, n_draft = 3000, 2
+    for row in range(n_draft if of_draft else n_draft + 1):
+        t, d = (rng.standard_normal((3, n, V)).astype(np.float32) for n in (n_draft + 1, n_draft))
+        d[...] = t[:, :n_draft]  # accepted wherever the number is below one
+        ids, u = np.argmax(t[:, :n_draft], 2).astype(np.uint32), np.full((3, n_draft + 1), 0.5)
+        check(dev, t, d, ids, None, top_k, 1.0, u)
+        _lib.call("wgpt_device_check", dev.handle)
+        x = d if of_draft else t
+        if value == np.inf:
+            x[1, row, 17] = value
+        else:
+            x[1, row] = value
+        accepted = check(dev, t, d, ids, None, top_k, 1.0, u)[1]
+        assert list(accepted) == [n_draft, row, n_draft]
+        with pytest.raises(_lib.WgptError) as e:
+            _lib.call("wgpt_device_check", dev.handle)
+        assert e.value.code == _lib.ERR_ARG and "row of logits" in e.value.message
+        if row < n_draft:  # turned down before it: the row decides nothing
+            ids[1, 0], u[1, 0] = np.argmin(t[1, 0] if row > 0 or of_draft else d[1, 0]), 1.0
+            if row > 0:
+                check(dev, t, d, ids, None, top_k, 1.0, u)
+                _lib.call("wgpt_device_check", dev.handle)
