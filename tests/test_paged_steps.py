@@ -190,3 +190,19 @@ def test_keep_past_the_longest_sequence(monkeypatch):
     for keep, recent in ((100, 101), (0, 0), (5, -1)):
         with pytest.raises(ValueError):
             c.evict(keep, recent)
+
+
+def test_an_eviction_that_is_refused_allocates_nothing(monkeypatch):
+    """While a pass list is being recorded writes are refused, and so is giving buffers back: none may have been made by then."""
+    c = PagedCache(Addresses(), 1, 1, 8, n_pages=8, page_size=4, max_length=16, weights=True)
+    keeper(monkeypatch, c)
+    c.advance(12)
+
+    def refused(self, array, offset=0):
+        raise OSError("recording")
+
+    made = len(c.device.made)
+    monkeypatch.setattr(FakeBuffer, "write", refused)
+    with pytest.raises(OSError):
+        c.evict(4, 1)
+    assert len(c.device.made) == made

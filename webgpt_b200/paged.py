@@ -142,13 +142,13 @@ class PagedCache:
             else:
                 runs.append([at, s, 1])
         row = self.max_length * 4
+        self._tables[1].write(self._table_of(pages))  # first: where it is refused, so is giving buffers back
         got, moved, kept = [], [], None
         try:
             kept = self.device.buffer(len(sequences) * keep * 4)
             for _ in range(self.n_layer):  # the weights that stay, zeros behind them
                 moved.append(self.device.buffer(len(sequences) * row))
                 moved[-1].write(np.zeros(len(sequences) * self.max_length, np.float32))
-            self._tables[1].write(self._table_of(pages))
             for i in range(self.n_layer):
                 for at, s, n in runs:
                     _lib.call("wgpt_paged_evict", self.device.handle, self.layer(i, 0, s, n).ptr, self.layer(i, 1, s, n).ptr, keep, recent,
