@@ -143,7 +143,8 @@ static bool paged_few(const wgpt_device *dev, const PagedAttention &a, int unit)
 
 // How many of the rows that share a head of the cache a CTA takes at once: what a sequence has of them on average. More row
 // tiles read the cache again, fewer rows leave room for more keys in flight. 16-bit types, head sizes up to 128: up to eight rows
-// are one tile of mma.sync, more go to tcgen05. Measured with both, f16, 4 heads of the cache, one new token, tcgen05 first: head size
+// are one tile of mma.sync, more go to tcgen05 (a rule on rows alone: long sequences with eight rows are better there, as the first of these
+// figures shows, the others are not). Measured with both, f16, 4 heads of the cache, one new token, tcgen05 first: head size
 // 128, 8 users of 8192 positions, 8 rows 27.4 / 30.8 us, 12 rows 28.3 / 41.7; 64 users of 1000, 35.4 / 33.1 and 36.4 / 50.9; head
 // size 64, 24.2 / 21.0 and 23.7 / 26.7, 32.2 / 24.6 and 32.1 / 31.0. 12 rows in tiles of 16 and of 32: 28.4 / 30.9 and 32.0 / 34.8.
 // f32, 8 users of 8192, 4 heads of 64, 2 rows in tiles of two and of four: 27.2 / 31.4, 4 rows in tiles of four and of eight: 31.5 / 41.7.
@@ -324,14 +325,15 @@ WGPT_EXPORT int32_t wgpt_verify_drafts(wgpt_device *dev, int32_t n_seq, int32_t 
   a.partial = static_cast<float2 *>(dev->scratch);
   const int warps = kVerifyThreads / 32;
   LAUNCH_PDL(dev, verify_sums_kernel, dim3((a.chunks + warps - 1) / warps, rows, n_seq), dim3(kVerifyThreads), 0, a);
-  // As many CTAs a sequence as are resident at once, two an SM: 64 sequences of 4 drafts over 50257 ids take 45.4 us with four CTAs each,
-  // 55.4 with eight (two waves), 57.2 with two. Where a few sequences leave half of the SMs empty anyway, a CTA may take all the registers:
-  // five logits of each row at once and one CTA an SM, against two and two: 1 sequence 15.6 / 16.1 us, 8 20.0 / 22.2, 16 30.0 / 26.8.
+  // As many CTAs a sequence as are resident at once, two an SM: 64 sequences of 4 drafts over 50257 ids take 43.5 us with four CTAs each,
+  // some 10 more with eight (two waves) or two. As long as one wave of clusters of eight has a CTA an SM (14 sequences; the SMs next to
+  // one another do not always make another cluster), a CTA may take all the registers: four logits of each row at once against two, and
+  // two CTAs an SM: 1 sequence 15.0 / 15.6 us, 8 19.4 / 21.3, 14 21.8 / 24.8, 16 28.9 / 25.1.
   int C = kDrawCluster;
   while (C > 1 && C * n_seq > 2 * dev->sm_count) C /= 2;
   const dim3 grid(C * n_seq), block(kDrawThreads);
-  if (C == kDrawCluster && 2 * C * n_seq <= dev->sm_count)
-    CK(launch_ex_x(dev->pdl, C, dev->stream, verify_draw_kernel<5, 1>, grid, block, 0, a));
+  if (C == kDrawCluster && 5 * C * n_seq <= 4 * dev->sm_count)
+    CK(launch_ex_x(dev->pdl, C, dev->stream, verify_draw_kernel<4, 1>, grid, block, 0, a));
   else
     CK(launch_ex_x(dev->pdl, C, dev->stream, verify_draw_kernel<2, 2>, grid, block, 0, a));
   dev->launches++;

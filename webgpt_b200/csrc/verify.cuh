@@ -258,8 +258,8 @@ __device__ __forceinline__ void write_ids(const Verify &a, int s, int accepted, 
 // tells them apart by the good sums. Equal rows have equal sums and leave zeros.
 // Every warp takes a stretch of ids; the sums of the stretches say in which one the running sum passes the number, and the warps of
 // its CTA add that stretch up id by id, a row of 32 ids each.
-// Bound by latency (logits, exponentials, three barriers of the cluster): one user with 4 drafts over 50257 ids 14.1 us with the sums, 64 users
-// 45.5.
+// Bound by latency (logits, exponentials, three barriers of the cluster): one user with 4 drafts over 50257 ids 15.0 us with the sums, 64 users
+// 43.5.
 constexpr int kDrawThreads = 512, kDrawWarps = kDrawThreads / 32, kDrawCluster = 8;
 // A row's sum in f32 is off by less than 1e-5 of itself: 70 roundings of a lane's additions and of its five rescalings (2^-24 each), six
 // exponentials (2^-22), and three roundings in each exponent's argument, (largest - logit) / temperature, whose mean over the
@@ -297,6 +297,8 @@ __global__ void __launch_bounds__(kDrawThreads, kCtas) verify_draw_kernel(const 
   // of every warp of the cluster, for each round: the target's row, the draft's, and both over the ids that count
   __shared__ double sums[2][4][kDrawCluster][kDrawWarps];
   __shared__ double s_row[2][32];  // sums of rows of 32 ids
+  __shared__ double s_found[4];    // total, the rows' sums, what lies before the stretch that has the id
+  __shared__ int s_owner;
   uint32_t C;
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(C));
   const int rank = (int)cluster_ctarank(), s = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -446,23 +448,24 @@ __global__ void __launch_bounds__(kDrawThreads, kCtas) verify_draw_kernel(const 
     cluster_arrive();
     cluster_wait();
   };
-  // of all warps' sums: what each counts and what lies before it, and their total; every warp for itself, four sums a lane
+  // Of all warps' sums, by one warp, four sums a lane: their total, and the last stretch with anything in it that begins at or below
+  // number * total, which has the id (rounding may put the beginning of an empty one there); -1: a number that is none. The other warps
+  // doing the same would keep it from the FP64 pipe.
   constexpr int kAll = kDrawCluster * kDrawWarps, kPer = kAll / 32;
-  double of[kPer], ahead[kPer];
   auto before_lane = [&](double upto) {  // no difference: a tiny sum ahead of a large one is not to be lost
     const double x = __shfl_up_sync(0xffffffffu, upto, 1);
     return lane > 0 ? x : 0.0;
   };
-  auto prefixes = [&]() {
+  auto find = [&]() {
     const double *v = &sums[round][0][0][0] + lane * kPer;
     const double *v2 = v + (rest ? 2 * kAll : 0);
-    double up2[kPer], up3[kPer], run2 = 0.0, run3 = 0.0;
+    double of[kPer], ahead[kPer], up2[kPer], up3[kPer], run2 = 0.0, run3 = 0.0;
 #pragma unroll
     for (int u = 0; u < kPer; u++) {
       up2[u] = run2;
       run2 += v2[u];
     }
-    double before2 = run2, before3 = 0.0, total;
+    double before2 = run2, total;
     if (two && rest) {
       zp = zq = 0.0;
 #pragma unroll
@@ -472,7 +475,7 @@ __global__ void __launch_bounds__(kDrawThreads, kCtas) verify_draw_kernel(const 
         zp += v[u];
         zq += v[kAll + u];
       }
-      before3 = run3;
+      double before3 = run3;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const double a2 = __shfl_up_sync(0xffffffffu, before2, o), a3 = __shfl_up_sync(0xffffffffu, before3, o);
@@ -486,13 +489,15 @@ __global__ void __launch_bounds__(kDrawThreads, kCtas) verify_draw_kernel(const 
       total = __shfl_sync(0xffffffffu, before2, 31) * zq - __shfl_sync(0xffffffffu, before3, 31) * zp;
       before2 = before_lane(before2);
       before3 = before_lane(before3);
+      bool left = false;
 #pragma unroll
       for (int u = 0; u < kPer; u++) {
         const double p = v2[u] * zq, w = p - v[3 * kAll + u] * zp;
         of[u] = w > kNoise * p ? w : 0.0;
+        left = left || of[u] > 0.0;
         ahead[u] = (before2 + up2[u]) * zq - (before3 + up3[u]) * zp;
       }
-      if (!__any_sync(0xffffffffu, of[0] + of[1] + of[2] + of[3] > 0.0)) total = 0.0;
+      if (!__any_sync(0xffffffffu, left)) total = 0.0;
     } else {
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -507,14 +512,32 @@ __global__ void __launch_bounds__(kDrawThreads, kCtas) verify_draw_kernel(const 
         ahead[u] = before2 + up2[u];
       }
     }
-    return total;
+    int mine = -1;
+    double from = 0.0;
+#pragma unroll
+    for (int u = 0; u < kPer; u++)
+      if (ahead[u] <= u01 * total && of[u] > 0.0) {
+        mine = lane * kPer + u;
+        from = ahead[u];
+      }
+    const int owner = __reduce_max_sync(0xffffffffu, mine);
+    if (lane == 0) {
+      s_found[0] = total;
+      s_found[1] = zp;
+      s_found[2] = zq;
+      s_owner = owner;
+    }
+    if (owner >= 0 && mine == owner) s_found[3] = from;
   };
-  static_assert(kPer == 4, "");
   double total;
   for (bool added = false;;) {  // the same for the whole cluster
     if (!added) add_up();
     added = true;
-    total = prefixes();
+    if (warp == 0) find();
+    __syncthreads();
+    total = s_found[0];
+    zp = s_found[1];
+    zq = s_found[2];
     if (two && rest && !none && round == 0 && total < kLeft * zp * zq) {  // again, with the good sums
       round = 1;
       added = false;
@@ -523,6 +546,7 @@ __global__ void __launch_bounds__(kDrawThreads, kCtas) verify_draw_kernel(const 
     } else {
       break;
     }
+    __syncthreads();  // before the places are written again
   }
   if (none) {
     if (rank == 0 && warp == 0) {
@@ -531,24 +555,14 @@ __global__ void __launch_bounds__(kDrawThreads, kCtas) verify_draw_kernel(const 
     }
     return;
   }
-  // the last stretch with anything in it that begins at or below the goal has the id (rounding may put the beginning of an empty
-  // one there)
   const double goal = u01 * total;
-  int mine = -1;
-#pragma unroll
-  for (int u = 0; u < kPer; u++)
-    if (ahead[u] <= goal && of[u] > 0.0) mine = lane * kPer + u;
-  const int owner = __reduce_max_sync(0xffffffffu, mine);
-  if (owner < 0) {  // a number that is none
+  const int owner = s_owner;
+  if (owner < 0) {
     if (rank == 0 && warp == 0) write_ids<32>(a, s, at, (uint32_t)(a.V - 1), lane);
     return;
   }
   if (owner / kDrawWarps != rank) return;
-  double before = 0.0;
-#pragma unroll
-  for (int u = 0; u < kPer; u++)
-    if (owner == lane * kPer + u) before = ahead[u];
-  before = __shfl_sync(0xffffffffu, before, owner / kPer);
+  double before = s_found[3];
   // The stretch's rows of 32 ids, two a warp at a time: their sums, then, in the first whose running sum passes the goal, id by
   // id. The stretch's sum was rounded in another order and may pass the goal where the running sum does not: the last id that counts then.
   constexpr int kRows = 2;
