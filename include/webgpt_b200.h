@@ -364,7 +364,8 @@ int32_t wgpt_paged_attention(wgpt_device *dev, const wgpt_paged_cache *cache, in
 /* Thins out every sequence that holds more than `keep` positions: the `recent` newest stay and, of the older ones, the
  * keep - recent with the largest accumulated weight (the lowest position among equals; NaN counts as the largest). What
  * stays keeps its order and goes to the positions 0, 1, ... of the cache `to`, which has the shape and type of `from` and
- * pages and a table of its own; its lengths (which may be from's array) are set to min(length, keep). Sequences of up to `keep`
+ * pages and a table of its own; its lengths (which may be from's array) are set to min(length, keep). Layers that share their
+ * lengths need another array for `to`: the second would find those that the first has set. Sequences of up to `keep`
  * positions are copied whole. The pages of `to` must not overlap the pages of `from` (slots that are read may be shared by sequences, so
  * nothing is moved in place): hand over free pages and take back the old ones. Key and value rows are copied as they are.
  * weights [n_seq, ld_weights] as above; weights_to [n_seq, ld_weights_to >= keep], or NULL: the weights of what stays, zeros

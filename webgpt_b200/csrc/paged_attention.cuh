@@ -1,7 +1,7 @@
 // Attention of new tokens over a paged cache.
 //   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = 2^(c s_ij - m_i),  s_ij = q_i . k_j,  c = scale / ln 2,  m_i = max_j c s_ij
 // in one pass over the keys, with the running maximum and sum in f32 (sums and values are multiplied by 2^(old - new maximum)
-// when it moves).
+// when it moves). Exponentials are ex2.approx, good to 2^-22; CUDA's exp2f promises two units in the last place, which is as much.
 //
 // What bounds it is the cache's bytes: a row of K and V is read once for all the query rows that share it (the heads of its
 // group, times the new tokens), at most a row tile of them; and for small calls a chain of about 7 us: lengths, pages, the first

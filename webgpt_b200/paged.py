@@ -3,6 +3,8 @@
 The pools, the page table and the lengths lie on the device, where wgpt_paged_append / _attention / _evict read them; this
 class keeps the free pages and a mirror of table and lengths, and hands out the descriptors. All layers share one table.
 A step is: advance() by the new tokens, append and attend per layer, retreat() by the drafts that were not accepted.
+With weights, attention adds those of all new tokens up, of drafts too: a retreat clears those of the positions that it drops, not
+what the dropped tokens gave to others.
 """
 import ctypes as C
 
@@ -107,9 +109,10 @@ class PagedCache:
     # ------------------------------------------------------------------ eviction
     def evict(self, keep, recent):
         """Thins out the sequences that hold more than keep positions, in every layer by its own weights; returns the
-        positions that stayed, [n_layer, n_seq, min(keep, max_length)], -1 behind them. Sequences of up to keep positions stay as they are.
-        What stays of the others goes to free pages: needs as many as one sequence of keep positions has. As many sequences
-        as there are pages for are thinned out together; a failure leaves those whole that had not come to it."""
+        positions that stayed, [n_layer, n_seq, min(keep, max_length)], -1 behind them. Sequences of up to keep positions
+        stay as they are. What stays of the others goes to free pages: needs as many as one sequence of keep positions
+        has. As many sequences as there are pages for are thinned out together; a failure leaves those whole whose turn
+        had not come."""
         if self._weights is None:
             raise ValueError("the cache keeps no weights: create it with weights=True")
         keep, recent = int(keep), int(recent)
