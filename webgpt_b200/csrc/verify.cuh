@@ -563,6 +563,7 @@ __global__ void __launch_bounds__(kDrawThreads, kCtas) verify_draw_kernel(const 
   }
   if (owner / kDrawWarps != rank) return;
   double before = s_found[3];
+  if (tid == 0) s_last = owner * stretch;  // an id whatever rounding does in very long stretches
   // The stretch's rows of 32 ids, two a warp at a time: their sums, then, in the first whose running sum passes the goal, id by
   // id. The stretch's sum was rounded in another order and may pass the goal where the running sum does not: the last id that counts then.
   constexpr int kRows = 2;
